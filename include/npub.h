@@ -292,6 +292,90 @@ int npub_rope_kv_store_freqs(void* qkv, int64_t ldx, int tokens, int tokens_per_
 int npub_rope_llama3_freqs(float* out, int head_dim, double theta, double factor, double low, double high,
                            double old_ctx);
 
+/* ------------------------------------------------ paged KV cache ----
+ * A paged cache is a pool of pages k_pages / v_pages, fp16
+ * [n_pages, kv_heads, page_size, head_dim] (contiguous, 16-byte aligned), and
+ * a table page_table int32 [batch, max_pages] (row stride ldt): key p of
+ * sequence b is slot p % page_size of page page_table[b, p / page_size].
+ * page_size is a power of two.  Sequences may hold the same page.  Packed rows: the new rows of
+ * all sequences one after the other, sequence b at rows
+ * [cu_seqlens[b], cu_seqlens[b + 1]) (int32 [batch + 1], ascending); rows
+ * outside [cu_seqlens[0], cu_seqlens[batch]) are neither computed nor
+ * written.  (The reference keeps no cache; its attention is
+ * llama_layer.py:114-137, its rotation llama_layer.py:96-112.)
+ *
+ * npub_rope_paged_append: RoPE, an optional RMSNorm of every q and k head and
+ * the cache append, in one pass over the fused rows qkv [tokens, ldx] (q
+ * heads | k heads | v heads, head_dim columns each).  Row t belongs to
+ * sequence t when cu_seqlens is NULL (a decode step, batch == tokens), else to
+ * the packed sequence that holds it.  Per q and k head x:
+ *   x_i <- x_i * gamma_i / sqrt(mean(x^2) + eps)   (q_gamma / k_gamma fp16 [head_dim]; NULL: no norm)
+ *   the first rot_dim columns rotated by the angles positions[t] * inv_freq[i]
+ *   (fp32 [rot_dim / 2], e.g. npub_rope_llama3_freqs): pairs (i, i + rot_dim/2),
+ *   or (2i, 2i + 1) when interleaved != 0; the other columns pass through
+ * in fp32 (the angle's product and reduction in fp64), rounded once.  q goes
+ * to q_out [tokens, ldq] (may alias the q columns of qkv), k and v to the
+ * cache at positions[t].  A row whose position lies outside
+ * [0, max_pages * page_size), or whose page id lies outside [0, n_pages), is
+ * rotated but not stored.  Two rows with the same slot: one of them is kept.
+ * head_dim % 16 == 0, <= 512; rot_dim % 16 == 0, 0 < rot_dim <= head_dim;
+ * page_size 1 .. 65536. */
+int npub_rope_paged_append(const void* qkv, int64_t ldx, void* q_out, int64_t ldq, int tokens, int q_heads,
+                           int kv_heads, int head_dim, int rot_dim, int interleaved, const int32_t* positions,
+                           const float* inv_freq, const void* q_gamma, const void* k_gamma, float eps, void* k_pages,
+                           void* v_pages, int n_pages, int page_size, const int32_t* page_table, int64_t ldt,
+                           int max_pages, const int32_t* cu_seqlens, int batch, void* stream);
+
+/* Attention of packed prompts of different lengths (llama_layer.py:114-137
+ * per sequence and head): q [total, heads*head_dim], k, v [total,
+ * kv_heads*head_dim] rows with strides ldq / ldk / ldv (multiples of 8), query
+ * head h reads kv head h / (heads / kv_heads), out fp16 [total,
+ * heads*head_dim] (ldo).  causal != 0: row i of a sequence sees its rows
+ * 0..i; else all of them.  max_len: the longest sequence's rows, or 0 when not
+ * known; a longer sequence's rows past it are not computed.  scale > 0;
+ * head_dim % 16 == 0.  head_dim > 128 or heads / kv_heads > 128 returns
+ * NPUB_ERR_UNSUPPORTED.  Nothing outside a sequence reaches its results, but
+ * the values of its own later rows have to be finite.  Needs no workspace. */
+int npub_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                          void* out, int64_t ldo, const int32_t* cu_seqlens, int batch, int total, int max_len,
+                          int heads, int kv_heads, int head_dim, float scale, int causal, void* stream);
+
+/* Attention of packed new rows over the paged cache (a prompt chunk behind
+ * what its pages hold, a prompt whose prefix is cached, drafted tokens): the
+ * keys of sequence b are positions 0 .. lens[b] - 1 (int32 [batch], clipped to
+ * [0, max_pages * page_size]), its n new rows the last n of them, so row i
+ * sees lens[b] - n + i + 1 keys (all of them when causal == 0); a row that
+ * sees none gives zeros.  max_new as max_len above; ctx_len: the largest
+ * lens[b] expected (0: the table's width), which only decides how the keys
+ * are split over CTAs.  A page id outside [0, n_pages) reads as zeros.
+ * page_size 16 .. 256; otherwise as npub_attention_packed.  Workspace:
+ * npub_attention_paged_workspace() bytes for the same sizes and ctx_len (the
+ * table's width where ctx_len is 0 or larger), 256-byte aligned; may be NULL when that is 0. */
+int npub_attention_paged(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int n_pages,
+                         int page_size, const int32_t* page_table, int64_t ldt, int max_pages, const int32_t* lens,
+                         const int32_t* cu_seqlens, int batch, int total, int max_new, int ctx_len, void* out,
+                         int64_t ldo, int heads, int kv_heads, int head_dim, float scale, int causal, void* workspace,
+                         size_t workspace_bytes, void* stream);
+size_t npub_attention_paged_workspace(int batch, int total, int max_new, int64_t ctx_len, int heads, int kv_heads,
+                                      int head_dim);
+
+/* Decode attention over the paged cache, one new row per sequence (row b of q
+ * and out), keys 0 .. lens[b] - 1.  shared_len > 0 (a multiple of page_size)
+ * says that the first shared_len keys of every sequence are in the same
+ * pages: they are read through row 0 of the table, once for the whole batch
+ * instead of once per sequence.  A sequence with lens[b] < shared_len sees the
+ * first lens[b] of them; lens[b] <= 0 gives zeros.  The result is that of
+ * shared_len 0 up to rounding.  ctx_len, workspace and limits as above
+ * (npub_attention_paged_decode_workspace with the same ctx_len and
+ * shared_len); batch <= 65535. */
+int npub_attention_paged_decode(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int n_pages,
+                                int page_size, const int32_t* page_table, int64_t ldt, int max_pages,
+                                const int32_t* lens, int batch, int ctx_len, int shared_len, void* out, int64_t ldo,
+                                int heads, int kv_heads, int head_dim, float scale, void* workspace,
+                                size_t workspace_bytes, void* stream);
+size_t npub_attention_paged_decode_workspace(int batch, int64_t ctx_len, int shared_len, int heads, int kv_heads,
+                                             int head_dim);
+
 /* ------------------------------------------------- NPU ISA semantics ----
  * One compute instruction of the NPU over PE buffers (_poc/mysim.cpp:114-141):
  * `word` is the 32-bit instruction (opcodes 0x01-0x13 vector, 0x40-0x43

@@ -68,6 +68,15 @@ SIGNATURES = {
     "npub_rope_kv_store_freqs": (_i, [_p, _i64, _i, _i, _i, _i, _i, _p, _p, _p, _p, _i64, _p]),
     "npub_rope_llama3_freqs": (_i, [_p, _i, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                                     ctypes.c_double]),
+    "npub_rope_paged_append": (_i, [_p, _i64, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _f, _p, _p, _i, _i,
+                                    _p, _i64, _i, _p, _i, _p]),
+    "npub_attention_packed": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i, _i, _i, _i, _i, _i, _f, _i, _p]),
+    "npub_attention_paged": (_i, [_p, _i64, _p, _p, _i, _i, _p, _i64, _i, _p, _p, _i, _i, _i, _i, _p, _i64, _i, _i,
+                                  _i, _f, _i, _p, _sz, _p]),
+    "npub_attention_paged_workspace": (_sz, [_i, _i, _i, _i64, _i, _i, _i]),
+    "npub_attention_paged_decode": (_i, [_p, _i64, _p, _p, _i, _i, _p, _i64, _i, _p, _i, _i, _i, _p, _i64, _i, _i, _i,
+                                         _f, _p, _sz, _p]),
+    "npub_attention_paged_decode_workspace": (_sz, [_i, _i64, _i, _i, _i, _i]),
     "npub_isa_vector": (_i, [_u32, _p, _p, _p, _p, _i64, _p]),
     "npub_f32_to_f16": (_i, [_p, _p, _i64, _p]),
     "npub_f16_to_f32": (_i, [_p, _p, _i64, _p]),

@@ -1,0 +1,644 @@
+// Attention of packed (ragged) query rows over packed K/V rows or a paged KV
+// cache, grouped heads, head_dim <= 128, on sm_100a.
+//
+// O = softmax(scale Q K^T + mask) V per sequence and head, the attention of
+// b_program_examples/llama_layer.py:114-137 in the max-subtracted form of
+// d_compiler/npu_compiler/model.py:145-150.  Query row i of a sequence with n
+// new rows and m keys sees keys 0 .. m - n + i (all m without the causal
+// mask); a row that sees no key gives zeros.
+//
+// A tile is 128 rows of one kv head: row r = (token r / G, head r % G) of its
+// G query heads, so that the group shares every K/V load and a prompt of few
+// tokens still fills rows.  A CTA takes two tiles, which share K and V:
+//   S_q(j) = Q_q K_j^T          tcgen05.mma, fp32 in TMEM
+//   P_q(j) = exp2(S c - m c)    one thread per row; fp16, over S_q's own TMEM columns
+//   O_q   += P_q(j) V_j         tcgen05.mma with A = P from TMEM, V read MN-major
+// O stays in TMEM over the whole key loop.  A row's reference maximum m moves
+// (and its O and sum are rescaled) only when the row maximum has grown by more
+// than 2^8: P then stays below 2^8, far inside fp16, and the rescale, which
+// reads and writes the O tile, is rare.  The tensor core works on one tile
+// while the other is in its softmax.
+//
+// Keys past a sequence's end inside its last 128-key block are whatever lies
+// behind them (the next sequence's rows, a page's stale slots): their scores
+// are masked by a select, and their V rows are zeroed in shared memory before
+// the product, since 0 * NaN and 0 * inf are NaN.
+//
+// Roles (384 threads): warps 0-3 and 4-7 softmax and output of tile 0 and 1,
+// warp 8 TMA, warp 9 tensor-memory allocation and MMA issue.
+#include "common.cuh"
+#include "fmha_packed.h"
+#include "gemm_tc.h"
+
+#include <cmath>
+
+namespace npub {
+namespace fpk {
+
+constexpr int kThreads = 384;
+constexpr int kBlk = 128;  // keys per block
+constexpr int kRows = 128;
+
+template <int HD>
+struct Smem {
+    static constexpr int kChunks = HD / 64;
+    static constexpr int kChunk = 128 * 128;           // 128 rows of one swizzled 128-byte row each
+    static constexpr int kTile = kChunks * kChunk;     // one K, V or Q tile
+    static constexpr int kStages = HD == 128 ? 5 : 8;  // ring of K and V tiles
+    static constexpr int kOffQ = 0;
+    static constexpr int kOffRing = 2 * kTile;
+    static constexpr int kOffBar = kOffRing + kStages * kTile;
+    static constexpr int kTotal = kOffBar + 256;
+    static_assert(kTotal <= 232448, "shared memory budget");
+};
+
+struct Params {
+    CUtensorMap tmQ, tmK, tmV;
+    const int32_t *cu, *lens, *table;
+    int64_t ldt;
+    int max_keys, page_shift, box_rows, n_pages;
+    int total_q, batch, heads, kv_heads, group, tpt, head_dim;
+    int tiles, n_items, splits, split_keys, first, split0, shared, causal;
+    float c;  // scale * log2(e)
+    __half* out;
+    int64_t ldo;
+    float* part_o;
+    float2* part_ml;
+    int* err;
+};
+
+struct Item {
+    int q_row0;      // first row of the sequence
+    int ntok, tok0;  // rows of the sequence, first row of tile 0
+    int kv_row0;     // packed K/V: first row of the sequence
+    int seq, kvh, split;
+    int off;         // row i sees keys <= off + i
+    int k0, kend;    // keys of this item
+    int n[2];        // key blocks of each tile
+};
+
+__device__ __forceinline__ void set_err(int* err, int code) {
+    if (err) atomicCAS(err, 0, code);
+}
+
+// Item -> rows and keys.  A whole warp: the tile's sequence is found by a scan
+// over the sequences' tile counts, 32 of them per step.  Reads cu and lens as
+// they are: whatever they hold, the rows stay inside [0, total_q) at the
+// stores and the keys inside the table, and the loop bounds are finite.
+template <bool PAGED>
+__device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
+    const int lane = threadIdx.x & 31;
+    it.split = idx % p.splits;
+    idx /= p.splits;
+    it.kvh = idx % p.kv_heads;
+    int tile = idx / p.kv_heads;
+    const int span = p.tiles * p.tpt;
+    if (PAGED && p.shared > 0) {
+        it.seq = 0;
+        it.q_row0 = 0;
+        it.ntok = p.total_q;
+        it.tok0 = tile * span;
+        it.kv_row0 = 0;
+        it.off = p.shared;  // no causal limit; each row has its own
+        it.k0 = it.split * p.split_keys;
+        it.kend = it.split == p.splits - 1 ? p.shared : min(p.shared, it.k0 + p.split_keys);
+        if (it.tok0 >= it.ntok) return false;
+        const int nb = it.kend > it.k0 ? (it.kend - it.k0 + kBlk - 1) / kBlk : 0;
+        it.n[0] = nb;
+        it.n[1] = (p.tiles == 2 && it.tok0 + p.tpt < it.ntok) ? nb : 0;
+        return true;
+    }
+    int b = -1, r0 = 0, r1 = 0;
+    for (int s0 = 0; s0 < p.batch; s0 += 32) {
+        int c0 = 0, c1 = 0;
+        if (s0 + lane < p.batch) {
+            c0 = p.cu ? max(0, min(p.total_q, __ldg(p.cu + s0 + lane))) : s0 + lane;
+            c1 = p.cu ? max(c0, min(p.total_q, __ldg(p.cu + s0 + lane + 1))) : c0 + 1;
+        }
+        const int cnt = (c1 - c0 + span - 1) / span;
+        int sum = cnt;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += v;
+        }
+        const uint32_t vote = __ballot_sync(0xffffffffu, sum > tile);
+        if (vote) {
+            const int l = __ffs(vote) - 1;
+            tile -= __shfl_sync(0xffffffffu, sum - cnt, l);
+            r0 = __shfl_sync(0xffffffffu, c0, l);
+            r1 = __shfl_sync(0xffffffffu, c1, l);
+            const int nt = __shfl_sync(0xffffffffu, cnt, l);
+            tile = nt - 1 - tile;  // longest causal rows first
+            b = s0 + l;
+            break;
+        }
+        tile -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (b < 0) return false;
+    it.seq = b;
+    it.q_row0 = r0;
+    it.kv_row0 = r0;
+    it.ntok = r1 - r0;
+    it.tok0 = tile * span;
+    const int klen = PAGED ? max(0, min(p.max_keys, __ldg(p.lens + b))) : it.ntok;
+    it.off = p.causal ? klen - it.ntok : klen;
+    it.k0 = p.first + it.split * p.split_keys;
+    it.kend = it.split == p.splits - 1 ? klen : min(klen, it.k0 + p.split_keys);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int t0 = it.tok0 + q * p.tpt, t1 = min(it.ntok, t0 + p.tpt);
+        const int lim = min(it.kend, p.causal ? it.off + t1 : klen);
+        it.n[q] = (q < p.tiles && t0 < it.ntok && lim > it.k0) ? (lim - it.k0 + kBlk - 1) / kBlk : 0;
+    }
+    return true;
+}
+
+// Keys that some row of tile q may see (a bound for its last block's steps).
+__device__ __forceinline__ int tile_limit(const Params& p, const Item& it, int q) {
+    const int t1 = min(it.ntok, it.tok0 + (q + 1) * p.tpt);
+    return (p.causal && p.shared == 0) ? min(it.kend, it.off + t1) : it.kend;
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+        "[%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort));
+}
+
+template <int HD, bool PAGED, bool PART>
+__global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_constant__ Params p) {
+    using L = Smem<HD>;
+    pdl_trigger();
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 1023u) {  // the swizzled tiles need 1024-byte alignment
+        if (threadIdx.x == 0) set_err(p.err, 0x500);
+        pdl_wait();
+        return;
+    }
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+    uint64_t* q_full = bars;       // 1
+    uint64_t* q_empty = bars + 1;  // 1
+    uint64_t* s_full = bars + 2;   // [2]
+    uint64_t* p_full = bars + 4;   // [2]
+    uint64_t* o_full = bars + 6;   // [2]
+    uint64_t* mma_done = bars + 8;
+    uint64_t* kv_full = bars + 9;  // [kStages]
+    uint64_t* kv_empty = kv_full + L::kStages;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + L::kStages);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_full[i], 1);
+        }
+        mbar_init(mma_done, 1);
+        for (int i = 0; i < L::kStages; ++i) {
+            mbar_init(&kv_full[i], 1);
+            mbar_init(&kv_empty[i], 1);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 8 && lane == 0) {
+        prefetch_tmap(&p.tmQ);
+        prefetch_tmap(&p.tmK);
+        prefetch_tmap(&p.tmV);
+    }
+    if (warp == 9) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    cta_sync_divergent();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    int never = 0;
+    volatile int* no_abort = &never;
+    pdl_wait();
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 8) {
+            // ------------------------------------------------------------ TMA producer
+            uint32_t n = 0, nz = 0;  // ring tiles and non-empty items so far
+            bool ok = true;
+            const int nbox = PAGED ? kBlk / p.box_rows : 1;
+            for (int idx = blockIdx.x; idx < p.n_items && ok; idx += gridDim.x) {
+                Item it;
+                if (!get_item<PAGED>(p, idx, it)) continue;
+                const int nblk = max(it.n[0], it.n[1]);
+                if (nblk == 0) continue;
+                ok = wait_all(q_empty, (nz & 1u) ^ 1u, abort_flag);
+                if (!ok) break;
+                const int nq = it.n[1] > 0 ? 2 : 1;
+                if (lane == 0) {
+                    const uint32_t bytes = (uint32_t)(p.group * p.tpt) * 128u * L::kChunks;
+                    mbar_arrive_expect_tx(q_full, bytes * nq);
+                    for (int q = 0; q < nq; ++q)
+                        for (int ch = 0; ch < L::kChunks; ++ch)
+                            tma_load_3d(smem + L::kOffQ + q * L::kTile + ch * L::kChunk, &p.tmQ, q_full, ch * 64,
+                                        it.kvh * p.group, it.q_row0 + it.tok0 + q * p.tpt);
+                }
+                ++nz;
+                for (int j = 0; j < nblk && ok; ++j) {
+                    int box = lane / L::kChunks, ch = lane % L::kChunks, c2 = 0, c3 = 0;
+                    const int key = it.k0 + j * kBlk;
+                    if (PAGED) {
+                        // lane -> (page piece, 64-column chunk); past the keys: a page outside the pool, which
+                        // the copy fills with zeros
+                        const int kk = key + box * p.box_rows;
+                        c3 = p.n_pages;
+                        if (box < nbox && kk < it.kend) {
+                            const int id = __ldg(p.table + (int64_t)it.seq * p.ldt + (kk >> p.page_shift));
+                            if (id >= 0 && id < p.n_pages) c3 = id;
+                        }
+                        c2 = kk & ((1 << p.page_shift) - 1);
+                    }
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv, ++n) {
+                        const uint32_t s = n % L::kStages, ph = (n / L::kStages) & 1u;
+                        ok = wait_all(&kv_empty[s], ph ^ 1u, abort_flag);
+                        if (!ok) break;
+                        uint8_t* dst = smem + L::kOffRing + s * L::kTile + ch * L::kChunk;
+                        if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], (uint32_t)L::kTile);
+                        __syncwarp();
+                        if (box < nbox) {
+                            if (PAGED)
+                                tma_load_4d(dst + box * p.box_rows * 128, kv ? &p.tmV : &p.tmK, &kv_full[s], ch * 64,
+                                            c2, it.kvh, c3);
+                            else
+                                tma_load_3d(dst, kv ? &p.tmV : &p.tmK, &kv_full[s], ch * 64, it.kvh,
+                                            it.kv_row0 + key);
+                        }
+                    }
+                }
+            }
+            if (!ok) {  // copies in flight land before the CTA leaves
+                if (lane == 0) {
+                    *abort_flag = 1;
+                    set_err(p.err, 0x501);
+                    if (nz) mbar_wait_bounded(q_full, (nz - 1) & 1u, no_abort, 200000000ull);
+                    for (uint32_t i = n > L::kStages ? n - L::kStages : 0; i < n; ++i)
+                        mbar_wait_bounded(&kv_full[i % L::kStages], (i / L::kStages) & 1u, no_abort, 200000000ull);
+                }
+            }
+        } else if (warp == 9) {
+            // ------------------------------------------------------------ MMA issuer
+            constexpr uint32_t idesc_s = umma_idesc_f16(kRows, kBlk);
+            constexpr uint32_t idesc_o = umma_idesc_f16_bmn(kRows, HD);
+            uint32_t base = 0, nz = 0, np[2] = {0, 0};
+            bool ok = true;
+            for (int idx = blockIdx.x; idx < p.n_items && ok; idx += gridDim.x) {
+                Item it;
+                if (!get_item<PAGED>(p, idx, it)) continue;
+                const int nblk = max(it.n[0], it.n[1]);
+                if (nblk == 0) continue;
+                ok = wait_all(q_full, nz & 1u, abort_flag);
+                ++nz;
+                for (int j = 0; ok && j <= nblk; ++j) {
+                    const uint32_t vn = base + 2 * j - 1, kn = base + 2 * j;
+                    const uint32_t vs = vn % L::kStages, ks = kn % L::kStages;
+                    const uint32_t va = smem_u32(smem + L::kOffRing + vs * L::kTile);
+                    const uint32_t ka = smem_u32(smem + L::kOffRing + ks * L::kTile);
+                    if (j >= 1) {
+                        ok = wait_all(&kv_full[vs], (vn / L::kStages) & 1u, abort_flag);
+                        if (!ok) break;
+                        const int vb = it.kend - (it.k0 + (j - 1) * kBlk);  // keys of this block
+                        if (vb < kBlk && (vb & 15)) {  // V rows behind the last key, up to the 16-key step's end
+                            const int n16 = (16 - (vb & 15)) * 8;
+                            for (int i = lane; i < n16 * L::kChunks; i += 32) {
+                                const int ch = i / n16, e = i - ch * n16;
+                                *reinterpret_cast<uint4*>(smem + L::kOffRing + vs * L::kTile + ch * L::kChunk +
+                                                          vb * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                        }
+                    }
+                    if (j < nblk) {
+                        ok = wait_all(&kv_full[ks], (kn / L::kStages) & 1u, abort_flag);
+                        if (!ok) break;
+                    }
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t sq = tmem + (uint32_t)(q * 128), oq = tmem + 256u + (uint32_t)(q * 128);
+                        if (j >= 1 && j - 1 < it.n[q]) {  // O_q += P_q(j-1) V_{j-1}
+                            ok = wait_all(&p_full[q], np[q] & 1u, abort_flag);
+                            if (!ok) break;
+                            ++np[q];
+                            tc_fence_after();
+                            if (lane == 0) {
+                                const int left = tile_limit(p, it, q) - (it.k0 + (j - 1) * kBlk);
+                                const int steps = min(kBlk / 16, (left + 15) >> 4);
+                                for (int kk = 0; kk < steps; ++kk)
+                                    tc_mma_f16_ts(oq, sq + (uint32_t)kk * 8u,
+                                                  umma_desc_sw128_mn(va + (uint32_t)kk * 2048u, (uint32_t)L::kChunk,
+                                                                     1024u),
+                                                  idesc_o, (j > 1 || kk > 0) ? 1u : 0u);
+                                if (j == it.n[q]) tc_commit(&o_full[q]);
+                            }
+                            __syncwarp();
+                        }
+                        if (j < it.n[q]) {  // S_q(j) = Q_q K_j^T
+                            tc_fence_after();
+                            if (lane == 0) {
+                                const uint32_t qa = smem_u32(smem + L::kOffQ + q * L::kTile);
+#pragma unroll
+                                for (int kk = 0; kk < HD / 16; ++kk) {
+                                    const uint32_t o = (uint32_t)((kk >> 2) * L::kChunk + (kk & 3) * 32);
+                                    tc_mma_f16(sq, umma_desc_sw128(qa + o), umma_desc_sw128(ka + o), idesc_s,
+                                               kk > 0 ? 1u : 0u);
+                                }
+                                tc_commit(&s_full[q]);
+                            }
+                            __syncwarp();
+                        }
+                    }
+                    if (!ok) break;
+                    if (lane == 0) {
+                        if (j >= 1) tc_commit(&kv_empty[vs]);
+                        if (j < nblk) tc_commit(&kv_empty[ks]);
+                        if (j == nblk - 1) tc_commit(q_empty);
+                    }
+                    __syncwarp();
+                }
+                base += 2 * nblk;
+            }
+            if (lane == 0) {
+                if (!ok) {
+                    *abort_flag = 1;
+                    set_err(p.err, 0x502);
+                }
+                tc_commit(mma_done);  // every MMA issued above completes before TMEM is freed
+                if (!mbar_wait_bounded(mma_done, 0, no_abort, 200000000ull)) set_err(p.err, 0x503);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ---------------------------------------------------------------- softmax / output
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int q = warp >> 2;
+        const int r = threadIdx.x & 127;  // row of the tile == TMEM lane
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t sq = tmem + lanes + (uint32_t)(q * 128), oq = tmem + lanes + 256u + (uint32_t)(q * 128);
+        const int tl = r / p.group, g = r - tl * p.group;
+        const float c = p.c;
+        uint32_t ns = 0, no = 0;
+        bool ok = true;
+        for (int idx = blockIdx.x; idx < p.n_items && ok; idx += gridDim.x) {
+            Item it;
+            if (!get_item<PAGED>(p, idx, it)) continue;
+            const int tok = it.tok0 + q * p.tpt + tl;
+            const bool valid = q < p.tiles && tl < p.tpt && tok < it.ntok;
+            int lim = it.kend;  // this row's keys end here
+            if (valid) {
+                if (PAGED && p.shared > 0) lim = min(lim, __ldg(p.lens + tok));
+                else if (p.causal) lim = min(lim, it.off + tok + 1);
+            }
+            float m = -INFINITY, l = 0.0f;
+            const int nb = it.n[q];
+            for (int j = 0; j < nb; ++j) {
+                ok = wait_all(&s_full[q], ns & 1u, abort_flag);
+                if (!ok) break;
+                ++ns;
+                tc_fence_after();
+                float x[128];
+                {
+                    uint32_t a[64], b[64];
+                    tmem_ld64(sq, a);
+                    tmem_ld64(sq + 64, b);
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) {
+                        x[e] = __uint_as_float(a[e]);
+                        x[64 + e] = __uint_as_float(b[e]);
+                    }
+                }
+                const int left = lim - (it.k0 + j * kBlk);
+                if (__any_sync(0xffffffffu, left < kBlk)) {
+#pragma unroll
+                    for (int e = 0; e < 128; ++e) x[e] = e < left ? x[e] : -INFINITY;
+                }
+                float m4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int e = 4; e < 128; ++e) m4[e & 3] = fmaxf(m4[e & 3], x[e]);
+                const float mx = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                if (j == 0) {
+                    m = mx;
+                } else {
+                    const bool need = (mx - m) * c > 8.0f;
+                    if (__any_sync(0xffffffffu, need)) {  // P_q(j-1) V_{j-1} is complete: S_q(j) was issued behind it
+                        const float corr = need ? ex2_approx((m - mx) * c) : 1.0f;
+                        if (need) m = mx;
+                        l *= corr;
+#pragma unroll 1
+                        for (int e0 = 0; e0 < HD; e0 += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(oq + (uint32_t)e0, o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                            tmem_st32(oq + (uint32_t)e0, o);
+                        }
+                    }
+                }
+                const float mc = m == -INFINITY ? 0.0f : m * c;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float p0 = ex2_approx(fmaf(x[h * 64 + 2 * e], c, -mc));
+                        const float p1 = ex2_approx(fmaf(x[h * 64 + 2 * e + 1], c, -mc));
+                        sum[e & 3] += p0 + p1;
+                        __half2 hh = __floats2half2_rn(p0, p1);
+                        pk[e] = *reinterpret_cast<uint32_t*>(&hh);
+                    }
+                    tmem_st32(sq + (uint32_t)(h * 32), pk);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[q]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            if (!ok) break;
+            if (nb > 0) {
+                ok = wait_all(&o_full[q], no & 1u, abort_flag);
+                if (!ok) break;
+                ++no;
+                tc_fence_after();
+            }
+            const int64_t row = (int64_t)it.q_row0 + tok;
+            const int head = it.kvh * p.group + g;
+            if (PART) {
+                const int64_t at = ((int64_t)(p.split0 + it.split) * p.total_q + row) * p.heads + head;
+                if (valid) p.part_ml[at] = make_float2(m == -INFINITY ? -INFINITY : m * c, l);
+                if (nb > 0) {
+#pragma unroll 1
+                    for (int e0 = 0; e0 < p.head_dim; e0 += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(oq + (uint32_t)e0, o);
+                        if (!valid || !(l != 0.0f)) continue;
+                        float* dst = p.part_o + at * p.head_dim + e0;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            if (e0 + e < p.head_dim)
+                                *reinterpret_cast<uint4*>(dst + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                }
+            } else {
+                const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+                __half* dst = p.out + row * p.ldo + (int64_t)head * p.head_dim;
+#pragma unroll 1
+                for (int e0 = 0; e0 < p.head_dim; e0 += 32) {
+                    uint32_t o[32];
+                    if (nb > 0) tmem_ld32(oq + (uint32_t)e0, o);
+                    if (!valid) continue;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        if (e0 + e >= p.head_dim) break;
+                        uint32_t pk[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            __half2 hh = __floats2half2_rn(__uint_as_float(o[e + 2 * i]) * inv,
+                                                           __uint_as_float(o[e + 2 * i + 1]) * inv);
+                            pk[i] = l != 0.0f ? *reinterpret_cast<uint32_t*>(&hh) : 0u;
+                        }
+                        *reinterpret_cast<uint4*>(dst + e0 + e) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                    }
+                }
+            }
+            tc_fence_before();  // the O reads above, before the next item's first P lets its product overwrite them
+        }
+        if (!ok) {
+            *abort_flag = 1;
+            set_err(p.err, 0x504);
+        }
+    }
+
+    tc_fence_before();
+    cta_sync_divergent();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int HD, bool PAGED, bool PART>
+int launch(const Params& p, int grid, cudaStream_t st) {
+    auto kern = fmha_packed_kernel<HD, PAGED, PART>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::kTotal);
+    if (e != cudaSuccess) {
+        npub_internal_set_cuda_error(e);
+        return NPUB_ERR_CUDA;
+    }
+    return launch_pdl(kern, dim3(grid), dim3(kThreads), Smem<HD>::kTotal, st, p);
+}
+
+}  // namespace fpk
+
+int64_t fmha_packed_items(int total_q, int batch, int heads, int kv_heads, int max_new, int tiles) {
+    const int64_t span = (int64_t)tiles * (128 / (heads / kv_heads));
+    int64_t n = total_q / span + batch;  // sum of ceil(rows / span) over the sequences is at most this
+    if (n > total_q) n = total_q;
+    if (max_new > 0 && n > batch * ((max_new + span - 1) / span)) n = batch * ((max_new + span - 1) / span);
+    return n;
+}
+
+int fmha_packed(const PackedArgs& a, cudaStream_t st) {
+    using namespace fpk;
+    const int group = a.heads / a.kv_heads;
+    const bool paged = a.kv.table != nullptr;
+    Params p;
+    memset(&p, 0, sizeof(p));
+    p.group = group;
+    p.tpt = kRows / group;
+    int rc = make_tmap_3d(&p.tmQ, false, a.q, (uint64_t)a.head_dim, (uint64_t)a.heads, (uint64_t)a.total_q,
+                          (uint64_t)a.head_dim, (uint64_t)a.ldq, (uint32_t)group, (uint32_t)p.tpt, true);
+    if (rc) return rc;
+    if (paged) {
+        p.box_rows = a.kv.page_size < kBlk ? a.kv.page_size : kBlk;
+        rc = make_tmap_pages(&p.tmK, a.kv.k, a.kv.n_pages, a.kv_heads, a.kv.page_size, a.head_dim, p.box_rows);
+        if (rc) return rc;
+        rc = make_tmap_pages(&p.tmV, a.kv.v, a.kv.n_pages, a.kv_heads, a.kv.page_size, a.head_dim, p.box_rows);
+        if (rc) return rc;
+        while ((1 << p.page_shift) < a.kv.page_size) ++p.page_shift;
+        const int64_t mk = (int64_t)a.kv.max_pages << p.page_shift;
+        p.max_keys = mk > 0x7fffff00 ? 0x7fffff00 : (int)mk;
+        p.n_pages = a.kv.n_pages;
+        p.table = a.kv.table;
+        p.ldt = a.kv.ldt;
+        p.lens = a.lens;
+    } else {
+        rc = make_tmap_3d(&p.tmK, false, a.kv.k, (uint64_t)a.head_dim, (uint64_t)a.kv_heads, (uint64_t)a.total_q,
+                          (uint64_t)a.head_dim, (uint64_t)a.kv.ldk, 1, kBlk, true);
+        if (rc) return rc;
+        rc = make_tmap_3d(&p.tmV, false, a.kv.v, (uint64_t)a.head_dim, (uint64_t)a.kv_heads, (uint64_t)a.total_q,
+                          (uint64_t)a.head_dim, (uint64_t)a.kv.ldv, 1, kBlk, true);
+        if (rc) return rc;
+    }
+    p.cu = a.cu;
+    p.total_q = a.total_q;
+    p.batch = a.batch;
+    p.heads = a.heads;
+    p.kv_heads = a.kv_heads;
+    p.head_dim = a.head_dim;
+    p.shared = a.shared;
+    p.causal = a.causal ? 1 : 0;
+    p.c = a.scale * 1.4426950408889634f;
+    p.out = reinterpret_cast<__half*>(a.out);
+    p.ldo = a.ldo;
+    p.part_o = a.part_o;
+    p.part_ml = a.part_ml;
+    p.err = npub_internal_device_error_word();
+    const bool part = a.part_o != nullptr;
+    p.splits = part ? a.splits : 1;
+    p.split_keys = a.split_keys;
+    p.first = a.first;
+    p.split0 = a.split0;
+    // One tile per CTA while that still leaves SMs free.
+    const int batch = a.shared > 0 ? 1 : a.batch;
+    const int64_t one = fmha_packed_items(a.total_q, batch, a.heads, a.kv_heads, a.max_new, 1);
+    p.tiles = one * a.kv_heads * p.splits <= num_sms() ? 1 : 2;
+    const int64_t items = fmha_packed_items(a.total_q, batch, a.heads, a.kv_heads, a.max_new, p.tiles) * a.kv_heads *
+                          p.splits;
+    if (items > 0x7fffffff) return NPUB_ERR_UNSUPPORTED;
+    p.n_items = (int)items;
+    const int grid = p.n_items;
+    const bool small = a.head_dim <= 64;
+    if (part) {
+        if (!paged) return NPUB_ERR_UNSUPPORTED;
+        return small ? launch<64, true, true>(p, grid, st) : launch<128, true, true>(p, grid, st);
+    }
+    if (paged) return small ? launch<64, true, false>(p, grid, st) : launch<128, true, false>(p, grid, st);
+    return small ? launch<64, false, false>(p, grid, st) : launch<128, false, false>(p, grid, st);
+}
+
+}  // namespace npub

@@ -21,6 +21,7 @@
 //   warps 4..7  int8 -> fp16 converters during the main loop, then the
 //               epilogue (warp 4+i reads TMEM lanes 32i..32i+31)
 #include "common.cuh"
+#include "fmha_packed.h"
 #include "gemm_tc.h"
 #include "gemm_w8a16_pair.h"
 #include "gemm_w8a16_skinny.h"
@@ -383,6 +384,22 @@ int make_tmap_3d(CUtensorMap* m, bool int8, const void* base, uint64_t d0, uint6
                      const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                      swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? NPUB_OK : NPUB_ERR_INVALID_ARG;
+}
+
+// 4-D map of a page pool [n_pages, kv_heads, page_size, head_dim] (fmha_packed.h).
+int make_tmap_pages(CUtensorMap* m, const void* base, int n_pages, int kv_heads, int page_size, int head_dim,
+                    int box_rows) {
+    auto enc = encode_fn();
+    if (!enc) return NPUB_ERR_CUDA;
+    cuuint64_t gdim[4] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)kv_heads, (cuuint64_t)n_pages};
+    const cuuint64_t s1 = (cuuint64_t)head_dim * 2;
+    cuuint64_t gstride[3] = {s1, s1 * page_size, s1 * page_size * kv_heads};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), gdim, gstride, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? NPUB_OK : NPUB_ERR_INVALID_ARG;
 }
 

@@ -1,0 +1,258 @@
+// C entries of the packed and paged attention: argument checks, the choice of
+// kernel (fmha_packed.cu: tcgen05 tiles of 128 rows; paged_decode.cu: up to 16
+// rows per kv head) and the split of the keys over CTAs.
+#include "common.cuh"
+#include "fmha_packed.h"
+#include "gemm_tc.h"
+#include "paged_decode.h"
+
+#include <cmath>
+
+namespace npub {
+namespace {
+
+bool dims_ok(int heads, int kv_heads, int head_dim, float scale) {
+    return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && head_dim > 0 && head_dim % 16 == 0 && scale > 0.0f &&
+           std::isfinite(scale);
+}
+
+// What the tile kernels implement beyond dims_ok: heads that fit two 64-column
+// chunks, groups that fit a tile, and at most 65535 heads.
+bool dims_supported(int heads, int kv_heads, int head_dim) {
+    return head_dim <= 128 && heads / kv_heads <= 128 && heads <= 65535;
+}
+
+bool pool_ok(const void* k, const void* v, int n_pages, int page_size, const int32_t* table, int64_t ldt,
+             int max_pages) {
+    return k && v && table && n_pages > 0 && page_size >= 16 && page_size <= 256 &&
+           (page_size & (page_size - 1)) == 0 && max_pages > 0 && ldt >= max_pages && npub_aligned(k, 16) &&
+           npub_aligned(v, 16);
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How the keys of a call are cut.  The partials are numbered through: the shared prefix's splits, then those of the
+// sequences' own keys.  The last split of either takes every key that is left, so ctx_len only decides the cut.
+struct Plan {
+    bool few;                     // own keys on paged_decode (else on the tiles)
+    int shared;                   // keys of the shared prefix phase (0: none)
+    int pre_splits, pre_keys;     // its splits and keys per split
+    int own_splits, own_keys;
+    bool part() const { return pre_splits + own_splits > 1; }
+    int total() const { return pre_splits + own_splits; }
+};
+
+// Cuts `keys` keys of `items` independent work items so that about `want` CTAs run, in ranges of at least `least`
+// keys and whole multiples of `unit`.
+void cut(int64_t keys, int64_t items, int64_t want, int64_t least, int64_t unit, int* splits, int* per) {
+    int64_t s = items > 0 ? ceil_div(want, items) : 1;
+    const int64_t most = ceil_div(keys, least);
+    if (s > most) s = most;
+    if (s < 1) s = 1;
+    int64_t k = ceil_div(ceil_div(keys, s), unit) * unit;
+    if (k < unit) k = unit;
+    if (k > 0x40000000) k = 0x40000000;
+    *per = (int)k;
+    *splits = (int)ceil_div(keys > 0 ? keys : 1, k);
+}
+
+Plan make_plan(int batch, int total, int max_new, int64_t ctx, int shared, int heads, int kv_heads) {
+    Plan pl = {};
+    const int group = heads / kv_heads, sms = num_sms();
+    pl.few = max_new > 0 && (int64_t)max_new * group <= kPagedDecodeRows && batch <= 65535;
+    if (batch < 2) shared = 0;  // nothing to share
+    pl.shared = shared;
+    if (shared > 0) {
+        const int64_t tiles = fmha_packed_items(total, 1, heads, kv_heads, 0, 2) * kv_heads;
+        cut(shared, tiles, sms, 256, 128, &pl.pre_splits, &pl.pre_keys);
+    }
+    const int64_t own = ctx > shared ? ctx - shared : 1;
+    if (pl.few) {
+        cut(own, (int64_t)batch * kv_heads, 4 * 2 * sms, 256, 64, &pl.own_splits, &pl.own_keys);
+    } else {
+        const int64_t tiles = fmha_packed_items(total, batch, heads, kv_heads, max_new, 2) * kv_heads;
+        if (tiles >= sms) {
+            pl.own_splits = 1;
+            pl.own_keys = 128;  // the last split takes every key that is left
+        } else {
+            cut(own, tiles, sms, 512, 128, &pl.own_splits, &pl.own_keys);
+        }
+    }
+    return pl;
+}
+
+size_t plan_bytes(const Plan& pl, int total, int heads, int head_dim) {
+    if (!pl.part()) return 0;
+    const size_t n = (size_t)pl.total() * total * heads;
+    return (n * sizeof(float2) + 255) / 256 * 256 + n * head_dim * sizeof(float);
+}
+
+int run_plan(const Plan& pl, PackedArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+    const size_t need = plan_bytes(pl, a.total_q, a.heads, a.head_dim);
+    if (need) {
+        if (!workspace || workspace_bytes < need) return NPUB_ERR_WORKSPACE;
+        NPUB_CHECK_ARG(npub_aligned(workspace, 256));
+        const size_t n = (size_t)pl.total() * a.total_q * a.heads;
+        a.part_ml = reinterpret_cast<float2*>(workspace);
+        a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (n * sizeof(float2) + 255) / 256 * 256);
+    }
+    if (pl.shared > 0) {
+        PackedArgs s = a;
+        s.shared = pl.shared;
+        s.causal = 0;
+        s.cu = nullptr;
+        s.max_new = 0;
+        s.splits = pl.pre_splits;
+        s.split_keys = pl.pre_keys;
+        const int rc = fmha_packed(s, st);
+        if (rc) return rc;
+    }
+    int rc;
+    if (pl.few) {
+        rc = paged_decode(a, pl.shared, pl.own_keys, pl.own_splits, pl.pre_splits, st);
+    } else {
+        a.first = pl.shared;
+        a.splits = pl.own_splits;
+        a.split0 = pl.pre_splits;
+        a.split_keys = pl.own_keys;
+        rc = fmha_packed(a, st);
+    }
+    if (rc || !need) return rc;
+    return paged_combine(a, pl.total(), st);
+}
+
+}  // namespace
+}  // namespace npub
+
+extern "C" int npub_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                                     int64_t ldv, void* out, int64_t ldo, const int32_t* cu_seqlens, int batch,
+                                     int total, int max_len, int heads, int kv_heads, int head_dim, float scale,
+                                     int causal, void* stream) {
+    using namespace npub;
+    NPUB_CHECK_ARG(batch >= 0 && total >= 0 && max_len >= 0 && dims_ok(heads, kv_heads, head_dim, scale));
+    if (batch == 0 || total == 0) return NPUB_OK;
+    NPUB_CHECK_ARG(q && k && v && out && cu_seqlens);
+    if (!dims_supported(heads, kv_heads, head_dim)) return NPUB_ERR_UNSUPPORTED;
+    NPUB_CHECK_ARG(ldq % 8 == 0 && ldk % 8 == 0 && ldv % 8 == 0 && ldo % 8 == 0);
+    NPUB_CHECK_ARG(ldq >= (int64_t)heads * head_dim && ldk >= (int64_t)kv_heads * head_dim &&
+                   ldv >= (int64_t)kv_heads * head_dim && ldo >= (int64_t)heads * head_dim);
+    NPUB_CHECK_ARG(npub_aligned(q, 16) && npub_aligned(k, 16) && npub_aligned(v, 16) && npub_aligned(out, 16));
+    PackedArgs a = {};
+    a.q = q;
+    a.ldq = ldq;
+    a.out = out;
+    a.ldo = ldo;
+    a.kv.k = k;
+    a.kv.v = v;
+    a.kv.ldk = ldk;
+    a.kv.ldv = ldv;
+    a.cu = cu_seqlens;
+    a.total_q = total;
+    a.batch = batch;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.max_new = max_len;
+    a.scale = scale;
+    a.causal = causal;
+    return fmha_packed(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int npub_attention_paged(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int n_pages,
+                                    int page_size, const int32_t* page_table, int64_t ldt, int max_pages,
+                                    const int32_t* lens, const int32_t* cu_seqlens, int batch, int total, int max_new,
+                                    int ctx_len, void* out, int64_t ldo, int heads, int kv_heads, int head_dim,
+                                    float scale, int causal, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace npub;
+    NPUB_CHECK_ARG(batch >= 0 && total >= 0 && max_new >= 0 && ctx_len >= 0 &&
+                   dims_ok(heads, kv_heads, head_dim, scale));
+    if (batch == 0 || total == 0) return NPUB_OK;
+    NPUB_CHECK_ARG(q && out && lens && cu_seqlens &&
+                   pool_ok(k_pages, v_pages, n_pages, page_size, page_table, ldt, max_pages));
+    if (!dims_supported(heads, kv_heads, head_dim)) return NPUB_ERR_UNSUPPORTED;
+    NPUB_CHECK_ARG(ldq % 8 == 0 && ldo % 8 == 0 && ldq >= (int64_t)heads * head_dim &&
+                   ldo >= (int64_t)heads * head_dim && npub_aligned(q, 16) && npub_aligned(out, 16));
+    PackedArgs a = {};
+    a.q = q;
+    a.ldq = ldq;
+    a.out = out;
+    a.ldo = ldo;
+    a.kv.k = k_pages;
+    a.kv.v = v_pages;
+    a.kv.table = page_table;
+    a.kv.ldt = ldt;
+    a.kv.max_pages = max_pages;
+    a.kv.n_pages = n_pages;
+    a.kv.page_size = page_size;
+    a.cu = cu_seqlens;
+    a.lens = lens;
+    a.total_q = total;
+    a.batch = batch;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.max_new = max_new;
+    a.scale = scale;
+    a.causal = causal;
+    const int64_t cap = (int64_t)max_pages * page_size;
+    const Plan pl = make_plan(batch, total, max_new, ctx_len > 0 && ctx_len < cap ? ctx_len : cap, 0, heads, kv_heads);
+    return run_plan(pl, a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t npub_attention_paged_workspace(int batch, int total, int max_new, int64_t ctx_len, int heads,
+                                                 int kv_heads, int head_dim) {
+    using namespace npub;
+    if (batch <= 0 || total <= 0 || max_new < 0 || ctx_len < 0 || !dims_ok(heads, kv_heads, head_dim, 1.0f) ||
+        !dims_supported(heads, kv_heads, head_dim))
+        return 0;
+    return plan_bytes(make_plan(batch, total, max_new, ctx_len, 0, heads, kv_heads), total, heads, head_dim);
+}
+
+extern "C" int npub_attention_paged_decode(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
+                                           int n_pages, int page_size, const int32_t* page_table, int64_t ldt,
+                                           int max_pages, const int32_t* lens, int batch, int ctx_len, int shared_len,
+                                           void* out, int64_t ldo, int heads, int kv_heads, int head_dim, float scale,
+                                           void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace npub;
+    NPUB_CHECK_ARG(batch >= 0 && ctx_len >= 0 && shared_len >= 0 && dims_ok(heads, kv_heads, head_dim, scale));
+    if (batch == 0) return NPUB_OK;
+    NPUB_CHECK_ARG(q && out && lens && pool_ok(k_pages, v_pages, n_pages, page_size, page_table, ldt, max_pages));
+    NPUB_CHECK_ARG(shared_len % page_size == 0 && shared_len <= (int64_t)max_pages * page_size);
+    if (!dims_supported(heads, kv_heads, head_dim) || batch > 65535) return NPUB_ERR_UNSUPPORTED;
+    NPUB_CHECK_ARG(ldq % 8 == 0 && ldo % 8 == 0 && ldq >= (int64_t)heads * head_dim &&
+                   ldo >= (int64_t)heads * head_dim && npub_aligned(q, 16) && npub_aligned(out, 16));
+    PackedArgs a = {};
+    a.q = q;
+    a.ldq = ldq;
+    a.out = out;
+    a.ldo = ldo;
+    a.kv.k = k_pages;
+    a.kv.v = v_pages;
+    a.kv.table = page_table;
+    a.kv.ldt = ldt;
+    a.kv.max_pages = max_pages;
+    a.kv.n_pages = n_pages;
+    a.kv.page_size = page_size;
+    a.lens = lens;
+    a.total_q = batch;
+    a.batch = batch;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.max_new = 1;
+    a.scale = scale;
+    a.causal = 1;
+    const int64_t cap = (int64_t)max_pages * page_size;
+    const Plan pl = make_plan(batch, batch, 1, ctx_len > 0 && ctx_len < cap ? ctx_len : cap, shared_len, heads,
+                              kv_heads);
+    return run_plan(pl, a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t npub_attention_paged_decode_workspace(int batch, int64_t ctx_len, int shared_len, int heads,
+                                                        int kv_heads, int head_dim) {
+    using namespace npub;
+    if (batch <= 0 || ctx_len < 0 || shared_len < 0 || !dims_ok(heads, kv_heads, head_dim, 1.0f) ||
+        !dims_supported(heads, kv_heads, head_dim))
+        return 0;
+    return plan_bytes(make_plan(batch, batch, 1, ctx_len, shared_len, heads, kv_heads), batch, heads, head_dim);
+}

@@ -27,6 +27,7 @@ __all__ = [
     "fp16", "quantize_w8", "matmul", "rmsnorm", "add", "swiglu", "softmax", "rope", "attention",
     "attention_decode", "kv_append", "rope_kv_append", "rope_kv_store", "matmul_swiglu", "interleave_gate_up",
     "matmul_rms", "rmsnorm_parts",
+    "rope_paged_append", "attention_packed", "attention_paged", "attention_paged_decode",
     "embed", "argmax", "isa_vector", "f32_to_f16_bits", "f16_bits_to_f32", "device_error", "NpubError",
 ]
 
@@ -552,6 +553,181 @@ def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v
         pos_ptr = pos.data_ptr()
     _lib.call("npub_kv_append", k_new.data_ptr(), ldk, v_new.data_ptr(), ldv, k_cache.data_ptr(), v_cache.data_ptr(),
               cap, pos_ptr, int(pos0), B, KVH, hd, _stream())
+
+
+# ------------------------------------------------------------ paged KV cache
+#
+# A paged cache is a pool k_pages / v_pages [n_pages, kv_heads, page_size,
+# head_dim] and a table page_table [batch, max_pages] of page ids: key p of
+# sequence b is slot p % page_size of page page_table[b, p // page_size].
+# Packed rows are the sequences' new rows one after the other, sequence b at
+# rows cu_seqlens[b] .. cu_seqlens[b + 1]; rows outside
+# cu_seqlens[0] .. cu_seqlens[-1] are neither computed nor written.
+
+def _on(*tensors):
+    """A context in which the tensors' one device is the current device (its
+    current stream is the one the op runs on)."""
+    devs = {t.device for t in tensors if t is not None}
+    _need(len(devs) == 1, f"all tensors must be on one device, got {sorted(map(str, devs))}")
+    return torch.cuda.device(devs.pop())
+
+
+def _ints(t: torch.Tensor, name: str, n: int) -> int:
+    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int32 and t.dim() == 1 and t.numel() == n
+          and t.is_contiguous(), f"{name} must be contiguous int32 CUDA [{n}]")
+    return t.data_ptr()
+
+
+def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor):
+    """Validate a paged cache; returns (n_pages, kv_heads, page_size, head_dim, batch, max_pages, ldt)."""
+    for t, nm in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float16 and t.dim() == 4
+              and t.is_contiguous(), f"{nm} must be contiguous fp16 CUDA [n_pages, kv_heads, page_size, head_dim]")
+    _need(k_pages.shape == v_pages.shape, "k_pages and v_pages must have the same shape")
+    ldt = _mat(page_table, "page_table", torch.int32)
+    return (*k_pages.shape, *page_table.shape, ldt)
+
+
+def rope_paged_append(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: int, positions: torch.Tensor,
+                      inv_freq: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                      page_table: torch.Tensor, *, cu_seqlens: Optional[torch.Tensor] = None,
+                      rot_dim: Optional[int] = None, interleaved: bool = False,
+                      q_gamma: Optional[torch.Tensor] = None, k_gamma: Optional[torch.Tensor] = None,
+                      eps: float = 1e-5, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The step between the QKV projection and the attention over a paged cache,
+    in one kernel: an RMSNorm of every q / k head (with q_gamma / k_gamma), RoPE
+    (llama_layer.py:96-112) of the q and k heads of the fused rows qkv
+    [tokens, (q_heads + 2 kv_heads) * head_dim], k and v written to the pages at
+    positions[t].  Returns q [tokens, q_heads * head_dim] (out; may be the q
+    columns of qkv).
+
+    cu_seqlens (int32 [batch + 1]): packed prompts; None: row t is sequence t's.
+    inv_freq (fp32 [rot_dim / 2], from rope_freqs): the rotation's rates;
+    rot_dim < head_dim rotates the first rot_dim columns only; interleaved
+    pairs columns (2i, 2i + 1) instead of (i, i + rot_dim / 2).  A position
+    outside the table, or a page id outside the pool, is rotated but not stored."""
+    ldx = _mat(qkv, "qkv", torch.float16)
+    T = qkv.shape[0]
+    R = head_dim if rot_dim is None else int(rot_dim)
+    _need(qkv.shape[1] >= (q_heads + 2 * kv_heads) * head_dim, "qkv has too few columns")
+    n_pages, kvh, ps, hd, B, W, ldt = _pool(k_pages, v_pages, page_table)
+    _need(kvh == kv_heads and hd == head_dim, "the pages' kv_heads and head_dim must match")
+    pos = _ints(positions, "positions", T)
+    _need(inv_freq.is_cuda and inv_freq.dtype == torch.float32 and inv_freq.is_contiguous()
+          and inv_freq.numel() * 2 == R, "inv_freq must be contiguous fp32 CUDA [rot_dim/2]")
+    for g, nm in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+        _need(g is None or (g.is_cuda and g.dtype == torch.float16 and g.numel() == head_dim and g.is_contiguous()),
+              f"{nm} must be a contiguous fp16 CUDA tensor of head_dim elements")
+    _need(cu_seqlens is not None or B == T, "without cu_seqlens the table needs one row per token")
+    cu = None if cu_seqlens is None else _ints(cu_seqlens, "cu_seqlens", B + 1)
+    with _on(qkv, positions, inv_freq, k_pages, v_pages, page_table, cu_seqlens, q_gamma, k_gamma, out):
+        if out is None:
+            out = torch.empty((T, q_heads * head_dim), dtype=torch.float16, device=qkv.device)
+        ldq = _mat(out, "out", torch.float16)
+        _need(tuple(out.shape) == (T, q_heads * head_dim), "out must be [tokens, q_heads * head_dim]")
+        _lib.call("npub_rope_paged_append", qkv.data_ptr(), ldx, out.data_ptr(), ldq, T, q_heads, kv_heads, head_dim,
+                  R, 1 if interleaved else 0, pos, inv_freq.data_ptr(), _ptr(q_gamma), _ptr(k_gamma), float(eps),
+                  k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps, page_table.data_ptr(), ldt, W, cu, B,
+                  _stream())
+    return out
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, heads: int,
+                     kv_heads: Optional[int] = None, *, head_dim: Optional[int] = None, max_len: int = 0,
+                     causal: bool = True, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """attention() (llama_layer.py:114-137) over packed prompts of different
+    lengths: q [total, heads*hd], k/v [total, kv_heads*hd], sequence b at rows
+    cu_seqlens[b] .. cu_seqlens[b + 1] (int32 [batch + 1]).  head_dim a multiple
+    of 16 up to 128.  max_len: at least the longest sequence's rows (0: not known)."""
+    kv_heads = kv_heads or heads
+    ldq = _mat(q, "q", torch.float16)
+    ldk = _mat(k, "k", torch.float16)
+    ldv = _mat(v, "v", torch.float16)
+    hd = head_dim or q.shape[1] // heads
+    T = q.shape[0]
+    _need(k.shape[0] == T and v.shape[0] == T, "q, k and v must have the same number of rows")
+    _need(q.shape[1] >= heads * hd and k.shape[1] >= kv_heads * hd and v.shape[1] >= kv_heads * hd,
+          "q, k or v is narrower than its heads")
+    _need(isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.numel() >= 1, "cu_seqlens must hold batch + 1 offsets")
+    B = cu_seqlens.numel() - 1
+    cu = _ints(cu_seqlens, "cu_seqlens", B + 1)
+    if scale is None:
+        scale = 1.0 / math.sqrt(hd)
+    with _on(q, k, v, cu_seqlens, out):
+        if out is None:
+            out = torch.empty((T, heads * hd), dtype=torch.float16, device=q.device)
+        ldo = _mat(out, "out", torch.float16)
+        _need(tuple(out.shape) == (T, heads * hd), "out must be [total, heads * head_dim]")
+        _lib.call("npub_attention_packed", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(),
+                  ldo, cu, B, T, int(max_len), heads, kv_heads, hd, float(scale), 1 if causal else 0, _stream())
+    return out
+
+
+def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    lens: torch.Tensor, cu_seqlens: torch.Tensor, *, heads: int, max_new: int = 0, ctx_len: int = 0,
+                    causal: bool = True, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of packed new rows q [total, heads*hd] over a paged cache that
+    holds them already: sequence b's keys are positions 0 .. lens[b] - 1 (int32
+    [batch]) and its new rows (cu_seqlens) the last of them.  Prompt chunks,
+    prompts behind a cached prefix, drafted tokens.
+
+    max_new: at least the new rows of any sequence (0: not known; when
+    max_new * heads / kv_heads <= 16 the kernel for few rows runs); ctx_len: the
+    largest lens expected (0: the table's width), which only decides how keys
+    are split over CTAs.  page_size 16 .. 256."""
+    ldq = _mat(q, "q", torch.float16)
+    T = q.shape[0]
+    n_pages, kv_heads, ps, hd, B, W, ldt = _pool(k_pages, v_pages, page_table)
+    _need(q.shape[1] == heads * hd, "q must be [total, heads * head_dim]")
+    ln = _ints(lens, "lens", B)
+    cu = _ints(cu_seqlens, "cu_seqlens", B + 1)
+    if scale is None:
+        scale = 1.0 / math.sqrt(hd)
+    ctx = min(int(ctx_len), W * ps) if ctx_len > 0 else W * ps
+    with _on(q, k_pages, v_pages, page_table, lens, cu_seqlens, out):
+        if out is None:
+            out = torch.empty((T, heads * hd), dtype=torch.float16, device=q.device)
+        ldo = _mat(out, "out", torch.float16)
+        _need(tuple(out.shape) == (T, heads * hd), "out must be [total, heads * head_dim]")
+        ws, wsb = _workspace(_lib.query("npub_attention_paged_workspace", B, T, int(max_new), ctx, heads, kv_heads,
+                                        hd), q.device)
+        _lib.call("npub_attention_paged", q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
+                  page_table.data_ptr(), ldt, W, ln, cu, B, T, int(max_new), ctx, out.data_ptr(), ldo, heads,
+                  kv_heads, hd, float(scale), 1 if causal else 0, _ptr(ws), wsb, _stream())
+    return out
+
+
+def attention_paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                           lens: torch.Tensor, *, heads: int, shared_len: int = 0, ctx_len: int = 0,
+                           scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """attention_decode() over a paged cache: q [batch, heads*hd], one new row
+    per sequence, keys 0 .. lens[b] - 1.
+
+    shared_len (a multiple of page_size): the first shared_len keys of every
+    sequence are in the same pages (a common prefix); they are read once for
+    the batch, through the table's first row.  The result is that of
+    shared_len=0 up to rounding, also for sequences shorter than shared_len.
+    ctx_len: the largest lens expected (0: the table's width)."""
+    ldq = _mat(q, "q", torch.float16)
+    n_pages, kv_heads, ps, hd, B, W, ldt = _pool(k_pages, v_pages, page_table)
+    _need(tuple(q.shape) == (B, heads * hd), "q must be [batch, heads * head_dim]")
+    ln = _ints(lens, "lens", B)
+    if scale is None:
+        scale = 1.0 / math.sqrt(hd)
+    ctx = min(int(ctx_len), W * ps) if ctx_len > 0 else W * ps
+    with _on(q, k_pages, v_pages, page_table, lens, out):
+        if out is None:
+            out = torch.empty((B, heads * hd), dtype=torch.float16, device=q.device)
+        ldo = _mat(out, "out", torch.float16)
+        _need(tuple(out.shape) == (B, heads * hd), "out must be [batch, heads * head_dim]")
+        ws, wsb = _workspace(_lib.query("npub_attention_paged_decode_workspace", B, ctx, int(shared_len), heads,
+                                        kv_heads, hd), q.device)
+        _lib.call("npub_attention_paged_decode", q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
+                  ps, page_table.data_ptr(), ldt, W, ln, B, ctx, int(shared_len), out.data_ptr(), ldo, heads,
+                  kv_heads, hd, float(scale), _ptr(ws), wsb, _stream())
+    return out
 
 
 # --------------------------------------------------------- NPU ISA semantics
