@@ -17,7 +17,19 @@
 // (and its O and sum are rescaled) only when the row maximum has grown by more
 // than 2^8: P then stays below 2^8, far inside fp16, and the rescale, which
 // reads and writes the O tile, is rare.  The tensor core works on one tile
-// while the other is in its softmax.
+// while the other is in its softmax; P is handed over in two halves of 64 keys.
+//
+// What bounds it (clock64 stamps in one CTA, 8192 causal tokens, 32/8 heads):
+// at head_dim 128 a pair of tiles takes 2820 cycles per key block, of which
+// the tensor core runs 2048; a tile's chain is its softmax (1850: 160 to read
+// S, 440 for the maximum and the rescale test, 1250 for the exponentials) and
+// then the second half of P V and the next S.  At head_dim 64 the products
+// are half as long and the exponentials bound it (16 per cycle and SM), so a
+// quarter of them runs as a polynomial on the FMA pipe there (437 against 469
+// us); at head_dim 128 that only costs issue slots and power (462 / 458 us).
+// The MMA thread is one elected thread for the whole loop: issuing from
+// "lane 0" branches of a warp cost 90-130 cycles per MMA (606 us) where the
+// tensor core needs 64.
 //
 // Keys past a sequence's end inside its last 128-key block are whatever lies
 // behind them (the next sequence's rows, a page's stale slots): their scores
@@ -25,7 +37,9 @@
 // the product, since 0 * NaN and 0 * inf are NaN.
 //
 // Roles (384 threads): warps 0-3 and 4-7 softmax and output of tile 0 and 1,
-// warp 8 TMA, warp 9 tensor-memory allocation and MMA issue.
+// warp 8 TMA, warp 9 tensor-memory allocation and MMA issue (one thread), warp
+// 10 the scheduler of this CTA's items (persistent grid), warp 11 the zeroing
+// of V rows behind the last key.
 #include "common.cuh"
 #include "fmha_packed.h"
 #include "gemm_tc.h"
@@ -48,7 +62,8 @@ struct Smem {
     static constexpr int kOffQ = 0;
     static constexpr int kOffRing = 2 * kTile;
     static constexpr int kOffBar = kOffRing + kStages * kTile;
-    static constexpr int kTotal = kOffBar + 256;
+    static constexpr int kOffItem = kOffBar + 320;
+    static constexpr int kTotal = kOffItem + 256;
     static_assert(kTotal <= 232448, "shared memory budget");
 };
 
@@ -58,7 +73,7 @@ struct Params {
     int64_t ldt;
     int max_keys, page_shift, box_rows, n_pages;
     int total_q, batch, heads, kv_heads, group, tpt, head_dim;
-    int tiles, n_items, splits, split_keys, first, split0, shared, causal;
+    int tiles, n_items, sorted, levels, splits, split_keys, first, split0, shared, causal;
     float c;  // scale * log2(e)
     __half* out;
     int64_t ldo;
@@ -75,16 +90,46 @@ struct Item {
     int off;         // row i sees keys <= off + i
     int k0, kend;    // keys of this item
     int n[2];        // key blocks of each tile
+    int steps[2];    // 16-key steps of its last block
+    int vfix;        // keys of the last block when V rows behind them need zeroing, else 0
+    int state;       // 1: an item, 0: the last one is behind
 };
+constexpr int kItemSlots = 2;  // the scheduler works one item ahead
 
 __device__ __forceinline__ void set_err(int* err, int code) {
     if (err) atomicCAS(err, 0, code);
 }
 
-// Item -> rows and keys.  A whole warp: the tile's sequence is found by a scan
-// over the sequences' tile counts, 32 of them per step.  Reads cu and lens as
-// they are: whatever they hold, the rows stay inside [0, total_q) at the
-// stores and the keys inside the table, and the loop bounds are finite.
+// Rows of sequence s0 + lane, [r0, r1), and its keys.  Reads cu and lens as
+// they are: whatever they hold, rows stay inside [0, total_q) and keys inside
+// the table.
+template <bool PAGED>
+__device__ __forceinline__ void seq_rows(const Params& p, int b, int& r0, int& r1, int& klen) {
+    r0 = r1 = klen = 0;
+    if (b >= p.batch) return;
+    r0 = p.cu ? max(0, min(p.total_q, __ldg(p.cu + b))) : b;
+    r1 = p.cu ? max(r0, min(p.total_q, __ldg(p.cu + b + 1))) : r0 + 1;
+    klen = PAGED ? max(0, min(p.max_keys, __ldg(p.lens + b))) : r1 - r0;
+}
+
+// Tiles of a sequence that reach into key block `level` or behind it: tile t
+// ends at key off + (t + 1) * span (a causal tile's cost; others all cost the
+// same and count as level 0).
+__device__ __forceinline__ int tiles_from(const Params& p, int ntok, int klen, int level, int span) {
+    const int nt = (ntok + span - 1) / span;
+    if (level <= 0) return nt;
+    if (!p.causal) return 0;
+    const int64_t first = (int64_t)level * kBlk - (klen - ntok);  // rows behind this one reach the level
+    const int64_t t = first <= 0 ? 0 : first / span;
+    return t >= nt ? 0 : nt - (int)t;
+}
+
+// Item number -> rows and keys, by the scheduler warp.  Tiles are numbered
+// from the most expensive down (p.sorted), so that the CTAs, which take items
+// round by round in alternating direction, end together: a bisection over the
+// key level whose tile count brackets the number, each step a sum over the
+// sequences (32 per warp step), then a scan for the sequence.  Without
+// p.sorted (no CTA has a second item) the scan alone.
 template <bool PAGED>
 __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
     const int lane = threadIdx.x & 31;
@@ -108,14 +153,44 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
         it.n[1] = (p.tiles == 2 && it.tok0 + p.tpt < it.ntok) ? nb : 0;
         return true;
     }
-    int b = -1, r0 = 0, r1 = 0;
-    for (int s0 = 0; s0 < p.batch; s0 += 32) {
-        int c0 = 0, c1 = 0;
-        if (s0 + lane < p.batch) {
-            c0 = p.cu ? max(0, min(p.total_q, __ldg(p.cu + s0 + lane))) : s0 + lane;
-            c1 = p.cu ? max(c0, min(p.total_q, __ldg(p.cu + s0 + lane + 1))) : c0 + 1;
+    int level = 0;
+    if (p.sorted) {
+        // the highest level with more than `tile` tiles from it on
+        int lo = 0, hi = p.levels;
+        bool any = false;
+        while (lo <= hi) {
+            const int mid = (lo + hi) >> 1;
+            int sum = 0;
+            for (int s0 = 0; s0 < p.batch; s0 += 32) {
+                int r0, r1, kl;
+                seq_rows<PAGED>(p, s0 + lane, r0, r1, kl);
+                sum += tiles_from(p, r1 - r0, kl, mid, span);
+            }
+            sum = __reduce_add_sync(0xffffffffu, sum);
+            if (sum > tile) {
+                level = mid;
+                any = true;
+                lo = mid + 1;
+            } else {
+                hi = mid - 1;
+            }
         }
-        const int cnt = (c1 - c0 + span - 1) / span;
+        if (!any) return false;
+        int above = 0;
+        for (int s0 = 0; s0 < p.batch; s0 += 32) {
+            int r0, r1, kl;
+            seq_rows<PAGED>(p, s0 + lane, r0, r1, kl);
+            above += tiles_from(p, r1 - r0, kl, level + 1, span);
+        }
+        tile -= __reduce_add_sync(0xffffffffu, above);
+    }
+    int b = -1, r0 = 0, r1 = 0, klen = 0;
+    for (int s0 = 0; s0 < p.batch; s0 += 32) {
+        int c0, c1, kl;
+        seq_rows<PAGED>(p, s0 + lane, c0, c1, kl);
+        const int all = (c1 - c0 + span - 1) / span;
+        const int over = p.sorted ? tiles_from(p, c1 - c0, kl, level + 1, span) : 0;
+        const int cnt = (p.sorted ? tiles_from(p, c1 - c0, kl, level, span) : all) - over;
         int sum = cnt;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -128,8 +203,8 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
             tile -= __shfl_sync(0xffffffffu, sum - cnt, l);
             r0 = __shfl_sync(0xffffffffu, c0, l);
             r1 = __shfl_sync(0xffffffffu, c1, l);
-            const int nt = __shfl_sync(0xffffffffu, cnt, l);
-            tile = nt - 1 - tile;  // longest causal rows first
+            klen = __shfl_sync(0xffffffffu, kl, l);
+            tile = __shfl_sync(0xffffffffu, all - 1 - over, l) - tile;  // longest causal rows first
             b = s0 + l;
             break;
         }
@@ -141,7 +216,6 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
     it.kv_row0 = r0;
     it.ntok = r1 - r0;
     it.tok0 = tile * span;
-    const int klen = PAGED ? max(0, min(p.max_keys, __ldg(p.lens + b))) : it.ntok;
     it.off = p.causal ? klen - it.ntok : klen;
     it.k0 = p.first + it.split * p.split_keys;
     it.kend = it.split == p.splits - 1 ? klen : min(klen, it.k0 + p.split_keys);
@@ -154,10 +228,17 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
     return true;
 }
 
-// Keys that some row of tile q may see (a bound for its last block's steps).
-__device__ __forceinline__ int tile_limit(const Params& p, const Item& it, int q) {
-    const int t1 = min(it.ntok, it.tok0 + (q + 1) * p.tpt);
-    return (p.causal && p.shared == 0) ? min(it.kend, it.off + t1) : it.kend;
+// The last block of each tile and of the item.
+__device__ __forceinline__ void finish_item(const Params& p, Item& it) {
+    const int nblk = max(it.n[0], it.n[1]);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int t1 = min(it.ntok, it.tok0 + (q + 1) * p.tpt);
+        const int lim = (p.causal && p.shared == 0) ? min(it.kend, it.off + t1) : it.kend;
+        it.steps[q] = min(kBlk / 16, (lim - it.k0 - (it.n[q] - 1) * kBlk + 15) >> 4);
+    }
+    const int vb = it.kend - it.k0 - (nblk - 1) * kBlk;  // > 128: the causal limit ends the item ahead of kend
+    it.vfix = nblk > 0 && vb < kBlk && (vb & 15) ? vb : 0;
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -174,6 +255,97 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         : "memory");
 }
 
+// A row's 128 scores, one wait.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&x)[128]) {
+    uint32_t r[4][32];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t(&v)[32] = r[i];
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+            "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+            : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+              "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+              "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+              "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+            : "r"(taddr + 32u * i)
+            : "memory");
+    }
+    // the wait takes every destination as an operand, so that no use (or copy) of one is moved before it
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t(&v)[32] = r[i];
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                       "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]),
+                       "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]),
+                       "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]),
+                       "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+                     :
+                     : "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[i * 32 + e] = __uint_as_float(r[i][e]);
+}
+
+// ---- pairs of fp32 (one instruction per pair)
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// The largest of three, NaN when one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t exp2_hw2(uint64_t y) {
+    float a, b;
+    unpack2(y, a, b);
+    return pack2(ex2_approx(a), ex2_approx(b));
+}
+// 2^y on the FMA pipe, y <= 8: y = n + f with n the nearest integer (by adding
+// 1.5 * 2^23, which leaves n in the low bits of the sum) and |f| <= 1/2, the
+// degree-4 interpolation of 2^f at the Chebyshev points of [-1/2, 1/2] (largest
+// relative error 4e-6, a hundredth of half a step of fp16), and n added to the
+// exponent field.  y is held at -126, below which P is zero in fp16 anyway.
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t y) {
+    float a, b;
+    unpack2(y, a, b);
+    y = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const uint64_t big = pack2(12582912.0f, 12582912.0f), nbig = pack2(-12582912.0f, -12582912.0f);
+    const uint64_t t = add2(y, big);
+    const uint64_t f = fma2(add2(t, nbig), pack2(-1.0f, -1.0f), y);
+    uint64_t r = pack2(0.00966636852f, 0.00966636852f);
+    r = fma2(r, f, pack2(0.0559219758f, 0.0559219758f));
+    r = fma2(r, f, pack2(0.24022349f, 0.24022349f));
+    r = fma2(r, f, pack2(0.693121045f, 0.693121045f));
+    r = fma2(r, f, pack2(1.0f, 1.0f));
+    float r0, r1, t0, t1;
+    unpack2(r, r0, r1);
+    unpack2(t, t0, t1);
+    return pack2(__uint_as_float(__float_as_uint(r0) + (__float_as_uint(t0) << 23)),
+                 __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t1) << 23)));
+}
+
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2,
                                             int c3) {
     asm volatile(
@@ -183,8 +355,72 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uin
         : "memory");
 }
 
+// One lane of a converged warp, by elect.sync: the compiler then knows that a
+// single thread runs the branch and keeps descriptors in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+// mbar_wait_bounded for waits on the critical path: the timer and the abort
+// flag are first read after 256 failed tries.
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort));
+    bool ok = mbar_try_wait(bar, parity);
+    if (!ok) {
+        uint64_t t0 = 0;
+        for (uint32_t i = 1;; ++i) {
+            ok = mbar_try_wait(bar, parity);
+            if (ok) break;
+            if ((i & 255u) == 0) {
+                const uint64_t t = globaltimer_ns();
+                if (t0 == 0) t0 = t;
+                if (*abort || t - t0 > 2000000000ull) break;
+            }
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+
+// The same for one thread.
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    if (mbar_try_wait(bar, parity)) return true;
+    uint64_t t0 = 0;
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255u) == 0) {
+            const uint64_t t = globaltimer_ns();
+            if (t0 == 0) t0 = t;
+            if (*abort || t - t0 > 2000000000ull) return false;
+        }
+    }
+}
+
+__device__ __forceinline__ float row_max(const float (&x)[128]) {
+    float m4[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m4[i] = max3_nan(x[i], x[4 + i], x[8 + i]);
+#pragma unroll
+    for (int e = 12; e < 124; e += 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m4[i] = max3_nan(m4[i], x[e + i], x[e + 4 + i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m4[i] = max3_nan(m4[i], x[124 + i], x[124 + i]);
+    return max3_nan(max3_nan(m4[0], m4[1], m4[2]), m4[3], m4[3]);
+}
+// The next item of this CTA, published by the scheduler warp; false at the end
+// or when a wait ran out (ok = false).  A whole warp.
+__device__ __forceinline__ bool next_item(const Item* slots, uint64_t* full, uint64_t* empty, uint32_t& k, Item& it,
+                                          volatile int* abort, bool& ok) {
+    const uint32_t s = k % kItemSlots;
+    ok = wait_all(&full[s], (k / kItemSlots) & 1u, abort);
+    if (!ok) return false;
+    it = slots[s];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&empty[s]);
+    ++k;
+    return it.state != 0;
 }
 
 template <int HD, bool PAGED, bool PART>
@@ -201,12 +437,18 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
     uint64_t* q_full = bars;       // 1
     uint64_t* q_empty = bars + 1;  // 1
     uint64_t* s_full = bars + 2;   // [2]
-    uint64_t* p_full = bars + 4;   // [2]
-    uint64_t* o_full = bars + 6;   // [2]
-    uint64_t* mma_done = bars + 8;
-    uint64_t* kv_full = bars + 9;  // [kStages]
+    uint64_t* p_full = bars + 4;   // [2 tiles][2 halves of the keys]
+    uint64_t* o_full = bars + 8;   // [2]
+    uint64_t* mma_done = bars + 10;
+    uint64_t* v_seen = bars + 11;
+    uint64_t* v_fixed = bars + 12;
+    uint64_t* kv_full = bars + 13;  // [kStages]
     uint64_t* kv_empty = kv_full + L::kStages;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + L::kStages);
+    uint64_t* it_full = kv_empty + L::kStages;  // [kItemSlots]
+    uint64_t* it_empty = it_full + kItemSlots;  // [kItemSlots]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(it_empty + kItemSlots);
+    Item* slots = reinterpret_cast<Item*>(smem + L::kOffItem);
+    static_assert(kItemSlots * sizeof(Item) <= 256 && (13 + 2 * L::kStages + 2 * kItemSlots) * 8 + 8 <= 320, "layout");
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -215,13 +457,20 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
         mbar_init(q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[2 * i], 4);
+            mbar_init(&p_full[2 * i + 1], 4);
             mbar_init(&o_full[i], 1);
         }
         mbar_init(mma_done, 1);
+        mbar_init(v_seen, 1);
+        mbar_init(v_fixed, 1);
         for (int i = 0; i < L::kStages; ++i) {
             mbar_init(&kv_full[i], 1);
             mbar_init(&kv_empty[i], 1);
+        }
+        for (int i = 0; i < kItemSlots; ++i) {
+            mbar_init(&it_full[i], 1);
+            mbar_init(&it_empty[i], 11);
         }
         *abort_flag = 0;
         fence_barrier_init();
@@ -247,12 +496,11 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 8) {
             // ------------------------------------------------------------ TMA producer
-            uint32_t n = 0, nz = 0;  // ring tiles and non-empty items so far
+            uint32_t n = 0, nz = 0, ni = 0;  // ring tiles, non-empty items, items so far
             bool ok = true;
             const int nbox = PAGED ? kBlk / p.box_rows : 1;
-            for (int idx = blockIdx.x; idx < p.n_items && ok; idx += gridDim.x) {
-                Item it;
-                if (!get_item<PAGED>(p, idx, it)) continue;
+            Item it;
+            while (ok && next_item(slots, it_full, it_empty, ni, it, abort_flag, ok)) {
                 const int nblk = max(it.n[0], it.n[1]);
                 if (nblk == 0) continue;
                 ok = wait_all(q_empty, (nz & 1u) ^ 1u, abort_flag);
@@ -310,88 +558,92 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 }
             }
         } else if (warp == 9) {
-            // ------------------------------------------------------------ MMA issuer
-            constexpr uint32_t idesc_s = umma_idesc_f16(kRows, kBlk);
-            constexpr uint32_t idesc_o = umma_idesc_f16_bmn(kRows, HD);
-            uint32_t base = 0, nz = 0, np[2] = {0, 0};
-            bool ok = true;
-            for (int idx = blockIdx.x; idx < p.n_items && ok; idx += gridDim.x) {
-                Item it;
-                if (!get_item<PAGED>(p, idx, it)) continue;
-                const int nblk = max(it.n[0], it.n[1]);
-                if (nblk == 0) continue;
-                ok = wait_all(q_full, nz & 1u, abort_flag);
-                ++nz;
-                for (int j = 0; ok && j <= nblk; ++j) {
-                    const uint32_t vn = base + 2 * j - 1, kn = base + 2 * j;
-                    const uint32_t vs = vn % L::kStages, ks = kn % L::kStages;
-                    const uint32_t va = smem_u32(smem + L::kOffRing + vs * L::kTile);
-                    const uint32_t ka = smem_u32(smem + L::kOffRing + ks * L::kTile);
-                    if (j >= 1) {
-                        ok = wait_all(&kv_full[vs], (vn / L::kStages) & 1u, abort_flag);
-                        if (!ok) break;
-                        const int vb = it.kend - (it.k0 + (j - 1) * kBlk);  // keys of this block
-                        if (vb < kBlk && (vb & 15)) {  // V rows behind the last key, up to the 16-key step's end
-                            const int n16 = (16 - (vb & 15)) * 8;
-                            for (int i = lane; i < n16 * L::kChunks; i += 32) {
-                                const int ch = i / n16, e = i - ch * n16;
-                                *reinterpret_cast<uint4*>(smem + L::kOffRing + vs * L::kTile + ch * L::kChunk +
-                                                          vb * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+            // ------------------------------------------------------------ MMA issuer: one thread
+            if (elect_one()) {
+                constexpr uint32_t idesc_s = umma_idesc_f16(kRows, kBlk);
+                constexpr uint32_t idesc_o = umma_idesc_f16_bmn(kRows, HD);
+                // descriptors step by 16-byte units in their low 14 bits: no carry below 256 KB
+                const uint64_t qd0 = umma_desc_sw128(smem_u32(smem + L::kOffQ));
+                const uint64_t kd0 = umma_desc_sw128(smem_u32(smem + L::kOffRing));
+                const uint64_t vd0 = umma_desc_sw128_mn(smem_u32(smem + L::kOffRing), (uint32_t)L::kChunk, 1024u);
+                uint32_t st = 0, ph = 0, nz = 0, ni = 0, np[2] = {0, 0}, nv = 0;
+                bool ok = true;
+                while (ok) {
+                    const uint32_t slot = ni % kItemSlots;
+                    ok = wait_one(&it_full[slot], (ni / kItemSlots) & 1u, abort_flag);
+                    if (!ok) break;
+                    const Item& it = slots[slot];
+                    const int n0 = it.n[0], n1 = it.n[1], state = it.state;
+                    const int last0 = it.steps[0], last1 = it.steps[1], vfix = it.vfix;
+                    mbar_arrive(&it_empty[slot]);
+                    ++ni;
+                    if (!state) break;
+                    const int nblk = max(n0, n1);
+                    if (nblk == 0) continue;
+                    ok = wait_one(q_full, nz & 1u, abort_flag);
+                    ++nz;
+                    for (int j = 0; ok && j <= nblk; ++j) {
+                        // this step's tiles of the ring: V_{j-1}, then K_j
+                        const uint32_t vs = st;
+                        if (j >= 1) {
+                            ok = wait_one(&kv_full[st], ph, abort_flag);
+                            if (ok && vfix && j == nblk) {  // warp 11's turn; P of this block takes longer
+                                mbar_arrive(v_seen);
+                                ok = wait_one(v_fixed, nv++ & 1u, abort_flag);
                             }
-                            fence_proxy_async_smem();
-                            __syncwarp();
+                            if (++st == L::kStages) st = 0, ph ^= 1u;
                         }
-                    }
-                    if (j < nblk) {
-                        ok = wait_all(&kv_full[ks], (kn / L::kStages) & 1u, abort_flag);
+                        const uint32_t ks = st;
+                        if (ok && j < nblk) {
+                            ok = wait_one(&kv_full[st], ph, abort_flag);
+                            if (++st == L::kStages) st = 0, ph ^= 1u;
+                        }
                         if (!ok) break;
-                    }
+                        const uint64_t vd = vd0 + (uint64_t)(vs * (L::kTile >> 4));
+                        const uint64_t kd = kd0 + (uint64_t)(ks * (L::kTile >> 4));
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const uint32_t sq = tmem + (uint32_t)(q * 128), oq = tmem + 256u + (uint32_t)(q * 128);
-                        if (j >= 1 && j - 1 < it.n[q]) {  // O_q += P_q(j-1) V_{j-1}
-                            ok = wait_all(&p_full[q], np[q] & 1u, abort_flag);
-                            if (!ok) break;
-                            ++np[q];
-                            tc_fence_after();
-                            if (lane == 0) {
-                                const int left = tile_limit(p, it, q) - (it.k0 + (j - 1) * kBlk);
-                                const int steps = min(kBlk / 16, (left + 15) >> 4);
-                                for (int kk = 0; kk < steps; ++kk)
-                                    tc_mma_f16_ts(oq, sq + (uint32_t)kk * 8u,
-                                                  umma_desc_sw128_mn(va + (uint32_t)kk * 2048u, (uint32_t)L::kChunk,
-                                                                     1024u),
-                                                  idesc_o, (j > 1 || kk > 0) ? 1u : 0u);
-                                if (j == it.n[q]) tc_commit(&o_full[q]);
+                        for (int q = 0; q < 2; ++q) {
+                            const int n = q ? n1 : n0;
+                            const uint32_t sq = tmem + (uint32_t)(q * 128), oq = tmem + 256u + (uint32_t)(q * 128);
+                            if (j >= 1 && j <= n) {  // O_q += P_q(j-1) V_{j-1}
+                                const int steps = j < n ? kBlk / 16 : (q ? last1 : last0);
+#pragma unroll
+                                for (int hf = 0; hf < 2; ++hf) {  // the first 64 keys' P is ready ahead of the rest
+                                    ok = wait_one(&p_full[2 * q + hf], np[q] & 1u, abort_flag);
+                                    if (!ok) break;
+                                    tc_fence_after();
+                                    if (steps == kBlk / 16) {
+#pragma unroll
+                                        for (int kk = hf * 4; kk < hf * 4 + 4; ++kk)
+                                            tc_mma_f16_ts(oq, sq + (uint32_t)kk * 8u, vd + (uint64_t)(kk * 128),
+                                                          idesc_o, (j > 1 || kk > 0) ? 1u : 0u);
+                                    } else {
+#pragma unroll 1
+                                        for (int kk = hf * 4; kk < min(steps, hf * 4 + 4); ++kk)
+                                            tc_mma_f16_ts(oq, sq + (uint32_t)kk * 8u, vd + (uint64_t)(kk * 128),
+                                                          idesc_o, (j > 1 || kk > 0) ? 1u : 0u);
+                                    }
+                                }
+                                if (!ok) break;
+                                ++np[q];
+                                if (j == n) tc_commit(&o_full[q]);
                             }
-                            __syncwarp();
-                        }
-                        if (j < it.n[q]) {  // S_q(j) = Q_q K_j^T
-                            tc_fence_after();
-                            if (lane == 0) {
-                                const uint32_t qa = smem_u32(smem + L::kOffQ + q * L::kTile);
+                            if (j < n) {  // S_q(j) = Q_q K_j^T
+                                const uint64_t qd = qd0 + (uint64_t)(q * (L::kTile >> 4));
 #pragma unroll
                                 for (int kk = 0; kk < HD / 16; ++kk) {
-                                    const uint32_t o = (uint32_t)((kk >> 2) * L::kChunk + (kk & 3) * 32);
-                                    tc_mma_f16(sq, umma_desc_sw128(qa + o), umma_desc_sw128(ka + o), idesc_s,
-                                               kk > 0 ? 1u : 0u);
+                                    const uint64_t o = (uint64_t)(((kk >> 2) * L::kChunk + (kk & 3) * 32) >> 4);
+                                    tc_mma_f16(sq, qd + o, kd + o, idesc_s, kk > 0 ? 1u : 0u);
                                 }
                                 tc_commit(&s_full[q]);
                             }
-                            __syncwarp();
                         }
-                    }
-                    if (!ok) break;
-                    if (lane == 0) {
+                        if (!ok) break;
                         if (j >= 1) tc_commit(&kv_empty[vs]);
                         if (j < nblk) tc_commit(&kv_empty[ks]);
                         if (j == nblk - 1) tc_commit(q_empty);
                     }
-                    __syncwarp();
                 }
-                base += 2 * nblk;
-            }
-            if (lane == 0) {
                 if (!ok) {
                     *abort_flag = 1;
                     set_err(p.err, 0x502);
@@ -400,6 +652,56 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 if (!mbar_wait_bounded(mma_done, 0, no_abort, 200000000ull)) set_err(p.err, 0x503);
             }
             __syncwarp();
+        } else if (warp == 11) {
+            // ------------------------------------------------------------ V rows behind the last key
+            uint32_t base = 0, ni = 0, nv = 0;
+            bool ok = true;
+            Item it;
+            while (ok && next_item(slots, it_full, it_empty, ni, it, abort_flag, ok)) {
+                const int nblk = max(it.n[0], it.n[1]);
+                if (it.vfix) {  // zeroed up to the end of the last 16-key step
+                    const uint32_t vs = (base + 2 * nblk - 1) % L::kStages;
+                    ok = wait_all(v_seen, nv++ & 1u, abort_flag);  // the MMA thread has seen the tile land
+                    if (!ok) break;
+                    const int vb = it.vfix, n16 = (16 - (vb & 15)) * 8;
+                    for (int i = lane; i < n16 * L::kChunks; i += 32) {
+                        const int ch = i / n16, e = i - ch * n16;
+                        *reinterpret_cast<uint4*>(smem + L::kOffRing + vs * L::kTile + ch * L::kChunk + vb * 128 +
+                                                  e * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(v_fixed);
+                }
+                base += 2 * nblk;
+            }
+        } else if (warp == 10) {
+            // ------------------------------------------------------------ scheduler
+            uint32_t k = 0;
+            bool ok = true;
+            for (int round = 0; ok; ++round) {
+                const int64_t base = (int64_t)round * gridDim.x;
+                const int64_t idx = base + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                Item it;
+                it.state = base < p.n_items ? 1 : 0;
+                if (it.state && (idx >= p.n_items || !get_item<PAGED>(p, (int)idx, it))) continue;
+                const uint32_t s = k % kItemSlots;
+                ok = wait_all(&it_empty[s], ((k / kItemSlots) & 1u) ^ 1u, abort_flag);
+                if (!ok) {
+                    if (lane == 0) {
+                        *abort_flag = 1;
+                        set_err(p.err, 0x505);
+                    }
+                    break;
+                }
+                finish_item(p, it);
+                if (lane == 0) {
+                    slots[s] = it;
+                    mbar_arrive(&it_full[s]);
+                }
+                ++k;
+                if (!it.state) break;
+            }
         }
     } else {
         // ---------------------------------------------------------------- softmax / output
@@ -410,11 +712,10 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
         const uint32_t sq = tmem + lanes + (uint32_t)(q * 128), oq = tmem + lanes + 256u + (uint32_t)(q * 128);
         const int tl = r / p.group, g = r - tl * p.group;
         const float c = p.c;
-        uint32_t ns = 0, no = 0;
+        uint32_t ns = 0, no = 0, ni = 0;
         bool ok = true;
-        for (int idx = blockIdx.x; idx < p.n_items && ok; idx += gridDim.x) {
-            Item it;
-            if (!get_item<PAGED>(p, idx, it)) continue;
+        Item it;
+        while (ok && next_item(slots, it_full, it_empty, ni, it, abort_flag, ok)) {
             const int tok = it.tok0 + q * p.tpt + tl;
             const bool valid = q < p.tiles && tl < p.tpt && tok < it.ntok;
             int lim = it.kend;  // this row's keys end here
@@ -423,36 +724,24 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 else if (p.causal) lim = min(lim, it.off + tok + 1);
             }
             float m = -INFINITY, l = 0.0f;
-            const int nb = it.n[q];
+            const int nb = q ? it.n[1] : it.n[0];
             for (int j = 0; j < nb; ++j) {
                 ok = wait_all(&s_full[q], ns & 1u, abort_flag);
                 if (!ok) break;
                 ++ns;
                 tc_fence_after();
                 float x[128];
-                {
-                    uint32_t a[64], b[64];
-                    tmem_ld64(sq, a);
-                    tmem_ld64(sq + 64, b);
-#pragma unroll
-                    for (int e = 0; e < 64; ++e) {
-                        x[e] = __uint_as_float(a[e]);
-                        x[64 + e] = __uint_as_float(b[e]);
-                    }
-                }
+                tmem_ld128(sq, x);
                 const int left = lim - (it.k0 + j * kBlk);
                 if (__any_sync(0xffffffffu, left < kBlk)) {
 #pragma unroll
                     for (int e = 0; e < 128; ++e) x[e] = e < left ? x[e] : -INFINITY;
                 }
-                float m4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int e = 4; e < 128; ++e) m4[e & 3] = fmaxf(m4[e & 3], x[e]);
-                const float mx = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                const float mx = max3_nan(m, row_max(x), m);
                 if (j == 0) {
                     m = mx;
                 } else {
-                    const bool need = (mx - m) * c > 8.0f;
+                    const bool need = mx != -INFINITY && !((mx - m) * c <= 8.0f);  // also when the maximum is NaN
                     if (__any_sync(0xffffffffu, need)) {  // P_q(j-1) V_{j-1} is complete: S_q(j) was issued behind it
                         const float corr = need ? ex2_approx((m - mx) * c) : 1.0f;
                         if (need) m = mx;
@@ -467,26 +756,31 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                         }
                     }
                 }
-                const float mc = m == -INFINITY ? 0.0f : m * c;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float mc = m == -INFINITY ? 0.0f : -m * c;  // 0: every exponential of the row is 2^-inf
+                const uint64_t c2 = pack2(c, c), mc2 = pack2(mc, mc);
+                uint64_t sum2[2] = {0, 0};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t pk[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const float p0 = ex2_approx(fmaf(x[h * 64 + 2 * e], c, -mc));
-                        const float p1 = ex2_approx(fmaf(x[h * 64 + 2 * e + 1], c, -mc));
-                        sum[e & 3] += p0 + p1;
+                        const uint64_t y = fma2(pack2(x[h * 64 + 2 * e], x[h * 64 + 2 * e + 1]), c2, mc2);
+                        const uint64_t pp = (HD == 64 && (e & 3) == 0) ? exp2_poly2(y) : exp2_hw2(y);
+                        sum2[e & 1] = add2(sum2[e & 1], pp);
+                        float p0, p1;
+                        unpack2(pp, p0, p1);
                         __half2 hh = __floats2half2_rn(p0, p1);
                         pk[e] = *reinterpret_cast<uint32_t*>(&hh);
                     }
                     tmem_st32(sq + (uint32_t)(h * 32), pk);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * q + h]);
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[q]);
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                float s0, s1;
+                unpack2(add2(sum2[0], sum2[1]), s0, s1);
+                l += s0 + s1;
             }
             if (!ok) break;
             if (nb > 0) {
@@ -499,13 +793,13 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             const int head = it.kvh * p.group + g;
             if (PART) {
                 const int64_t at = ((int64_t)(p.split0 + it.split) * p.total_q + row) * p.heads + head;
-                if (valid) p.part_ml[at] = make_float2(m == -INFINITY ? -INFINITY : m * c, l);
+                if (valid) p.part_ml[at] = m == -INFINITY ? make_float2(-INFINITY, 0.0f) : make_float2(m * c, l);
                 if (nb > 0) {
 #pragma unroll 1
                     for (int e0 = 0; e0 < p.head_dim; e0 += 32) {
                         uint32_t o[32];
                         tmem_ld32(oq + (uint32_t)e0, o);
-                        if (!valid || !(l != 0.0f)) continue;
+                        if (!valid || m == -INFINITY) continue;
                         float* dst = p.part_o + at * p.head_dim + e0;
 #pragma unroll
                         for (int e = 0; e < 32; e += 4)
@@ -514,7 +808,8 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                     }
                 }
             } else {
-                const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+                const bool none = m == -INFINITY;  // no key
+                const float inv = 1.0f / l;
                 __half* dst = p.out + row * p.ldo + (int64_t)head * p.head_dim;
 #pragma unroll 1
                 for (int e0 = 0; e0 < p.head_dim; e0 += 32) {
@@ -529,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                         for (int i = 0; i < 4; ++i) {
                             __half2 hh = __floats2half2_rn(__uint_as_float(o[e + 2 * i]) * inv,
                                                            __uint_as_float(o[e + 2 * i + 1]) * inv);
-                            pk[i] = l != 0.0f ? *reinterpret_cast<uint32_t*>(&hh) : 0u;
+                            pk[i] = none ? 0u : *reinterpret_cast<uint32_t*>(&hh);
                         }
                         *reinterpret_cast<uint4*>(dst + e0 + e) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
                     }
@@ -631,7 +926,9 @@ int fmha_packed(const PackedArgs& a, cudaStream_t st) {
                           p.splits;
     if (items > 0x7fffffff) return NPUB_ERR_UNSUPPORTED;
     p.n_items = (int)items;
-    const int grid = p.n_items;
+    const int grid = p.n_items < num_sms() ? p.n_items : num_sms();
+    p.sorted = p.n_items > grid && a.shared == 0;
+    p.levels = (int)(((paged ? (int64_t)p.max_keys : (int64_t)a.total_q) + kBlk - 1) / kBlk);
     const bool small = a.head_dim <= 64;
     if (part) {
         if (!paged) return NPUB_ERR_UNSUPPORTED;
