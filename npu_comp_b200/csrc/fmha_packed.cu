@@ -73,10 +73,11 @@ struct Params {
     int64_t ldt;
     int max_keys, page_shift, box_rows, n_pages;
     int total_q, batch, heads, kv_heads, group, tpt, head_dim;
-    int tiles, n_items, sorted, levels, splits, split_keys, first, split0, shared, causal;
+    int tiles, n_items, sorted, levels, splits, first, split0, shared, causal;
     float c;  // scale * log2(e)
     __half* out;
     int64_t ldo;
+    int out32;  // output rows are 32-byte aligned
     float* part_o;
     float2* part_ml;
     int* err;
@@ -120,8 +121,9 @@ __device__ __forceinline__ int tiles_from(const Params& p, int ntok, int klen, i
     if (level <= 0) return nt;
     if (!p.causal) return 0;
     const int64_t first = (int64_t)level * kBlk - (klen - ntok);  // rows behind this one reach the level
-    const int64_t t = first <= 0 ? 0 : first / span;
-    return t >= nt ? 0 : nt - (int)t;
+    if (first <= 0) return nt;
+    if (first >= ntok) return 0;
+    return nt - (int)((uint32_t)first / (uint32_t)span);
 }
 
 // Item number -> rows and keys, by the scheduler warp.  Tiles are numbered
@@ -145,8 +147,9 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
         it.tok0 = tile * span;
         it.kv_row0 = 0;
         it.off = p.shared;  // no causal limit; each row has its own
-        it.k0 = it.split * p.split_keys;
-        it.kend = it.split == p.splits - 1 ? p.shared : min(p.shared, it.k0 + p.split_keys);
+        const int per = ((p.shared + kBlk - 1) / kBlk + p.splits - 1) / p.splits * kBlk;
+        it.k0 = min(p.shared, it.split * per);
+        it.kend = min(p.shared, it.k0 + per);
         if (it.tok0 >= it.ntok) return false;
         const int nb = it.kend > it.k0 ? (it.kend - it.k0 + kBlk - 1) / kBlk : 0;
         it.n[0] = nb;
@@ -217,8 +220,10 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
     it.ntok = r1 - r0;
     it.tok0 = tile * span;
     it.off = p.causal ? klen - it.ntok : klen;
-    it.k0 = p.first + it.split * p.split_keys;
-    it.kend = it.split == p.splits - 1 ? klen : min(klen, it.k0 + p.split_keys);
+    // every sequence's own keys in p.splits equal ranges of whole blocks
+    const int per = ((max(0, klen - p.first) + kBlk - 1) / kBlk + p.splits - 1) / p.splits * kBlk;
+    it.k0 = min(klen, p.first + it.split * per);
+    it.kend = it.split == p.splits - 1 ? klen : min(klen, it.k0 + per);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const int t0 = it.tok0 + q * p.tpt, t1 = min(it.ntok, t0 + p.tpt);
@@ -253,6 +258,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr)
         : "memory");
+}
+
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 // A row's 128 scores, one wait.
@@ -426,7 +437,10 @@ __device__ __forceinline__ bool next_item(const Item* slots, uint64_t* full, uin
 template <int HD, bool PAGED, bool PART>
 __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_constant__ Params p) {
     using L = Smem<HD>;
-    pdl_trigger();
+    // A shared-prefix phase lets its successor start only behind its own wait: the successor (paged_decode on the
+    // sequences' own keys) then needs none before its loads and runs beside this kernel.
+    const bool late = PART && p.shared > 0;
+    if (!late) pdl_trigger();
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // the swizzled tiles need 1024-byte alignment
         if (threadIdx.x == 0) set_err(p.err, 0x500);
@@ -491,6 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
     int never = 0;
     volatile int* no_abort = &never;
     pdl_wait();
+    if (late) pdl_trigger();
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -789,44 +804,47 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 ++no;
                 tc_fence_after();
             }
+            // Output straight from a lane's registers, whole 32-byte sectors where the row allows it.  (Through shared
+            // memory, for 128-byte lines, it took as long: the staging competes with the operand reads of the other
+            // tile's MMAs, which use all of the shared-memory bandwidth.)
             const int64_t row = (int64_t)it.q_row0 + tok;
             const int head = it.kvh * p.group + g;
-            if (PART) {
-                const int64_t at = ((int64_t)(p.split0 + it.split) * p.total_q + row) * p.heads + head;
-                if (valid) p.part_ml[at] = m == -INFINITY ? make_float2(-INFINITY, 0.0f) : make_float2(m * c, l);
-                if (nb > 0) {
-#pragma unroll 1
-                    for (int e0 = 0; e0 < p.head_dim; e0 += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(oq + (uint32_t)e0, o);
-                        if (!valid || m == -INFINITY) continue;
-                        float* dst = p.part_o + at * p.head_dim + e0;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            if (e0 + e < p.head_dim)
-                                *reinterpret_cast<uint4*>(dst + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                    }
-                }
-            } else {
-                const bool none = m == -INFINITY;  // no key
-                const float inv = 1.0f / l;
-                __half* dst = p.out + row * p.ldo + (int64_t)head * p.head_dim;
+            const bool none = m == -INFINITY;  // no key: zeros (no partial)
+            const int64_t at = PART ? ((int64_t)(p.split0 + it.split) * p.total_q + row) * p.heads + head : 0;
+            if (PART && valid) p.part_ml[at] = none ? make_float2(-INFINITY, 0.0f) : make_float2(m * c, l);
+            const bool put = valid && !(PART && none);
+            const float inv = none ? 0.0f : 1.0f / l;
+            float* dstf = p.part_o + at * p.head_dim;
+            __half* dsth = p.out + row * p.ldo + (int64_t)head * p.head_dim;
+            if (__any_sync(0xffffffffu, put)) {
 #pragma unroll 1
                 for (int e0 = 0; e0 < p.head_dim; e0 += 32) {
                     uint32_t o[32];
                     if (nb > 0) tmem_ld32(oq + (uint32_t)e0, o);
-                    if (!valid) continue;
+                    if (!put) continue;
+                    if (PART) {
+                        const int n = p.head_dim - e0 < 32 ? p.head_dim - e0 : 32;  // a multiple of 16
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        if (e0 + e >= p.head_dim) break;
-                        uint32_t pk[4];
+                        for (int e = 0; e < 32; e += 8)
+                            if (e < n) st_global_v8(dstf + e0 + e, &o[e]);
+                    } else {
+                        uint32_t pk[16];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            __half2 hh = __floats2half2_rn(__uint_as_float(o[e + 2 * i]) * inv,
-                                                           __uint_as_float(o[e + 2 * i + 1]) * inv);
+                        for (int i = 0; i < 16; ++i) {
+                            __half2 hh = __floats2half2_rn(__uint_as_float(o[2 * i]) * inv,
+                                                           __uint_as_float(o[2 * i + 1]) * inv);
                             pk[i] = none ? 0u : *reinterpret_cast<uint32_t*>(&hh);
                         }
-                        *reinterpret_cast<uint4*>(dst + e0 + e) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                        if (p.out32) {
+                            st_global_v8(dsth + e0, pk);
+                            if (e0 + 16 < p.head_dim) st_global_v8(dsth + e0 + 16, pk + 8);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (e0 + i * 8 < p.head_dim)
+                                    *reinterpret_cast<uint4*>(dsth + e0 + i * 8) =
+                                        make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+                        }
                     }
                 }
             }
@@ -910,12 +928,12 @@ int fmha_packed(const PackedArgs& a, cudaStream_t st) {
     p.c = a.scale * 1.4426950408889634f;
     p.out = reinterpret_cast<__half*>(a.out);
     p.ldo = a.ldo;
+    p.out32 = npub_aligned(a.out, 32) && a.ldo % 16 == 0;
     p.part_o = a.part_o;
     p.part_ml = a.part_ml;
     p.err = npub_internal_device_error_word();
     const bool part = a.part_o != nullptr;
     p.splits = part ? a.splits : 1;
-    p.split_keys = a.split_keys;
     p.first = a.first;
     p.split0 = a.split0;
     // One tile per CTA while that still leaves SMs free.

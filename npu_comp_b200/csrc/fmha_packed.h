@@ -32,8 +32,8 @@ struct PackedArgs {
     float scale;
     int causal;
     // splits > 1 (or shared): fp32 partials instead of out
-    int splits, split_keys;
-    int first, split0;    // the splits' first key, and the index of split 0 among the partials
+    int splits;           // equal ranges of every sequence's keys from `first` on
+    int first, split0;    // split0: index of split 0 among the partials
     float* part_o;        // [splits, total_q, heads, head_dim]
     float2* part_ml;      // [splits, total_q, heads]: (row maximum * scale * log2 e, sum of exponentials)
 };

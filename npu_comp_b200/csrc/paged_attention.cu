@@ -36,47 +36,50 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Plan {
     bool few;                     // own keys on paged_decode (else on the tiles)
     int shared;                   // keys of the shared prefix phase (0: none)
-    int pre_splits, pre_keys;     // its splits and keys per split
-    int own_splits, own_keys;
+    int pre_splits, own_splits;
     bool part() const { return pre_splits + own_splits > 1; }
     int total() const { return pre_splits + own_splits; }
 };
 
-// Cuts `keys` keys of `items` independent work items so that about `want` CTAs run, in ranges of at least `least`
-// keys and whole multiples of `unit`.
-void cut(int64_t keys, int64_t items, int64_t want, int64_t least, int64_t unit, int* splits, int* per) {
-    int64_t s = items > 0 ? ceil_div(want, items) : 1;
-    const int64_t most = ceil_div(keys, least);
-    if (s > most) s = most;
-    if (s < 1) s = 1;
-    int64_t k = ceil_div(ceil_div(keys, s), unit) * unit;
-    if (k < unit) k = unit;
-    if (k > 0x40000000) k = 0x40000000;
-    *per = (int)k;
-    *splits = (int)ceil_div(keys > 0 ? keys : 1, k);
+// Number of key ranges for `items` work items of up to `keys` keys on `slots` resident CTAs: the s that makes
+// waves * (start + key units of a range * per unit) + combination smallest, times in us.  `part_us`: what the partials
+// of one more split cost (written, read), `fixed`: a combination pass runs anyway.
+int pick_splits(int64_t keys, int64_t items, int64_t slots, int unit, double start, double per_unit, double part_us,
+                bool fixed) {
+    const int64_t units = ceil_div(keys > 0 ? keys : 1, unit);
+    double best = 0.0;
+    int pick = 1;
+    for (int s = 1; s <= 64 && s <= units; ++s) {
+        const double t = (double)ceil_div(items * s, slots) * (start + (double)ceil_div(units, s) * per_unit) +
+                         (s > 1 || fixed ? s * (part_us + 0.15) : 0.0) + (s > 1 && !fixed ? 4.0 : 0.0);
+        if (s == 1 || t < 0.95 * best) {
+            best = t;
+            pick = s;
+        }
+    }
+    return pick;
 }
 
-Plan make_plan(int batch, int total, int max_new, int64_t ctx, int shared, int heads, int kv_heads) {
+Plan make_plan(int batch, int total, int max_new, int64_t ctx, int shared, int heads, int kv_heads, int head_dim) {
     Plan pl = {};
     const int group = heads / kv_heads, sms = num_sms();
     pl.few = max_new > 0 && (int64_t)max_new * group <= kPagedDecodeRows && batch <= 65535;
     if (batch < 2) shared = 0;  // nothing to share
     pl.shared = shared;
+    // Measured: a pair of tiles takes 1.5 us per 128 keys and 4 us to start and end; a few-row CTA, two of which share
+    // an SM, takes 1.5 us per 64 keys of 128 columns and 2.5 us; partials move at about 4 TB/s (they stay in L2).
+    const double part_us = (double)total * heads * head_dim * 8.0 / 4e6;
     if (shared > 0) {
         const int64_t tiles = fmha_packed_items(total, 1, heads, kv_heads, 0, 2) * kv_heads;
-        cut(shared, tiles, sms, 256, 128, &pl.pre_splits, &pl.pre_keys);
+        pl.pre_splits = pick_splits(shared, tiles, sms, 128, 4.0, 1.5, part_us, true);
     }
     const int64_t own = ctx > shared ? ctx - shared : 1;
     if (pl.few) {
-        cut(own, (int64_t)batch * kv_heads, 4 * 2 * sms, 256, 64, &pl.own_splits, &pl.own_keys);
+        const int64_t items = (int64_t)batch * kv_heads;
+        pl.own_splits = pick_splits(own, items, 2 * sms, 64, 2.5, head_dim > 64 ? 1.5 : 0.8, part_us, shared > 0);
     } else {
         const int64_t tiles = fmha_packed_items(total, batch, heads, kv_heads, max_new, 2) * kv_heads;
-        if (tiles >= sms) {
-            pl.own_splits = 1;
-            pl.own_keys = 128;  // the last split takes every key that is left
-        } else {
-            cut(own, tiles, sms, 512, 128, &pl.own_splits, &pl.own_keys);
-        }
+        pl.own_splits = pick_splits(own, tiles, sms, 128, 4.0, 1.5, part_us, shared > 0);
     }
     return pl;
 }
@@ -103,20 +106,13 @@ int run_plan(const Plan& pl, PackedArgs& a, void* workspace, size_t workspace_by
         s.cu = nullptr;
         s.max_new = 0;
         s.splits = pl.pre_splits;
-        s.split_keys = pl.pre_keys;
         const int rc = fmha_packed(s, st);
         if (rc) return rc;
     }
-    int rc;
-    if (pl.few) {
-        rc = paged_decode(a, pl.shared, pl.own_keys, pl.own_splits, pl.pre_splits, st);
-    } else {
-        a.first = pl.shared;
-        a.splits = pl.own_splits;
-        a.split0 = pl.pre_splits;
-        a.split_keys = pl.own_keys;
-        rc = fmha_packed(a, st);
-    }
+    a.first = pl.shared;
+    a.splits = pl.own_splits;
+    a.split0 = pl.pre_splits;
+    const int rc = pl.few ? paged_decode(a, st) : fmha_packed(a, st);
     if (rc || !need) return rc;
     return paged_combine(a, pl.total(), st);
 }
@@ -195,7 +191,8 @@ extern "C" int npub_attention_paged(const void* q, int64_t ldq, const void* k_pa
     a.scale = scale;
     a.causal = causal;
     const int64_t cap = (int64_t)max_pages * page_size;
-    const Plan pl = make_plan(batch, total, max_new, ctx_len > 0 && ctx_len < cap ? ctx_len : cap, 0, heads, kv_heads);
+    const Plan pl = make_plan(batch, total, max_new, ctx_len > 0 && ctx_len < cap ? ctx_len : cap, 0, heads, kv_heads,
+                              head_dim);
     return run_plan(pl, a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -205,7 +202,7 @@ extern "C" size_t npub_attention_paged_workspace(int batch, int total, int max_n
     if (batch <= 0 || total <= 0 || max_new < 0 || ctx_len < 0 || !dims_ok(heads, kv_heads, head_dim, 1.0f) ||
         !dims_supported(heads, kv_heads, head_dim))
         return 0;
-    return plan_bytes(make_plan(batch, total, max_new, ctx_len, 0, heads, kv_heads), total, heads, head_dim);
+    return plan_bytes(make_plan(batch, total, max_new, ctx_len, 0, heads, kv_heads, head_dim), total, heads, head_dim);
 }
 
 extern "C" int npub_attention_paged_decode(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
@@ -244,7 +241,7 @@ extern "C" int npub_attention_paged_decode(const void* q, int64_t ldq, const voi
     a.causal = 1;
     const int64_t cap = (int64_t)max_pages * page_size;
     const Plan pl = make_plan(batch, batch, 1, ctx_len > 0 && ctx_len < cap ? ctx_len : cap, shared_len, heads,
-                              kv_heads);
+                              kv_heads, head_dim);
     return run_plan(pl, a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -254,5 +251,5 @@ extern "C" size_t npub_attention_paged_decode_workspace(int batch, int64_t ctx_l
     if (batch <= 0 || ctx_len < 0 || shared_len < 0 || !dims_ok(heads, kv_heads, head_dim, 1.0f) ||
         !dims_supported(heads, kv_heads, head_dim))
         return 0;
-    return plan_bytes(make_plan(batch, batch, 1, ctx_len, shared_len, heads, kv_heads), batch, heads, head_dim);
+    return plan_bytes(make_plan(batch, batch, 1, ctx_len, shared_len, heads, kv_heads, head_dim), batch, heads, head_dim);
 }

@@ -48,8 +48,9 @@ struct Params {
     int64_t ldt;
     int max_keys, page_shift, box_rows, n_pages;
     int total_q, heads, kv_heads, group, head_dim, causal;
-    int first, chunk, splits;  // keys [first + split * chunk, + chunk); the last split takes all that are left
+    int first, splits;         // every sequence's keys from `first` on in `splits` equal ranges
     int split0;                // index of split 0 among the partials
+    int beside;                // launched behind a shared-prefix phase, which has waited for all earlier work
     float c;
     __half* out;
     int64_t ldo;
@@ -123,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
         prefetch_tmap(&p.tmV);
     }
     cta_sync_divergent();
-    pdl_wait();
+    if (!p.beside) pdl_wait();
 
     // rows of this sequence, its keys, and this CTA's range of them
     int row0 = b, nrow = 1;
@@ -134,9 +135,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     }
     const int R = nrow * p.group;
     const int len = max(0, min(p.lens[b], p.max_keys));
-    const int64_t first = (int64_t)p.first + (int64_t)split * p.chunk;
-    const int k0 = (int)min(first, (int64_t)len);
-    const int k1 = R == 0 ? k0 : split == p.splits - 1 ? len : (int)min(first + p.chunk, (int64_t)len);
+    const int own = max(0, len - p.first);
+    const int per = ((own + kKeys - 1) / kKeys + p.splits - 1) / p.splits * kKeys;  // whole stages
+    const int k0 = R == 0 ? 0 : p.first + min(own, split * per);
+    const int k1 = R == 0 ? 0 : p.first + min(own, split * per + per);
     const int nst = (k1 - k0 + kKeys - 1) / kKeys;
     const bool part = p.part_o != nullptr;
 
@@ -170,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
             for (int i = max(0, j - L::kStages); i < j; ++i)
                 mbar_wait_bounded(&full[i % L::kStages], (uint32_t)(i / L::kStages) & 1u, &never, 200000000ull);
         }
+        if (p.beside) pdl_wait();
         return;
     }
 
@@ -341,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
             *reinterpret_cast<uint2*>(p.out + (int64_t)(row0 + t) * p.ldo + (int64_t)head * p.head_dim + d) = w;
         }
     }
+    if (p.beside) pdl_wait();  // this grid's end then means the prefix phase's end to the combination behind it
 }
 
 // out[row, head] = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over the
@@ -362,28 +366,44 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const float* __restr
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
-    const int d0 = lane * 4;
-    const bool act = d0 < hd;
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        const float2 ml = part_ml[(int64_t)s * n + id];
-        if (ml.y == 0.0f) continue;
-        const float f = ex2_approx(ml.x - m);
-        sum += f * ml.y;
-        if (act) {
-            const float4 v = *reinterpret_cast<const float4*>(part_o + ((int64_t)s * n + id) * hd + d0);
-            acc[0] += f * v.x;
-            acc[1] += f * v.y;
-            acc[2] += f * v.z;
-            acc[3] += f * v.w;
+    const bool act = lane * 4 < hd;
+    for (int s0 = 0; s0 < splits; s0 += 32) {
+        // lane s: the weight of split s0 + s (0 where it saw no key and has no partial)
+        float f = 0.0f;
+        if (s0 + lane < splits) {
+            const float2 ml = part_ml[(int64_t)(s0 + lane) * n + id];
+            if (ml.y != 0.0f) f = ex2_approx(ml.x - m);
+            sum += f * ml.y;
+        }
+        const float* src = part_o + ((int64_t)s0 * n + id) * hd + lane * 4;
+        const int cnt = min(32, splits - s0);
+        for (int s = 0; s < cnt; s += 8) {  // eight loads in flight
+            float4 v[8];
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                w[i] = __shfl_sync(0xffffffffu, f, (s + i) & 31);
+                if (s + i >= cnt) w[i] = 0.0f;
+                v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (act && w[i] != 0.0f) v[i] = __ldcs(reinterpret_cast<const float4*>(src + (int64_t)(s + i) * n * hd));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                acc[0] += w[i] * v[i].x;
+                acc[1] += w[i] * v[i].y;
+                acc[2] += w[i] * v[i].z;
+                acc[3] += w[i] * v[i].w;
+            }
         }
     }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (!act) return;
     const float inv = 1.0f / sum;
     uint2 w;
     w.x = sum != 0.0f ? h2(acc[0] * inv, acc[1] * inv) : 0u;
     w.y = sum != 0.0f ? h2(acc[2] * inv, acc[3] * inv) : 0u;
-    *reinterpret_cast<uint2*>(out + row * ldo + (id - row * heads) * hd + d0) = w;
+    *reinterpret_cast<uint2*>(out + row * ldo + (id - row * heads) * hd + lane * 4) = w;
 }
 
 template <int HD>
@@ -399,7 +419,7 @@ int launch(const Params& p, int batch, cudaStream_t st) {
 
 }  // namespace pdec
 
-int paged_decode(const PackedArgs& a, int first, int chunk, int splits, int split0, cudaStream_t st) {
+int paged_decode(const PackedArgs& a, cudaStream_t st) {
     using namespace pdec;
     Params p;
     memset(&p, 0, sizeof(p));
@@ -424,10 +444,10 @@ int paged_decode(const PackedArgs& a, int first, int chunk, int splits, int spli
     p.group = a.heads / a.kv_heads;
     p.head_dim = a.head_dim;
     p.causal = a.causal ? 1 : 0;
-    p.first = first;
-    p.chunk = chunk;
-    p.splits = splits;
-    p.split0 = split0;
+    p.first = a.first;
+    p.splits = a.part_o ? a.splits : 1;
+    p.split0 = a.split0;
+    p.beside = a.first > 0;
     p.c = a.scale * 1.4426950408889634f;
     p.out = reinterpret_cast<__half*>(a.out);
     p.ldo = a.ldo;
