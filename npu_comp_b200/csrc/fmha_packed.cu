@@ -89,10 +89,12 @@ struct Item {
     int kv_row0;     // packed K/V: first row of the sequence
     int seq, kvh, split;
     int off;         // row i sees keys <= off + i
-    int k0, kend;    // keys of this item
+    int kb[2];       // first key of each tile's range
+    int ke[2];       // its end
     int n[2];        // key blocks of each tile
     int steps[2];    // 16-key steps of its last block
     int vfix;        // keys of the last block when V rows behind them need zeroing, else 0
+    int vfix_q;      // its tile (two ranges)
     int state;       // 1: an item, 0: the last one is behind
 };
 constexpr int kItemSlots = 2;  // the scheduler works one item ahead
@@ -126,13 +128,39 @@ __device__ __forceinline__ int tiles_from(const Params& p, int ntok, int klen, i
     return nt - (int)((uint32_t)first / (uint32_t)span);
 }
 
+// Key blocks of the item's keys [k0, kend): the same for both tiles, or (DUAL)
+// one half for each, and what the last ones need.  lim[q]: keys that some row
+// of tile q may see end here; used[q]: the tile has rows.
+template <bool DUAL>
+__device__ __forceinline__ void cut_item(Item& it, int k0, int kend, const int (&lim)[2], const bool (&used)[2]) {
+    const int mid = DUAL ? min(kend, k0 + ((kend - k0 + kBlk - 1) / kBlk + 1) / 2 * kBlk) : kend;
+    it.vfix = it.vfix_q = 0;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        it.kb[q] = DUAL && q ? mid : k0;
+        it.ke[q] = DUAL && !q ? mid : kend;
+        const int end = min(lim[q], it.ke[q]);
+        it.n[q] = used[q] && end > it.kb[q] ? (end - it.kb[q] + kBlk - 1) / kBlk : 0;
+        it.steps[q] = min(kBlk / 16, (end - it.kb[q] - (it.n[q] - 1) * kBlk + 15) >> 4);
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int nb = DUAL ? it.n[q] : max(it.n[0], it.n[1]);
+        const int vb = it.ke[q] - it.kb[q] - (nb - 1) * kBlk;  // > 128: the causal limit ends the range earlier
+        if (nb > 0 && vb < kBlk && (vb & 15)) {
+            it.vfix = vb;
+            it.vfix_q = q;
+        }
+    }
+}
+
 // Item number -> rows and keys, by the scheduler warp.  Tiles are numbered
 // from the most expensive down (p.sorted), so that the CTAs, which take items
 // round by round in alternating direction, end together: a bisection over the
 // key level whose tile count brackets the number, each step a sum over the
 // sequences (32 per warp step), then a scan for the sequence.  Without
 // p.sorted (no CTA has a second item) the scan alone.
-template <bool PAGED>
+template <bool PAGED, bool DUAL>
 __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
     const int lane = threadIdx.x & 31;
     it.split = idx % p.splits;
@@ -148,12 +176,10 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
         it.kv_row0 = 0;
         it.off = p.shared;  // no causal limit; each row has its own
         const int per = ((p.shared + kBlk - 1) / kBlk + p.splits - 1) / p.splits * kBlk;
-        it.k0 = min(p.shared, it.split * per);
-        it.kend = min(p.shared, it.k0 + per);
+        const int k0 = min(p.shared, it.split * per);
         if (it.tok0 >= it.ntok) return false;
-        const int nb = it.kend > it.k0 ? (it.kend - it.k0 + kBlk - 1) / kBlk : 0;
-        it.n[0] = nb;
-        it.n[1] = (p.tiles == 2 && it.tok0 + p.tpt < it.ntok) ? nb : 0;
+        cut_item<DUAL>(it, k0, min(p.shared, k0 + per), {p.shared, p.shared},
+                       {true, DUAL || (p.tiles == 2 && it.tok0 + p.tpt < it.ntok)});
         return true;
     }
     int level = 0;
@@ -222,28 +248,12 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
     it.off = p.causal ? klen - it.ntok : klen;
     // every sequence's own keys in p.splits equal ranges of whole blocks
     const int per = ((max(0, klen - p.first) + kBlk - 1) / kBlk + p.splits - 1) / p.splits * kBlk;
-    it.k0 = min(klen, p.first + it.split * per);
-    it.kend = it.split == p.splits - 1 ? klen : min(klen, it.k0 + per);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int t0 = it.tok0 + q * p.tpt, t1 = min(it.ntok, t0 + p.tpt);
-        const int lim = min(it.kend, p.causal ? it.off + t1 : klen);
-        it.n[q] = (q < p.tiles && t0 < it.ntok && lim > it.k0) ? (lim - it.k0 + kBlk - 1) / kBlk : 0;
-    }
+    const int k0 = min(klen, p.first + it.split * per);
+    const int t0 = it.tok0 + (DUAL ? 0 : p.tpt), t1 = min(it.ntok, it.tok0 + p.tpt), t2 = min(it.ntok, t0 + p.tpt);
+    cut_item<DUAL>(it, k0, it.split == p.splits - 1 ? klen : min(klen, k0 + per),
+                   {p.causal ? it.off + t1 : klen, p.causal ? it.off + t2 : klen},
+                   {true, DUAL || (p.tiles == 2 && t0 < it.ntok)});
     return true;
-}
-
-// The last block of each tile and of the item.
-__device__ __forceinline__ void finish_item(const Params& p, Item& it) {
-    const int nblk = max(it.n[0], it.n[1]);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int t1 = min(it.ntok, it.tok0 + (q + 1) * p.tpt);
-        const int lim = (p.causal && p.shared == 0) ? min(it.kend, it.off + t1) : it.kend;
-        it.steps[q] = min(kBlk / 16, (lim - it.k0 - (it.n[q] - 1) * kBlk + 15) >> 4);
-    }
-    const int vb = it.kend - it.k0 - (nblk - 1) * kBlk;  // > 128: the causal limit ends the item ahead of kend
-    it.vfix = nblk > 0 && vb < kBlk && (vb & 15) ? vb : 0;
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -434,7 +444,10 @@ __device__ __forceinline__ bool next_item(const Item* slots, uint64_t* full, uin
     return it.state != 0;
 }
 
-template <int HD, bool PAGED, bool PART>
+// DUAL (partials only): the two tiles are the same rows on the two halves of the
+// item's keys, for items whose rows fill one tile: two chains of products and
+// softmax keep a CTA's loads going where one would wait for itself.
+template <int HD, bool PAGED, bool PART, bool DUAL>
 __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_constant__ Params p) {
     using L = Smem<HD>;
     // A shared-prefix phase lets its successor start only behind its own wait: the successor (paged_decode on the
@@ -461,8 +474,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
     uint64_t* it_full = kv_empty + L::kStages;  // [kItemSlots]
     uint64_t* it_empty = it_full + kItemSlots;  // [kItemSlots]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(it_empty + kItemSlots);
+    volatile uint32_t* vfix_stage = tmem_slot + 2;
     Item* slots = reinterpret_cast<Item*>(smem + L::kOffItem);
-    static_assert(kItemSlots * sizeof(Item) <= 256 && (13 + 2 * L::kStages + 2 * kItemSlots) * 8 + 8 <= 320, "layout");
+    static_assert(kItemSlots * sizeof(Item) <= 256 && (13 + 2 * L::kStages + 2 * kItemSlots) * 8 + 12 <= 320, "layout");
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -520,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 if (nblk == 0) continue;
                 ok = wait_all(q_empty, (nz & 1u) ^ 1u, abort_flag);
                 if (!ok) break;
-                const int nq = it.n[1] > 0 ? 2 : 1;
+                const int nq = !DUAL && it.n[1] > 0 ? 2 : 1;
                 if (lane == 0) {
                     const uint32_t bytes = (uint32_t)(p.group * p.tpt) * 128u * L::kChunks;
                     mbar_arrive_expect_tx(q_full, bytes * nq);
@@ -530,22 +544,26 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                                         it.kvh * p.group, it.q_row0 + it.tok0 + q * p.tpt);
                 }
                 ++nz;
-                for (int j = 0; j < nblk && ok; ++j) {
-                    int box = lane / L::kChunks, ch = lane % L::kChunks, c2 = 0, c3 = 0;
-                    const int key = it.k0 + j * kBlk;
-                    if (PAGED) {
-                        // lane -> (page piece, 64-column chunk); past the keys: a page outside the pool, which
-                        // the copy fills with zeros
-                        const int kk = key + box * p.box_rows;
-                        c3 = p.n_pages;
-                        if (box < nbox && kk < it.kend) {
-                            const int id = __ldg(p.table + (int64_t)it.seq * p.ldt + (kk >> p.page_shift));
-                            if (id >= 0 && id < p.n_pages) c3 = id;
-                        }
-                        c2 = kk & ((1 << p.page_shift) - 1);
-                    }
+                // in the order of their use: V of block j - 1, K of block j (of both ranges in turn)
+                const int box = lane / L::kChunks, ch = lane % L::kChunks;
+                for (int j = 0; j <= nblk && ok; ++j) {
 #pragma unroll
-                    for (int kv = 0; kv < 2; ++kv, ++n) {
+                    for (int u = 0; u < (DUAL ? 4 : 2); ++u) {
+                        const int q = u >> 1, kv = 1 - (u & 1), jb = j - kv;
+                        if (jb < 0 || jb >= (DUAL ? it.n[q] : nblk)) continue;
+                        const int key = it.kb[q] + jb * kBlk;
+                        int c2 = 0, c3 = 0;
+                        if (PAGED) {
+                            // lane -> (page piece, 64-column chunk); past the keys: a page outside the pool, which
+                            // the copy fills with zeros
+                            const int kk = key + box * p.box_rows;
+                            c3 = p.n_pages;
+                            if (box < nbox && kk < it.ke[q]) {
+                                const int id = __ldg(p.table + (int64_t)it.seq * p.ldt + (kk >> p.page_shift));
+                                if (id >= 0 && id < p.n_pages) c3 = id;
+                            }
+                            c2 = kk & ((1 << p.page_shift) - 1);
+                        }
                         const uint32_t s = n % L::kStages, ph = (n / L::kStages) & 1u;
                         ok = wait_all(&kv_empty[s], ph ^ 1u, abort_flag);
                         if (!ok) break;
@@ -560,6 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                                 tma_load_3d(dst, kv ? &p.tmV : &p.tmK, &kv_full[s], ch * 64, it.kvh,
                                             it.kv_row0 + key);
                         }
+                        ++n;
                     }
                 }
             }
@@ -589,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                     if (!ok) break;
                     const Item& it = slots[slot];
                     const int n0 = it.n[0], n1 = it.n[1], state = it.state;
-                    const int last0 = it.steps[0], last1 = it.steps[1], vfix = it.vfix;
+                    const int last0 = it.steps[0], last1 = it.steps[1], vfix = it.vfix, vfix_q = it.vfix_q;
                     mbar_arrive(&it_empty[slot]);
                     ++ni;
                     if (!state) break;
@@ -598,29 +617,25 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                     ok = wait_one(q_full, nz & 1u, abort_flag);
                     ++nz;
                     for (int j = 0; ok && j <= nblk; ++j) {
-                        // this step's tiles of the ring: V_{j-1}, then K_j
-                        const uint32_t vs = st;
-                        if (j >= 1) {
-                            ok = wait_one(&kv_full[st], ph, abort_flag);
-                            if (ok && vfix && j == nblk) {  // warp 11's turn; P of this block takes longer
-                                mbar_arrive(v_seen);
-                                ok = wait_one(v_fixed, nv++ & 1u, abort_flag);
-                            }
-                            if (++st == L::kStages) st = 0, ph ^= 1u;
-                        }
-                        const uint32_t ks = st;
-                        if (ok && j < nblk) {
-                            ok = wait_one(&kv_full[st], ph, abort_flag);
-                            if (++st == L::kStages) st = 0, ph ^= 1u;
-                        }
-                        if (!ok) break;
-                        const uint64_t vd = vd0 + (uint64_t)(vs * (L::kTile >> 4));
-                        const uint64_t kd = kd0 + (uint64_t)(ks * (L::kTile >> 4));
+                        uint32_t vs = 0, ks = 0;
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
-                            const int n = q ? n1 : n0;
+                            const int n = q ? n1 : n0, nkv = DUAL ? n : nblk;
                             const uint32_t sq = tmem + (uint32_t)(q * 128), oq = tmem + 256u + (uint32_t)(q * 128);
+                            const bool mine = DUAL || q == 0;  // this tile takes the next K and V off the ring
+                            if (mine && j >= 1 && j <= nkv) {  // V_{j-1}
+                                vs = st;
+                                ok = wait_one(&kv_full[st], ph, abort_flag);
+                                if (++st == L::kStages) st = 0, ph ^= 1u;
+                                if (ok && vfix && j == nkv && (!DUAL || q == vfix_q)) {  // warp 11's turn; P takes longer
+                                    *vfix_stage = vs;
+                                    mbar_arrive(v_seen);
+                                    ok = wait_one(v_fixed, nv++ & 1u, abort_flag);
+                                }
+                                if (!ok) break;
+                            }
                             if (j >= 1 && j <= n) {  // O_q += P_q(j-1) V_{j-1}
+                                const uint64_t vd = vd0 + (uint64_t)(vs * (L::kTile >> 4));
                                 const int steps = j < n ? kBlk / 16 : (q ? last1 : last0);
 #pragma unroll
                                 for (int hf = 0; hf < 2; ++hf) {  // the first 64 keys' P is ready ahead of the rest
@@ -642,20 +657,31 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                                 if (!ok) break;
                                 ++np[q];
                                 if (j == n) tc_commit(&o_full[q]);
+                                if (DUAL) tc_commit(&kv_empty[vs]);
+                            }
+                            if (mine && j < nkv) {  // K_j
+                                ks = st;
+                                ok = wait_one(&kv_full[st], ph, abort_flag);
+                                if (++st == L::kStages) st = 0, ph ^= 1u;
+                                if (!ok) break;
                             }
                             if (j < n) {  // S_q(j) = Q_q K_j^T
-                                const uint64_t qd = qd0 + (uint64_t)(q * (L::kTile >> 4));
+                                const uint64_t kd = kd0 + (uint64_t)(ks * (L::kTile >> 4));
+                                const uint64_t qd = qd0 + (uint64_t)((DUAL ? 0 : q) * (L::kTile >> 4));
 #pragma unroll
                                 for (int kk = 0; kk < HD / 16; ++kk) {
                                     const uint64_t o = (uint64_t)(((kk >> 2) * L::kChunk + (kk & 3) * 32) >> 4);
                                     tc_mma_f16(sq, qd + o, kd + o, idesc_s, kk > 0 ? 1u : 0u);
                                 }
                                 tc_commit(&s_full[q]);
+                                if (DUAL) tc_commit(&kv_empty[ks]);
                             }
                         }
                         if (!ok) break;
-                        if (j >= 1) tc_commit(&kv_empty[vs]);
-                        if (j < nblk) tc_commit(&kv_empty[ks]);
+                        if (!DUAL) {
+                            if (j >= 1) tc_commit(&kv_empty[vs]);
+                            if (j < nblk) tc_commit(&kv_empty[ks]);
+                        }
                         if (j == nblk - 1) tc_commit(q_empty);
                     }
                 }
@@ -669,26 +695,22 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             __syncwarp();
         } else if (warp == 11) {
             // ------------------------------------------------------------ V rows behind the last key
-            uint32_t base = 0, ni = 0, nv = 0;
+            uint32_t ni = 0, nv = 0;
             bool ok = true;
             Item it;
             while (ok && next_item(slots, it_full, it_empty, ni, it, abort_flag, ok)) {
-                const int nblk = max(it.n[0], it.n[1]);
-                if (it.vfix) {  // zeroed up to the end of the last 16-key step
-                    const uint32_t vs = (base + 2 * nblk - 1) % L::kStages;
-                    ok = wait_all(v_seen, nv++ & 1u, abort_flag);  // the MMA thread has seen the tile land
-                    if (!ok) break;
-                    const int vb = it.vfix, n16 = (16 - (vb & 15)) * 8;
-                    for (int i = lane; i < n16 * L::kChunks; i += 32) {
-                        const int ch = i / n16, e = i - ch * n16;
-                        *reinterpret_cast<uint4*>(smem + L::kOffRing + vs * L::kTile + ch * L::kChunk + vb * 128 +
-                                                  e * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(v_fixed);
+                if (!it.vfix) continue;
+                ok = wait_all(v_seen, nv++ & 1u, abort_flag);  // the MMA thread has seen the tile land
+                if (!ok) break;
+                uint8_t* v = smem + L::kOffRing + *vfix_stage * L::kTile;
+                const int vb = it.vfix, n16 = (16 - (vb & 15)) * 8;  // zeroed up to the end of the last 16-key step
+                for (int i = lane; i < n16 * L::kChunks; i += 32) {
+                    const int ch = i / n16, e = i - ch * n16;
+                    *reinterpret_cast<uint4*>(v + ch * L::kChunk + vb * 128 + e * 16) = make_uint4(0, 0, 0, 0);
                 }
-                base += 2 * nblk;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_fixed);
             }
         } else if (warp == 10) {
             // ------------------------------------------------------------ scheduler
@@ -699,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 const int64_t idx = base + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
                 Item it;
                 it.state = base < p.n_items ? 1 : 0;
-                if (it.state && (idx >= p.n_items || !get_item<PAGED>(p, (int)idx, it))) continue;
+                if (it.state && (idx >= p.n_items || !get_item<PAGED, DUAL>(p, (int)idx, it))) continue;
                 const uint32_t s = k % kItemSlots;
                 ok = wait_all(&it_empty[s], ((k / kItemSlots) & 1u) ^ 1u, abort_flag);
                 if (!ok) {
@@ -709,7 +731,6 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                     }
                     break;
                 }
-                finish_item(p, it);
                 if (lane == 0) {
                     slots[s] = it;
                     mbar_arrive(&it_full[s]);
@@ -731,9 +752,10 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
         bool ok = true;
         Item it;
         while (ok && next_item(slots, it_full, it_empty, ni, it, abort_flag, ok)) {
-            const int tok = it.tok0 + q * p.tpt + tl;
-            const bool valid = q < p.tiles && tl < p.tpt && tok < it.ntok;
-            int lim = it.kend;  // this row's keys end here
+            const int tok = it.tok0 + (DUAL ? 0 : q * p.tpt) + tl;
+            const bool valid = (DUAL || q < p.tiles) && tl < p.tpt && tok < it.ntok;
+            const int kb = q ? it.kb[1] : it.kb[0];
+            int lim = q ? it.ke[1] : it.ke[0];  // this row's keys end here
             if (valid) {
                 if (PAGED && p.shared > 0) lim = min(lim, __ldg(p.lens + tok));
                 else if (p.causal) lim = min(lim, it.off + tok + 1);
@@ -747,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 tc_fence_after();
                 float x[128];
                 tmem_ld128(sq, x);
-                const int left = lim - (it.k0 + j * kBlk);
+                const int left = lim - (kb + j * kBlk);
                 if (__any_sync(0xffffffffu, left < kBlk)) {
 #pragma unroll
                     for (int e = 0; e < 128; ++e) x[e] = e < left ? x[e] : -INFINITY;
@@ -810,7 +832,8 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             const int64_t row = (int64_t)it.q_row0 + tok;
             const int head = it.kvh * p.group + g;
             const bool none = m == -INFINITY;  // no key: zeros (no partial)
-            const int64_t at = PART ? ((int64_t)(p.split0 + it.split) * p.total_q + row) * p.heads + head : 0;
+            const int sp = p.split0 + (DUAL ? 2 * it.split + q : it.split);
+            const int64_t at = PART ? ((int64_t)sp * p.total_q + row) * p.heads + head : 0;
             if (PART && valid) p.part_ml[at] = none ? make_float2(-INFINITY, 0.0f) : make_float2(m * c, l);
             const bool put = valid && !(PART && none);
             const float inv = none ? 0.0f : 1.0f / l;
@@ -864,9 +887,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
     }
 }
 
-template <int HD, bool PAGED, bool PART>
+template <int HD, bool PAGED, bool PART, bool DUAL = false>
 int launch(const Params& p, int grid, cudaStream_t st) {
-    auto kern = fmha_packed_kernel<HD, PAGED, PART>;
+    auto kern = fmha_packed_kernel<HD, PAGED, PART, DUAL>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::kTotal);
     if (e != cudaSuccess) {
         npub_internal_set_cuda_error(e);
@@ -936,10 +959,12 @@ int fmha_packed(const PackedArgs& a, cudaStream_t st) {
     p.splits = part ? a.splits : 1;
     p.first = a.first;
     p.split0 = a.split0;
-    // One tile per CTA while that still leaves SMs free.
     const int batch = a.shared > 0 ? 1 : a.batch;
-    const int64_t one = fmha_packed_items(a.total_q, batch, a.heads, a.kv_heads, a.max_new, 1);
-    p.tiles = one * a.kv_heads * p.splits <= num_sms() ? 1 : 2;
+    p.tiles = a.tiles;
+    if (p.tiles == 0) {  // one tile per CTA while that still leaves SMs free
+        const int64_t one = fmha_packed_items(a.total_q, batch, a.heads, a.kv_heads, a.max_new, 1);
+        p.tiles = one * a.kv_heads <= num_sms() ? 1 : 2;
+    }
     const int64_t items = fmha_packed_items(a.total_q, batch, a.heads, a.kv_heads, a.max_new, p.tiles) * a.kv_heads *
                           p.splits;
     if (items > 0x7fffffff) return NPUB_ERR_UNSUPPORTED;
@@ -950,6 +975,7 @@ int fmha_packed(const PackedArgs& a, cudaStream_t st) {
     const bool small = a.head_dim <= 64;
     if (part) {
         if (!paged) return NPUB_ERR_UNSUPPORTED;
+        if (a.dual) return small ? launch<64, true, true, true>(p, grid, st) : launch<128, true, true, true>(p, grid, st);
         return small ? launch<64, true, true>(p, grid, st) : launch<128, true, true>(p, grid, st);
     }
     if (paged) return small ? launch<64, true, false>(p, grid, st) : launch<128, true, false>(p, grid, st);

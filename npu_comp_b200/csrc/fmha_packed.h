@@ -32,6 +32,8 @@ struct PackedArgs {
     float scale;
     int causal;
     // splits > 1 (or shared): fp32 partials instead of out
+    int tiles;            // row tiles of an item: 1, 2, or 0 (chosen by the number of items)
+    int dual;             // partials, tiles == 1: an item's keys in two halves, two partials for each split
     int splits;           // equal ranges of every sequence's keys from `first` on
     int first, split0;    // split0: index of split 0 among the partials
     float* part_o;        // [splits, total_q, heads, head_dim]

@@ -33,31 +33,55 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How the keys of a call are cut.  The partials are numbered through: the shared prefix's splits, then those of the
 // sequences' own keys.  The last split of either takes every key that is left, so ctx_len only decides the cut.
+struct Phase {
+    int tiles, dual;  // tile kernel: rows of an item, and whether its keys go in two halves
+    int splits;
+    int partials() const { return splits * (dual ? 2 : 1); }
+};
 struct Plan {
-    bool few;                     // own keys on paged_decode (else on the tiles)
-    int shared;                   // keys of the shared prefix phase (0: none)
-    int pre_splits, own_splits;
-    bool part() const { return pre_splits + own_splits > 1; }
-    int total() const { return pre_splits + own_splits; }
+    bool few;    // own keys on paged_decode (else on the tiles)
+    int shared;  // keys of the shared prefix phase (0: none)
+    Phase pre, own;
+    int total() const { return (shared > 0 ? pre.partials() : 0) + own.partials(); }
+    bool part() const { return total() > 1; }
 };
 
 // Number of key ranges for `items` work items of up to `keys` keys on `slots` resident CTAs: the s that makes
-// waves * (start + key units of a range * per unit) + combination smallest, times in us.  `part_us`: what the partials
-// of one more split cost (written, read), `fixed`: a combination pass runs anyway.
+// waves * (start + key units of a range * per unit) + combination smallest, times in us.  `part_us`: what one more
+// split's partials cost (written, read), `per`: partials of a range, `fixed`: a combination pass runs anyway.
 int pick_splits(int64_t keys, int64_t items, int64_t slots, int unit, double start, double per_unit, double part_us,
-                bool fixed) {
+                int per, bool fixed, double* us) {
     const int64_t units = ceil_div(keys > 0 ? keys : 1, unit);
-    double best = 0.0;
     int pick = 1;
     for (int s = 1; s <= 64 && s <= units; ++s) {
-        const double t = (double)ceil_div(items * s, slots) * (start + (double)ceil_div(units, s) * per_unit) +
-                         (s > 1 || fixed ? s * (part_us + 0.15) : 0.0) + (s > 1 && !fixed ? 4.0 : 0.0);
-        if (s == 1 || t < 0.95 * best) {
-            best = t;
+        const double unit_us = items * s <= slots / 2 ? 0.6 * per_unit : per_unit;  // few CTAs: bandwidth to spare
+        const bool part = s * per > 1;
+        const double t = (double)ceil_div(items * s, slots) * (start + (double)ceil_div(units, s) * unit_us) +
+                         (part || fixed ? s * per * (part_us + 0.15) : 0.0) + (part && !fixed ? 4.0 : 0.0);
+        if (s == 1 || t < 0.95 * *us) {
+            *us = t;
             pick = s;
         }
     }
     return pick;
+}
+
+// A phase on the tile kernel: pairs of tiles (1.5 us per 128 keys of a pair, 4 us to start and end), or, where the rows
+// fill one tile, one tile on two halves of the keys (1.5 us per 256 keys).
+Phase tile_phase(int total, int batch, int heads, int kv_heads, int max_new, int64_t keys, double part_us, bool fixed) {
+    const int64_t sms = num_sms();
+    const int64_t one = fmha_packed_items(total, batch, heads, kv_heads, max_new, 1) * kv_heads;
+    const int64_t two = fmha_packed_items(total, batch, heads, kv_heads, max_new, 2) * kv_heads;
+    Phase a = {}, b = {};
+    double ua, ub;
+    a.tiles = 2;
+    a.splits = pick_splits(keys, two, sms, 128, 4.0, 1.5, part_us, 1, fixed, &ua);
+    b.tiles = 1;
+    b.dual = 1;
+    b.splits = pick_splits(keys, one, sms, 256, 4.0, 1.5, part_us, 2, fixed, &ub);
+    if (ub < ua) return b;
+    if (a.splits == 1) a.tiles = 0;
+    return a;
 }
 
 Plan make_plan(int batch, int total, int max_new, int64_t ctx, int shared, int heads, int kv_heads, int head_dim) {
@@ -66,20 +90,16 @@ Plan make_plan(int batch, int total, int max_new, int64_t ctx, int shared, int h
     pl.few = max_new > 0 && (int64_t)max_new * group <= kPagedDecodeRows && batch <= 65535;
     if (batch < 2) shared = 0;  // nothing to share
     pl.shared = shared;
-    // Measured: a pair of tiles takes 1.5 us per 128 keys and 4 us to start and end; a few-row CTA, two of which share
-    // an SM, takes 1.5 us per 64 keys of 128 columns and 2.5 us; partials move at about 4 TB/s (they stay in L2).
-    const double part_us = (double)total * heads * head_dim * 8.0 / 4e6;
-    if (shared > 0) {
-        const int64_t tiles = fmha_packed_items(total, 1, heads, kv_heads, 0, 2) * kv_heads;
-        pl.pre_splits = pick_splits(shared, tiles, sms, 128, 4.0, 1.5, part_us, true);
-    }
+    const double part_us = (double)total * heads * head_dim * 8.0 / 4e6;  // about 4 TB/s: they stay in L2
+    if (shared > 0) pl.pre = tile_phase(total, 1, heads, kv_heads, 0, shared, part_us, true);
     const int64_t own = ctx > shared ? ctx - shared : 1;
     if (pl.few) {
-        const int64_t items = (int64_t)batch * kv_heads;
-        pl.own_splits = pick_splits(own, items, 2 * sms, 64, 2.5, head_dim > 64 ? 1.5 : 0.8, part_us, shared > 0);
+        // a few-row CTA, two of which share an SM, takes 1.5 us per 64 keys of 128 columns and 2.5 us
+        double us;
+        pl.own.splits = pick_splits(own, (int64_t)batch * kv_heads, 2 * sms, 64, 2.5, head_dim > 64 ? 1.5 : 0.8,
+                                    part_us, 1, shared > 0, &us);
     } else {
-        const int64_t tiles = fmha_packed_items(total, batch, heads, kv_heads, max_new, 2) * kv_heads;
-        pl.own_splits = pick_splits(own, tiles, sms, 128, 4.0, 1.5, part_us, shared > 0);
+        pl.own = tile_phase(total, batch, heads, kv_heads, max_new, own, part_us, shared > 0);
     }
     return pl;
 }
@@ -105,13 +125,17 @@ int run_plan(const Plan& pl, PackedArgs& a, void* workspace, size_t workspace_by
         s.causal = 0;
         s.cu = nullptr;
         s.max_new = 0;
-        s.splits = pl.pre_splits;
+        s.splits = pl.pre.splits;
+        s.tiles = pl.pre.tiles;
+        s.dual = pl.pre.dual;
         const int rc = fmha_packed(s, st);
         if (rc) return rc;
     }
     a.first = pl.shared;
-    a.splits = pl.own_splits;
-    a.split0 = pl.pre_splits;
+    a.splits = pl.own.splits;
+    a.tiles = pl.own.tiles;
+    a.dual = pl.own.dual;
+    a.split0 = pl.shared > 0 ? pl.pre.partials() : 0;
     const int rc = pl.few ? paged_decode(a, st) : fmha_packed(a, st);
     if (rc || !need) return rc;
     return paged_combine(a, pl.total(), st);

@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     const int R = nrow * p.group;
     const int len = max(0, min(p.lens[b], p.max_keys));
     const int own = max(0, len - p.first);
-    const int per = ((own + kKeys - 1) / kKeys + p.splits - 1) / p.splits * kKeys;  // whole stages
+    // whole stages, at least 256 keys: what a short sequence does not fill ends at once
+    const int per = max(4, ((own + kKeys - 1) / kKeys + p.splits - 1) / p.splits) * kKeys;
     const int k0 = R == 0 ? 0 : p.first + min(own, split * per);
     const int k1 = R == 0 ? 0 : p.first + min(own, split * per + per);
     const int nst = (k1 - k0 + kKeys - 1) / kKeys;
