@@ -128,9 +128,27 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Call an npub_* function and raise on a non-zero status."""
-    lib = load()
-    st = getattr(lib, name)(*args)
+    st = getattr(load(), name)(*args)
     if st != NPUB_OK:
+        fail(name, st)
+
+
+_bound = {}
+
+
+def bound(name: str):
+    """The npub_* function itself, for callers that check its status with
+    fail(): without the lock and the attribute lookup of every call()."""
+    f = _bound.get(name)
+    if f is None or _lib is None:
+        f = _bound[name] = getattr(load(), name)
+    return f
+
+
+def fail(name: str, st: int) -> None:
+    """Raise for a non-zero status of an npub_* function."""
+    if st != NPUB_OK:
+        lib = load()
         text = lib.npub_strerror(st).decode()
         if st == NPUB_ERR_CUDA:
             text += f" (cudaError {lib.npub_last_cuda_error()})"

@@ -73,6 +73,7 @@ struct Params {
     int64_t ldt;
     int max_keys, page_shift, box_rows, n_pages;
     int total_q, batch, heads, kv_heads, group, tpt, head_dim;
+    uint32_t span_inv;  // ceil(2^32 / (tiles * tpt))
     int tiles, n_items, sorted, levels, splits, first, split0, shared, causal;
     float c;  // scale * log2(e)
     __half* out;
@@ -106,8 +107,17 @@ __device__ __forceinline__ void set_err(int* err, int code) {
 // Rows of sequence s0 + lane, [r0, r1), and its keys.  Reads cu and lens as
 // they are: whatever they hold, rows stay inside [0, total_q) and keys inside
 // the table.
+struct SeqRows {
+    int r0, r1, klen;
+};
 template <bool PAGED>
-__device__ __forceinline__ void seq_rows(const Params& p, int b, int& r0, int& r1, int& klen) {
+__device__ __forceinline__ void seq_rows(const Params& p, int b, const SeqRows& near, int& r0, int& r1, int& klen) {
+    if (b < 32) {  // the lane's own, loaded once
+        r0 = near.r0;
+        r1 = near.r1;
+        klen = near.klen;
+        return;
+    }
     r0 = r1 = klen = 0;
     if (b >= p.batch) return;
     r0 = p.cu ? max(0, min(p.total_q, __ldg(p.cu + b))) : b;
@@ -125,7 +135,9 @@ __device__ __forceinline__ int tiles_from(const Params& p, int ntok, int klen, i
     const int64_t first = (int64_t)level * kBlk - (klen - ntok);  // rows behind this one reach the level
     if (first <= 0) return nt;
     if (first >= ntok) return 0;
-    return nt - (int)((uint32_t)first / (uint32_t)span);
+    uint32_t t = __umulhi((uint32_t)first, p.span_inv);  // first / span, at most one too large
+    t -= t * (uint32_t)span > (uint32_t)first ? 1u : 0u;
+    return nt - (int)t;
 }
 
 // Key blocks of the item's keys [k0, kend): the same for both tiles, or (DUAL)
@@ -161,7 +173,7 @@ __device__ __forceinline__ void cut_item(Item& it, int k0, int kend, const int (
 // sequences (32 per warp step), then a scan for the sequence.  Without
 // p.sorted (no CTA has a second item) the scan alone.
 template <bool PAGED, bool DUAL>
-__device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
+__device__ __forceinline__ bool get_item(const Params& p, const SeqRows& near, int idx, Item& it) {
     const int lane = threadIdx.x & 31;
     it.split = idx % p.splits;
     idx /= p.splits;
@@ -192,7 +204,7 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
             int sum = 0;
             for (int s0 = 0; s0 < p.batch; s0 += 32) {
                 int r0, r1, kl;
-                seq_rows<PAGED>(p, s0 + lane, r0, r1, kl);
+                seq_rows<PAGED>(p, s0 + lane, near, r0, r1, kl);
                 sum += tiles_from(p, r1 - r0, kl, mid, span);
             }
             sum = __reduce_add_sync(0xffffffffu, sum);
@@ -208,7 +220,7 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
         int above = 0;
         for (int s0 = 0; s0 < p.batch; s0 += 32) {
             int r0, r1, kl;
-            seq_rows<PAGED>(p, s0 + lane, r0, r1, kl);
+            seq_rows<PAGED>(p, s0 + lane, near, r0, r1, kl);
             above += tiles_from(p, r1 - r0, kl, level + 1, span);
         }
         tile -= __reduce_add_sync(0xffffffffu, above);
@@ -216,7 +228,7 @@ __device__ __forceinline__ bool get_item(const Params& p, int idx, Item& it) {
     int b = -1, r0 = 0, r1 = 0, klen = 0;
     for (int s0 = 0; s0 < p.batch; s0 += 32) {
         int c0, c1, kl;
-        seq_rows<PAGED>(p, s0 + lane, c0, c1, kl);
+        seq_rows<PAGED>(p, s0 + lane, near, c0, c1, kl);
         const int all = (c1 - c0 + span - 1) / span;
         const int over = p.sorted ? tiles_from(p, c1 - c0, kl, level + 1, span) : 0;
         const int cnt = (p.sorted ? tiles_from(p, c1 - c0, kl, level, span) : all) - over;
@@ -716,12 +728,18 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             // ------------------------------------------------------------ scheduler
             uint32_t k = 0;
             bool ok = true;
+            SeqRows near = {0, 0, 0};
+            if (lane < p.batch && !(PAGED && p.shared > 0)) {
+                near.r0 = p.cu ? max(0, min(p.total_q, __ldg(p.cu + lane))) : lane;
+                near.r1 = p.cu ? max(near.r0, min(p.total_q, __ldg(p.cu + lane + 1))) : lane + 1;
+                near.klen = PAGED ? max(0, min(p.max_keys, __ldg(p.lens + lane))) : near.r1 - near.r0;
+            }
             for (int round = 0; ok; ++round) {
                 const int64_t base = (int64_t)round * gridDim.x;
                 const int64_t idx = base + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
                 Item it;
                 it.state = base < p.n_items ? 1 : 0;
-                if (it.state && (idx >= p.n_items || !get_item<PAGED, DUAL>(p, (int)idx, it))) continue;
+                if (it.state && (idx >= p.n_items || !get_item<PAGED, DUAL>(p, near, (int)idx, it))) continue;
                 const uint32_t s = k % kItemSlots;
                 ok = wait_all(&it_empty[s], ((k / kItemSlots) & 1u) ^ 1u, abort_flag);
                 if (!ok) {
@@ -971,6 +989,7 @@ int fmha_packed(const PackedArgs& a, cudaStream_t st) {
     p.n_items = (int)items;
     const int grid = p.n_items < num_sms() ? p.n_items : num_sms();
     p.sorted = p.n_items > grid && a.shared == 0;
+    p.span_inv = (uint32_t)((0x100000000ull + p.tiles * p.tpt - 1) / (p.tiles * p.tpt) - (p.tiles * p.tpt == 1));
     p.levels = (int)(((paged ? (int64_t)p.max_keys : (int64_t)a.total_q) + kBlk - 1) / kBlk);
     const bool small = a.head_dim <= 64;
     if (part) {

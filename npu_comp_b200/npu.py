@@ -568,88 +568,99 @@ def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v
 # These ops run between two launches of a decode step, where 10 us of Python
 # are more than the kernels take: their checks build no message unless they
 # fail, and read the stream's handle without making a Stream object (a decode
-# step's append 30 -> 13 us per call, of which 5 us are the C call).
+# step's append: 30 us per call with the checks of the ops above, HOSTUS so, of
+# which 5 us are the C call).
 
-def _on_own_device(f):
-    """Run the op with its first tensor's device current (its current stream is
-    the one the op runs on)."""
-    @functools.wraps(f)
-    def op(*args, **kw):
-        x = args[0] if args else next(iter(kw.values()), None)
-        d = x.get_device() if isinstance(x, torch.Tensor) else -1
-        if d < 0 or d == torch.cuda.current_device():
-            return f(*args, **kw)
-        with torch.cuda.device(d):
-            return f(*args, **kw)
-    return op
+_Tensor, _f16, _i32 = torch.Tensor, torch.float16, torch.int32
 
 
-def _rows16(t: torch.Tensor, name: str, dev: int) -> int:
-    """_mat() for fp16 rows on device index dev."""
-    if (isinstance(t, torch.Tensor) and t.dtype is torch.float16 and t.dim() == 2 and t.is_cuda
-            and t.get_device() == dev):
-        s0, s1 = t.stride()
-        n, c = t.shape
-        if s1 == 1 or c == 1:
-            return max(s0, c) if n <= 1 else s0
-    ld = _mat(t, name, torch.float16)  # raises, or
-    _need(t.get_device() == dev, f"{name} must be on the same device as the first argument")
-    return ld
+def _launch(name: str, dev: int, *args) -> None:
+    """Call an entry point on device index dev's current stream (the last argument)."""
+    f = _lib.bound(name)
+    if torch._C._cuda_getDevice() == dev:
+        st = f(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            st = f(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail(name, st)
+
+
+def _first16(t: torch.Tensor, name: str):
+    """(device index, rows, columns, leading dimension) of an op's first fp16 matrix."""
+    if isinstance(t, _Tensor) and t.dtype is _f16 and t.is_cuda:
+        s = t.stride()
+        if len(s) == 2:
+            n, c = t.shape
+            if s[1] == 1 or c == 1:
+                return t.get_device(), n, c, s[0] if n > 1 else max(s[0], c)
+    _mat(t, name, torch.float16)  # raises
+    raise ValueError(f"{name} must be a row-major fp16 CUDA matrix")
+
+
+def _rows16(t: torch.Tensor, name: str, dev: int):
+    """(rows, columns, leading dimension) of a further one, on the same device."""
+    d, n, c, ld = _first16(t, name)
+    if d != dev:
+        raise ValueError(f"{name} must be on the same device as the first argument")
+    return n, c, ld
 
 
 def _ints(t: torch.Tensor, name: str, n: int, dev: int) -> int:
-    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.is_cuda and t.get_device() == dev
-            and t.dim() == 1 and t.numel() == n and t.is_contiguous()):
+    if not (isinstance(t, _Tensor) and t.dtype is _i32 and t.get_device() == dev and t.dim() == 1 and t.numel() == n
+            and t.is_contiguous()):
         raise ValueError(f"{name} must be contiguous int32 CUDA [{n}] on the same device as the first argument")
     return t.data_ptr()
 
 
 def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, dev: int):
-    """Validate a paged cache; returns (n_pages, kv_heads, page_size, head_dim, batch, max_pages, ldt)."""
-    for t, nm in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if not (isinstance(t, torch.Tensor) and t.dtype is torch.float16 and t.is_cuda and t.get_device() == dev
-                and t.dim() == 4 and t.is_contiguous()):
-            raise ValueError(f"{nm} must be contiguous fp16 CUDA [n_pages, kv_heads, page_size, head_dim] on the "
-                             "same device as the first argument")
+    """Validate a paged cache; returns ((n_pages, kv_heads, page_size, head_dim), batch, max_pages, ldt)."""
+    if not (isinstance(k_pages, _Tensor) and k_pages.dtype is _f16 and k_pages.get_device() == dev
+            and k_pages.dim() == 4 and k_pages.is_contiguous() and isinstance(v_pages, _Tensor)
+            and v_pages.dtype is _f16 and v_pages.get_device() == dev and v_pages.is_contiguous()):
+        raise ValueError("k_pages and v_pages must be contiguous fp16 CUDA [n_pages, kv_heads, page_size, head_dim] on "
+                         "the same device as the first argument")
     shape = k_pages.shape
     if v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must have the same shape")
-    ldt = _mat(page_table, "page_table", torch.int32) if not (
-        isinstance(page_table, torch.Tensor) and page_table.dtype is torch.int32 and page_table.is_cuda
-        and page_table.is_contiguous() and page_table.dim() == 2) else page_table.shape[1]
-    if page_table.get_device() != dev:
-        raise ValueError("page_table must be on the same device as the first argument")
-    return (*shape, *page_table.shape, ldt)
+    if not (isinstance(page_table, _Tensor) and page_table.dtype is _i32 and page_table.get_device() == dev):
+        raise ValueError("page_table must be int32 CUDA [batch, max_pages] on the same device as the first argument")
+    s = page_table.stride()
+    if len(s) != 2 or (s[1] != 1 and page_table.shape[1] != 1):
+        raise ValueError("page_table must be [batch, max_pages] with unit stride along its last dim")
+    B, W = page_table.shape
+    return shape, B, W, s[0] if B > 1 else max(s[0], W)
 
 
 def _out16(out: Optional[torch.Tensor], like: torch.Tensor, rows: int, cols: int, dev: int):
     """(output [rows, cols], its leading dimension)"""
     if out is None:
         return like.new_empty((rows, cols)), cols
-    ld = _rows16(out, "out", dev)
-    if out.shape[0] != rows or out.shape[1] != cols:
+    n, c, ld = _rows16(out, "out", dev)
+    if n != rows or c != cols:
         raise ValueError(f"out must be [{rows}, {cols}]")
     return out, ld
 
 
 @functools.lru_cache(maxsize=4096)
 def _paged_query(dev: int, name: str, *sizes: int) -> int:
-    return _lib.query(name, *sizes)  # a function of the sizes and the device's SM count
+    with torch.cuda.device(dev):
+        return _lib.query(name, *sizes)  # a function of the sizes and the device's SM count
 
 
-def _paged_workspace(like: torch.Tensor, name: str, *sizes: int):
-    n = _paged_query(like.get_device(), name, *sizes)
+def _paged_workspace(like: torch.Tensor, dev: int, name: str, *sizes: int):
+    """(tensor that holds the workspace or None, its address or None, its size)"""
+    n = _paged_query(dev, name, *sizes)
     if n == 0:
-        return None, 0
+        return None, None, 0
     ws = torch.empty(n, dtype=torch.uint8, device=like.device)
-    return (ws, n) if ws.data_ptr() % 256 == 0 else _workspace(n, like.device)
+    p = ws.data_ptr()
+    if p % 256:
+        ws, _ = _workspace(n, like.device)
+        p = ws.data_ptr()
+    return ws, p, n
 
 
-def _raw_stream(dev: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev)
-
-
-@_on_own_device
 def rope_paged_append(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: int, positions: torch.Tensor,
                       inv_freq: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                       page_table: torch.Tensor, *, cu_seqlens: Optional[torch.Tensor] = None,
@@ -668,35 +679,37 @@ def rope_paged_append(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: 
     rot_dim < head_dim rotates the first rot_dim columns only; interleaved
     pairs columns (2i, 2i + 1) instead of (i, i + rot_dim / 2).  A position
     outside the table, or a page id outside the pool, is rotated but not stored."""
-    dev = qkv.get_device() if isinstance(qkv, torch.Tensor) else -1
-    ldx = _rows16(qkv, "qkv", dev)
-    T = qkv.shape[0]
+    dev, T, cols, ldx = _first16(qkv, "qkv")
     R = head_dim if rot_dim is None else int(rot_dim)
-    if qkv.shape[1] < (q_heads + 2 * kv_heads) * head_dim:
+    if cols < (q_heads + 2 * kv_heads) * head_dim:
         raise ValueError("qkv has too few columns")
-    n_pages, kvh, ps, hd, B, W, ldt = _pool(k_pages, v_pages, page_table, dev)
+    (n_pages, kvh, ps, hd), B, W, ldt = _pool(k_pages, v_pages, page_table, dev)
     if kvh != kv_heads or hd != head_dim:
         raise ValueError("the pages' kv_heads and head_dim must match")
     pos = _ints(positions, "positions", T, dev)
-    if not (inv_freq.dtype is torch.float32 and inv_freq.get_device() == dev and inv_freq.is_contiguous()
-            and inv_freq.numel() * 2 == R):
+    if not (isinstance(inv_freq, _Tensor) and inv_freq.dtype is torch.float32 and inv_freq.get_device() == dev
+            and inv_freq.is_contiguous() and inv_freq.numel() * 2 == R):
         raise ValueError("inv_freq must be contiguous fp32 CUDA [rot_dim/2]")
-    for g in (q_gamma, k_gamma):
-        if g is not None and not (g.dtype is torch.float16 and g.get_device() == dev and g.numel() == head_dim
-                                  and g.is_contiguous()):
-            raise ValueError("q_gamma and k_gamma must be contiguous fp16 CUDA tensors of head_dim elements")
-    if cu_seqlens is None and B != T:
-        raise ValueError("without cu_seqlens the table needs one row per token")
-    cu = None if cu_seqlens is None else _ints(cu_seqlens, "cu_seqlens", B + 1, dev)
+    gq = gk = None
+    if q_gamma is not None or k_gamma is not None:
+        for g in (q_gamma, k_gamma):
+            if g is not None and not (isinstance(g, _Tensor) and g.dtype is _f16 and g.get_device() == dev
+                                      and g.numel() == head_dim and g.is_contiguous()):
+                raise ValueError("q_gamma and k_gamma must be contiguous fp16 CUDA tensors of head_dim elements")
+        gq, gk = _ptr(q_gamma), _ptr(k_gamma)
+    if cu_seqlens is None:
+        if B != T:
+            raise ValueError("without cu_seqlens the table needs one row per token")
+        cu = None
+    else:
+        cu = _ints(cu_seqlens, "cu_seqlens", B + 1, dev)
     out, ldq = _out16(out, qkv, T, q_heads * head_dim, dev)
-    _lib.call("npub_rope_paged_append", qkv.data_ptr(), ldx, out.data_ptr(), ldq, T, q_heads, kv_heads, head_dim, R,
-              1 if interleaved else 0, pos, inv_freq.data_ptr(), _ptr(q_gamma), _ptr(k_gamma), eps,
-              k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps, page_table.data_ptr(), ldt, W, cu, B,
-              _raw_stream(dev))
+    _launch("npub_rope_paged_append", dev, qkv.data_ptr(), ldx, out.data_ptr(), ldq, T, q_heads, kv_heads, head_dim, R,
+            1 if interleaved else 0, pos, inv_freq.data_ptr(), gq, gk, eps, k_pages.data_ptr(), v_pages.data_ptr(),
+            n_pages, ps, page_table.data_ptr(), ldt, W, cu, B)
     return out
 
 
-@_on_own_device
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, heads: int,
                      kv_heads: Optional[int] = None, *, head_dim: Optional[int] = None, max_len: int = 0,
                      causal: bool = True, scale: Optional[float] = None,
@@ -706,28 +719,27 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     cu_seqlens[b] .. cu_seqlens[b + 1] (int32 [batch + 1]).  head_dim a multiple
     of 16 up to 128.  max_len: at least the longest sequence's rows (0: not known)."""
     kv_heads = kv_heads or heads
-    dev = q.get_device() if isinstance(q, torch.Tensor) else -1
-    ldq, ldk, ldv = _rows16(q, "q", dev), _rows16(k, "k", dev), _rows16(v, "v", dev)
-    T, qc = q.shape
-    _need(heads > 0, "heads must be positive")
+    _need(heads > 0 and kv_heads > 0, "heads and kv_heads must be positive")
+    dev, T, qc, ldq = _first16(q, "q")
+    Tk, kc, ldk = _rows16(k, "k", dev)
+    Tv, vc, ldv = _rows16(v, "v", dev)
     hd = head_dim or qc // heads
-    if k.shape[0] != T or v.shape[0] != T:
+    if Tk != T or Tv != T:
         raise ValueError("q, k and v must have the same number of rows")
-    if qc < heads * hd or k.shape[1] < kv_heads * hd or v.shape[1] < kv_heads * hd:
+    if qc < heads * hd or kc < kv_heads * hd or vc < kv_heads * hd:
         raise ValueError("q, k or v is narrower than its heads")
-    B = (cu_seqlens.numel() if isinstance(cu_seqlens, torch.Tensor) else 0) - 1
+    B = (cu_seqlens.numel() if isinstance(cu_seqlens, _Tensor) else 0) - 1
     if B < 0:
         raise ValueError("cu_seqlens must hold batch + 1 offsets")
     cu = _ints(cu_seqlens, "cu_seqlens", B + 1, dev)
     if scale is None:
         scale = 1.0 / math.sqrt(max(hd, 1))
     out, ldo = _out16(out, q, T, heads * hd, dev)
-    _lib.call("npub_attention_packed", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
-              cu, B, T, int(max_len), heads, kv_heads, hd, scale, 1 if causal else 0, _raw_stream(dev))
+    _launch("npub_attention_packed", dev, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
+            cu, B, T, int(max_len), heads, kv_heads, hd, scale, 1 if causal else 0)
     return out
 
 
-@_on_own_device
 def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                     lens: torch.Tensor, cu_seqlens: torch.Tensor, *, heads: int, max_new: int = 0, ctx_len: int = 0,
                     causal: bool = True, scale: Optional[float] = None,
@@ -741,10 +753,8 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     max_new * heads / kv_heads <= 16 the kernel for few rows runs); ctx_len: the
     largest lens expected (0: the table's width), which only decides how keys
     are split over CTAs.  page_size 16 .. 256."""
-    dev = q.get_device() if isinstance(q, torch.Tensor) else -1
-    ldq = _rows16(q, "q", dev)
-    T, qc = q.shape
-    n_pages, kv_heads, ps, hd, B, W, ldt = _pool(k_pages, v_pages, page_table, dev)
+    dev, T, qc, ldq = _first16(q, "q")
+    (n_pages, kv_heads, ps, hd), B, W, ldt = _pool(k_pages, v_pages, page_table, dev)
     if qc != heads * hd:
         raise ValueError("q must be [total, heads * head_dim]")
     ln = _ints(lens, "lens", B, dev)
@@ -754,14 +764,13 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     max_new = int(max_new)
     ctx = min(int(ctx_len), W * ps) if ctx_len > 0 else W * ps
     out, ldo = _out16(out, q, T, heads * hd, dev)
-    ws, wsb = _paged_workspace(q, "npub_attention_paged_workspace", B, T, max_new, ctx, heads, kv_heads, hd)
-    _lib.call("npub_attention_paged", q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
-              page_table.data_ptr(), ldt, W, ln, cu, B, T, max_new, ctx, out.data_ptr(), ldo, heads, kv_heads, hd,
-              scale, 1 if causal else 0, _ptr(ws), wsb, _raw_stream(dev))
+    ws, wsp, wsb = _paged_workspace(q, dev, "npub_attention_paged_workspace", B, T, max_new, ctx, heads, kv_heads, hd)
+    _launch("npub_attention_paged", dev, q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
+            page_table.data_ptr(), ldt, W, ln, cu, B, T, max_new, ctx, out.data_ptr(), ldo, heads, kv_heads, hd, scale,
+            1 if causal else 0, wsp, wsb)
     return out
 
 
-@_on_own_device
 def attention_paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                            lens: torch.Tensor, *, heads: int, shared_len: int = 0, ctx_len: int = 0,
                            scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -773,10 +782,9 @@ def attention_paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     the batch, through the table's first row.  The result is that of
     shared_len=0 up to rounding, also for sequences shorter than shared_len.
     ctx_len: the largest lens expected (0: the table's width)."""
-    dev = q.get_device() if isinstance(q, torch.Tensor) else -1
-    ldq = _rows16(q, "q", dev)
-    n_pages, kv_heads, ps, hd, B, W, ldt = _pool(k_pages, v_pages, page_table, dev)
-    if q.shape[0] != B or q.shape[1] != heads * hd:
+    dev, n, qc, ldq = _first16(q, "q")
+    (n_pages, kv_heads, ps, hd), B, W, ldt = _pool(k_pages, v_pages, page_table, dev)
+    if n != B or qc != heads * hd:
         raise ValueError("q must be [batch, heads * head_dim]")
     ln = _ints(lens, "lens", B, dev)
     if scale is None:
@@ -784,10 +792,11 @@ def attention_paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     shared_len = int(shared_len)
     ctx = min(int(ctx_len), W * ps) if ctx_len > 0 else W * ps
     out, ldo = _out16(out, q, B, heads * hd, dev)
-    ws, wsb = _paged_workspace(q, "npub_attention_paged_decode_workspace", B, ctx, shared_len, heads, kv_heads, hd)
-    _lib.call("npub_attention_paged_decode", q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
-              page_table.data_ptr(), ldt, W, ln, B, ctx, shared_len, out.data_ptr(), ldo, heads, kv_heads, hd, scale,
-              _ptr(ws), wsb, _raw_stream(dev))
+    ws, wsp, wsb = _paged_workspace(q, dev, "npub_attention_paged_decode_workspace", B, ctx, shared_len, heads,
+                                    kv_heads, hd)
+    _launch("npub_attention_paged_decode", dev, q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
+            page_table.data_ptr(), ldt, W, ln, B, ctx, shared_len, out.data_ptr(), ldo, heads, kv_heads, hd, scale,
+            wsp, wsb)
     return out
 
 
