@@ -41,6 +41,7 @@
 // 10 the scheduler of this CTA's items (persistent grid), warp 11 the zeroing
 // of V rows behind the last key.
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "fmha_packed.h"
 #include "gemm_tc.h"
 
@@ -73,7 +74,7 @@ struct Params {
     int64_t ldt;
     int max_keys, page_shift, box_rows, n_pages;
     int total_q, batch, heads, kv_heads, group, tpt, head_dim;
-    uint32_t span_inv;  // ceil(2^32 / (tiles * tpt))
+    uint32_t span_inv;  // ceil(2^32 / (tiles * tpt)), 2^32 - 1 for 1
     int tiles, n_items, sorted, levels, splits, first, split0, shared, causal;
     float c;  // scale * log2(e)
     __half* out;
@@ -135,8 +136,9 @@ __device__ __forceinline__ int tiles_from(const Params& p, int ntok, int klen, i
     const int64_t first = (int64_t)level * kBlk - (klen - ntok);  // rows behind this one reach the level
     if (first <= 0) return nt;
     if (first >= ntok) return 0;
-    uint32_t t = __umulhi((uint32_t)first, p.span_inv);  // first / span, at most one too large
-    t -= t * (uint32_t)span > (uint32_t)first ? 1u : 0u;
+    uint32_t t = __umulhi((uint32_t)first, p.span_inv);  // first / span, at most one off
+    if (t * (uint32_t)span > (uint32_t)first) --t;
+    else if ((uint32_t)first - t * (uint32_t)span >= (uint32_t)span) ++t;
     return nt - (int)t;
 }
 
@@ -324,25 +326,6 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&x)[128]) {
         for (int e = 0; e < 32; ++e) x[i * 32 + e] = __uint_as_float(r[i][e]);
 }
 
-// ---- pairs of fp32 (one instruction per pair)
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 // The largest of three, NaN when one is.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float r;

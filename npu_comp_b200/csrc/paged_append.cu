@@ -18,12 +18,13 @@
 //
 // Bound: HBM, every row read and written once.
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "gemm_tc.h"
 
 namespace npub {
 namespace {
 
-constexpr int kAppThreads = 256;
+constexpr int kAppThreads = 128;
 constexpr int kMaxHalf = 256;  // rot_dim / 2
 
 struct AppendArgs {
@@ -46,21 +47,25 @@ struct AppendArgs {
     int batch;
 };
 
-__device__ __forceinline__ void unpack8f(const uint4& r, float* f) {
+// Eight fp16 as four pairs of fp32, and back.
+__device__ __forceinline__ void unpack8(const uint4& r, uint64_t (&f)[4]) {
     const __half2* h = reinterpret_cast<const __half2*>(&r);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 t = __half22float2(h[i]);
-        f[2 * i] = t.x;
-        f[2 * i + 1] = t.y;
+        f[i] = pack2(t.x, t.y);
     }
 }
 
-__device__ __forceinline__ uint4 pack8h(const float* f) {
+__device__ __forceinline__ uint4 pack8(const uint64_t (&f)[4]) {
     uint4 r;
     __half2* h = reinterpret_cast<__half2*>(&r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) {
+        float a, b;
+        unpack2(f[i], a, b);
+        h[i] = __floats2half2_rn(a, b);
+    }
     return r;
 }
 
@@ -79,101 +84,153 @@ __device__ __forceinline__ int seq_of_row(const int32_t* __restrict__ cu, int ba
     return -1;
 }
 
+// Block (x, y): TOK tokens, and of their 16-element units every gridDim.y-th run
+// of kAppThreads, one unit per thread and step.  A thread loads its first unit
+// before the block forms the angles and looks up the pages.
+//
+// Measured at 8192 packed tokens of 32 / 8 heads of 128 with norms (201 MB):
+// 40.8 us with two tokens and 128 threads, 4.9 TB/s or 0.76 of the copy rate;
+// 43.5 with 256 threads, 46-48 with two or three units in flight per thread
+// (their registers cost more warps than they bring loads), 51 with the
+// arithmetic one element at a time: the instructions, not the loads, are what
+// competes with HBM here, so it runs on pairs (f32x2) and v heads are copied.
+template <int TOK>
 __global__ void __launch_bounds__(kAppThreads) rope_paged_append_kernel(const AppendArgs a) {
     pdl_trigger();
-    __shared__ float cs[kMaxHalf], sn[kMaxHalf];
+    // {cos, cos', sin, sin'} of the pairs 8 u + 2 e and 8 u + 2 e + 1 at [e][u]: the lanes of a head (u = 0, 1, ...)
+    // read neighbouring words
+    __shared__ float4 turn[TOK][kMaxHalf / 2];
+    __shared__ int page_of[TOK], slot_of[TOK];
     pdl_wait();
-    const int t = blockIdx.x;
-    int seq = t;
-    if (a.cu) {
-        seq = seq_of_row(a.cu, a.batch, t);
-        if (seq < 0) return;  // block-uniform: a row of no sequence stays as it is
-    }
-    const int p = a.pos[t];
-    for (int i = threadIdx.x; i < a.half; i += kAppThreads) {
-        const double turns = (double)p * (double)a.inv_freq[i] * 0.15915494309189535;  // 1 / (2 pi)
-        float s, c;
-        sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-        cs[i] = c;
-        sn[i] = s;
-    }
-    int page = -1;  // a position outside the table, or a page outside the pool, is not stored
-    if (p >= 0 && (p >> a.page_shift) < a.max_pages) {
-        const int id = a.table[(int64_t)seq * a.ldt + (p >> a.page_shift)];
-        if (id >= 0 && id < a.n_pages) page = id;
-    }
-    __syncthreads();
-    const int slot = p & ((1 << a.page_shift) - 1);
-    const __half* row = a.x + (int64_t)t * a.ldx;
+    const int t0 = blockIdx.x * TOK;
     const int heads = a.hq + 2 * a.hk;
-    const int total = ((heads << a.units_log2) + 31) & ~31;  // whole warps: the norm's shuffles
+    const int total = ((heads << a.units_log2) + 31) & ~31;  // units of a token, whole warps (the norm's shuffles)
     const int rot_units = a.half >> 3;
     const bool any_norm = a.gq || a.gk;
-    for (int i = blockIdx.y * kAppThreads + threadIdx.x; i < total; i += gridDim.y * kAppThreads) {
+    bool first = true;
+    for (int base = blockIdx.y * kAppThreads; base < TOK * total; base += gridDim.y * kAppThreads) {
+        int i = base + threadIdx.x, tk = 0;
+#pragma unroll
+        for (int n = 0; n < (TOK > 1 ? TOK : 0); ++n)
+            if (i >= total) {
+                i -= total;
+                ++tk;
+            }
+        const bool in = tk < TOK && t0 + tk < a.tokens;  // the same for a whole warp
         const int h = i >> a.units_log2, u = i & (a.units_p2 - 1);
-        const bool act = h < heads && u < a.units;
-        const bool isq = h < a.hq, isv = h >= a.hq + a.hk;
+        const bool act = in && h < heads && u < a.units;
         // the unit's two 8-element chunks: the two halves of a rotated pair, else neighbours
         const bool split = !a.interleaved && u < rot_units;
-        const int c0 = split ? u * 8 : u * 16;
-        const int c1 = split ? c0 + a.half : c0 + 8;
-        uint4 r0 = make_uint4(0, 0, 0, 0), r1 = r0;
+        const int c0 = split ? u * 8 : u * 16, c1 = split ? c0 + a.half : c0 + 8;
+        uint4 o0 = make_uint4(0, 0, 0, 0), o1 = o0;
         if (act) {
-            r0 = *reinterpret_cast<const uint4*>(row + (int64_t)h * a.hd + c0);
-            r1 = *reinterpret_cast<const uint4*>(row + (int64_t)h * a.hd + c1);
+            const __half* x = a.x + (int64_t)(t0 + tk) * a.ldx + (int64_t)h * a.hd;
+            o0 = *reinterpret_cast<const uint4*>(x + c0);
+            o1 = *reinterpret_cast<const uint4*>(x + c1);
         }
-        float x0[8], x1[8];
-        unpack8f(r0, x0);
-        unpack8f(r1, x1);
+        if (first) {
+            first = false;
+#pragma unroll
+            for (int tk = 0; tk < TOK; ++tk) {
+                const int t = t0 + tk;
+                if (t >= a.tokens) break;
+                const int p = a.pos[t];
+                for (int i = threadIdx.x; i < a.half; i += kAppThreads) {
+                    const double turns = (double)p * (double)a.inv_freq[i] * 0.15915494309189535;  // 1 / (2 pi)
+                    float s, c;
+                    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+                    float* w = reinterpret_cast<float*>(&turn[tk][((i & 7) >> 1) * rot_units + (i >> 3)]) + (i & 1);
+                    w[0] = c;
+                    w[2] = s;
+                }
+                if ((threadIdx.x >> 5) == kAppThreads / 32 - 1 - tk) {  // one warp per token, from the last on
+                    const int seq = a.cu ? seq_of_row(a.cu, a.batch, t) : t;
+                    // a position outside the table, or a page outside the pool, is not stored (-1); a row of no
+                    // sequence stays as it is (-2)
+                    int page = seq < 0 ? -2 : -1;
+                    if (seq >= 0 && p >= 0 && (p >> a.page_shift) < a.max_pages) {
+                        const int id = a.table[(int64_t)seq * a.ldt + (p >> a.page_shift)];
+                        if (id >= 0 && id < a.n_pages) page = id;
+                    }
+                    if ((threadIdx.x & 31) == 0) {
+                        page_of[tk] = page;
+                        slot_of[tk] = p & ((1 << a.page_shift) - 1);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (!in) continue;
+        const bool isq = h < a.hq, isv = h >= a.hq + a.hk;
+        const int page = page_of[tk];
         const __half* g = isv ? nullptr : isq ? a.gq : a.gk;
-        if (any_norm) {
-            float ss = 0.0f;
+        const bool turns = !isv && u < rot_units;
+        if (__any_sync(0xffffffffu, turns || g)) {  // a warp of v heads copies
+            uint64_t x0[4], x1[4];
+            unpack8(o0, x0);
+            unpack8(o1, x1);
+            if (any_norm) {
+                uint64_t s2 = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss += x0[e] * x0[e] + x1[e] * x1[e];
-            for (int m = a.units_p2 >> 1; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-            if (g && act) {
-                const float inv = 1.0f / sqrtf(ss * a.inv_hd + a.eps);
-                float g0[8], g1[8];
-                unpack8f(__ldg(reinterpret_cast<const uint4*>(g + c0)), g0);
-                unpack8f(__ldg(reinterpret_cast<const uint4*>(g + c1)), g1);
+                for (int e = 0; e < 4; ++e) s2 = fma2(x1[e], x1[e], fma2(x0[e], x0[e], s2));
+                float ss, sb;
+                unpack2(s2, ss, sb);
+                ss += sb;
+                for (int m = a.units_p2 >> 1; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+                if (g && act) {
+                    const float inv = rsqrtf(ss * a.inv_hd + a.eps);
+                    const uint64_t inv2 = pack2(inv, inv);
+                    uint64_t g0[4], g1[4];
+                    unpack8(__ldg(reinterpret_cast<const uint4*>(g + c0)), g0);
+                    unpack8(__ldg(reinterpret_cast<const uint4*>(g + c1)), g1);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x0[e] *= inv * g0[e];
-                    x1[e] *= inv * g1[e];
+                    for (int e = 0; e < 4; ++e) {
+                        x0[e] = mul2(x0[e], mul2(inv2, g0[e]));
+                        x1[e] = mul2(x1[e], mul2(inv2, g1[e]));
+                    }
                 }
             }
-        }
-        if (!act) continue;
-        if (!isv && u < rot_units) {
-            if (split) {
+            if (turns) {
+                const float4* cs = &turn[tk][u];
+                if (split) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float c = cs[c0 + e], s = sn[c0 + e], v0 = x0[e], v1 = x1[e];
-                    x0[e] = v0 * c - v1 * s;
-                    x1[e] = v1 * c + v0 * s;
-                }
-            } else {
+                    for (int e = 0; e < 4; ++e) {
+                        const float4 w = cs[e * rot_units];
+                        const uint64_t c = pack2(w.x, w.y), s = pack2(w.z, w.w), ns = pack2(-w.z, -w.w);
+                        const uint64_t v0 = x0[e], v1 = x1[e];
+                        x0[e] = fma2(v0, c, mul2(v1, ns));
+                        x1[e] = fma2(v1, c, mul2(v0, s));
+                    }
+                } else {
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const int f0 = u * 8 + (e >> 1), f1 = f0 + 4;
-                    const float a0 = x0[e], b0 = x0[e + 1], a1 = x1[e], b1 = x1[e + 1];
-                    x0[e] = a0 * cs[f0] - b0 * sn[f0];
-                    x0[e + 1] = b0 * cs[f0] + a0 * sn[f0];
-                    x1[e] = a1 * cs[f1] - b1 * sn[f1];
-                    x1[e + 1] = b1 * cs[f1] + a1 * sn[f1];
+                    for (int e = 0; e < 4; ++e) {
+                        const float4 w = cs[(e >> 1) * rot_units], v = cs[((e >> 1) + 2) * rot_units];
+                        const float c0 = (e & 1) ? w.y : w.x, s0 = (e & 1) ? w.w : w.z;
+                        const float c1 = (e & 1) ? v.y : v.x, s1 = (e & 1) ? v.w : v.z;
+                        float p, q;
+                        unpack2(x0[e], p, q);
+                        x0[e] = pack2(p * c0 - q * s0, q * c0 + p * s0);
+                        unpack2(x1[e], p, q);
+                        x1[e] = pack2(p * c1 - q * s1, q * c1 + p * s1);
+                    }
                 }
             }
+            if (!isv) {
+                o0 = pack8(x0);
+                o1 = pack8(x1);
+            }
         }
+        if (!act || page == -2) continue;
         __half* dst;
         if (isq) {
-            dst = a.q + (int64_t)t * a.ldq + (int64_t)h * a.hd;
+            dst = a.q + (int64_t)(t0 + tk) * a.ldq + (int64_t)h * a.hd;
         } else {
             if (page < 0) continue;
             const int kvh = isv ? h - a.hq - a.hk : h - a.hq;
-            dst = (isv ? a.vp : a.kp) + ((((int64_t)page * a.hk + kvh) << a.page_shift) + slot) * a.hd;
+            dst = (isv ? a.vp : a.kp) + ((((int64_t)page * a.hk + kvh) << a.page_shift) + slot_of[tk]) * a.hd;
         }
-        *reinterpret_cast<uint4*>(dst + c0) = pack8h(x0);
-        *reinterpret_cast<uint4*>(dst + c1) = pack8h(x1);
+        *reinterpret_cast<uint4*>(dst + c0) = o0;
+        *reinterpret_cast<uint4*>(dst + c1) = o1;
     }
 }
 
@@ -230,9 +287,11 @@ extern "C" int npub_rope_paged_append(const void* qkv, int64_t ldx, void* q_out,
     a.max_pages = max_pages;
     a.cu = cu_seqlens;
     a.batch = batch;
-    const int total = (q_heads + 2 * kv_heads) << a.units_log2;
-    int groups = 1;  // blocks per token: one while the tokens alone fill the GPU
-    if (tokens < 2 * num_sms()) groups = (total + kAppThreads - 1) / kAppThreads;
-    return launch_pdl(rope_paged_append_kernel, dim3(tokens, groups), dim3(kAppThreads), 0,
-                      reinterpret_cast<cudaStream_t>(stream), a);
+    const int total = (((q_heads + 2 * kv_heads) << a.units_log2) + 31) & ~31;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (tokens < 4 * num_sms()) {  // one unit per thread, blocks over the heads
+        const int groups = (total + kAppThreads - 1) / kAppThreads;
+        return launch_pdl(rope_paged_append_kernel<1>, dim3(tokens, groups), dim3(kAppThreads), 0, st, a);
+    }
+    return launch_pdl(rope_paged_append_kernel<2>, dim3((tokens + 1) / 2), dim3(kAppThreads), 0, st, a);
 }
