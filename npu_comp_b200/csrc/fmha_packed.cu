@@ -904,6 +904,7 @@ int launch(const Params& p, int grid, cudaStream_t st) {
 int64_t fmha_packed_items(int total_q, int batch, int heads, int kv_heads, int max_new, int tiles) {
     const int64_t span = (int64_t)tiles * (128 / (heads / kv_heads));
     int64_t n = total_q / span + batch;  // sum of ceil(rows / span) over the sequences is at most this
+    if (batch == 1) n = (total_q + span - 1) / span;
     if (n > total_q) n = total_q;
     if (max_new > 0 && n > batch * ((max_new + span - 1) / span)) n = batch * ((max_new + span - 1) / span);
     return n;

@@ -46,17 +46,24 @@ struct Plan {
     bool part() const { return total() > 1; }
 };
 
+// What a kernel takes, in us: `first` to start, then per item `item` and `unit_us` for every `unit` keys (`alone` while
+// at most half of the slots are taken: bandwidth to spare).
+struct Cost {
+    double first, item, unit_us, alone;
+    int unit;
+};
+
 // Number of key ranges for `items` work items of up to `keys` keys on `slots` resident CTAs: the s that makes
-// waves * (start + key units of a range * per unit) + combination smallest, times in us.  `part_us`: what one more
-// split's partials cost (written, read), `per`: partials of a range, `fixed`: a combination pass runs anyway.
-int pick_splits(int64_t keys, int64_t items, int64_t slots, int unit, double start, double per_unit, double part_us,
-                int per, bool fixed, double* us) {
-    const int64_t units = ceil_div(keys > 0 ? keys : 1, unit);
+// first + waves * (item + units of a range * unit_us) + combination smallest.  `part_us`: what one more split's
+// partials cost (written, read), `per`: partials of a range, `fixed`: a combination pass runs anyway.
+int pick_splits(int64_t keys, int64_t items, int64_t slots, const Cost& c, double part_us, int per, bool fixed,
+                double* us) {
+    const int64_t units = ceil_div(keys > 0 ? keys : 1, c.unit);
     int pick = 1;
     for (int s = 1; s <= 64 && s <= units; ++s) {
-        const double unit_us = items * s <= slots / 2 ? 0.6 * per_unit : per_unit;  // few CTAs: bandwidth to spare
+        const double unit_us = items * s <= slots / 2 ? c.alone : c.unit_us;
         const bool part = s * per > 1;
-        const double t = (double)ceil_div(items * s, slots) * (start + (double)ceil_div(units, s) * unit_us) +
+        const double t = c.first + (double)ceil_div(items * s, slots) * (c.item + (double)ceil_div(units, s) * unit_us) +
                          (part || fixed ? s * per * (part_us + 0.15) : 0.0) + (part && !fixed ? 4.0 : 0.0);
         if (s == 1 || t < 0.95 * *us) {
             *us = t;
@@ -66,21 +73,21 @@ int pick_splits(int64_t keys, int64_t items, int64_t slots, int unit, double sta
     return pick;
 }
 
-// A phase on the tile kernel: pairs of tiles (1.5 us per 128 keys of a pair, 4 us to start and end), or, where the rows
-// fill one tile, one tile on two halves of the keys (1.5 us per 256 keys).
-Phase tile_phase(int total, int batch, int heads, int kv_heads, int max_new, int64_t keys, double part_us, bool fixed) {
-    const int64_t sms = num_sms();
+// A phase on the tile kernel (measured: 7 us to start, 2 us to change items, 1.6 us per 128 keys of a pair of tiles),
+// on `slots` SMs: pairs of tiles, or, where the rows fill one tile, one tile on two halves of the keys.
+Phase tile_phase(int total, int batch, int heads, int kv_heads, int max_new, int64_t keys, int64_t slots,
+                 double part_us, bool fixed) {
     const int64_t one = fmha_packed_items(total, batch, heads, kv_heads, max_new, 1) * kv_heads;
     const int64_t two = fmha_packed_items(total, batch, heads, kv_heads, max_new, 2) * kv_heads;
     Phase a = {}, b = {};
     double ua, ub;
     a.tiles = 2;
-    a.splits = pick_splits(keys, two, sms, 128, 4.0, 1.5, part_us, 1, fixed, &ua);
+    a.splits = pick_splits(keys, two, slots, Cost{7.0, 2.0, 1.6, 1.6, 128}, part_us, 1, fixed, &ua);
     b.tiles = 1;
     b.dual = 1;
-    b.splits = pick_splits(keys, one, sms, 256, 4.0, 1.5, part_us, 2, fixed, &ub);
+    b.splits = pick_splits(keys, one, slots, Cost{7.0, 2.0, 1.6, 1.6, 256}, part_us, 2, fixed, &ub);
     if (ub < ua) return b;
-    if (a.splits == 1) a.tiles = 0;
+    if (a.splits == 1 && !fixed) a.tiles = 0;
     return a;
 }
 
@@ -91,15 +98,17 @@ Plan make_plan(int batch, int total, int max_new, int64_t ctx, int shared, int h
     if (batch < 2) shared = 0;  // nothing to share
     pl.shared = shared;
     const double part_us = (double)total * heads * head_dim * 8.0 / 4e6;  // about 4 TB/s: they stay in L2
-    if (shared > 0) pl.pre = tile_phase(total, 1, heads, kv_heads, 0, shared, part_us, true);
+    // The prefix phase takes half of the SMs and the own keys run beside it (64 sequences, 32 / 8 heads, 8192 shared
+    // and 265 own keys on average: 36 us; on all SMs, one phase after the other, 46 us).
+    if (shared > 0) pl.pre = tile_phase(total, 1, heads, kv_heads, 0, shared, sms / 2, part_us, true);
     const int64_t own = ctx > shared ? ctx - shared : 1;
     if (pl.few) {
-        // a few-row CTA, two of which share an SM, takes 1.5 us per 64 keys of 128 columns and 2.5 us
+        // a few-row CTA, two of which share an SM, takes 2.5 us and 6 us per 256 keys of 128 columns
+        const Cost c = head_dim > 64 ? Cost{0.0, 2.5, 6.0, 3.6, 256} : Cost{0.0, 2.5, 3.2, 1.9, 256};
         double us;
-        pl.own.splits = pick_splits(own, (int64_t)batch * kv_heads, 2 * sms, 64, 2.5, head_dim > 64 ? 1.5 : 0.8,
-                                    part_us, 1, shared > 0, &us);
+        pl.own.splits = pick_splits(own, (int64_t)batch * kv_heads, 2 * sms, c, part_us, 1, shared > 0, &us);
     } else {
-        pl.own = tile_phase(total, batch, heads, kv_heads, max_new, own, part_us, shared > 0);
+        pl.own = tile_phase(total, batch, heads, kv_heads, max_new, own, sms, part_us, shared > 0);
     }
     return pl;
 }

@@ -111,21 +111,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + L::kStages);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kvh = (int)blockIdx.x / p.splits, split = (int)blockIdx.x - kvh * p.splits, b = blockIdx.y;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < L::kStages; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], kWarps);
-        }
-        *abort_flag = 0;
-        fence_barrier_init();
-    }
-    if (warp == kWarps && lane == 0) {
-        prefetch_tmap(&p.tmK);
-        prefetch_tmap(&p.tmV);
-    }
-    cta_sync_divergent();
+    const bool part = p.part_o != nullptr;
+    // Beside a prefix phase the last CTA waits for that phase at its end: this grid's completion then means the prefix's
+    // to the combination behind it.  (All CTAs waiting would keep their slots from the CTAs behind them.)
+    const bool holds = p.beside && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
     if (!p.beside) pdl_wait();
-
     // rows of this sequence, its keys, and this CTA's range of them
     int row0 = b, nrow = 1;
     if (p.cu) {
@@ -141,7 +131,34 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     const int k0 = R == 0 ? 0 : p.first + min(own, split * per);
     const int k1 = R == 0 ? 0 : p.first + min(own, split * per + per);
     const int nst = (k1 - k0 + kKeys - 1) / kKeys;
-    const bool part = p.part_o != nullptr;
+    if (nst == 0) {
+        for (int r = threadIdx.x; r < R; r += kThreads) {
+            const int t = r / p.group, head = kvh * p.group + r - t * p.group;
+            if (part) {
+                p.part_ml[((int64_t)(p.split0 + split) * p.total_q + row0 + t) * p.heads + head] =
+                    make_float2(-INFINITY, 0.0f);
+            } else {
+                for (int d = 0; d < p.head_dim; d += 4)
+                    *reinterpret_cast<uint2*>(p.out + (int64_t)(row0 + t) * p.ldo + (int64_t)head * p.head_dim + d) =
+                        make_uint2(0, 0);
+            }
+        }
+        if (holds) pdl_wait();
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kWarps);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == kWarps && lane == 0) {
+        prefetch_tmap(&p.tmK);
+        prefetch_tmap(&p.tmV);
+    }
+    cta_sync_divergent();
 
     if (warp == kWarps) {
         // -------------------------------------------------------------------- producer
@@ -173,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
             for (int i = max(0, j - L::kStages); i < j; ++i)
                 mbar_wait_bounded(&full[i % L::kStages], (uint32_t)(i / L::kStages) & 1u, &never, 200000000ull);
         }
-        if (p.beside) pdl_wait();
+        if (holds) pdl_wait();
         return;
     }
 
@@ -345,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
             *reinterpret_cast<uint2*>(p.out + (int64_t)(row0 + t) * p.ldo + (int64_t)head * p.head_dim + d) = w;
         }
     }
-    if (p.beside) pdl_wait();  // this grid's end then means the prefix phase's end to the combination behind it
+    if (holds) pdl_wait();
 }
 
 // out[row, head] = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over the
