@@ -41,36 +41,46 @@ struct Phase {
 struct Plan {
     bool few;    // own keys on paged_decode (else on the tiles)
     int shared;  // keys of the shared prefix phase (0: none)
+    bool cluster;  // paged_decode combines its ranges itself
     Phase pre, own;
     int total() const { return (shared > 0 ? pre.partials() : 0) + own.partials(); }
-    bool part() const { return total() > 1; }
+    bool part() const { return total() > 1 && !cluster; }
 };
 
-// What a kernel takes, in us: `first` to start, then per item `item` and `unit_us` for every `unit` keys (`alone` while
-// at most half of the slots are taken: bandwidth to spare).
+// What a kernel takes, in us: `first` to start, then per item `item` and `unit_us` for every `unit` keys.
 struct Cost {
-    double first, item, unit_us, alone;
+    double first, item, unit_us;
     int unit;
 };
 
-// Number of key ranges for `items` work items of up to `keys` keys on `slots` resident CTAs: the s that makes
-// first + waves * (item + units of a range * unit_us) + combination smallest.  `part_us`: what one more split's
-// partials cost (written, read), `per`: partials of a range, `fixed`: a combination pass runs anyway.
-int pick_splits(int64_t keys, int64_t items, int64_t slots, const Cost& c, double part_us, int per, bool fixed,
-                double* us) {
+// The number of key ranges s <= most for `items` items of up to `keys` keys on `slots` resident CTAs that makes the
+// estimate below smallest.  `range_us`: what one more range's partials cost (written, read); `fixed`: a combination
+// pass runs anyway, else it adds `pass_us` where there is more than one partial (`per` of them for a range).
+//   equal   items of one length, in waves: first + waves * (item + range)
+//   ragged  lengths below `keys` (0.7 of it on average), CTAs taken in order as slots come free: the work over the
+//           slots and half of the longest CTA, or that CTA where the slots are not filled
+struct Split {
+    int s;
+    double us;
+};
+Split pick_splits(int64_t keys, int64_t items, int64_t slots, const Cost& c, bool ragged, int most, double range_us,
+                  int per, bool fixed, double pass_us) {
     const int64_t units = ceil_div(keys > 0 ? keys : 1, c.unit);
-    int pick = 1;
-    for (int s = 1; s <= 64 && s <= units; ++s) {
-        const double unit_us = items * s <= slots / 2 ? c.alone : c.unit_us;
-        const bool part = s * per > 1;
-        const double t = c.first + (double)ceil_div(items * s, slots) * (c.item + (double)ceil_div(units, s) * unit_us) +
-                         (part || fixed ? s * per * (part_us + 0.15) : 0.0) + (part && !fixed ? 4.0 : 0.0);
-        if (s == 1 || t < 0.95 * *us) {
-            *us = t;
-            pick = s;
+    Split best = {1, 0.0};
+    for (int s = 1; s <= most && s <= units; ++s) {
+        const double cta = c.item + (double)ceil_div(units, s) * c.unit_us;
+        double t;
+        if (ragged) {
+            const double bulk = (double)items * (s * c.item + 0.7 * (double)units * c.unit_us) / (double)slots;
+            t = bulk + 0.5 * cta > cta ? bulk + 0.5 * cta : cta;
+        } else {
+            t = (double)ceil_div(items * s, slots) * cta;
         }
+        t += c.first;
+        if (s * per > 1 || fixed) t += s * per * range_us + (fixed ? 0.0 : pass_us);
+        if (s == 1 || t < 0.97 * best.us) best = Split{s, t};
     }
-    return pick;
+    return best;
 }
 
 // A phase on the tile kernel (measured: 7 us to start, 2 us to change items, 1.6 us per 128 keys of a pair of tiles),
@@ -80,15 +90,15 @@ Phase tile_phase(int total, int batch, int heads, int kv_heads, int max_new, int
     const int64_t one = fmha_packed_items(total, batch, heads, kv_heads, max_new, 1) * kv_heads;
     const int64_t two = fmha_packed_items(total, batch, heads, kv_heads, max_new, 2) * kv_heads;
     Phase a = {}, b = {};
-    double ua, ub;
-    a.tiles = 2;
-    a.splits = pick_splits(keys, two, slots, Cost{7.0, 2.0, 1.6, 1.6, 128}, part_us, 1, fixed, &ua);
+    const double range_us = part_us + 0.15;
+    const Split sa = pick_splits(keys, two, slots, Cost{7.0, 2.0, 1.6, 128}, false, 64, range_us, 1, fixed, 4.0);
+    const Split sb = pick_splits(keys, one, slots, Cost{7.0, 2.0, 1.6, 256}, false, 64, range_us, 2, fixed, 4.0);
+    a.tiles = sa.s == 1 && !fixed ? 0 : 2;
+    a.splits = sa.s;
     b.tiles = 1;
     b.dual = 1;
-    b.splits = pick_splits(keys, one, slots, Cost{7.0, 2.0, 1.6, 1.6, 256}, part_us, 2, fixed, &ub);
-    if (ub < ua) return b;
-    if (a.splits == 1 && !fixed) a.tiles = 0;
-    return a;
+    b.splits = sb.s;
+    return sb.us < sa.us ? b : a;
 }
 
 Plan make_plan(int batch, int total, int max_new, int64_t ctx, int shared, int heads, int kv_heads, int head_dim) {
@@ -103,10 +113,19 @@ Plan make_plan(int batch, int total, int max_new, int64_t ctx, int shared, int h
     if (shared > 0) pl.pre = tile_phase(total, 1, heads, kv_heads, 0, shared, sms / 2, part_us, true);
     const int64_t own = ctx > shared ? ctx - shared : 1;
     if (pl.few) {
-        // a few-row CTA, two of which share an SM, takes 2.5 us and 6 us per 256 keys of 128 columns
-        const Cost c = head_dim > 64 ? Cost{0.0, 2.5, 6.0, 3.6, 256} : Cost{0.0, 2.5, 3.2, 1.9, 256};
-        double us;
-        pl.own.splits = pick_splits(own, (int64_t)batch * kv_heads, 2 * sms, c, part_us, 1, shared > 0, &us);
+        // a few-row CTA, two of which share an SM, takes 4 us (in a cluster 5) and 3 us per 128 keys of 128 columns
+        const Cost c = {0.0, 4.0, head_dim > 64 ? 3.0 : 1.6, 128}, cc = {0.0, 5.0, c.unit_us, 128};
+        const bool ragged = batch > 1;
+        const int64_t items = (int64_t)batch * kv_heads;
+        const Split sp = pick_splits(own, items, 2 * sms, c, ragged, 64, part_us + 0.15, 1, shared > 0, 4.0);
+        pl.own.splits = sp.s;
+        if (shared == 0) {
+            const Split sc = pick_splits(own, items, 2 * sms, cc, ragged, kPagedDecodeCluster, 0.0, 1, true, 0.0);
+            if (sc.us <= sp.us) {
+                pl.own.splits = sc.s;
+                pl.cluster = true;
+            }
+        }
     } else {
         pl.own = tile_phase(total, batch, heads, kv_heads, max_new, own, sms, part_us, shared > 0);
     }

@@ -11,7 +11,9 @@
 // flight: a producer warp streams stages of 64 keys (K and V, 32 KB at
 // head_dim 128) through a ring by TMA, its lanes issuing one page piece each;
 // four consumer warps take 16 keys of every stage, each with its own running
-// maximum and sum, and meet only at the end.
+// maximum and sum, and meet only at the end.  Up to eight ranges of one item
+// are a cluster and combine through one another's shared memory; more of them,
+// or a shared prefix, leave partials for a second kernel.
 //
 // As in fmha_packed.cu the running maximum moves only when it has grown by
 // more than 2^8; keys past the sequence's end are masked by a select and their
@@ -37,7 +39,11 @@ struct Smem {
     static constexpr int kStages = HD == 128 ? 3 : 6;
     static constexpr int kOffBar = kStages * 2 * kTile;
     static constexpr int kTotal = kOffBar + 256;
-    static_assert(kWarps * kMaxRows * HD * 4 + kWarps * kMaxRows * 8 <= kOffBar, "the merge reuses the ring");
+    // the merge reuses the ring: the warps' partials, then (clusters) the CTA's own
+    static constexpr int kOffMl = kWarps * kMaxRows * HD * 4;
+    static constexpr int kOffOwn = kOffMl + kWarps * kMaxRows * 8;
+    static constexpr int kOffOwnMl = kOffOwn + kMaxRows * HD * 4;
+    static_assert(kOffOwnMl + kMaxRows * 8 <= kOffBar, "layout");
 };
 
 struct Params {
@@ -50,6 +56,7 @@ struct Params {
     int total_q, heads, kv_heads, group, head_dim, causal;
     int first, splits;         // every sequence's keys from `first` on in `splits` equal ranges
     int split0;                // index of split 0 among the partials
+    int cluster;               // the splits of an item are a cluster, which combines them itself
     int beside;                // launched behind a shared-prefix phase, which has waited for all earlier work
     float c;
     __half* out;
@@ -90,6 +97,19 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a)
+                 : "memory");
+    return v;
+}
 __device__ __forceinline__ uint32_t h2(float a, float b) {
     __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
@@ -126,8 +146,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     const int R = nrow * p.group;
     const int len = max(0, min(p.lens[b], p.max_keys));
     const int own = max(0, len - p.first);
-    // whole stages, at least 256 keys: what a short sequence does not fill ends at once
-    const int per = max(4, ((own + kKeys - 1) / kKeys + p.splits - 1) / p.splits) * kKeys;
+    // whole stages, at least 128 keys: the CTAs that a short sequence does not fill end at once
+    const int per = max(2, ((own + kKeys - 1) / kKeys + p.splits - 1) / p.splits) * kKeys;
     const int k0 = R == 0 ? 0 : p.first + min(own, split * per);
     const int k1 = R == 0 ? 0 : p.first + min(own, split * per + per);
     const int nst = (k1 - k0 + kKeys - 1) / kKeys;
@@ -137,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
             if (part) {
                 p.part_ml[((int64_t)(p.split0 + split) * p.total_q + row0 + t) * p.heads + head] =
                     make_float2(-INFINITY, 0.0f);
-            } else {
+            } else if (split == 0) {
                 for (int d = 0; d < p.head_dim; d += 4)
                     *reinterpret_cast<uint2*>(p.out + (int64_t)(row0 + t) * p.ldo + (int64_t)head * p.head_dim + d) =
                         make_uint2(0, 0);
@@ -317,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     }
     consumer_bar();  // nobody reads the ring any more
     float* so = reinterpret_cast<float*>(smem);                                    // [warp][row][HD]
-    float2* sml = reinterpret_cast<float2*>(smem + kWarps * kMaxRows * HD * 4);    // [warp][row]
+    float2* sml = reinterpret_cast<float2*>(smem + L::kOffMl);                      // [warp][row]
     if ((lane & 3) == 0) {
         sml[warp * kMaxRows + ra] = make_float2(m[0], l[0]);
         sml[warp * kMaxRows + rb] = make_float2(m[1], l[1]);
@@ -349,7 +369,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
             acc[3] += f * v.w;
         }
         const int t = r / p.group, head = kvh * p.group + r - t * p.group;
-        if (part) {
+        if (p.cluster) {
+            if (d == 0)
+                *reinterpret_cast<float2*>(smem + L::kOffOwnMl + r * 8) =
+                    make_float2(mm == -INFINITY ? -INFINITY : mm * c, sum);
+            *reinterpret_cast<float4*>(smem + L::kOffOwn + (r * HD + d) * 4) =
+                make_float4(acc[0], acc[1], acc[2], acc[3]);
+        } else if (part) {
             const int64_t at = ((int64_t)(p.split0 + split) * p.total_q + row0 + t) * p.heads + head;
             if (d == 0) p.part_ml[at] = make_float2(mm == -INFINITY ? -INFINITY : mm * c, sum);
             if (sum != 0.0f)
@@ -361,6 +387,40 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
             w.y = sum != 0.0f ? h2(acc[2] * inv, acc[3] * inv) : 0u;
             *reinterpret_cast<uint2*>(p.out + (int64_t)(row0 + t) * p.ldo + (int64_t)head * p.head_dim + d) = w;
         }
+    }
+    if (p.cluster) {
+        // the CTAs of the cluster with keys (the producers and the CTAs without have left, and do not count) each
+        // combine a part of the rows from all of their shared memories
+        const int n = (own + per - 1) / per;
+        cluster_arrive();
+        cluster_wait();
+        for (int i = split * (kWarps * 32) + threadIdx.x; i < R * cols; i += n * (kWarps * 32)) {
+            const int r = i / cols, d = (i - r * cols) * 4;
+            const uint32_t ml_at = smem_u32(smem + L::kOffOwnMl + r * 8);
+            const uint32_t o_at = smem_u32(smem + L::kOffOwn + (r * HD + d) * 4);
+            float mm = -INFINITY;
+            for (int t = 0; t < n; ++t) mm = fmaxf(mm, ld_cluster_f2(mapa_shared(ml_at, t)).x);
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+            for (int t = 0; t < n; ++t) {
+                const float2 ml = ld_cluster_f2(mapa_shared(ml_at, t));
+                if (ml.y == 0.0f) continue;
+                const float f = ex2_approx(ml.x - mm);
+                const float4 v = ld_cluster_f4(mapa_shared(o_at, t));
+                sum += f * ml.y;
+                acc[0] += f * v.x;
+                acc[1] += f * v.y;
+                acc[2] += f * v.z;
+                acc[3] += f * v.w;
+            }
+            const float inv = 1.0f / sum;
+            uint2 w;
+            w.x = sum != 0.0f ? h2(acc[0] * inv, acc[1] * inv) : 0u;
+            w.y = sum != 0.0f ? h2(acc[2] * inv, acc[3] * inv) : 0u;
+            const int t = r / p.group, head = kvh * p.group + r - t * p.group;
+            *reinterpret_cast<uint2*>(p.out + (int64_t)(row0 + t) * p.ldo + (int64_t)head * p.head_dim + d) = w;
+        }
+        cluster_arrive();  // nobody leaves while its shared memory is read
+        cluster_wait();
     }
     if (holds) pdl_wait();
 }
@@ -432,7 +492,28 @@ int launch(const Params& p, int batch, cudaStream_t st) {
         npub_internal_set_cuda_error(e);
         return NPUB_ERR_CUDA;
     }
-    return launch_pdl(kern, dim3(p.kv_heads * p.splits, batch), dim3(kThreads), Smem<HD>::kTotal, st, p);
+    if (!p.cluster)
+        return launch_pdl(kern, dim3(p.kv_heads * p.splits, batch), dim3(kThreads), Smem<HD>::kTotal, st, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.kv_heads * p.splits, batch);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Smem<HD>::kTotal;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = npub_internal_pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.splits;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t le = cudaLaunchKernelEx(&cfg, kern, p);
+    if (le != cudaSuccess) {
+        npub_internal_set_cuda_error(le);
+        return NPUB_ERR_CUDA;
+    }
+    return npub_internal_launch_status();
 }
 
 }  // namespace pdec
@@ -463,7 +544,8 @@ int paged_decode(const PackedArgs& a, cudaStream_t st) {
     p.head_dim = a.head_dim;
     p.causal = a.causal ? 1 : 0;
     p.first = a.first;
-    p.splits = a.part_o ? a.splits : 1;
+    p.splits = a.splits;
+    p.cluster = !a.part_o && a.splits > 1;
     p.split0 = a.split0;
     p.beside = a.first > 0;
     p.c = a.scale * 1.4426950408889634f;

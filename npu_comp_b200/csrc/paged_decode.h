@@ -8,8 +8,10 @@ namespace npub {
 
 constexpr int kPagedDecodeRows = 16;  // rows per kv head that paged_decode takes
 
+constexpr int kPagedDecodeCluster = 8;  // ranges that a cluster combines
+
 // a.splits equal ranges of every sequence's keys from a.first on: partials a.split0 + s when a.part_o is set, else
-// (one range) the result.  a.cu null: one row per sequence.
+// (up to kPagedDecodeCluster ranges) the result.  a.cu null: one row per sequence.
 int paged_decode(const PackedArgs& a, cudaStream_t st);
 int paged_combine(const PackedArgs& a, int splits, cudaStream_t st);
 

@@ -82,5 +82,5 @@ def test_workspace_queries(libnpub_path):
     assert p(0, 8, 0, 100, 4, 2, 128) == 0 and p(2, 8, 0, 64, 4, 2, 128) == 0
     assert p(2, 100000, 0, 100000, 32, 8, 128) == 0  # enough tiles: no split
     # partials are (2 + head_dim) floats per row, head and split
-    n = p(1, 4, 4, 4096, 4, 2, 128)
+    n = p(1, 4, 4, 65536, 4, 2, 128)
     assert n > 0 and n % (4 * 4 * 130 * 4) < 256
