@@ -331,21 +331,22 @@ int npub_rope_paged_append(const void* qkv, int64_t ldx, void* q_out, int64_t ld
  * kv_heads*head_dim] rows with strides ldq / ldk / ldv (multiples of 8), query
  * head h reads kv head h / (heads / kv_heads), out fp16 [total,
  * heads*head_dim] (ldo).  causal != 0: row i of a sequence sees its rows
- * 0..i; else all of them.  max_len: the longest sequence's rows, or 0 when not
- * known; a longer sequence's rows past it are not computed.  scale > 0;
+ * 0..i; else all of them.  scale > 0;
  * head_dim % 16 == 0.  head_dim > 128 or heads / kv_heads > 128 returns
  * NPUB_ERR_UNSUPPORTED.  Nothing outside a sequence reaches its results, but
  * the values of its own later rows have to be finite.  Needs no workspace. */
 int npub_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
-                          void* out, int64_t ldo, const int32_t* cu_seqlens, int batch, int total, int max_len,
-                          int heads, int kv_heads, int head_dim, float scale, int causal, void* stream);
+                          void* out, int64_t ldo, const int32_t* cu_seqlens, int batch, int total, int heads,
+                          int kv_heads, int head_dim, float scale, int causal, void* stream);
 
 /* Attention of packed new rows over the paged cache (a prompt chunk behind
  * what its pages hold, a prompt whose prefix is cached, drafted tokens): the
  * keys of sequence b are positions 0 .. lens[b] - 1 (int32 [batch], clipped to
  * [0, max_pages * page_size]), its n new rows the last n of them, so row i
  * sees lens[b] - n + i + 1 keys (all of them when causal == 0); a row that
- * sees none gives zeros.  max_new as max_len above; ctx_len: the largest
+ * sees none gives zeros.  max_new: at least the new rows of any sequence (rows
+ * past it may be left out), or 0 when not known; up to 16 / (heads /
+ * kv_heads) of them run on a kernel for few rows.  ctx_len: the largest
  * lens[b] expected (0: the table's width), which only decides how the keys
  * are split over CTAs.  A page id outside [0, n_pages) reads as zeros.
  * page_size 16 .. 256; otherwise as npub_attention_packed.  Workspace:

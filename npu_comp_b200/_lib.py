@@ -70,7 +70,7 @@ SIGNATURES = {
                                     ctypes.c_double]),
     "npub_rope_paged_append": (_i, [_p, _i64, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _f, _p, _p, _i, _i,
                                     _p, _i64, _i, _p, _i, _p]),
-    "npub_attention_packed": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i, _i, _i, _i, _i, _i, _f, _i, _p]),
+    "npub_attention_packed": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i, _i, _i, _i, _i, _f, _i, _p]),
     "npub_attention_paged": (_i, [_p, _i64, _p, _p, _i, _i, _p, _i64, _i, _p, _p, _i, _i, _i, _i, _p, _i64, _i, _i,
                                   _i, _f, _i, _p, _sz, _p]),
     "npub_attention_paged_workspace": (_sz, [_i, _i, _i, _i64, _i, _i, _i]),

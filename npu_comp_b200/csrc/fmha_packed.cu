@@ -23,10 +23,16 @@
 // at head_dim 128 a pair of tiles takes 2820 cycles per key block, of which
 // the tensor core runs 2048; a tile's chain is its softmax (1850: 160 to read
 // S, 440 for the maximum and the rescale test, 1250 for the exponentials) and
-// then the second half of P V and the next S.  At head_dim 64 the products
-// are half as long and the exponentials bound it (16 per cycle and SM), so a
-// quarter of them runs as a polynomial on the FMA pipe there (437 against 469
-// us); at head_dim 128 that only costs issue slots and power (462 / 458 us).
+// then the second half of P V and the next S.  446 us, 1230 TFLOP/s: 0.74 of
+// the burst rate, 0.87 of the sustained one, with the clock down to 1.6 GHz
+// under the power limit.  At head_dim 64 the products are half as long and the
+// exponentials bound it (16 per cycle and SM), so a quarter of them runs as a
+// polynomial on the FMA pipe there (437 against 469 us when it was added); at
+// head_dim 128 that only costs issue slots and power (462 / 458 us).  Tried and
+// left out: P beside S at head_dim 64, so that the next S is formed during the
+// softmax (8192 tokens 207 -> 204 us, twelve ragged prompts 48 -> 51); the
+// exponentials formed with the old maximum while the new one is found (458 ->
+// 487 us: spills); the output through shared memory.
 // The MMA thread is one elected thread for the whole loop: issuing from
 // "lane 0" branches of a warp cost 90-130 cycles per MMA (606 us) where the
 // tensor core needs 64.
@@ -59,11 +65,11 @@ struct Smem {
     static constexpr int kChunks = HD / 64;
     static constexpr int kChunk = 128 * 128;           // 128 rows of one swizzled 128-byte row each
     static constexpr int kTile = kChunks * kChunk;     // one K, V or Q tile
-    static constexpr int kStages = HD == 128 ? 5 : 8;  // ring of K and V tiles
+    static constexpr int kStages = HD == 128 ? 5 : 10;  // ring of K and V tiles
     static constexpr int kOffQ = 0;
     static constexpr int kOffRing = 2 * kTile;
     static constexpr int kOffBar = kOffRing + kStages * kTile;
-    static constexpr int kOffItem = kOffBar + 320;
+    static constexpr int kOffItem = kOffBar + 384;
     static constexpr int kTotal = kOffItem + 256;
     static_assert(kTotal <= 232448, "shared memory budget");
 };
@@ -105,7 +111,7 @@ __device__ __forceinline__ void set_err(int* err, int code) {
     if (err) atomicCAS(err, 0, code);
 }
 
-// Rows of sequence s0 + lane, [r0, r1), and its keys.  Reads cu and lens as
+// Rows of sequence b, [r0, r1), and its keys.  Reads cu and lens as
 // they are: whatever they hold, rows stay inside [0, total_q) and keys inside
 // the table.
 struct SeqRows {
@@ -173,7 +179,7 @@ __device__ __forceinline__ void cut_item(Item& it, int k0, int kend, const int (
 // round by round in alternating direction, end together: a bisection over the
 // key level whose tile count brackets the number, each step a sum over the
 // sequences (32 per warp step), then a scan for the sequence.  Without
-// p.sorted (no CTA has a second item) the scan alone.
+// p.sorted (no CTA has a second item, or the order is given) the scan alone.
 template <bool PAGED, bool DUAL>
 __device__ __forceinline__ bool get_item(const Params& p, const SeqRows& near, int idx, Item& it) {
     const int lane = threadIdx.x & 31;
@@ -363,54 +369,12 @@ __device__ __forceinline__ uint64_t exp2_poly2(uint64_t y) {
                  __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t1) << 23)));
 }
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2,
-                                            int c3) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
-        "[%2];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-        : "memory");
-}
-
 // One lane of a converged warp, by elect.sync: the compiler then knows that a
 // single thread runs the branch and keeps descriptors in uniform registers.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p != 0;
-}
-
-// mbar_wait_bounded for waits on the critical path: the timer and the abort
-// flag are first read after 256 failed tries.
-__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    bool ok = mbar_try_wait(bar, parity);
-    if (!ok) {
-        uint64_t t0 = 0;
-        for (uint32_t i = 1;; ++i) {
-            ok = mbar_try_wait(bar, parity);
-            if (ok) break;
-            if ((i & 255u) == 0) {
-                const uint64_t t = globaltimer_ns();
-                if (t0 == 0) t0 = t;
-                if (*abort || t - t0 > 2000000000ull) break;
-            }
-        }
-    }
-    return __all_sync(0xffffffffu, ok);
-}
-
-// The same for one thread.
-__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    if (mbar_try_wait(bar, parity)) return true;
-    uint64_t t0 = 0;
-    for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 255u) == 0) {
-            const uint64_t t = globaltimer_ns();
-            if (t0 == 0) t0 = t;
-            if (*abort || t - t0 > 2000000000ull) return false;
-        }
-    }
 }
 
 __device__ __forceinline__ float row_max(const float (&x)[128]) {
@@ -431,7 +395,7 @@ __device__ __forceinline__ float row_max(const float (&x)[128]) {
 __device__ __forceinline__ bool next_item(const Item* slots, uint64_t* full, uint64_t* empty, uint32_t& k, Item& it,
                                           volatile int* abort, bool& ok) {
     const uint32_t s = k % kItemSlots;
-    ok = wait_all(&full[s], (k / kItemSlots) & 1u, abort);
+    ok = mbar_wait_warp(&full[s], (k / kItemSlots) & 1u, abort);
     if (!ok) return false;
     it = slots[s];
     __syncwarp();
@@ -446,10 +410,10 @@ __device__ __forceinline__ bool next_item(const Item* slots, uint64_t* full, uin
 template <int HD, bool PAGED, bool PART, bool DUAL>
 __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_constant__ Params p) {
     using L = Smem<HD>;
-    // A shared-prefix phase lets its successor start only behind its own wait: the successor (paged_decode on the
-    // sequences' own keys) then needs none before its loads and runs beside this kernel.
+    // The successor may start once every CTA holds its tensor memory (it may want some itself and then wait for this
+    // kernel).  Behind a shared-prefix phase it may start only after this kernel's own wait: paged_decode on the
+    // sequences' own keys then needs no wait before its loads and runs beside this kernel.
     const bool late = PART && p.shared > 0;
-    if (!late) pdl_trigger();
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // the swizzled tiles need 1024-byte alignment
         if (threadIdx.x == 0) set_err(p.err, 0x500);
@@ -472,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(it_empty + kItemSlots);
     volatile uint32_t* vfix_stage = tmem_slot + 2;
     Item* slots = reinterpret_cast<Item*>(smem + L::kOffItem);
-    static_assert(kItemSlots * sizeof(Item) <= 256 && (13 + 2 * L::kStages + 2 * kItemSlots) * 8 + 12 <= 320, "layout");
+    static_assert(kItemSlots * sizeof(Item) <= 256 && (13 + 2 * L::kStages + 2 * kItemSlots) * 8 + 12 <= 384, "layout");
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -514,6 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
     const uint32_t tmem = *tmem_slot;
     int never = 0;
     volatile int* no_abort = &never;
+    if (!late) pdl_trigger();
     pdl_wait();
     if (late) pdl_trigger();
 
@@ -528,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             while (ok && next_item(slots, it_full, it_empty, ni, it, abort_flag, ok)) {
                 const int nblk = max(it.n[0], it.n[1]);
                 if (nblk == 0) continue;
-                ok = wait_all(q_empty, (nz & 1u) ^ 1u, abort_flag);
+                ok = mbar_wait_warp(q_empty, (nz & 1u) ^ 1u, abort_flag);
                 if (!ok) break;
                 const int nq = !DUAL && it.n[1] > 0 ? 2 : 1;
                 if (lane == 0) {
@@ -561,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                             c2 = kk & ((1 << p.page_shift) - 1);
                         }
                         const uint32_t s = n % L::kStages, ph = (n / L::kStages) & 1u;
-                        ok = wait_all(&kv_empty[s], ph ^ 1u, abort_flag);
+                        ok = mbar_wait_warp(&kv_empty[s], ph ^ 1u, abort_flag);
                         if (!ok) break;
                         uint8_t* dst = smem + L::kOffRing + s * L::kTile + ch * L::kChunk;
                         if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], (uint32_t)L::kTile);
@@ -600,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 bool ok = true;
                 while (ok) {
                     const uint32_t slot = ni % kItemSlots;
-                    ok = wait_one(&it_full[slot], (ni / kItemSlots) & 1u, abort_flag);
+                    ok = mbar_wait_quick(&it_full[slot], (ni / kItemSlots) & 1u, abort_flag);
                     if (!ok) break;
                     const Item& it = slots[slot];
                     const int n0 = it.n[0], n1 = it.n[1], state = it.state;
@@ -610,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                     if (!state) break;
                     const int nblk = max(n0, n1);
                     if (nblk == 0) continue;
-                    ok = wait_one(q_full, nz & 1u, abort_flag);
+                    ok = mbar_wait_quick(q_full, nz & 1u, abort_flag);
                     ++nz;
                     for (int j = 0; ok && j <= nblk; ++j) {
                         uint32_t vs = 0, ks = 0;
@@ -621,12 +586,12 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                             const bool mine = DUAL || q == 0;  // this tile takes the next K and V off the ring
                             if (mine && j >= 1 && j <= nkv) {  // V_{j-1}
                                 vs = st;
-                                ok = wait_one(&kv_full[st], ph, abort_flag);
+                                ok = mbar_wait_quick(&kv_full[st], ph, abort_flag);
                                 if (++st == L::kStages) st = 0, ph ^= 1u;
                                 if (ok && vfix && j == nkv && (!DUAL || q == vfix_q)) {  // warp 11's turn; P takes longer
                                     *vfix_stage = vs;
                                     mbar_arrive(v_seen);
-                                    ok = wait_one(v_fixed, nv++ & 1u, abort_flag);
+                                    ok = mbar_wait_quick(v_fixed, nv++ & 1u, abort_flag);
                                 }
                                 if (!ok) break;
                             }
@@ -635,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                                 const int steps = j < n ? kBlk / 16 : (q ? last1 : last0);
 #pragma unroll
                                 for (int hf = 0; hf < 2; ++hf) {  // the first 64 keys' P is ready ahead of the rest
-                                    ok = wait_one(&p_full[2 * q + hf], np[q] & 1u, abort_flag);
+                                    ok = mbar_wait_quick(&p_full[2 * q + hf], np[q] & 1u, abort_flag);
                                     if (!ok) break;
                                     tc_fence_after();
                                     if (steps == kBlk / 16) {
@@ -657,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                             }
                             if (mine && j < nkv) {  // K_j
                                 ks = st;
-                                ok = wait_one(&kv_full[st], ph, abort_flag);
+                                ok = mbar_wait_quick(&kv_full[st], ph, abort_flag);
                                 if (++st == L::kStages) st = 0, ph ^= 1u;
                                 if (!ok) break;
                             }
@@ -696,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             Item it;
             while (ok && next_item(slots, it_full, it_empty, ni, it, abort_flag, ok)) {
                 if (!it.vfix) continue;
-                ok = wait_all(v_seen, nv++ & 1u, abort_flag);  // the MMA thread has seen the tile land
+                ok = mbar_wait_warp(v_seen, nv++ & 1u, abort_flag);  // the MMA thread has seen the tile land
                 if (!ok) break;
                 uint8_t* v = smem + L::kOffRing + *vfix_stage * L::kTile;
                 const int vb = it.vfix, n16 = (16 - (vb & 15)) * 8;  // zeroed up to the end of the last 16-key step
@@ -725,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 it.state = base < p.n_items ? 1 : 0;
                 if (it.state && (idx >= p.n_items || !get_item<PAGED, DUAL>(p, near, (int)idx, it))) continue;
                 const uint32_t s = k % kItemSlots;
-                ok = wait_all(&it_empty[s], ((k / kItemSlots) & 1u) ^ 1u, abort_flag);
+                ok = mbar_wait_warp(&it_empty[s], ((k / kItemSlots) & 1u) ^ 1u, abort_flag);
                 if (!ok) {
                     if (lane == 0) {
                         *abort_flag = 1;
@@ -765,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             float m = -INFINITY, l = 0.0f;
             const int nb = q ? it.n[1] : it.n[0];
             for (int j = 0; j < nb; ++j) {
-                ok = wait_all(&s_full[q], ns & 1u, abort_flag);
+                ok = mbar_wait_warp(&s_full[q], ns & 1u, abort_flag);
                 if (!ok) break;
                 ++ns;
                 tc_fence_after();
@@ -823,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             }
             if (!ok) break;
             if (nb > 0) {
-                ok = wait_all(&o_full[q], no & 1u, abort_flag);
+                ok = mbar_wait_warp(&o_full[q], no & 1u, abort_flag);
                 if (!ok) break;
                 ++no;
                 tc_fence_after();
@@ -930,7 +895,7 @@ int fmha_packed(const PackedArgs& a, cudaStream_t st) {
         if (rc) return rc;
         while ((1 << p.page_shift) < a.kv.page_size) ++p.page_shift;
         const int64_t mk = (int64_t)a.kv.max_pages << p.page_shift;
-        p.max_keys = mk > 0x7fffff00 ? 0x7fffff00 : (int)mk;
+        p.max_keys = mk > 0x7ff00000 ? 0x7ff00000 : (int)mk;
         p.n_pages = a.kv.n_pages;
         p.table = a.kv.table;
         p.ldt = a.kv.ldt;
@@ -965,11 +930,11 @@ int fmha_packed(const PackedArgs& a, cudaStream_t st) {
     const int batch = a.shared > 0 ? 1 : a.batch;
     p.tiles = a.tiles;
     if (p.tiles == 0) {  // one tile per CTA while that still leaves SMs free
-        const int64_t one = fmha_packed_items(a.total_q, batch, a.heads, a.kv_heads, a.max_new, 1);
+        const int64_t one = fmha_packed_items(a.total_q, batch, a.heads, a.kv_heads, 0, 1);
         p.tiles = one * a.kv_heads <= num_sms() ? 1 : 2;
     }
-    const int64_t items = fmha_packed_items(a.total_q, batch, a.heads, a.kv_heads, a.max_new, p.tiles) * a.kv_heads *
-                          p.splits;
+    // a bound that no value of the offsets exceeds while they ascend
+    const int64_t items = fmha_packed_items(a.total_q, batch, a.heads, a.kv_heads, 0, p.tiles) * a.kv_heads * p.splits;
     if (items > 0x7fffffff) return NPUB_ERR_UNSUPPORTED;
     p.n_items = (int)items;
     const int grid = p.n_items < num_sms() ? p.n_items : num_sms();

@@ -174,10 +174,10 @@ int run_plan(const Plan& pl, PackedArgs& a, void* workspace, size_t workspace_by
 
 extern "C" int npub_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
                                      int64_t ldv, void* out, int64_t ldo, const int32_t* cu_seqlens, int batch,
-                                     int total, int max_len, int heads, int kv_heads, int head_dim, float scale,
+                                     int total, int heads, int kv_heads, int head_dim, float scale,
                                      int causal, void* stream) {
     using namespace npub;
-    NPUB_CHECK_ARG(batch >= 0 && total >= 0 && max_len >= 0 && dims_ok(heads, kv_heads, head_dim, scale));
+    NPUB_CHECK_ARG(batch >= 0 && total >= 0 && dims_ok(heads, kv_heads, head_dim, scale));
     if (batch == 0 || total == 0) return NPUB_OK;
     NPUB_CHECK_ARG(q && k && v && out && cu_seqlens);
     if (!dims_supported(heads, kv_heads, head_dim)) return NPUB_ERR_UNSUPPORTED;
@@ -200,7 +200,6 @@ extern "C" int npub_attention_packed(const void* q, int64_t ldq, const void* k, 
     a.heads = heads;
     a.kv_heads = kv_heads;
     a.head_dim = head_dim;
-    a.max_new = max_len;
     a.scale = scale;
     a.causal = causal;
     return fmha_packed(a, reinterpret_cast<cudaStream_t>(stream));

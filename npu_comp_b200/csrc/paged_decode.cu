@@ -71,14 +71,6 @@ __device__ __forceinline__ void set_err(int* err, int code) {
 }
 __device__ __forceinline__ void consumer_bar() { asm volatile("barrier.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2,
-                                            int c3) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
-        "[%2];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-        : "memory");
-}
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -194,8 +186,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
                 const int id = __ldg(p.table + (int64_t)b * p.ldt + (key >> p.page_shift));
                 if (id >= 0 && id < p.n_pages) page = id;
             }
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait_bounded(&empty[s], ((uint32_t)(j / L::kStages) & 1u) ^ 1u, abort_flag));
+            ok = mbar_wait_warp(&empty[s], ((uint32_t)(j / L::kStages) & 1u) ^ 1u, abort_flag);
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(&full[s], 2u * L::kTile);
             __syncwarp();
@@ -248,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     bool ok = true;
     for (int j = 0; j < nst; ++j) {
         const int s = j % L::kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[s], (uint32_t)(j / L::kStages) & 1u, abort_flag));
+        ok = mbar_wait_warp(&full[s], (uint32_t)(j / L::kStages) & 1u, abort_flag);
         if (!ok) break;
         const int kb = k0 + j * kKeys + warp * 16;  // first key of this warp
         if (kb < k1) {
@@ -529,7 +520,7 @@ int paged_decode(const PackedArgs& a, cudaStream_t st) {
     if (rc) return rc;
     while ((1 << p.page_shift) < a.kv.page_size) ++p.page_shift;
     const int64_t mk = (int64_t)a.kv.max_pages << p.page_shift;
-    p.max_keys = mk > 0x7fffff00 ? 0x7fffff00 : (int)mk;
+    p.max_keys = mk > 0x7ff00000 ? 0x7ff00000 : (int)mk;
     p.n_pages = a.kv.n_pages;
     p.table = a.kv.table;
     p.ldt = a.kv.ldt;

@@ -711,13 +711,13 @@ def rope_paged_append(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: 
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, heads: int,
-                     kv_heads: Optional[int] = None, *, head_dim: Optional[int] = None, max_len: int = 0,
-                     causal: bool = True, scale: Optional[float] = None,
+                     kv_heads: Optional[int] = None, *, head_dim: Optional[int] = None, causal: bool = True,
+                     scale: Optional[float] = None,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """attention() (llama_layer.py:114-137) over packed prompts of different
     lengths: q [total, heads*hd], k/v [total, kv_heads*hd], sequence b at rows
     cu_seqlens[b] .. cu_seqlens[b + 1] (int32 [batch + 1]).  head_dim a multiple
-    of 16 up to 128.  max_len: at least the longest sequence's rows (0: not known)."""
+    of 16 up to 128."""
     kv_heads = kv_heads or heads
     _need(heads > 0 and kv_heads > 0, "heads and kv_heads must be positive")
     dev, T, qc, ldq = _first16(q, "q")
@@ -736,7 +736,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         scale = 1.0 / math.sqrt(max(hd, 1))
     out, ldo = _out16(out, q, T, heads * hd, dev)
     _launch("npub_attention_packed", dev, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
-            cu, B, T, int(max_len), heads, kv_heads, hd, scale, 1 if causal else 0)
+            cu, B, T, heads, kv_heads, hd, scale, 1 if causal else 0)
     return out
 
 
@@ -749,8 +749,9 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     [batch]) and its new rows (cu_seqlens) the last of them.  Prompt chunks,
     prompts behind a cached prefix, drafted tokens.
 
-    max_new: at least the new rows of any sequence (0: not known; when
-    max_new * heads / kv_heads <= 16 the kernel for few rows runs); ctx_len: the
+    max_new: at least the new rows of any sequence (rows past it may be left
+    out; 0: not known); up to 16 * kv_heads / heads of them run on the kernel
+    for few rows.  ctx_len: the
     largest lens expected (0: the table's width), which only decides how keys
     are split over CTAs.  page_size 16 .. 256."""
     dev, T, qc, ldq = _first16(q, "q")

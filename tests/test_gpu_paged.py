@@ -100,7 +100,7 @@ def test_append_unstored_rows_and_in_place(cuda_device):
 
 # ------------------------------------------------------------------- packed
 
-def run_packed(dev, lens, H, KV, hd, causal=True, behind=3, max_len=0, bad=(), scale=None, spread=1.0):
+def run_packed(dev, lens, H, KV, hd, causal=True, behind=3, bad=(), scale=None, spread=1.0):
     g = torch.Generator(device=dev).manual_seed(sum(lens) * 7 + H)
     T = sum(lens)
     x = spread * torch.randn((T + behind, (H + 2 * KV) * hd), generator=g, device=dev)
@@ -111,7 +111,7 @@ def run_packed(dev, lens, H, KV, hd, causal=True, behind=3, max_len=0, bad=(), s
     x[T:] = float("nan")
     q, k, v = x[:, :H * hd], x[:, H * hd:(H + KV) * hd], x[:, (H + KV) * hd:]
     out = torch.full((T + behind, H * hd), 3.0, dtype=torch.float16, device=dev)
-    o = nb.attention_packed(q, k, v, cu, H, KV, head_dim=hd, max_len=max_len, causal=causal, scale=scale, out=out)
+    o = nb.attention_packed(q, k, v, cu, H, KV, head_dim=hd, causal=causal, scale=scale, out=out)
     assert npu.device_error() == 0
     assert (o[T:] == 3.0).all()
     sc = scale or 1 / math.sqrt(hd)
@@ -132,7 +132,7 @@ def run_packed(dev, lens, H, KV, hd, causal=True, behind=3, max_len=0, bad=(), s
 ])
 @pytest.mark.parametrize("causal", [True, False])
 def test_packed(cuda_device, lens, H, KV, hd, causal):
-    run_packed(cuda_device, lens, H, KV, hd, causal, max_len=max(lens) if sum(lens) % 2 else 0)
+    run_packed(cuda_device, lens, H, KV, hd, causal)
 
 
 def test_packed_neighbours_do_not_leak(cuda_device):
@@ -422,6 +422,102 @@ def test_graph_replay_and_streams(cuda_device):
         check_rows(o, q, kp, vp, table, [1] * B, keys, H, ps)
         check_rows(o2, other, kp, vp, table, [1] * B, lens2.tolist(), H, ps)
     del graph
+
+
+def test_rows_outside_the_offsets_stay(cuda_device):
+    """Offsets that start behind row 0 and end ahead of the last row, and
+    outputs whose rows are only 16-byte aligned."""
+    dev, H, KV, hd, ps = cuda_device, 4, 2, 80, 16
+    g = torch.Generator(device=dev).manual_seed(8)
+    T, cu = 60, torch.tensor([5, 5, 40, 57], dtype=torch.int32, device=dev)
+    x = torch.randn((T, (H + 2 * KV) * hd), generator=g, device=dev).half()
+    q, k, v = x[:, :H * hd], x[:, H * hd:(H + KV) * hd], x[:, (H + KV) * hd:]
+    kp, vp, table, lens = make_cache(dev, [7, 200, 90], KV, hd, ps)
+    f = nb.rope_freqs(hd, device=dev)
+    for run in (lambda o: nb.attention_packed(q, k, v, cu, H, KV, head_dim=hd, out=o),
+                lambda o: nb.attention_paged(q.contiguous(), kp, vp, table, lens, cu, heads=H, out=o),
+                lambda o: nb.attention_paged(q.contiguous(), kp, vp, table, lens, cu, heads=H, ctx_len=64, out=o),
+                lambda o: nb.rope_paged_append(x, H, KV, hd, torch.zeros(T, dtype=torch.int32, device=dev), f,
+                                               kp.clone(), vp.clone(), table, cu_seqlens=cu, out=o)):
+        outs = []
+        for off, pad in ((0, 0), (8, 24)):
+            base = torch.full((T, off + H * hd + pad), 3.0, dtype=torch.float16, device=dev)
+            o = run(base[:, off:off + H * hd])
+            assert (o[:5] == 3.0).all() and (o[57:] == 3.0).all() and (o[5:57] != 3.0).any(dim=1).all()
+            assert (base[:, :off] == 3.0).all() and (base[:, off + H * hd:] == 3.0).all()
+            outs.append(o.clone())
+        assert torch.equal(*outs)
+    o = nb.attention_packed(q, k, v, cu, H, KV, head_dim=hd)
+    e, b = attention64(q[40:57].reshape(-1, H, hd), k[40:57].reshape(-1, KV, hd), v[40:57].reshape(-1, KV, hd),
+                       1 / math.sqrt(hd))
+    within(o[40:57], e, b)
+
+
+def test_many_sequences(cuda_device):
+    """More sequences than a warp holds, of 0 to 90 rows, and a long one."""
+    lens = [(i * 37) % 91 for i in range(200)] + [900]
+    run_packed(cuda_device, lens, 8, 2, 64)
+    run_packed(cuda_device, lens, 16, 16, 128)
+    dev, H, KV, hd, ps = cuda_device, 8, 2, 128, 16
+    new = [(i * 5) % 7 for i in range(100)] + [70]
+    keys = [n + (i * 53) % 300 for i, n in enumerate(new)]
+    kp, vp, table, ln = make_cache(dev, keys, KV, hd, ps)
+    q = torch.randn((sum(new), H * hd), device=dev).half()
+    check_rows(nb.attention_paged(q, kp, vp, table, ln, offsets(new, dev), heads=H), q, kp, vp, table, new, keys, H, ps)
+
+
+@pytest.mark.parametrize("H,KV,hd", [(8, 8, 128), (16, 1, 64), (64, 1, 128)])
+def test_long_context(cuda_device, H, KV, hd):
+    """Contexts past 2^16 keys: the largest numbers of key ranges."""
+    dev, ps, keys = cuda_device, 64, [70001, 1, 66000]
+    kp, vp, table, lens = make_cache(dev, keys, KV, hd, ps)
+    q = torch.randn((3, H * hd), device=dev).half()
+    for kw in (dict(), dict(ctx_len=70001)):
+        check_rows(nb.attention_paged_decode(q, kp, vp, table, lens, heads=H, **kw), q, kp, vp, table, [1] * 3, keys,
+                   H, ps)
+    check_rows(nb.attention_paged_decode(q[:1], kp, vp, table[:1], lens[:1], heads=H), q[:1], kp, vp, table[:1], [1],
+               keys[:1], H, ps)
+
+
+def test_prompt_graph_replay(cuda_device):
+    """Packed prompts and chunks captured once, replayed with other offsets and
+    lengths of the same totals; two graphs do not share scratch."""
+    dev, H, KV, hd, ps, B, T = cuda_device, 8, 2, 128, 16, 3, 90
+    keys = [400, 500, 300]
+    kp, vp, table, lens = make_cache(dev, keys, KV, hd, ps)
+    g = torch.Generator(device=dev).manual_seed(6)
+    x = torch.randn((T, (H + 2 * KV) * hd), generator=g, device=dev).half()
+    q, k, v = x[:, :H * hd], x[:, H * hd:(H + KV) * hd], x[:, (H + KV) * hd:]
+    qc = q.contiguous()
+    cu = offsets([30, 30, 30], dev)
+    nb.attention_paged(qc, kp, vp, table, lens, cu, heads=H)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            a = nb.attention_packed(q, k, v, cu, H, KV, head_dim=hd)
+            b = nb.attention_paged(qc, kp, vp, table, lens, cu, heads=H)
+        graphs.append((graph, a, b))
+    side = torch.cuda.Stream(device=dev)
+    for new, left in (([1, 60, 29], [400, 77, 300]), ([0, 0, 90], [1, 500, 90])):
+        cu.copy_(offsets(new, dev))
+        lens.copy_(torch.tensor(left))
+        torch.cuda.synchronize()
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+        torch.cuda.synchronize()
+        for _, a, b in graphs:
+            at = 0
+            for n in new:
+                if n:
+                    r = slice(at, at + n)
+                    e, bound = attention64(q[r].reshape(n, H, hd), k[r].reshape(n, KV, hd), v[r].reshape(n, KV, hd),
+                                           1 / math.sqrt(hd))
+                    within(a[r], e, bound)
+                at += n
+            check_rows(b, qc, kp, vp, table, new, left, H, ps)
+    graphs.clear()
 
 
 def test_python_refusals(cuda_device):

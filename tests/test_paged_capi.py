@@ -25,9 +25,9 @@ def test_append_refusals(libnpub_path):
         assert append(lib, **kw) == -1, kw
 
 
-def packed(lib, q=P, ldq=512, k=P, ldk=256, v=P, ldv=256, out=P, ldo=512, cu=P, batch=2, total=8, max_len=0, h=4,
-           kv=2, hd=128, scale=0.1):
-    return lib.npub_attention_packed(q, ldq, k, ldk, v, ldv, out, ldo, cu, batch, total, max_len, h, kv, hd, scale, 1,
+def packed(lib, q=P, ldq=512, k=P, ldk=256, v=P, ldv=256, out=P, ldo=512, cu=P, batch=2, total=8, h=4, kv=2,
+           hd=128, scale=0.1):
+    return lib.npub_attention_packed(q, ldq, k, ldk, v, ldv, out, ldo, cu, batch, total, h, kv, hd, scale, 1,
                                      None)
 
 
@@ -37,7 +37,7 @@ def test_packed_refusals(libnpub_path):
     for kw in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(cu=None), dict(q=ODD), dict(k=ODD),
                dict(v=ODD), dict(out=ODD), dict(ldq=504), dict(ldk=248), dict(ldv=260), dict(ldo=511), dict(h=3),
                dict(kv=0), dict(hd=0), dict(hd=100), dict(scale=0.0), dict(scale=float("inf")),
-               dict(scale=float("nan")), dict(max_len=-1), dict(total=-1), dict(batch=-1)):
+               dict(scale=float("nan")), dict(total=-1), dict(batch=-1)):
         assert packed(lib, **kw) == -1, kw
     assert packed(lib, hd=144, ldq=1024, ldk=512, ldv=512, ldo=1024) == -2
     assert packed(lib, h=256, kv=1, hd=16, ldq=4096, ldo=4096) == -2
