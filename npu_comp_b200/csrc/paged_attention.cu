@@ -31,8 +31,8 @@ bool pool_ok(const void* k, const void* v, int n_pages, int page_size, const int
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How the keys of a call are cut.  The partials are numbered through: the shared prefix's splits, then those of the
-// sequences' own keys.  The last split of either takes every key that is left, so ctx_len only decides the cut.
+// How the keys of a call are cut.  The partials are numbered through: the shared prefix's, then those of the sequences'
+// own keys.  The ranges are equal parts of what each sequence holds, so ctx_len only decides their number.
 struct Phase {
     int tiles, dual;  // tile kernel: rows of an item, and whether its keys go in two halves
     int splits;
