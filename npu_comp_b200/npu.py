@@ -568,22 +568,28 @@ def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v
 # These ops run between two launches of a decode step, where 10 us of Python
 # are more than the kernels take: their checks build no message unless they
 # fail, and read the stream's handle without making a Stream object (a decode
-# step's append: 30 us per call with the checks of the ops above, HOSTUS so, of
+# step's append: 30 us per call with the checks of the ops above, 12 us so, of
 # which 5 us are the C call).
 
 _Tensor, _f16, _i32 = torch.Tensor, torch.float16, torch.int32
 
 
-def _launch(name: str, dev: int, *args) -> None:
-    """Call an entry point on device index dev's current stream (the last argument)."""
-    f = _lib.bound(name)
-    if torch._C._cuda_getDevice() == dev:
-        st = f(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            st = f(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if st:
-        _lib.fail(name, st)
+class _Here:
+    """The context of a tensor on the current device: nothing to do."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def _device(dev: int):
+    """A context in which device index dev is current."""
+    return _here if torch._C._cuda_getDevice() == dev else torch.cuda.device(dev)
 
 
 def _first16(t: torch.Tensor, name: str):
@@ -635,7 +641,7 @@ def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor
 def _out16(out: Optional[torch.Tensor], like: torch.Tensor, rows: int, cols: int, dev: int):
     """(output [rows, cols], its leading dimension)"""
     if out is None:
-        return like.new_empty((rows, cols)), cols
+        return like.new_empty(rows, cols), cols
     n, c, ld = _rows16(out, "out", dev)
     if n != rows or c != cols:
         raise ValueError(f"out must be [{rows}, {cols}]")
@@ -704,9 +710,13 @@ def rope_paged_append(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: 
     else:
         cu = _ints(cu_seqlens, "cu_seqlens", B + 1, dev)
     out, ldq = _out16(out, qkv, T, q_heads * head_dim, dev)
-    _launch("npub_rope_paged_append", dev, qkv.data_ptr(), ldx, out.data_ptr(), ldq, T, q_heads, kv_heads, head_dim, R,
+    with _device(dev):
+        st = _lib.bound("npub_rope_paged_append")(
+            qkv.data_ptr(), ldx, out.data_ptr(), ldq, T, q_heads, kv_heads, head_dim, R,
             1 if interleaved else 0, pos, inv_freq.data_ptr(), gq, gk, eps, k_pages.data_ptr(), v_pages.data_ptr(),
-            n_pages, ps, page_table.data_ptr(), ldt, W, cu, B)
+            n_pages, ps, page_table.data_ptr(), ldt, W, cu, B, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail("npub_rope_paged_append", st)
     return out
 
 
@@ -735,8 +745,12 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if scale is None:
         scale = 1.0 / math.sqrt(max(hd, 1))
     out, ldo = _out16(out, q, T, heads * hd, dev)
-    _launch("npub_attention_packed", dev, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
-            cu, B, T, heads, kv_heads, hd, scale, 1 if causal else 0)
+    with _device(dev):
+        st = _lib.bound("npub_attention_packed")(
+            q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
+            cu, B, T, heads, kv_heads, hd, scale, 1 if causal else 0, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail("npub_attention_packed", st)
     return out
 
 
@@ -766,9 +780,13 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ctx = min(int(ctx_len), W * ps) if ctx_len > 0 else W * ps
     out, ldo = _out16(out, q, T, heads * hd, dev)
     ws, wsp, wsb = _paged_workspace(q, dev, "npub_attention_paged_workspace", B, T, max_new, ctx, heads, kv_heads, hd)
-    _launch("npub_attention_paged", dev, q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
+    with _device(dev):
+        st = _lib.bound("npub_attention_paged")(
+            q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
             page_table.data_ptr(), ldt, W, ln, cu, B, T, max_new, ctx, out.data_ptr(), ldo, heads, kv_heads, hd, scale,
-            1 if causal else 0, wsp, wsb)
+            1 if causal else 0, wsp, wsb, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail("npub_attention_paged", st)
     return out
 
 
@@ -795,9 +813,13 @@ def attention_paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     out, ldo = _out16(out, q, B, heads * hd, dev)
     ws, wsp, wsb = _paged_workspace(q, dev, "npub_attention_paged_decode_workspace", B, ctx, shared_len, heads,
                                     kv_heads, hd)
-    _launch("npub_attention_paged_decode", dev, q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
+    with _device(dev):
+        st = _lib.bound("npub_attention_paged_decode")(
+            q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, ps,
             page_table.data_ptr(), ldt, W, ln, B, ctx, shared_len, out.data_ptr(), ldo, heads, kv_heads, hd, scale,
-            wsp, wsb)
+            wsp, wsb, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail("npub_attention_paged_decode", st)
     return out
 
 
