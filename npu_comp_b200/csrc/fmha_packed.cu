@@ -30,9 +30,12 @@
 // polynomial on the FMA pipe there (437 against 469 us when it was added); at
 // head_dim 128 that only costs issue slots and power (462 / 458 us).  Tried and
 // left out: P beside S at head_dim 64, so that the next S is formed during the
-// softmax (8192 tokens 207 -> 204 us, twelve ragged prompts 48 -> 51); the
+// softmax (8192 tokens 207 -> 204 us, twelve ragged prompts 48 -> 51); two
+// threads per row, 16 softmax warps (454 -> 495-553 us, 48 -> 56: the pairs'
+// exchange and the second read of S, which 104 registers force); the
 // exponentials formed with the old maximum while the new one is found (458 ->
-// 487 us: spills); the output through shared memory.
+// 487 us: spills); P handed over as 96 + 32 keys (no difference); the output
+// through shared memory.
 // The MMA thread is one elected thread for the whole loop: issuing from
 // "lane 0" branches of a warp cost 90-130 cycles per MMA (606 us) where the
 // tensor core needs 64.

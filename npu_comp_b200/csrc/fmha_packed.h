@@ -27,7 +27,6 @@ struct PackedArgs {
     const int32_t* cu;    // [batch + 1]; null: one row per sequence
     const int32_t* lens;  // pages: keys of each sequence (shared-prefix phase: of each row)
     int total_q, batch, heads, kv_heads, head_dim;
-    int max_new;          // rows of the longest sequence (0: not known)
     int shared;           // > 0: shared-prefix phase, the first `shared` keys of row 0's pages for all rows
     float scale;
     int causal;
@@ -41,7 +40,8 @@ struct PackedArgs {
 };
 
 int fmha_packed(const PackedArgs& a, cudaStream_t st);
-// Row-tile items (per kv head) that fmha_packed runs for these sizes, an upper bound.
+// Items (per kv head) of `tiles` row tiles: at most this many for rows in ascending offsets; max_new > 0: for sequences
+// of no more rows (estimates only).
 int64_t fmha_packed_items(int total_q, int batch, int heads, int kv_heads, int max_new, int tiles);
 // 4-D map of a page pool [n_pages, kv_heads, page_size, head_dim], box {64, box_rows, 1, 1}, 128-byte swizzle.
 int make_tmap_pages(CUtensorMap* m, const void* base, int n_pages, int kv_heads, int page_size, int head_dim,

@@ -152,7 +152,6 @@ int run_plan(const Plan& pl, PackedArgs& a, void* workspace, size_t workspace_by
         s.shared = pl.shared;
         s.causal = 0;
         s.cu = nullptr;
-        s.max_new = 0;
         s.splits = pl.pre.splits;
         s.tiles = pl.pre.tiles;
         s.dual = pl.pre.dual;
@@ -238,7 +237,6 @@ extern "C" int npub_attention_paged(const void* q, int64_t ldq, const void* k_pa
     a.heads = heads;
     a.kv_heads = kv_heads;
     a.head_dim = head_dim;
-    a.max_new = max_new;
     a.scale = scale;
     a.causal = causal;
     const int64_t cap = (int64_t)max_pages * page_size;
@@ -287,7 +285,6 @@ extern "C" int npub_attention_paged_decode(const void* q, int64_t ldq, const voi
     a.heads = heads;
     a.kv_heads = kv_heads;
     a.head_dim = head_dim;
-    a.max_new = 1;
     a.scale = scale;
     a.causal = 1;
     const int64_t cap = (int64_t)max_pages * page_size;
