@@ -84,85 +84,73 @@ __device__ __forceinline__ int seq_of_row(const int32_t* __restrict__ cu, int ba
     return -1;
 }
 
-// Block (x, y): TOK tokens, and of their 16-element units every gridDim.y-th run
-// of kAppThreads, one unit per thread and step.  A thread loads its first unit
-// before the block forms the angles and looks up the pages.
+// Block (x, y): token x, and of its 16-element units every gridDim.y-th run of
+// kAppThreads, one unit per thread and step.  A thread loads its first unit
+// before the block forms the angles and looks up the page.
 //
 // Measured at 8192 packed tokens of 32 / 8 heads of 128 with norms (201 MB):
-// 40.8 us with two tokens and 128 threads, 4.9 TB/s or 0.76 of the copy rate;
-// 43.5 with 256 threads, 46-48 with two or three units in flight per thread
-// (their registers cost more warps than they bring loads), 51 with the
-// arithmetic one element at a time: the instructions, not the loads, are what
-// competes with HBM here, so it runs on pairs (f32x2) and v heads are copied.
-template <int TOK>
+// 37.2 us with 128 threads, 5.4 TB/s or 0.83 of the copy rate (39.3 and 41.9
+// with the heads of a token over two and three blocks); 43 with 96 or
+// 192 threads, 39.6 and 45 with two and four tokens per block, 46-48 with two
+// or three units in flight per thread (their registers cost more warps than
+// they bring loads), 51 with the arithmetic one element at a time: the
+// instructions, not the loads, are what competes with HBM here, so it runs on
+// pairs (f32x2) and v heads are copied.
 __global__ void __launch_bounds__(kAppThreads) rope_paged_append_kernel(const AppendArgs a) {
     pdl_trigger();
     // {cos, cos', sin, sin'} of the pairs 8 u + 2 e and 8 u + 2 e + 1 at [e][u]: the lanes of a head (u = 0, 1, ...)
     // read neighbouring words
-    __shared__ float4 turn[TOK][kMaxHalf / 2];
-    __shared__ int page_of[TOK], slot_of[TOK];
+    __shared__ float4 turn[kMaxHalf / 2];
+    __shared__ int page_of, slot_of;
     pdl_wait();
-    const int t0 = blockIdx.x * TOK;
+    const int t = blockIdx.x;
     const int heads = a.hq + 2 * a.hk;
     const int total = ((heads << a.units_log2) + 31) & ~31;  // units of a token, whole warps (the norm's shuffles)
     const int rot_units = a.half >> 3;
     const bool any_norm = a.gq || a.gk;
     bool first = true;
-    for (int base = blockIdx.y * kAppThreads; base < TOK * total; base += gridDim.y * kAppThreads) {
-        int i = base + threadIdx.x, tk = 0;
-#pragma unroll
-        for (int n = 0; n < (TOK > 1 ? TOK : 0); ++n)
-            if (i >= total) {
-                i -= total;
-                ++tk;
-            }
-        const bool in = tk < TOK && t0 + tk < a.tokens;  // the same for a whole warp
+    for (int base = blockIdx.y * kAppThreads; base < total; base += gridDim.y * kAppThreads) {
+        const int i = base + threadIdx.x;
         const int h = i >> a.units_log2, u = i & (a.units_p2 - 1);
-        const bool act = in && h < heads && u < a.units;
+        const bool act = h < heads && u < a.units;
         // the unit's two 8-element chunks: the two halves of a rotated pair, else neighbours
         const bool split = !a.interleaved && u < rot_units;
         const int c0 = split ? u * 8 : u * 16, c1 = split ? c0 + a.half : c0 + 8;
         uint4 o0 = make_uint4(0, 0, 0, 0), o1 = o0;
         if (act) {
-            const __half* x = a.x + (int64_t)(t0 + tk) * a.ldx + (int64_t)h * a.hd;
+            const __half* x = a.x + (int64_t)t * a.ldx + (int64_t)h * a.hd;
             o0 = *reinterpret_cast<const uint4*>(x + c0);
             o1 = *reinterpret_cast<const uint4*>(x + c1);
         }
         if (first) {
             first = false;
-#pragma unroll
-            for (int tk = 0; tk < TOK; ++tk) {
-                const int t = t0 + tk;
-                if (t >= a.tokens) break;
-                const int p = a.pos[t];
-                for (int i = threadIdx.x; i < a.half; i += kAppThreads) {
-                    const double turns = (double)p * (double)a.inv_freq[i] * 0.15915494309189535;  // 1 / (2 pi)
-                    float s, c;
-                    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-                    float* w = reinterpret_cast<float*>(&turn[tk][((i & 7) >> 1) * rot_units + (i >> 3)]) + (i & 1);
-                    w[0] = c;
-                    w[2] = s;
+            const int p = a.pos[t];
+            for (int k = threadIdx.x; k < a.half; k += kAppThreads) {
+                const double turns = (double)p * (double)a.inv_freq[k] * 0.15915494309189535;  // 1 / (2 pi)
+                float s, c;
+                sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+                float* w = reinterpret_cast<float*>(&turn[((k & 7) >> 1) * rot_units + (k >> 3)]) + (k & 1);
+                w[0] = c;
+                w[2] = s;
+            }
+            if ((threadIdx.x >> 5) == kAppThreads / 32 - 1) {  // the last warp has the fewest angles
+                const int seq = a.cu ? seq_of_row(a.cu, a.batch, t) : t;
+                // a position outside the table, or a page outside the pool, is not stored (-1); a row of no sequence
+                // stays as it is (-2)
+                int page = seq < 0 ? -2 : -1;
+                if (seq >= 0 && p >= 0 && (p >> a.page_shift) < a.max_pages) {
+                    const int id = a.table[(int64_t)seq * a.ldt + (p >> a.page_shift)];
+                    if (id >= 0 && id < a.n_pages) page = id;
                 }
-                if ((threadIdx.x >> 5) == kAppThreads / 32 - 1 - tk) {  // one warp per token, from the last on
-                    const int seq = a.cu ? seq_of_row(a.cu, a.batch, t) : t;
-                    // a position outside the table, or a page outside the pool, is not stored (-1); a row of no
-                    // sequence stays as it is (-2)
-                    int page = seq < 0 ? -2 : -1;
-                    if (seq >= 0 && p >= 0 && (p >> a.page_shift) < a.max_pages) {
-                        const int id = a.table[(int64_t)seq * a.ldt + (p >> a.page_shift)];
-                        if (id >= 0 && id < a.n_pages) page = id;
-                    }
-                    if ((threadIdx.x & 31) == 0) {
-                        page_of[tk] = page;
-                        slot_of[tk] = p & ((1 << a.page_shift) - 1);
-                    }
+                if ((threadIdx.x & 31) == 0) {
+                    page_of = page;
+                    slot_of = p & ((1 << a.page_shift) - 1);
                 }
             }
             __syncthreads();
         }
-        if (!in) continue;
         const bool isq = h < a.hq, isv = h >= a.hq + a.hk;
-        const int page = page_of[tk];
+        const int page = page_of;
         const __half* g = isv ? nullptr : isq ? a.gq : a.gk;
         const bool turns = !isv && u < rot_units;
         if (__any_sync(0xffffffffu, turns || g)) {  // a warp of v heads copies
@@ -191,7 +179,7 @@ __global__ void __launch_bounds__(kAppThreads) rope_paged_append_kernel(const Ap
                 }
             }
             if (turns) {
-                const float4* cs = &turn[tk][u];
+                const float4* cs = &turn[u];
                 if (split) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -223,11 +211,11 @@ __global__ void __launch_bounds__(kAppThreads) rope_paged_append_kernel(const Ap
         if (!act || page == -2) continue;
         __half* dst;
         if (isq) {
-            dst = a.q + (int64_t)(t0 + tk) * a.ldq + (int64_t)h * a.hd;
+            dst = a.q + (int64_t)t * a.ldq + (int64_t)h * a.hd;
         } else {
             if (page < 0) continue;
             const int kvh = isv ? h - a.hq - a.hk : h - a.hq;
-            dst = (isv ? a.vp : a.kp) + ((((int64_t)page * a.hk + kvh) << a.page_shift) + slot_of[tk]) * a.hd;
+            dst = (isv ? a.vp : a.kp) + ((((int64_t)page * a.hk + kvh) << a.page_shift) + slot_of) * a.hd;
         }
         *reinterpret_cast<uint4*>(dst + c0) = o0;
         *reinterpret_cast<uint4*>(dst + c1) = o1;
@@ -289,9 +277,7 @@ extern "C" int npub_rope_paged_append(const void* qkv, int64_t ldx, void* q_out,
     a.batch = batch;
     const int total = (((q_heads + 2 * kv_heads) << a.units_log2) + 31) & ~31;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (tokens < 4 * num_sms()) {  // one unit per thread, blocks over the heads
-        const int groups = (total + kAppThreads - 1) / kAppThreads;
-        return launch_pdl(rope_paged_append_kernel<1>, dim3(tokens, groups), dim3(kAppThreads), 0, st, a);
-    }
-    return launch_pdl(rope_paged_append_kernel<2>, dim3((tokens + 1) / 2), dim3(kAppThreads), 0, st, a);
+    // few tokens: blocks over the heads too, one unit per thread
+    const int groups = tokens < 4 * num_sms() ? (total + kAppThreads - 1) / kAppThreads : 1;
+    return launch_pdl(rope_paged_append_kernel, dim3(tokens, groups), dim3(kAppThreads), 0, st, a);
 }
