@@ -352,7 +352,8 @@ __device__ __forceinline__ uint64_t exp2_hw2(uint64_t y) {
 // 1.5 * 2^23, which leaves n in the low bits of the sum) and |f| <= 1/2, the
 // degree-4 interpolation of 2^f at the Chebyshev points of [-1/2, 1/2] (largest
 // relative error 4e-6, a hundredth of half a step of fp16), and n added to the
-// exponent field.  y is held at -126, below which P is zero in fp16 anyway.
+// exponent field.  y is held at -126, below which P is zero in fp16 anyway; so is
+// a NaN, which the row's end puts right.
 __device__ __forceinline__ uint64_t exp2_poly2(uint64_t y) {
     float a, b;
     unpack2(y, a, b);
@@ -802,6 +803,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             const int64_t row = (int64_t)it.q_row0 + tok;
             const int head = it.kvh * p.group + g;
             const bool none = m == -INFINITY;  // no key: zeros (no partial)
+            // A score of +inf or NaN: the row is NaN, as x - m is in the formula.  Its weights need not be: exp2_poly2
+            // holds a NaN at 2^-126, and the sum and O would then be zeros.
+            if (!(m < INFINITY)) l = NAN;
             const int sp = p.split0 + (DUAL ? 2 * it.split + q : it.split);
             const int64_t at = PART ? ((int64_t)sp * p.total_q + row) * p.heads + head : 0;
             if (PART && valid) p.part_ml[at] = none ? make_float2(-INFINITY, 0.0f) : make_float2(m * c, l);

@@ -1,0 +1,96 @@
+"""The paged-cache operators on the GPU where calls go wrong most easily
+(paged_exact.py derives the bounds)."""
+import math
+
+import pytest
+import torch
+
+import npu_comp_b200 as nb
+from npu_comp_b200 import npu
+from paged_exact import attention_exact, same, to_pages
+
+pytestmark = pytest.mark.gpu
+
+
+def offsets(lens, dev):
+    return torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32, device=dev)
+
+
+# How a call reaches each kernel: new rows and keys per sequence, heads, the keys that take turns in the test.
+#   packed / tiles: tile kernel, keys whole; ranges: the tile kernel's partials; few: up to 16 rows per kv head, keys
+#   whole, in a cluster, or as partials; decode, prefix: one row, with and without a shared prefix
+PATHS = {
+    "packed": ([200, 70, 1], [200, 70, 1], 4, 2),
+    "tiles": ([150, 3, 9], [300, 77, 4], 4, 2),
+    "ranges": ([40, 2], [9000, 300], 8, 2),
+    "few": ([3, 1, 4], [100, 70, 2], 4, 2),
+    "few_long": ([3, 1, 4], [6000, 70, 700], 4, 2),
+    "decode": ([1] * 4, [300, 0, 65, 2000], 8, 2),
+    "prefix": ([1] * 4, [700, 520, 600, 513], 8, 2),
+}
+
+
+class Call:
+    """One call of PATHS with random inputs; x.run() compares every row with the 64-bit form."""
+
+    def __init__(self, dev, path, hd, causal=True, ps=16):
+        self.path, self.hd, self.causal, self.ps, self.dev = path, hd, causal, ps, dev
+        self.new, self.keys, self.H, self.KV = PATHS[path]
+        g = torch.Generator(device=dev).manual_seed(hd + sum(self.keys))
+        rnd = lambda *s: torch.randn(s, generator=g, device=dev).half()  # noqa: E731
+        self.q = [rnd(n, self.H, hd) for n in self.new]
+        self.k = [rnd(n, self.KV, hd) for n in self.keys]
+        self.v = [rnd(n, self.KV, hd) for n in self.keys]
+        self.shared = 512 if path == "prefix" else 0
+        for x in (self.k, self.v):
+            for y in x[1:]:
+                y[:self.shared] = x[0][:self.shared]
+
+    def run(self):
+        dev, H, KV, hd = self.dev, self.H, self.KV, self.hd
+        q, cu = torch.cat(self.q).reshape(-1, H * hd), offsets(self.new, dev)
+        if self.path == "packed":
+            o = nb.attention_packed(q, torch.cat(self.k).reshape(-1, KV * hd), torch.cat(self.v).reshape(-1, KV * hd),
+                                    cu, H, KV, head_dim=hd, causal=self.causal)
+        else:
+            kp, vp, table, lens = to_pages(self.k, self.v, self.ps, shared=self.shared)
+            if self.path in ("decode", "prefix"):
+                o = nb.attention_paged_decode(q, kp, vp, table, lens, heads=H, shared_len=self.shared)
+            else:
+                o = nb.attention_paged(q, kp, vp, table, lens, cu, heads=H, causal=self.causal,
+                                       max_new=max(self.new) if "few" in self.path else 0)
+        assert npu.device_error() == 0
+        want = [attention_exact(a, b, c, 1 / math.sqrt(hd), self.causal) for a, b, c in zip(self.q, self.k, self.v)]
+        same(o, torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want]))
+        return o
+
+
+@pytest.mark.parametrize("hd", [16, 64, 96, 128])
+@pytest.mark.parametrize("path", PATHS)
+def test_infinite_and_nan_scores(cuda_device, path, hd):
+    """A key whose score is +inf or NaN makes the rows that see it NaN, and no
+    other row: at every place of a group of eight keys, in the first, a middle
+    and the last block of a row's keys."""
+    for causal in (True, False) if path not in ("decode", "prefix") else (True,):
+        c = Call(cuda_device, path, hd, causal)
+        m = c.keys[0]
+        for j in sorted({*range(8), 64, 65, min(129, m - 1), m // 2, *range(m - 9, m)}):
+            for value in (math.inf, math.nan):
+                if value != value and j % 8 != 1:
+                    continue
+                k = c.k[0].clone()
+                c.q[0][..., 3] = c.q[0][..., 3].abs() + 0.125
+                c.k[0][j, 0, 3] = value
+                if c.shared:
+                    held = [y[:c.shared].clone() for y in c.k]
+                    for y in c.k[1:]:
+                        y[:c.shared] = c.k[0][:c.shared]
+                    if j < c.shared:  # all of them see it
+                        for y in c.q[1:]:
+                            y[..., 3] = y[..., 3].abs() + 0.125
+                o = c.run()
+                assert torch.isnan(o).any()
+                c.k[0] = k
+                if c.shared:
+                    for y, h in zip(c.k[1:], held[1:]):
+                        y[:c.shared] = h
