@@ -802,14 +802,18 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             // tile's MMAs, which use all of the shared-memory bandwidth.)
             const int64_t row = (int64_t)it.q_row0 + tok;
             const int head = it.kvh * p.group + g;
-            const bool none = m == -INFINITY;  // no key: zeros (no partial)
+            const bool none = lim <= kb;  // no key in the range: zeros (no partial)
             // A score of +inf or NaN: the row is NaN, as x - m is in the formula.  Its weights need not be: exp2_poly2
             // holds a NaN at 2^-126, and the sum and O would then be zeros.
             if (!(m < INFINITY)) l = NAN;
+            // Keys, but all scores -inf: 0 / 0 in the formula.  A partial (m = -inf, l = 1) weighs 2^-inf beside others
+            // that have a maximum, and NaN where none has.
+            const bool flat = m == -INFINITY;
+            if (flat) l = none ? 0.0f : PART ? 1.0f : NAN;
             const int sp = p.split0 + (DUAL ? 2 * it.split + q : it.split);
             const int64_t at = PART ? ((int64_t)sp * p.total_q + row) * p.heads + head : 0;
-            if (PART && valid) p.part_ml[at] = none ? make_float2(-INFINITY, 0.0f) : make_float2(m * c, l);
-            const bool put = valid && !(PART && none);
+            if (PART && valid) p.part_ml[at] = make_float2(flat ? -INFINITY : m * c, l);
+            const bool put = valid && !(PART && flat);
             const float inv = none ? 0.0f : 1.0f / l;
             float* dstf = p.part_o + at * p.head_dim;
             __half* dsth = p.out + row * p.ldo + (int64_t)head * p.head_dim;

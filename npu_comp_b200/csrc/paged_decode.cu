@@ -360,6 +360,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
             acc[3] += f * v.w;
         }
         const int t = r / p.group, head = kvh * p.group + r - t * p.group;
+        // keys, but all scores -inf: 0 / 0 in the formula, (-inf, 1) for a combination
+        const bool flat = mm == -INFINITY && sum == 0.0f && (p.causal ? min(k1, len - nrow + t + 1) : k1) > k0;
+        if (flat) sum = 1.0f;
         if (p.cluster) {
             if (d == 0)
                 *reinterpret_cast<float2*>(smem + L::kOffOwnMl + r * 8) =
@@ -369,10 +372,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
         } else if (part) {
             const int64_t at = ((int64_t)(p.split0 + split) * p.total_q + row0 + t) * p.heads + head;
             if (d == 0) p.part_ml[at] = make_float2(mm == -INFINITY ? -INFINITY : mm * c, sum);
-            if (sum != 0.0f)
+            if (sum != 0.0f && !flat)
                 *reinterpret_cast<float4*>(p.part_o + at * p.head_dim + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         } else {
-            const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+            const float inv = flat ? NAN : sum != 0.0f ? 1.0f / sum : 0.0f;
             uint2 w;
             w.x = sum != 0.0f ? h2(acc[0] * inv, acc[1] * inv) : 0u;
             w.y = sum != 0.0f ? h2(acc[2] * inv, acc[3] * inv) : 0u;

@@ -94,3 +94,23 @@ def test_infinite_and_nan_scores(cuda_device, path, hd):
                 if c.shared:
                     for y, h in zip(c.k[1:], held[1:]):
                         y[:c.shared] = h
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("path", PATHS)
+def test_scores_of_minus_infinity(cuda_device, path, hd):
+    """Scores of -inf weigh nothing beside finite ones, in whole blocks and key
+    ranges too; a row all of whose scores are -inf is NaN (0 / 0), unlike a row
+    that sees no key, which is zero."""
+    c = Call(cuda_device, path, hd)
+    m = c.keys[0]
+    for n in sorted({1, 2, 64, 130, m // 2, m - 1, m}):  # the first n keys
+        k = c.k[0].clone()
+        c.q[0][..., 3] = c.q[0][..., 3].abs() + 0.125
+        c.k[0][:n, 0, 3] = -math.inf
+        if c.shared:
+            for y, x in zip(c.k[1:], c.q[1:]):
+                y[:c.shared] = c.k[0][:c.shared]
+                x[..., 3] = x[..., 3].abs() + 0.125
+        o = c.run()
+        assert torch.isnan(o).any() == (n > m - c.new[0])
+        c.k[0] = k
