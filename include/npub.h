@@ -345,9 +345,10 @@ int npub_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk
  * keys of sequence b are positions 0 .. lens[b] - 1 (int32 [batch], clipped to
  * [0, max_pages * page_size]), its n new rows the last n of them, so row i
  * sees lens[b] - n + i + 1 keys (all of them when causal == 0); a row that
- * sees none gives zeros.  max_new: at least the new rows of any sequence (rows
- * past it may be left out), or 0 when not known; up to 16 / (heads /
- * kv_heads) of them run on a kernel for few rows.  ctx_len: the largest
+ * sees none gives zeros.  max_new: at least the new rows of any sequence, or 0
+ * when not known; up to r = 16 / (heads / kv_heads) of them run on a kernel for
+ * few rows (a sequence that has more than r rows all the same gets zeros for
+ * those past its first r).  ctx_len: the largest
  * lens[b] expected (0: the table's width), which only decides how the keys
  * are split over CTAs.  A page id outside [0, n_pages) reads as zeros.
  * page_size 16 .. 256; otherwise as npub_attention_packed.  Workspace:

@@ -107,6 +107,16 @@ __device__ __forceinline__ uint32_t h2(float a, float b) {
     return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// What a row and head without keys in this range leaves: an empty partial, or a row of zeros.
+__device__ __forceinline__ void no_keys(const Params& p, bool part, int split, int row, int head) {
+    if (part) {
+        p.part_ml[((int64_t)(p.split0 + split) * p.total_q + row) * p.heads + head] = make_float2(-INFINITY, 0.0f);
+    } else {
+        for (int d = 0; d < p.head_dim; d += 4)
+            *reinterpret_cast<uint2*>(p.out + (int64_t)row * p.ldo + (int64_t)head * p.head_dim + d) = make_uint2(0, 0);
+    }
+}
+
 // grid (kv_heads * splits, batch)
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_constant__ Params p) {
@@ -129,11 +139,18 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     const bool holds = p.beside && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
     if (!p.beside) pdl_wait();
     // rows of this sequence, its keys, and this CTA's range of them
-    int row0 = b, nrow = 1;
+    int row0 = b, nseq = 1, nrow = 1;
     if (p.cu) {
         row0 = max(0, min(p.total_q, p.cu[b]));
-        nrow = max(0, min(p.total_q, p.cu[b + 1]) - row0);
-        nrow = min(nrow, kMaxRows / p.group);
+        nseq = max(0, min(p.total_q, p.cu[b + 1]) - row0);
+        nrow = min(nseq, kMaxRows / p.group);
+        if (nrow < nseq && (part || split == 0)) {  // a caller's max_new below the sequence's rows: the rest are zeros
+            const int rest = (nseq - nrow) * p.group;
+            for (int i = threadIdx.x; i < rest; i += kThreads) {
+                const int t = i / p.group;
+                no_keys(p, part, split, row0 + nrow + t, kvh * p.group + i - t * p.group);
+            }
+        }
     }
     const int R = nrow * p.group;
     const int len = max(0, min(p.lens[b], p.max_keys));
@@ -145,15 +162,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     const int nst = (k1 - k0 + kKeys - 1) / kKeys;
     if (nst == 0) {
         for (int r = threadIdx.x; r < R; r += kThreads) {
-            const int t = r / p.group, head = kvh * p.group + r - t * p.group;
-            if (part) {
-                p.part_ml[((int64_t)(p.split0 + split) * p.total_q + row0 + t) * p.heads + head] =
-                    make_float2(-INFINITY, 0.0f);
-            } else if (split == 0) {
-                for (int d = 0; d < p.head_dim; d += 4)
-                    *reinterpret_cast<uint2*>(p.out + (int64_t)(row0 + t) * p.ldo + (int64_t)head * p.head_dim + d) =
-                        make_uint2(0, 0);
-            }
+            const int t = r / p.group;
+            if (part || split == 0) no_keys(p, part, split, row0 + t, kvh * p.group + r - t * p.group);
         }
         if (holds) pdl_wait();
         return;
@@ -224,8 +234,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     }
     int lim[2] = {len, len};  // keys of rows ra and rb end here
     if (p.causal) {
-        lim[0] = len - nrow + ra / p.group + 1;
-        lim[1] = len - nrow + rb / p.group + 1;
+        lim[0] = len - nseq + ra / p.group + 1;
+        lim[1] = len - nseq + rb / p.group + 1;
     }
     lim[0] = min(lim[0], k1);
     lim[1] = min(lim[1], k1);
@@ -361,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
         }
         const int t = r / p.group, head = kvh * p.group + r - t * p.group;
         // keys, but all scores -inf: 0 / 0 in the formula, (-inf, 1) for a combination
-        const bool flat = mm == -INFINITY && sum == 0.0f && (p.causal ? min(k1, len - nrow + t + 1) : k1) > k0;
+        const bool flat = mm == -INFINITY && sum == 0.0f && (p.causal ? min(k1, len - nseq + t + 1) : k1) > k0;
         if (flat) sum = 1.0f;
         if (p.cluster) {
             if (d == 0)

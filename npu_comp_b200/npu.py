@@ -763,11 +763,11 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     [batch]) and its new rows (cu_seqlens) the last of them.  Prompt chunks,
     prompts behind a cached prefix, drafted tokens.
 
-    max_new: at least the new rows of any sequence (rows past it may be left
-    out; 0: not known); up to 16 * kv_heads / heads of them run on the kernel
-    for few rows.  ctx_len: the
-    largest lens expected (0: the table's width), which only decides how keys
-    are split over CTAs.  page_size 16 .. 256."""
+    max_new: at least the new rows of any sequence (0: not known); up to
+    r = 16 * kv_heads / heads of them run on the kernel for few rows, where a
+    sequence that has more than r rows all the same gets zeros for those past
+    its first r.  ctx_len: the largest lens expected (0: the table's width),
+    which only decides how keys are split over CTAs.  page_size 16 .. 256."""
     dev, T, qc, ldq = _first16(q, "q")
     (n_pages, kv_heads, ps, hd), B, W, ldt = _pool(k_pages, v_pages, page_table, dev)
     if qc != heads * hd:

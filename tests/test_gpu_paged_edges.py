@@ -114,3 +114,33 @@ def test_scores_of_minus_infinity(cuda_device, path, hd):
         o = c.run()
         assert torch.isnan(o).any() == (n > m - c.new[0])
         c.k[0] = k
+
+@pytest.mark.parametrize("keys", [[40, 9, 30, 7], [900, 9, 30, 1200], [30000, 9, 30, 20000]])  # whole, cluster, partials
+@pytest.mark.parametrize("H,KV", [(8, 2), (16, 1), (3, 3)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_more_rows_than_max_new(cuda_device, keys, H, KV, causal):
+    """max_new below a sequence's rows: the rows up to 16 * kv_heads / heads see
+    the keys they should, the others are zero; where max_new takes the call to
+    the tile kernel, all rows are computed."""
+    dev, hd, ps, new = cuda_device, 128, 16, [7, 1, 23, 7]
+    g = torch.Generator(device=dev).manual_seed(sum(keys) + H)
+    q = [torch.randn((n, H, hd), generator=g, device=dev).half() for n in new]
+    k, v = ([torch.randn((n, KV, hd), generator=g, device=dev).half() for n in keys] for _ in range(2))
+    kp, vp, table, lens = to_pages(k, v, ps)
+    cu, T = offsets(new, dev) + 2, sum(new)
+    x = torch.cat([torch.zeros_like(q[0][:2]), *q, torch.zeros_like(q[0][:2])]).reshape(T + 4, H * hd)
+    want = [attention_exact(a, b, c, 1 / math.sqrt(hd), causal) for a, b, c in zip(q, k, v)]
+    for max_new in (1, 4, 17):
+        few = max_new * (H // KV) <= 16
+        kept = [min(n, 16 // (H // KV)) if few else n for n in new]
+        o, b = ([w[i].clone() for w in want] for i in (0, 1))
+        for i, n in enumerate(kept):
+            o[i][n:], b[i][n:] = 0.0, 0.0
+        out = torch.full_like(x, 3.0)
+        npu._paged_query.cache_clear()
+        held = torch.full((64 << 20,), float("nan"), device=dev)  # scratch that is used unwritten shows as NaN
+        del held
+        nb.attention_paged(x, kp, vp, table, lens, cu, heads=H, max_new=max_new, causal=causal, out=out)
+        assert npu.device_error() == 0
+        same(out[2:T + 2], torch.cat(o), torch.cat(b))
+        assert (out[:2] == 3.0).all() and (out[T + 2:] == 3.0).all()
