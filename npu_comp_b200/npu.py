@@ -648,6 +648,11 @@ def _out16(out: Optional[torch.Tensor], like: torch.Tensor, rows: int, cols: int
     return out, ld
 
 
+def _context(ctx_len: int, width: int) -> int:
+    """The keys that a call's split is planned for, as the C entries take them (a table may be wider than an int)."""
+    return min(int(ctx_len) if ctx_len > 0 else width, width, 2 ** 31 - 1)
+
+
 @functools.lru_cache(maxsize=4096)
 def _paged_query(dev: int, name: str, *sizes: int) -> int:
     with torch.cuda.device(dev):
@@ -776,8 +781,8 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     cu = _ints(cu_seqlens, "cu_seqlens", B + 1, dev)
     if scale is None:
         scale = 1.0 / math.sqrt(max(hd, 1))
-    max_new = int(max_new)
-    ctx = min(int(ctx_len), W * ps) if ctx_len > 0 else W * ps
+    max_new = min(int(max_new), 2 ** 31 - 1)
+    ctx = _context(ctx_len, W * ps)
     out, ldo = _out16(out, q, T, heads * hd, dev)
     ws, wsp, wsb = _paged_workspace(q, dev, "npub_attention_paged_workspace", B, T, max_new, ctx, heads, kv_heads, hd)
     with _device(dev):
@@ -809,7 +814,9 @@ def attention_paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if scale is None:
         scale = 1.0 / math.sqrt(max(hd, 1))
     shared_len = int(shared_len)
-    ctx = min(int(ctx_len), W * ps) if ctx_len > 0 else W * ps
+    if not 0 <= shared_len <= min(W * ps, 2 ** 31 - 1):
+        raise ValueError("shared_len must lie within the table, below 2^31")
+    ctx = _context(ctx_len, W * ps)
     out, ldo = _out16(out, q, B, heads * hd, dev)
     ws, wsp, wsb = _paged_workspace(q, dev, "npub_attention_paged_decode_workspace", B, ctx, shared_len, heads,
                                     kv_heads, hd)

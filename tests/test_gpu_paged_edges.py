@@ -144,3 +144,39 @@ def test_more_rows_than_max_new(cuda_device, keys, H, KV, causal):
         assert npu.device_error() == 0
         same(out[2:T + 2], torch.cat(o), torch.cat(b))
         assert (out[:2] == 3.0).all() and (out[T + 2:] == 3.0).all()
+
+@pytest.mark.parametrize("pages", [2 ** 23, 2 ** 23 + 1, 2 ** 24 + 4])
+def test_tables_past_32_bits_of_keys(cuda_device, pages):
+    """A table wider than 2^31 keys (pages * 256) is no reason to refuse a call,
+    nor to plan it for another number of keys than its workspace."""
+    dev, H, KV, hd, ps = cuda_device, 4, 2, 64, 256
+    g = torch.Generator(device=dev).manual_seed(3)
+    k, v = ([torch.randn((900, KV, hd), generator=g, device=dev).half()] for _ in range(2))
+    q = torch.randn((1, H, hd), generator=g, device=dev).half()
+    kp, vp, narrow, lens = to_pages(k, v, ps)
+    table = torch.zeros((1, pages), dtype=torch.int32, device=dev)
+    table[:, :narrow.shape[1]] = narrow
+    o, b = attention_exact(q, k[0], v[0], 1 / math.sqrt(hd))
+    x = q.reshape(1, H * hd)
+    for ctx in (0, 900, 2 ** 31, 2 ** 33):
+        same(nb.attention_paged_decode(x, kp, vp, table, lens, heads=H, ctx_len=ctx), o, b)
+        for max_new in (0, 1):
+            same(nb.attention_paged(x, kp, vp, table, lens, offsets([1], dev), heads=H, ctx_len=ctx, max_new=max_new),
+                 o, b)
+    assert npu.device_error() == 0
+
+
+def test_hints_past_32_bits(cuda_device):
+    """A max_new or shared_len past an int is not taken for its low 32 bits."""
+    dev, H, KV, hd, ps, new = cuda_device, 4, 2, 64, 16, [20, 3]
+    g = torch.Generator(device=dev).manual_seed(5)
+    k, v = ([torch.randn((n, KV, hd), generator=g, device=dev).half() for n in (90, 40)] for _ in range(2))
+    q = [torch.randn((n, H, hd), generator=g, device=dev).half() for n in new]
+    kp, vp, table, lens = to_pages(k, v, ps)
+    want = [attention_exact(a, b, c, 1 / math.sqrt(hd)) for a, b, c in zip(q, k, v)]
+    x = torch.cat(q).reshape(-1, H * hd)
+    o = nb.attention_paged(x, kp, vp, table, lens, offsets(new, dev), heads=H, max_new=2 ** 32 + 1)
+    same(o, torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want]))
+    for n in (2 ** 32, 2 ** 32 + 16, -2 ** 32):
+        with pytest.raises(ValueError):
+            nb.attention_paged_decode(x[:2], kp, vp, table, lens, heads=H, shared_len=n)
