@@ -308,7 +308,7 @@ int npub_rope_llama3_freqs(float* out, int head_dim, double theta, double factor
  * the cache append, in one pass over the fused rows qkv [tokens, ldx] (q
  * heads | k heads | v heads, head_dim columns each).  Row t belongs to
  * sequence t when cu_seqlens is NULL (a decode step, batch == tokens), else to
- * the packed sequence that holds it.  Per q and k head x:
+ * the packed sequence that holds it (batch >= 1).  Per q and k head x:
  *   x_i <- x_i * gamma_i / sqrt(mean(x^2) + eps)   (q_gamma / k_gamma fp16 [head_dim]; NULL: no norm)
  *   the first rot_dim columns rotated by the angles positions[t] * inv_freq[i]
  *   (fp32 [rot_dim / 2], e.g. npub_rope_llama3_freqs): pairs (i, i + rot_dim/2),
@@ -317,7 +317,8 @@ int npub_rope_llama3_freqs(float* out, int head_dim, double theta, double factor
  * to q_out [tokens, ldq] (may alias the q columns of qkv), k and v to the
  * cache at positions[t].  A row whose position lies outside
  * [0, max_pages * page_size), or whose page id lies outside [0, n_pages), is
- * rotated but not stored.  Two rows with the same slot: one of them is kept.
+ * rotated but not stored.  Rows with the same slot are stored in no order, and
+ * not as wholes: the slot then holds columns of several of them.
  * head_dim % 16 == 0, <= 512; rot_dim % 16 == 0, 0 < rot_dim <= head_dim;
  * page_size 1 .. 65536. */
 int npub_rope_paged_append(const void* qkv, int64_t ldx, void* q_out, int64_t ldq, int tokens, int q_heads,

@@ -689,7 +689,8 @@ def rope_paged_append(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: 
     inv_freq (fp32 [rot_dim / 2], from rope_freqs): the rotation's rates;
     rot_dim < head_dim rotates the first rot_dim columns only; interleaved
     pairs columns (2i, 2i + 1) instead of (i, i + rot_dim / 2).  A position
-    outside the table, or a page id outside the pool, is rotated but not stored."""
+    outside the table, or a page id outside the pool, is rotated but not stored.
+    Rows with the same slot leave columns of several of them in it."""
     dev, T, cols, ldx = _first16(qkv, "qkv")
     R = head_dim if rot_dim is None else int(rot_dim)
     if cols < (q_heads + 2 * kv_heads) * head_dim:

@@ -180,3 +180,24 @@ def test_hints_past_32_bits(cuda_device):
     for n in (2 ** 32, 2 ** 32 + 16, -2 ** 32):
         with pytest.raises(ValueError):
             nb.attention_paged_decode(x[:2], kp, vp, table, lens, heads=H, shared_len=n)
+
+def test_rows_of_one_slot(cuda_device):
+    """Rows at the same position of the same pages: every run of eight columns of
+    the slot comes from one of them, and no other slot changes."""
+    dev, H, KV, hd, ps, n = cuda_device, 4, 2, 128, 16, 6
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn((n, (H + 2 * KV) * hd), generator=g, device=dev).half()
+    f, table = nb.rope_freqs(hd, device=dev), torch.tensor([[1, 0, 2]] * n, dtype=torch.int32, device=dev)
+    pos = torch.full((n,), 19, dtype=torch.int32, device=dev)
+    kp = torch.full((3, KV, ps, hd), 3.0, dtype=torch.float16, device=dev)
+    vp = kp.clone()
+    q = nb.rope_paged_append(x, H, KV, hd, pos, f, kp, vp, table)
+    one = [torch.full((n + 2, KV, ps, hd), 3.0, dtype=torch.float16, device=dev) for _ in range(2)]
+    own = torch.arange(n, device=dev)[:, None] + torch.tensor([2, 0, 2], device=dev)  # the rows in pages of their own
+    assert torch.equal(q, nb.rope_paged_append(x, H, KV, hd, pos, f, *one, own.int()))
+    for got, rows in zip((kp, vp), one):
+        cand = rows[:n, :, 3].reshape(n, KV, hd // 8, 8)
+        slot = got[0, :, 3].reshape(1, KV, hd // 8, 8)
+        assert (cand == slot).all(-1).any(0).all()
+        got[0, :, 3] = 3.0
+        assert (got == 3.0).all()
