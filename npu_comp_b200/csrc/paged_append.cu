@@ -32,7 +32,7 @@ struct AppendArgs {
     int64_t ldx;
     __half* q;
     int64_t ldq;
-    int tokens, hq, hk, hd, half, interleaved;
+    int hq, hk, hd, half, interleaved;
     int units, units_p2, units_log2;  // 16-element units per head, padded to a power of two
     const int32_t* pos;
     const float* inv_freq;
@@ -249,7 +249,6 @@ extern "C" int npub_rope_paged_append(const void* qkv, int64_t ldx, void* q_out,
     a.ldx = ldx;
     a.q = reinterpret_cast<__half*>(q_out);
     a.ldq = ldq;
-    a.tokens = tokens;
     a.hq = q_heads;
     a.hk = kv_heads;
     a.hd = head_dim;
