@@ -6,8 +6,8 @@ import pytest
 import torch
 
 import npu_comp_b200 as nb
-from npu_comp_b200 import npu
-from paged_exact import attention_exact, same, to_pages
+from npu_comp_b200 import _lib, npu
+from paged_exact import attention_exact, planted, same, to_pages
 
 pytestmark = pytest.mark.gpu
 
@@ -201,3 +201,158 @@ def test_rows_of_one_slot(cuda_device):
         assert (cand == slot).all(-1).any(0).all()
         got[0, :, 3] = 3.0
         assert (got == 3.0).all()
+
+# ------------------------------------------------- long contexts, planted keys
+
+@pytest.mark.parametrize("H,KV,hd", [(8, 8, 128), (16, 1, 64), (64, 1, 128)])
+def test_long_planted_contexts(cuda_device, H, KV, hd):
+    """Contexts of up to 70001 keys over the largest numbers of key ranges: every
+    64 keys hold one that the result cannot do without (test_paged_exact.py),
+    by one row, a chunk of rows, and behind a shared prefix."""
+    dev, ps, keys, shared = cuda_device, 64, [70001, 300, 66000], 0
+    sc = 1 / math.sqrt(hd)
+    plant = [planted(m, KV, hd, every=64, gen=torch.Generator().manual_seed(m), dev=dev) for m in keys]
+    q = torch.stack([u.repeat_interleave(H // KV, 0) for u, _, _ in plant])
+    k, v = [p[1] for p in plant], [p[2] for p in plant]
+    kp, vp, table, lens = to_pages(k, v, ps)
+    want = [attention_exact(q[b:b + 1], k[b], v[b], sc) for b in range(3)]
+    o, bound = torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want])
+    x = q.reshape(3, H * hd)
+    for kw in (dict(), dict(ctx_len=70001), dict(ctx_len=500)):
+        same(nb.attention_paged_decode(x, kp, vp, table, lens, heads=H, **kw), o, bound)
+        same(nb.attention_paged(x, kp, vp, table, lens, offsets([1] * 3, dev), heads=H, **kw), o, bound)
+    same(nb.attention_paged_decode(x[:1], kp, vp, table[:1], lens[:1], heads=H), o[:1], bound[:1])
+    n = 20  # a chunk of the longest: partials of the tile kernel
+    rows = q[:1].expand(n, H, hd).contiguous()
+    e, b = attention_exact(rows, k[0], v[0], sc)
+    y = rows.reshape(n, H * hd)
+    assert _lib.query("npub_attention_paged_workspace", 1, n, 0, 70001, H, KV, hd) > 0
+    same(nb.attention_paged(y, kp, vp, table[:1], lens[:1], offsets([n], dev), heads=H, ctx_len=70001), e, b)
+    assert npu.device_error() == 0
+
+
+@pytest.mark.parametrize("H,KV,hd,B", [(8, 2, 128, 5), (4, 4, 64, 3), (32, 1, 128, 2)])
+def test_long_planted_prefix(cuda_device, H, KV, hd, B):
+    """A shared prefix of 20032 keys with own keys behind it, one sequence inside
+    the prefix: every 64 keys of both phases hold one that shows."""
+    dev, ps, shared, sc = cuda_device, 64, 20032, 1 / math.sqrt(hd)
+    gen = torch.Generator().manual_seed(B)
+    u, k0, v0 = planted(shared, KV, hd, every=64, gen=gen, dev=dev)
+    k, v = [], []
+    for b in range(B):
+        m = [4368, 700, 64, 1, 9000][b]
+        _, kb, vb = planted(m, KV, hd, every=64, gen=gen, dev=dev)
+        flat = (kb.abs() == 1).all(-1)  # the planted ones, against the prefix's query
+        kb[flat] = u.expand_as(kb)[flat]
+        k.append(torch.cat([k0, kb]))
+        v.append(torch.cat([v0, vb]))
+    kp, vp, table, lens = to_pages(k, v, ps, shared=shared)
+    lens[-1] = 15001  # ends inside the prefix
+    keys = lens.tolist()
+    q = u.repeat_interleave(H // KV, 0).expand(B, H, hd).contiguous()
+    want = [attention_exact(q[b:b + 1], k[b][:keys[b]], v[b][:keys[b]], sc) for b in range(B)]
+    o, bound = torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want])
+    for kw in (dict(shared_len=shared), dict(shared_len=shared, ctx_len=max(keys)), dict()):
+        same(nb.attention_paged_decode(q.reshape(B, H * hd), kp, vp, table, lens, heads=H, **kw), o, bound)
+    assert npu.device_error() == 0
+
+# ------------------------------------------------------------ calls in flight
+
+def serving_inputs(dev, seed, B=4, H=8, KV=2, hd=128, m=6000):
+    """q, its pages, and the 64-bit result of a decode batch and of chunks whose
+    calls use scratch: other values for every seed."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g, device=dev).half()  # noqa: E731
+    keys, new = [m - 701 * b - 13 * seed for b in range(B)], [9, 2, 30, 5]
+    k, v = [r(n, KV, hd) for n in keys], [r(n, KV, hd) for n in keys]
+    for x in (k, v):
+        for y in x[1:]:
+            y[:512] = x[0][:512]
+    q1, qn = r(B, H, hd), r(sum(new), H, hd)
+    sc = 1 / math.sqrt(hd)
+    w1 = [attention_exact(q1[b:b + 1], k[b], v[b], sc) for b in range(B)]
+    wn = [attention_exact(a, k[b], v[b], sc) for b, a in enumerate(qn.split(new))]
+    cat = lambda w: tuple(torch.cat([y[i] for y in w]) for i in (0, 1))  # noqa: E731
+    pages = to_pages(k, v, 16, shared=512, seed=seed)
+    # both calls leave partials in scratch
+    W = pages[2].shape[1] * 16
+    assert _lib.query("npub_attention_paged_decode_workspace", B, W, 512, H, KV, hd) > 0
+    assert _lib.query("npub_attention_paged_workspace", B, sum(new), 0, W, H, KV, hd) > 0
+    cu = offsets(new, dev)
+
+    def step():
+        kp, vp, table, lens = pages
+        return (nb.attention_paged_decode(q1.reshape(B, -1), kp, vp, table, lens, heads=H, shared_len=512),
+                nb.attention_paged(qn.reshape(-1, H * hd), kp, vp, table, lens, cu, heads=H))
+
+    def check(outs):
+        for got, (o, b) in zip(outs, (cat(w1), cat(wn))):
+            same(got, o, b)
+
+    return step, check
+
+
+def captured(step):
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    return graph, outs
+
+
+def test_two_graphs_in_flight(cuda_device):
+    """Two captured steps of different inputs, replayed on two streams with
+    nothing between them: neither writes the other's scratch or outputs."""
+    calls = [serving_inputs(cuda_device, s) for s in (1, 2)]
+    graphs = [captured(step) for step, _ in calls]
+    streams = [torch.cuda.Stream(device=cuda_device) for _ in graphs]
+    for _ in range(5):
+        for _, outs in graphs:
+            for o in outs:
+                o.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for (graph, _), st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for (_, outs), (_, check) in zip(graphs, calls):
+            check(outs)
+    assert npu.device_error() == 0
+    del graph
+    graphs.clear()
+
+
+def test_graph_beside_eager_calls(cuda_device):
+    """A captured step replayed on a stream of its own while another stream runs
+    the same operators on other inputs, with no wait between the two."""
+    dev = cuda_device
+    (step1, check1), (step2, check2) = serving_inputs(dev, 3), serving_inputs(dev, 4)
+    graph, outs = captured(step1)
+    sides = [torch.cuda.Stream(device=dev) for _ in range(2)]
+    for _ in range(5):
+        for o in outs:
+            o.fill_(float("nan"))
+        torch.cuda.synchronize()
+        eager = []
+        for _ in range(10):
+            with torch.cuda.stream(sides[0]):
+                graph.replay()
+            with torch.cuda.stream(sides[1]):
+                eager.append(step2())
+        torch.cuda.synchronize()
+        check1(outs)
+        for x in eager:
+            check2(x)
+    assert npu.device_error() == 0
+    del graph
+
+
+@pytest.mark.parametrize("path", PATHS)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_same_bits_every_time(cuda_device, path, hd):
+    c = Call(cuda_device, path, hd)
+    first = c.run()
+    for _ in range(3):
+        assert torch.equal(c.run(), first)
