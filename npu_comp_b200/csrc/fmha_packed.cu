@@ -84,7 +84,7 @@ struct Params {
     int max_keys, page_shift, box_rows, n_pages;
     int total_q, batch, heads, kv_heads, group, tpt, head_dim;
     uint32_t span_inv;  // ceil(2^32 / (tiles * tpt)), 2^32 - 1 for 1
-    int tiles, n_items, sorted, levels, splits, first, split0, shared, causal;
+    int tiles, n_items, sorted, splits, first, split0, shared, causal;
     float c;  // scale * log2(e)
     __half* out;
     int64_t ldo;
@@ -114,25 +114,21 @@ __device__ __forceinline__ void set_err(int* err, int code) {
     if (err) atomicCAS(err, 0, code);
 }
 
-// Rows of sequence b, [r0, r1), and its keys.  Reads cu and lens as
-// they are: whatever they hold, rows stay inside [0, total_q) and keys inside
-// the table.
+// Rows of a sequence, [r0, r1), and its keys.
 struct SeqRows {
     int r0, r1, klen;
 };
+// Those of sequence b (none past the batch).  Reads cu and lens as they are:
+// whatever they hold, rows stay inside [0, total_q) and keys inside the table.
 template <bool PAGED>
-__device__ __forceinline__ void seq_rows(const Params& p, int b, const SeqRows& near, int& r0, int& r1, int& klen) {
-    if (b < 32) {  // the lane's own, loaded once
-        r0 = near.r0;
-        r1 = near.r1;
-        klen = near.klen;
-        return;
+__device__ __forceinline__ SeqRows seq_rows(const Params& p, int b) {
+    SeqRows r = {0, 0, 0};
+    if (b < p.batch) {
+        r.r0 = p.cu ? max(0, min(p.total_q, __ldg(p.cu + b))) : b;
+        r.r1 = p.cu ? max(r.r0, min(p.total_q, __ldg(p.cu + b + 1))) : r.r0 + 1;
+        r.klen = PAGED ? max(0, min(p.max_keys, __ldg(p.lens + b))) : r.r1 - r.r0;
     }
-    r0 = r1 = klen = 0;
-    if (b >= p.batch) return;
-    r0 = p.cu ? max(0, min(p.total_q, __ldg(p.cu + b))) : b;
-    r1 = p.cu ? max(r0, min(p.total_q, __ldg(p.cu + b + 1))) : r0 + 1;
-    klen = PAGED ? max(0, min(p.max_keys, __ldg(p.lens + b))) : r1 - r0;
+    return r;
 }
 
 // Tiles of a sequence that reach into key block `level` or behind it: tile t
@@ -177,14 +173,48 @@ __device__ __forceinline__ void cut_item(Item& it, int k0, int kend, const int (
     }
 }
 
+// Tiles of the whole batch that reach into `level` or behind it, by a warp;
+// near: the lane's own of the first 32 sequences.
+template <bool PAGED>
+__device__ __forceinline__ int batch_tiles_from(const Params& p, const SeqRows& near, int level, int span) {
+    int sum = tiles_from(p, near.r1 - near.r0, near.klen, level, span);
+#pragma unroll 1
+    for (int b = 32 + (threadIdx.x & 31); b - (int)(threadIdx.x & 31) < p.batch; b += 32) {
+        const SeqRows r = seq_rows<PAGED>(p, b);
+        sum += tiles_from(p, r.r1 - r.r0, r.klen, level, span);
+    }
+    return __reduce_add_sync(0xffffffffu, sum);
+}
+
+// Where the scheduler stands.  A CTA's item numbers only ascend, so each search
+// goes on from the last one: 1000 prompts of 100 rows, 32 / 8 heads of 64, in
+// 470 us (11.9 ms with a search of the whole batch for every item, 86 us each).
+// In shared memory: its warp's 56 registers do not hold it without spills.
+struct Place {
+    int level;       // tiles of this level are handed out (sorted; else all tiles are one level)
+    int above;       // tiles of the levels above
+    int here;        // tiles of this level
+    int s0, before;  // the 32 sequences that the last tile was found in, and the tiles of this level ahead of them
+};
+template <bool PAGED>
+__device__ __forceinline__ Place first_place(const Params& p, const SeqRows& near) {
+    if (!p.sorted) return Place{0, 0, 0x7fffffff, 0, 0};
+    int keys = near.klen;
+#pragma unroll 1
+    for (int b = 32 + (threadIdx.x & 31); b - (int)(threadIdx.x & 31) < p.batch; b += 32)
+        keys = max(keys, seq_rows<PAGED>(p, b).klen);
+    return Place{(int)(__reduce_max_sync(0xffffffffu, (unsigned)keys) / kBlk) + 1, 0, 0, 0, 0};  // no tile reaches it
+}
+
 // Item number -> rows and keys, by the scheduler warp.  Tiles are numbered
 // from the most expensive down (p.sorted), so that the CTAs, which take items
-// round by round in alternating direction, end together: a bisection over the
-// key level whose tile count brackets the number, each step a sum over the
-// sequences (32 per warp step), then a scan for the sequence.  Without
-// p.sorted (no CTA has a second item, or the order is given) the scan alone.
+// round by round in alternating direction, end together: the tiles of a key
+// level, then those of the next level that has any, found from the last one
+// down in doubling steps and a bisection, each step a sum over the sequences
+// (32 per warp step); within a level a scan for the sequence.  Without p.sorted
+// (no CTA has a second item, or the order is given) the scan alone.
 template <bool PAGED, bool DUAL>
-__device__ __forceinline__ bool get_item(const Params& p, const SeqRows& near, int idx, Item& it) {
+__device__ __forceinline__ bool get_item(const Params& p, const SeqRows& near, Place& at, int idx, Item& it) {
     const int lane = threadIdx.x & 31;
     it.split = idx % p.splits;
     idx /= p.splits;
@@ -205,45 +235,37 @@ __device__ __forceinline__ bool get_item(const Params& p, const SeqRows& near, i
                        {true, DUAL || (p.tiles == 2 && it.tok0 + p.tpt < it.ntok)});
         return true;
     }
-    int level = 0;
-    if (p.sorted) {
-        // the highest level with more than `tile` tiles from it on
-        int lo = 0, hi = p.levels;
-        if (p.batch <= 32) hi = min(hi, (int)(__reduce_max_sync(0xffffffffu, (unsigned)near.klen) / kBlk));
-        bool any = false;
-        while (lo <= hi) {
-            const int mid = (lo + hi) >> 1;
-            int sum = 0;
-            for (int s0 = 0; s0 < p.batch; s0 += 32) {
-                int r0, r1, kl;
-                seq_rows<PAGED>(p, s0 + lane, near, r0, r1, kl);
-                sum += tiles_from(p, r1 - r0, kl, mid, span);
-            }
-            sum = __reduce_add_sync(0xffffffffu, sum);
-            if (sum > tile) {
-                level = mid;
-                any = true;
-                lo = mid + 1;
+    if (tile - at.above >= at.here) {  // (sorted) the next level: tiles from `lo` on > tile >= tiles from `hi` on
+        int hi = at.level, nhi = at.above + at.here, lo = hi, nlo = nhi;
+        for (int step = 1; nlo <= tile; step *= 2) {
+            if (lo == 0) return false;  // behind the last tile
+            hi = lo;
+            nhi = nlo;
+            lo = max(0, lo - step);
+            nlo = batch_tiles_from<PAGED>(p, near, lo, span);
+        }
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1, n = batch_tiles_from<PAGED>(p, near, mid, span);
+            if (n > tile) {
+                lo = mid;
+                nlo = n;
             } else {
-                hi = mid - 1;
+                hi = mid;
+                nhi = n;
             }
         }
-        if (!any) return false;
-        int above = 0;
-        for (int s0 = 0; s0 < p.batch; s0 += 32) {
-            int r0, r1, kl;
-            seq_rows<PAGED>(p, s0 + lane, near, r0, r1, kl);
-            above += tiles_from(p, r1 - r0, kl, level + 1, span);
-        }
-        tile -= __reduce_add_sync(0xffffffffu, above);
+        __syncwarp();
+        at = Place{lo, nhi, nlo - nhi, 0, 0};
+        __syncwarp();
     }
+    tile -= at.above + at.before;
     int b = -1, r0 = 0, r1 = 0, klen = 0;
-    for (int s0 = 0; s0 < p.batch; s0 += 32) {
-        int c0, c1, kl;
-        seq_rows<PAGED>(p, s0 + lane, near, c0, c1, kl);
-        const int all = (c1 - c0 + span - 1) / span;
-        const int over = p.sorted ? tiles_from(p, c1 - c0, kl, level + 1, span) : 0;
-        const int cnt = (p.sorted ? tiles_from(p, c1 - c0, kl, level, span) : all) - over;
+    int s0 = at.s0;
+    for (; s0 < p.batch; s0 += 32) {
+        const SeqRows r = s0 == 0 ? near : seq_rows<PAGED>(p, s0 + lane);
+        const int n = r.r1 - r.r0, all = (n + span - 1) / span;
+        const int over = p.sorted ? tiles_from(p, n, r.klen, at.level + 1, span) : 0;
+        const int cnt = (p.sorted ? tiles_from(p, n, r.klen, at.level, span) : all) - over;
         int sum = cnt;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -254,15 +276,20 @@ __device__ __forceinline__ bool get_item(const Params& p, const SeqRows& near, i
         if (vote) {
             const int l = __ffs(vote) - 1;
             tile -= __shfl_sync(0xffffffffu, sum - cnt, l);
-            r0 = __shfl_sync(0xffffffffu, c0, l);
-            r1 = __shfl_sync(0xffffffffu, c1, l);
-            klen = __shfl_sync(0xffffffffu, kl, l);
+            r0 = __shfl_sync(0xffffffffu, r.r0, l);
+            r1 = __shfl_sync(0xffffffffu, r.r1, l);
+            klen = __shfl_sync(0xffffffffu, r.klen, l);
             tile = __shfl_sync(0xffffffffu, all - 1 - over, l) - tile;  // longest causal rows first
             b = s0 + l;
             break;
         }
-        tile -= __shfl_sync(0xffffffffu, sum, 31);
+        sum = __shfl_sync(0xffffffffu, sum, 31);
+        tile -= sum;
+        __syncwarp();
+        if (lane == 0) at.before += sum;
     }
+    if (lane == 0) at.s0 = s0;
+    __syncwarp();
     if (b < 0) return false;
     it.seq = b;
     it.q_row0 = r0;
@@ -440,7 +467,8 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(it_empty + kItemSlots);
     volatile uint32_t* vfix_stage = tmem_slot + 2;
     Item* slots = reinterpret_cast<Item*>(smem + L::kOffItem);
-    static_assert(kItemSlots * sizeof(Item) <= 256 && (13 + 2 * L::kStages + 2 * kItemSlots) * 8 + 12 <= 384, "layout");
+    Place* place = reinterpret_cast<Place*>(slots + kItemSlots);
+    static_assert(kItemSlots * sizeof(Item) + sizeof(Place) <= 256 && (13 + 2 * L::kStages + 2 * kItemSlots) * 8 + 12 <= 384, "layout");
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -681,18 +709,16 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             // ------------------------------------------------------------ scheduler
             uint32_t k = 0;
             bool ok = true;
-            SeqRows near = {0, 0, 0};
-            if (lane < p.batch && !(PAGED && p.shared > 0)) {
-                near.r0 = p.cu ? max(0, min(p.total_q, __ldg(p.cu + lane))) : lane;
-                near.r1 = p.cu ? max(near.r0, min(p.total_q, __ldg(p.cu + lane + 1))) : lane + 1;
-                near.klen = PAGED ? max(0, min(p.max_keys, __ldg(p.lens + lane))) : near.r1 - near.r0;
-            }
-            for (int round = 0; ok; ++round) {
-                const int64_t base = (int64_t)round * gridDim.x;
-                const int64_t idx = base + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            SeqRows near = {0, 0, 0};  // of the first 32 sequences, loaded once
+            if (!(PAGED && p.shared > 0)) near = seq_rows<PAGED>(p, lane);
+            Place& at = *place;
+            at = first_place<PAGED>(p, near);
+            __syncwarp();
+            for (uint32_t round = 0; ok; ++round) {
+                const uint32_t idx = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
                 Item it;
-                it.state = base < p.n_items ? 1 : 0;
-                if (it.state && (idx >= p.n_items || !get_item<PAGED, DUAL>(p, near, (int)idx, it))) continue;
+                // no item with this number: none with the later ones either
+                it.state = idx < (uint32_t)p.n_items && get_item<PAGED, DUAL>(p, near, at, (int)idx, it) ? 1 : 0;
                 const uint32_t s = k % kItemSlots;
                 ok = mbar_wait_warp(&it_empty[s], ((k / kItemSlots) & 1u) ^ 1u, abort_flag);
                 if (!ok) {
@@ -954,7 +980,6 @@ int fmha_packed(const PackedArgs& a, cudaStream_t st) {
     // against 50.8).
     p.sorted = p.n_items > grid && a.shared == 0 && a.batch > 1 && a.causal;
     p.span_inv = (uint32_t)((0x100000000ull + p.tiles * p.tpt - 1) / (p.tiles * p.tpt) - (p.tiles * p.tpt == 1));
-    p.levels = (int)(((paged ? (int64_t)p.max_keys : (int64_t)a.total_q) + kBlk - 1) / kBlk);
     const bool small = a.head_dim <= 64;
     if (part) {
         if (!paged) return NPUB_ERR_UNSUPPORTED;

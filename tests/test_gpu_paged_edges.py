@@ -356,3 +356,77 @@ def test_same_bits_every_time(cuda_device, path, hd):
     first = c.run()
     for _ in range(3):
         assert torch.equal(c.run(), first)
+
+# --------------------------------------------------------------- many prompts
+
+@pytest.mark.parametrize("H,KV,hd", [(8, 2, 64), (4, 4, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_hundreds_of_prompts(cuda_device, H, KV, hd, causal):
+    """Ragged prompts past what one step of the scheduler looks at, empty ones
+    and long ones among them, packed and over pages."""
+    dev = cuda_device
+    new = [(i * 37) % 91 if i % 11 else 0 for i in range(1100)] + [0] * 70 + [700, 1, 2, 300]
+    g = torch.Generator(device=dev).manual_seed(hd)
+    x = torch.randn((sum(new), H + 2 * KV, hd), generator=g, device=dev).half()
+    q, k, v = x[:, :H], x[:, H:H + KV], x[:, H + KV:]
+    o = nb.attention_packed(q.reshape(-1, H * hd), k.reshape(-1, KV * hd), v.reshape(-1, KV * hd), offsets(new, dev), H,
+                            KV, head_dim=hd, causal=causal)
+    cut = lambda t: t.split(new)  # noqa: E731
+    want = [attention_exact(a, b, c, 1 / math.sqrt(hd), causal) for a, b, c in zip(cut(q), cut(k), cut(v))]
+    same(o, torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want]))
+    # the last rows of each, the first ones cached already
+    late = [n // 2 for n in new]
+    rows = torch.cat([t[n - m:] for t, n, m in zip(cut(q), new, late)]).reshape(-1, H * hd)
+    kp, vp, table, lens = to_pages(cut(k), cut(v), 16)
+    want = [(w[0][n - m:], w[1][n - m:]) for w, n, m in zip(want, new, late)]
+    o = nb.attention_paged(rows, kp, vp, table, lens, offsets(late, dev), heads=H, causal=causal)
+    same(o, torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want]))
+    assert npu.device_error() == 0
+
+
+def test_more_sequences_than_a_grid_row(cuda_device):
+    """70000 sequences, most of one row that sees its own key alone (its v)."""
+    dev, H, KV, hd, B = cuda_device, 4, 2, 64, 70000
+    g = torch.Generator(device=dev).manual_seed(7)
+    x = torch.randn((B, (H + 2 * KV) * hd), generator=g, device=dev).half()
+    q, k, v = x[:, :H * hd], x[:, H * hd:(H + KV) * hd], x[:, (H + KV) * hd:]
+    cu = torch.arange(B + 1, dtype=torch.int32, device=dev)
+    cu[500:900] = 500  # 400 empty ones, then one of 400 rows
+    o = nb.attention_packed(q, k, v, cu, H, KV, head_dim=hd).view(B, H, hd)
+    own = v.reshape(B, KV, hd).repeat_interleave(H // KV, 1)
+    alone = torch.ones(B, dtype=torch.bool, device=dev)
+    alone[500:900] = False
+    assert torch.equal(o[alone], own[alone])
+    r = slice(500, 900)
+    e, b = attention_exact(q[r].reshape(-1, H, hd), k[r].reshape(-1, KV, hd), v[r].reshape(-1, KV, hd), 1 / math.sqrt(hd))
+    same(o[r].reshape(400, -1), e, b)
+    kp, vp = torch.zeros((B, KV, 16, hd), dtype=torch.float16, device=dev), torch.zeros((B, KV, 16, hd), dtype=torch.float16, device=dev)
+    kp[:, :, 0], vp[:, :, 0] = k.reshape(B, KV, hd), v.reshape(B, KV, hd)
+    table = torch.arange(B, dtype=torch.int32, device=dev)[:, None]
+    ones, cu = torch.ones(B, dtype=torch.int32, device=dev), torch.arange(B + 1, dtype=torch.int32, device=dev)
+    for max_new in (0, 1):
+        o = nb.attention_paged(q.contiguous(), kp, vp, table, ones, cu, heads=H, max_new=max_new)
+        assert torch.equal(o.view(B, H, hd), own)
+    assert npu.device_error() == 0
+
+
+def test_many_short_prompts_take_no_longer_than_equal_ones(cuda_device):
+    """1000 prompts of 100 rows: the packed kernel, which looks up whose rows it
+    takes, against attention() on the same rows, which is told (a ninth of its
+    time; with a search of all sequences for every item it took three times it)."""
+    dev, B, T, H, KV, hd = cuda_device, 1000, 100, 32, 8, 64
+    x = torch.randn((B * T, (H + 2 * KV) * hd), generator=torch.Generator(device=dev).manual_seed(1), device=dev).half()
+    q, k, v = x[:, :H * hd], x[:, H * hd:(H + KV) * hd], x[:, (H + KV) * hd:]
+    cu = offsets([T] * B, dev)
+    took = []
+    for call in (lambda: nb.attention_packed(q, k, v, cu, H, KV, head_dim=hd),
+                 lambda: nb.attention(q, k, v, H, KV, head_dim=hd, batch=B)):
+        call()
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(5):
+            call()
+        b.record()
+        b.synchronize()
+        took.append(a.elapsed_time(b))
+    assert took[0] < took[1], took
