@@ -36,15 +36,17 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Phase {
     int tiles, dual;  // tile kernel: rows of an item, and whether its keys go in two halves
     int splits;
+    bool cluster;     // paged_decode combines its ranges itself
+    double us;        // the estimate
+    int64_t ctas;     // tile kernel: items of all ranges
     int partials() const { return splits * (dual ? 2 : 1); }
 };
 struct Plan {
     bool few;    // own keys on paged_decode (else on the tiles)
     int shared;  // keys of the shared prefix phase (0: none)
-    bool cluster;  // paged_decode combines its ranges itself
     Phase pre, own;
     int total() const { return (shared > 0 ? pre.partials() : 0) + own.partials(); }
-    bool part() const { return total() > 1 && !cluster; }
+    bool part() const { return total() > 1 && !own.cluster; }
 };
 
 // What a kernel takes, in us: `first` to start, then per item `item` and `unit_us` for every `unit` keys.
@@ -95,39 +97,70 @@ Phase tile_phase(int total, int batch, int heads, int kv_heads, int max_new, int
     const Split sb = pick_splits(keys, one, slots, Cost{7.0, 2.0, 1.6, 256}, false, 64, range_us, 2, fixed, 4.0);
     a.tiles = sa.s == 1 && !fixed ? 0 : 2;
     a.splits = sa.s;
+    a.us = sa.us;
+    a.ctas = two * sa.s;
     b.tiles = 1;
     b.dual = 1;
     b.splits = sb.s;
+    b.us = sb.us;
+    b.ctas = one * sb.s;
     return sb.us < sa.us ? b : a;
+}
+
+// The few-row kernel on up to `keys` keys of each sequence; behind: a shared
+// prefix's partials are combined with its own.  One of its CTAs, two of which
+// share an SM, takes 4 us (in a cluster 5) and 3 us per 128 keys of 128 columns.
+Phase few_phase(int batch, int kv_heads, int head_dim, int64_t keys, double part_us, bool behind) {
+    const Cost c = {0.0, 4.0, head_dim > 64 ? 3.0 : 1.6, 128}, cc = {0.0, 5.0, c.unit_us, 128};
+    const bool ragged = batch > 1;
+    const int64_t items = (int64_t)batch * kv_heads, slots = 2 * num_sms();
+    Phase ph = {};
+    const Split sp = pick_splits(keys, items, slots, c, ragged, 64, part_us + 0.15, 1, behind, 4.0);
+    ph.splits = sp.s;
+    ph.us = sp.us;
+    if (!behind) {
+        const Split sc = pick_splits(keys, items, slots, cc, ragged, kPagedDecodeCluster, 0.0, 1, true, 0.0);
+        if (sc.us <= sp.us) {
+            ph.splits = sc.s;
+            ph.us = sc.us;
+            ph.cluster = true;
+        }
+    }
+    return ph;
 }
 
 Plan make_plan(int batch, int total, int max_new, int64_t ctx, int shared, int heads, int kv_heads, int head_dim) {
     Plan pl = {};
     const int group = heads / kv_heads, sms = num_sms();
     pl.few = max_new > 0 && (int64_t)max_new * group <= kPagedDecodeRows && batch <= 65535;
-    if (batch < 2) shared = 0;  // nothing to share
-    pl.shared = shared;
     const double part_us = (double)total * heads * head_dim * 8.0 / 4e6;  // about 4 TB/s: they stay in L2
-    // The prefix phase takes half of the SMs and the own keys run beside it (64 sequences, 32 / 8 heads, 8192 shared
-    // and 265 own keys on average: 36 us; on all SMs, one phase after the other, 46 us).
-    if (shared > 0) pl.pre = tile_phase(total, 1, heads, kv_heads, 0, shared, sms / 2, part_us, true);
-    const int64_t own = ctx > shared ? ctx - shared : 1;
-    if (pl.few) {
-        // a few-row CTA, two of which share an SM, takes 4 us (in a cluster 5) and 3 us per 128 keys of 128 columns
-        const Cost c = {0.0, 4.0, head_dim > 64 ? 3.0 : 1.6, 128}, cc = {0.0, 5.0, c.unit_us, 128};
-        const bool ragged = batch > 1;
-        const int64_t items = (int64_t)batch * kv_heads;
-        const Split sp = pick_splits(own, items, 2 * sms, c, ragged, 64, part_us + 0.15, 1, shared > 0, 4.0);
-        pl.own.splits = sp.s;
-        if (shared == 0) {
-            const Split sc = pick_splits(own, items, 2 * sms, cc, ragged, kPagedDecodeCluster, 0.0, 1, true, 0.0);
-            if (sc.us <= sp.us) {
-                pl.own.splits = sc.s;
-                pl.cluster = true;
-            }
+    auto own = [&](int64_t keys, bool behind) {
+        return pl.few ? few_phase(batch, kv_heads, head_dim, keys, part_us, behind)
+                      : tile_phase(total, batch, heads, kv_heads, max_new, keys, sms, part_us, behind);
+    };
+    pl.own = own(ctx, false);
+    if (shared <= 0 || batch < 2) return pl;  // nothing to share
+    // The prefix phase takes a part of the SMs and the own keys run beside it on the others, then on all: together
+    // they take the longer of the prefix's time and the sum of both phases' shares of the SMs, and 4 us to combine.
+    // It is left out where reading the prefix for every sequence is estimated to be as quick.  Measured, 32 / 8 heads
+    // of 128, with the phase and without: 2 sequences of 100 own keys behind 512 keys 9.4 and 6.8 us, 64 of 200 behind
+    // 128 22.7 and 18.7, 16 of 200 behind 2048 15.0 and 25.3.  (The estimate without it takes no account of the L2,
+    // from which all but the first read the prefix: near the border it keeps the phase, 4 sequences behind 4096 16.6
+    // and 13.0.)  Its SMs: 64 sequences of 100 own keys behind 131072 take 213 us on half of them, 163 on all;
+    // 64 of 265 behind 8192 36 on half, 46 on all.
+    double best = pl.own.us;
+    const Phase mine = own(ctx > shared ? ctx - shared : 1, true);
+    for (int quarters = 2; quarters <= 4; ++quarters) {
+        const Phase pre = tile_phase(total, 1, heads, kv_heads, 0, shared, sms * quarters / 4, part_us, true);
+        const double both = mine.us + pre.us * (pre.ctas < sms ? (double)pre.ctas / sms : 1.0);
+        const double us = 4.0 + (pre.us > both ? pre.us : both);
+        if (us < best) {
+            best = us;
+            pl.shared = shared;
+            pl.pre = pre;
+            pl.own = mine;
         }
-    } else {
-        pl.own = tile_phase(total, batch, heads, kv_heads, max_new, own, sms, part_us, shared > 0);
+        if (pre.us <= both) break;  // more SMs for the prefix would only take them from the own keys
     }
     return pl;
 }

@@ -466,3 +466,77 @@ def test_append_to_many_sequences(cuda_device):
     nb.rope_paged_append(torch.cat([x[:2], x]), H, KV, hd, torch.cat([two, pos]), f, kp, vp, wide, cu_seqlens=cu3, out=q)
     assert (q[:2] == 3.0).all() and torch.equal(q[2:], outs[0][0])
     assert torch.equal(kp, outs[0][1]) and torch.equal(vp, outs[0][2])
+
+# ------------------------------------------------------ the shared prefix's plan
+
+def launches(call):
+    n = _lib.launch_count()
+    call()
+    return _lib.launch_count() - n
+
+
+@pytest.mark.parametrize("keys,shared,H,KV,hd,ps", [
+    ([4100 + i for i in range(40)], 4096, 16, 2, 128, 16),                       # several row tiles
+    ([9000, 10, 0, 8192, 8191, 8193] + [8300] * 20, 8192, 6, 2, 128, 64),         # sequences inside the prefix
+    ([4096] * 33, 4096, 8, 8, 64, 256),                                          # nothing but the prefix
+    ([16700, 16900] * 12, 16384, 32, 1, 128, 16),                                # groups of 32: tiles on the own keys
+    ([4500, 4097, 4100, 5003] * 8, 4096, 40, 8, 96, 32),
+    ([40000 + i for i in range(20)], 39936, 32, 8, 128, 64),                     # the prefix on most SMs
+])
+def test_prefix_phase(cuda_device, keys, shared, H, KV, hd, ps):
+    """Batches whose prefix has a phase of its own (three launches), with other
+    lengths than the plan was made for too."""
+    dev, B = cuda_device, len(keys)
+    g = torch.Generator(device=dev).manual_seed(B + shared)
+    rnd = lambda *s: torch.randn(s, generator=g, device=dev).half()  # noqa: E731
+    full = [max(n, shared) for n in keys]  # every sequence holds the prefix's pages, used or not
+    k, v = ([rnd(n, KV, hd) for n in full] for _ in range(2))
+    for x in (k, v):
+        for y in x[1:]:
+            y[:shared] = x[0][:shared]
+    kp, vp, table, lens = to_pages(k, v, ps, shared=shared)
+    q = rnd(B, H, hd)
+    for lengths in (keys, [max(0, n - 700 - 13 * b) for b, n in enumerate(keys)]):
+        lens.copy_(torch.tensor(lengths))
+        out = torch.empty((B, H * hd), dtype=torch.float16, device=dev)
+        n = launches(lambda: nb.attention_paged_decode(q.reshape(B, -1), kp, vp, table, lens, heads=H, shared_len=shared,
+                                                       ctx_len=max(keys), out=out))
+        assert n == 3 and npu.device_error() == 0
+        want = [attention_exact(q[b:b + 1], k[b][:m], v[b][:m], 1 / math.sqrt(hd)) for b, m in enumerate(lengths)]
+        same(out, torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want]))
+
+
+@pytest.mark.parametrize("B,shared,own", [(2, 64, 100), (2, 512, 100), (4, 512, 100), (64, 131072, 100)])
+def test_a_prefix_costs_nothing(cuda_device, B, shared, own):
+    """Telling of a shared prefix takes no longer than not telling of it (short
+    ones took up to 1.6 times as long, through a phase of their own)."""
+    dev, H, KV, hd, ps = cuda_device, 32, 8, 128, 64
+    g = torch.Generator(device=dev).manual_seed(B)
+    pages = shared // ps + B * -(-own // ps)
+    kp, vp = (torch.randn((pages, KV, ps, hd), generator=g, device=dev).half() for _ in range(2))
+    at = shared // ps
+    table = torch.arange(pages, dtype=torch.int32, device=dev)
+    table = torch.cat([table[:at].expand(B, at), table[at:].view(B, -1)], 1).contiguous()
+    lens = torch.full((B,), shared + own, dtype=torch.int32, device=dev)
+    q = torch.randn((B, H * hd), generator=g, device=dev).half()
+    took = []
+    for sl in (shared, 0):
+        graph = torch.cuda.CUDAGraph()
+        run = lambda: nb.attention_paged_decode(q, kp, vp, table, lens, heads=H, shared_len=sl)  # noqa: E731
+        run()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            for _ in range(20):
+                run()
+        graph.replay()
+        best = math.inf
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            graph.replay()
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        took.append(best)
+        del graph
+    assert took[0] < 1.2 * took[1], took
