@@ -366,8 +366,9 @@ size_t npub_attention_paged_workspace(int batch, int total, int max_new, int64_t
 /* Decode attention over the paged cache, one new row per sequence (row b of q
  * and out), keys 0 .. lens[b] - 1.  shared_len > 0 (a multiple of page_size)
  * says that the first shared_len keys of every sequence are in the same
- * pages: they are read through row 0 of the table, once for the whole batch
- * instead of once per sequence.  A sequence with lens[b] < shared_len sees the
+ * pages: they are read through row 0 of the table (what the other rows hold
+ * there is not looked at), where it pays once for the whole batch instead of
+ * once per sequence.  A sequence with lens[b] < shared_len sees the
  * first lens[b] of them; lens[b] <= 0 gives zeros.  The result is that of
  * shared_len 0 up to rounding.  ctx_len, workspace and limits as above
  * (npub_attention_paged_decode_workspace with the same ctx_len and

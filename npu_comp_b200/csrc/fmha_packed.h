@@ -16,6 +16,7 @@ struct KvSource {
     const int32_t* table;    // pages: [batch, max_pages] page ids, row stride ldt
     int64_t ldt;
     int max_pages, n_pages, page_size;
+    int common;              // pages, paged_decode: the first `common` keys of all sequences are looked up in row 0
 };
 
 struct PackedArgs {

@@ -142,13 +142,14 @@ Plan make_plan(int batch, int total, int max_new, int64_t ctx, int shared, int h
     if (shared <= 0 || batch < 2) return pl;  // nothing to share
     // The prefix phase takes a part of the SMs and the own keys run beside it on the others, then on all: together
     // they take the longer of the prefix's time and the sum of both phases' shares of the SMs, and 4 us to combine.
-    // It is left out where reading the prefix for every sequence is estimated to be as quick.  Measured, 32 / 8 heads
+    // It is left out where the few-row kernel is estimated to read the prefix for every sequence as quickly (through row
+    // 0 of the table; the same look-up in the tile kernel costs chunks of prompts 1 %).  Measured, 32 / 8 heads
     // of 128, with the phase and without: 2 sequences of 100 own keys behind 512 keys 9.4 and 6.8 us, 64 of 200 behind
     // 128 22.7 and 18.7, 16 of 200 behind 2048 15.0 and 25.3.  (The estimate without it takes no account of the L2,
     // from which all but the first read the prefix: near the border it keeps the phase, 4 sequences behind 4096 16.6
     // and 13.0.)  Its SMs: 64 sequences of 100 own keys behind 131072 take 213 us on half of them, 163 on all;
     // 64 of 265 behind 8192 36 on half, 46 on all.
-    double best = pl.own.us;
+    double best = pl.few ? pl.own.us : 1e30;
     const Phase mine = own(ctx > shared ? ctx - shared : 1, true);
     for (int quarters = 2; quarters <= 4; ++quarters) {
         const Phase pre = tile_phase(total, 1, heads, kv_heads, 0, shared, sms * quarters / 4, part_us, true);
@@ -312,6 +313,7 @@ extern "C" int npub_attention_paged_decode(const void* q, int64_t ldq, const voi
     a.kv.max_pages = max_pages;
     a.kv.n_pages = n_pages;
     a.kv.page_size = page_size;
+    a.kv.common = shared_len;
     a.lens = lens;
     a.total_q = batch;
     a.batch = batch;

@@ -52,7 +52,7 @@ struct Params {
     int64_t ldq;
     const int32_t *cu, *lens, *table;
     int64_t ldt;
-    int max_keys, page_shift, box_rows, n_pages;
+    int max_keys, page_shift, box_rows, n_pages, common;
     int total_q, heads, kv_heads, group, head_dim, causal;
     int first, splits;         // every sequence's keys from `first` on in `splits` equal ranges
     int split0;                // index of split 0 among the partials
@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
             const int key = k0 + j * kKeys + box * p.box_rows;
             int page = p.n_pages;  // past the keys: outside the pool, filled with zeros
             if (box < nbox && key < k1) {
-                const int id = __ldg(p.table + (int64_t)b * p.ldt + (key >> p.page_shift));
+                const int64_t row = key < p.common ? 0 : b;
+                const int id = __ldg(p.table + row * p.ldt + (key >> p.page_shift));
                 if (id >= 0 && id < p.n_pages) page = id;
             }
             ok = mbar_wait_warp(&empty[s], ((uint32_t)(j / L::kStages) & 1u) ^ 1u, abort_flag);
@@ -535,6 +536,7 @@ int paged_decode(const PackedArgs& a, cudaStream_t st) {
     const int64_t mk = (int64_t)a.kv.max_pages << p.page_shift;
     p.max_keys = mk > 0x7ff00000 ? 0x7ff00000 : (int)mk;
     p.n_pages = a.kv.n_pages;
+    p.common = a.kv.common;
     p.table = a.kv.table;
     p.ldt = a.kv.ldt;
     p.lens = a.lens;

@@ -803,8 +803,8 @@ def attention_paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     per sequence, keys 0 .. lens[b] - 1.
 
     shared_len (a multiple of page_size): the first shared_len keys of every
-    sequence are in the same pages (a common prefix); they are read once for
-    the batch, through the table's first row.  The result is that of
+    sequence are in the same pages (a common prefix); they are read through the
+    table's first row, where it pays once for the batch.  The result is that of
     shared_len=0 up to rounding, also for sequences shorter than shared_len.
     ctx_len: the largest lens expected (0: the table's width)."""
     dev, n, qc, ldq = _first16(q, "q")

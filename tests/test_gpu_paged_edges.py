@@ -480,6 +480,8 @@ def launches(call):
     ([9000, 10, 0, 8192, 8191, 8193] + [8300] * 20, 8192, 6, 2, 128, 64),         # sequences inside the prefix
     ([4096] * 33, 4096, 8, 8, 64, 256),                                          # nothing but the prefix
     ([16700, 16900] * 12, 16384, 32, 1, 128, 16),                                # groups of 32: tiles on the own keys
+    ([900, 1100, 640], 640, 32, 1, 64, 16),                                      # which keep the phase in any case
+    ([6200, 6512, 5000, 600], 512, 32, 1, 128, 64),
     ([4500, 4097, 4100, 5003] * 8, 4096, 40, 8, 96, 32),
     ([40000 + i for i in range(20)], 39936, 32, 8, 128, 64),                     # the prefix on most SMs
 ])
@@ -495,6 +497,7 @@ def test_prefix_phase(cuda_device, keys, shared, H, KV, hd, ps):
         for y in x[1:]:
             y[:shared] = x[0][:shared]
     kp, vp, table, lens = to_pages(k, v, ps, shared=shared)
+    table[1:, :shared // ps] = 1 << 30  # the prefix is looked up in row 0
     q = rnd(B, H, hd)
     for lengths in (keys, [max(0, n - 700 - 13 * b) for b, n in enumerate(keys)]):
         lens.copy_(torch.tensor(lengths))
@@ -540,3 +543,30 @@ def test_a_prefix_costs_nothing(cuda_device, B, shared, own):
         took.append(best)
         del graph
     assert took[0] < 1.2 * took[1], took
+
+
+@pytest.mark.parametrize("keys,shared,H,KV,hd,ps", [
+    ([700, 300, 0, 512, 511, 513], 512, 8, 2, 128, 16),   # few rows, in a cluster or whole
+    ([12000, 4200], 4096, 8, 2, 128, 64),                  # as partials
+    ([9000], 8192, 4, 2, 128, 128),
+])
+def test_prefix_without_a_phase(cuda_device, keys, shared, H, KV, hd, ps):
+    """Batches that are quicker without a phase for the prefix find it in row 0
+    of the table all the same."""
+    dev, B = cuda_device, len(keys)
+    g = torch.Generator(device=dev).manual_seed(shared)
+    rnd = lambda *s: torch.randn(s, generator=g, device=dev).half()  # noqa: E731
+    k, v = ([rnd(max(n, shared), KV, hd) for n in keys] for _ in range(2))
+    for x in (k, v):
+        for y in x[1:]:
+            y[:shared] = x[0][:shared]
+    kp, vp, table, lens = to_pages(k, v, ps, shared=shared)
+    lens.copy_(torch.tensor(keys))
+    table[1:, :shared // ps] = 1 << 30
+    q = rnd(B, H, hd)
+    out = torch.empty((B, H * hd), dtype=torch.float16, device=dev)
+    n = launches(lambda: nb.attention_paged_decode(q.reshape(B, -1), kp, vp, table, lens, heads=H, shared_len=shared,
+                                                   ctx_len=max(keys), out=out))
+    assert n < 3 and npu.device_error() == 0
+    want = [attention_exact(q[b:b + 1], k[b][:m], v[b][:m], 1 / math.sqrt(hd)) for b, m in enumerate(keys)]
+    same(out, torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want]))
