@@ -363,6 +363,17 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&x)[128]) {
         for (int e = 0; e < 32; ++e) x[i * 32 + e] = __uint_as_float(r[i][e]);
 }
 
+// An exponent is x c - m c in one FMA.  From |m c| = 1024 on the rounding of m c
+// (2^-14 there) would weigh blocks and key ranges with other references
+// differently by more than a quarter of P's rounding, and from 2^28 on overflow
+// P: the warp's rows then subtract their reference from the scores first.  (The
+// branch costs twelve ragged prompts at head_dim 64 47.7 -> 48.5 us and drafted
+// rows 1 %, long prompts nothing; subtracting always 49.3 and 1 % everywhere, a
+// copy of the exponentials for it 48.9.)
+__device__ __forceinline__ bool far_off(float m, float c) {
+    return __any_sync(0xffffffffu, m != -INFINITY && !(fabsf(m) * c <= 1024.0f));
+}
+
 // The largest of three, NaN when one is.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float r;
@@ -758,6 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 else if (p.causal) lim = min(lim, it.off + tok + 1);
             }
             float m = -INFINITY, l = 0.0f;
+            bool far = false;  // some row's reference is, in this warp
             const int nb = q ? it.n[1] : it.n[0];
             for (int j = 0; j < nb; ++j) {
                 ok = mbar_wait_warp(&s_full[q], ns & 1u, abort_flag);
@@ -774,11 +786,13 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                 const float mx = max3_nan(m, row_max(x), m);
                 if (j == 0) {
                     m = mx;
+                    far = far_off(m, c);
                 } else {
                     const bool need = mx != -INFINITY && !((mx - m) * c <= 8.0f);  // also when the maximum is NaN
                     if (__any_sync(0xffffffffu, need)) {  // P_q(j-1) V_{j-1} is complete: S_q(j) was issued behind it
                         const float corr = need ? ex2_approx((m - mx) * c) : 1.0f;
                         if (need) m = mx;
+                        far |= far_off(m, c);
                         l *= corr;
 #pragma unroll 1
                         for (int e0 = 0; e0 < HD; e0 += 32) {
@@ -790,7 +804,13 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
                         }
                     }
                 }
-                const float mc = m == -INFINITY ? 0.0f : -m * c;  // 0: every exponential of the row is 2^-inf
+                const float ref = m == -INFINITY ? 0.0f : m;  // 0: every exponential of the row is 2^-inf
+                float mc = -ref * c;
+                if (far) {
+                    mc = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 128; ++e) x[e] -= ref;
+                }
                 const uint64_t c2 = pack2(c, c), mc2 = pack2(mc, mc);
                 uint64_t sum2[2] = {0, 0};
 #pragma unroll
@@ -838,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_packed_kernel(const __grid_c
             if (flat) l = none ? 0.0f : PART ? 1.0f : NAN;
             const int sp = p.split0 + (DUAL ? 2 * it.split + q : it.split);
             const int64_t at = PART ? ((int64_t)sp * p.total_q + row) * p.heads + head : 0;
-            if (PART && valid) p.part_ml[at] = make_float2(flat ? -INFINITY : m * c, l);
+            if (PART && valid) p.part_ml[at] = make_float2(m, l);
             const bool put = valid && !(PART && flat);
             const float inv = none ? 0.0f : 1.0f / l;
             float* dstf = p.part_o + at * p.head_dim;

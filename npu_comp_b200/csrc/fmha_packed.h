@@ -37,7 +37,7 @@ struct PackedArgs {
     int splits;           // equal ranges of every sequence's keys from `first` on
     int first, split0;    // split0: index of split 0 among the partials
     float* part_o;        // [splits, total_q, heads, head_dim]
-    // [splits, total_q, heads]: (row maximum * scale * log2 e, sum of exponentials); (-inf, 0) where the row has no key
+    // [splits, total_q, heads]: (row's reference score, sum of exponentials); (-inf, 0) where the row has no key
     // in the range, (-inf, 1) where all its scores there are -inf (part_o is not written then)
     float2* part_ml;
 };

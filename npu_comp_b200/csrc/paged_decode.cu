@@ -299,12 +299,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
                         o[n][2 * r + 1] *= corr;
                     }
                 }
-                const float mc = m[r] == -INFINITY ? 0.0f : m[r] * c;
+                const float ref = m[r] == -INFINITY ? 0.0f : m[r];
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float pv = ex2_approx(fmaf(x[n][2 * r + e], c, -mc));
+                        const float pv = ex2_approx((x[n][2 * r + e] - ref) * c);
                         x[n][2 * r + e] = pv;
                         l[r] += pv;
                     }
@@ -377,12 +377,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
         if (p.cluster) {
             if (d == 0)
                 *reinterpret_cast<float2*>(smem + L::kOffOwnMl + r * 8) =
-                    make_float2(mm == -INFINITY ? -INFINITY : mm * c, sum);
+                    make_float2(mm, sum);
             *reinterpret_cast<float4*>(smem + L::kOffOwn + (r * HD + d) * 4) =
                 make_float4(acc[0], acc[1], acc[2], acc[3]);
         } else if (part) {
             const int64_t at = ((int64_t)(p.split0 + split) * p.total_q + row0 + t) * p.heads + head;
-            if (d == 0) p.part_ml[at] = make_float2(mm == -INFINITY ? -INFINITY : mm * c, sum);
+            if (d == 0) p.part_ml[at] = make_float2(mm, sum);
             if (sum != 0.0f && !flat)
                 *reinterpret_cast<float4*>(p.part_o + at * p.head_dim + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         } else {
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
             for (int t = 0; t < n; ++t) {
                 const float2 ml = ld_cluster_f2(mapa_shared(ml_at, t));
                 if (ml.y == 0.0f) continue;
-                const float f = ex2_approx(ml.x - mm);
+                const float f = ex2_approx((ml.x - mm) * c);
                 const float4 v = ld_cluster_f4(mapa_shared(o_at, t));
                 sum += f * ml.y;
                 acc[0] += f * v.x;
@@ -430,13 +430,14 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const __grid_
     if (holds) pdl_wait();
 }
 
-// out[row, head] = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s over the
+// out[row, head] = sum_s 2^((m_s - m) c) o_s / sum_s 2^((m_s - m) c) l_s over the
 // splits that saw a key; one warp per (row, head).  Rows outside
 // [cu[0], cu[batch]) are left as they are.
 __global__ void __launch_bounds__(128) paged_combine_kernel(const float* __restrict__ part_o,
                                                             const float2* __restrict__ part_ml, int splits, int rows,
                                                             int heads, int hd, const int32_t* __restrict__ cu,
-                                                            int batch, __half* __restrict__ out, int64_t ldo) {
+                                                            int batch, float c, __half* __restrict__ out,
+                                                            int64_t ldo) {
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31;
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const float* __restr
         float f = 0.0f;
         if (s0 + lane < splits) {
             const float2 ml = part_ml[(int64_t)(s0 + lane) * n + id];
-            if (ml.y != 0.0f) f = ex2_approx(ml.x - m);
+            if (ml.y != 0.0f) f = ex2_approx((ml.x - m) * c);
             sum += f * ml.y;
         }
         const float* src = part_o + ((int64_t)s0 * n + id) * hd + lane * 4;
@@ -567,7 +568,7 @@ int paged_combine(const PackedArgs& a, int splits, cudaStream_t st) {
     const int64_t n = (int64_t)a.total_q * a.heads;
     if ((n + 3) / 4 > 0x7fffffff) return NPUB_ERR_UNSUPPORTED;
     return launch_pdl(pdec::paged_combine_kernel, dim3((unsigned)((n + 3) / 4)), dim3(128), 0, st, a.part_o,
-                      a.part_ml, splits, a.total_q, a.heads, a.head_dim, a.cu, a.batch,
+                      a.part_ml, splits, a.total_q, a.heads, a.head_dim, a.cu, a.batch, a.scale * 1.4426950408889634f,
                       reinterpret_cast<__half*>(a.out), a.ldo);
 }
 

@@ -18,7 +18,8 @@ def offsets(lens, dev):
 
 # How a call reaches each kernel: new rows and keys per sequence, heads, the keys that take turns in the test.
 #   packed / tiles: tile kernel, keys whole; ranges: the tile kernel's partials; few: up to 16 rows per kv head, keys
-#   whole, in a cluster, or as partials; decode, prefix: one row, with and without a shared prefix
+#   whole, in a cluster, or as partials; decode, prefix, prefix_phase: one row, without a shared prefix, with one that
+#   every sequence reads, and with one that has a phase of its own
 PATHS = {
     "packed": ([200, 70, 1], [200, 70, 1], 4, 2),
     "tiles": ([150, 3, 9], [300, 77, 4], 4, 2),
@@ -27,6 +28,7 @@ PATHS = {
     "few_long": ([3, 1, 4], [6000, 70, 700], 4, 2),
     "decode": ([1] * 4, [300, 0, 65, 2000], 8, 2),
     "prefix": ([1] * 4, [700, 520, 600, 513], 8, 2),
+    "prefix_phase": ([1] * 20, [2500, 2049, 2048] + [2100 + 7 * i for i in range(17)], 32, 8),
 }
 
 
@@ -36,31 +38,33 @@ class Call:
     def __init__(self, dev, path, hd, causal=True, ps=16):
         self.path, self.hd, self.causal, self.ps, self.dev = path, hd, causal, ps, dev
         self.new, self.keys, self.H, self.KV = PATHS[path]
+        self.decode = path in ("decode", "prefix", "prefix_phase")
         g = torch.Generator(device=dev).manual_seed(hd + sum(self.keys))
         rnd = lambda *s: torch.randn(s, generator=g, device=dev).half()  # noqa: E731
         self.q = [rnd(n, self.H, hd) for n in self.new]
         self.k = [rnd(n, self.KV, hd) for n in self.keys]
         self.v = [rnd(n, self.KV, hd) for n in self.keys]
-        self.shared = 512 if path == "prefix" else 0
+        self.shared = {"prefix": 512, "prefix_phase": 2048}.get(path, 0)
         for x in (self.k, self.v):
             for y in x[1:]:
                 y[:self.shared] = x[0][:self.shared]
 
-    def run(self):
+    def run(self, scale=None):
         dev, H, KV, hd = self.dev, self.H, self.KV, self.hd
         q, cu = torch.cat(self.q).reshape(-1, H * hd), offsets(self.new, dev)
         if self.path == "packed":
             o = nb.attention_packed(q, torch.cat(self.k).reshape(-1, KV * hd), torch.cat(self.v).reshape(-1, KV * hd),
-                                    cu, H, KV, head_dim=hd, causal=self.causal)
+                                    cu, H, KV, head_dim=hd, causal=self.causal, scale=scale)
         else:
             kp, vp, table, lens = to_pages(self.k, self.v, self.ps, shared=self.shared)
-            if self.path in ("decode", "prefix"):
-                o = nb.attention_paged_decode(q, kp, vp, table, lens, heads=H, shared_len=self.shared)
+            if self.decode:
+                o = nb.attention_paged_decode(q, kp, vp, table, lens, heads=H, shared_len=self.shared, scale=scale)
             else:
-                o = nb.attention_paged(q, kp, vp, table, lens, cu, heads=H, causal=self.causal,
+                o = nb.attention_paged(q, kp, vp, table, lens, cu, heads=H, causal=self.causal, scale=scale,
                                        max_new=max(self.new) if "few" in self.path else 0)
         assert npu.device_error() == 0
-        want = [attention_exact(a, b, c, 1 / math.sqrt(hd), self.causal) for a, b, c in zip(self.q, self.k, self.v)]
+        scale = scale or 1 / math.sqrt(hd)
+        want = [attention_exact(a, b, c, scale, self.causal) for a, b, c in zip(self.q, self.k, self.v)]
         same(o, torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want]))
         return o
 
@@ -71,8 +75,10 @@ def test_infinite_and_nan_scores(cuda_device, path, hd):
     """A key whose score is +inf or NaN makes the rows that see it NaN, and no
     other row: at every place of a group of eight keys, in the first, a middle
     and the last block of a row's keys."""
-    for causal in (True, False) if path not in ("decode", "prefix") else (True,):
+    for causal in (True, False):
         c = Call(cuda_device, path, hd, causal)
+        if c.decode and not causal:
+            continue
         m = c.keys[0]
         for j in sorted({*range(8), 64, 65, min(129, m - 1), m // 2, *range(m - 9, m)}):
             for value in (math.inf, math.nan):
@@ -112,7 +118,8 @@ def test_scores_of_minus_infinity(cuda_device, path, hd):
                 y[:c.shared] = c.k[0][:c.shared]
                 x[..., 3] = x[..., 3].abs() + 0.125
         o = c.run()
-        assert torch.isnan(o).any() == (n > m - c.new[0])
+        # the first sequence's first row sees nothing else, or another sequence whose keys end with the prefix
+        assert torch.isnan(o).any() == (n > m - c.new[0] or 0 < min(c.keys) <= min(n, c.shared))
         c.k[0] = k
 
 @pytest.mark.parametrize("keys", [[40, 9, 30, 7], [900, 9, 30, 1200], [30000, 9, 30, 20000]])  # whole, cluster, partials
@@ -570,3 +577,43 @@ def test_prefix_without_a_phase(cuda_device, keys, shared, H, KV, hd, ps):
     assert n < 3 and npu.device_error() == 0
     want = [attention_exact(q[b:b + 1], k[b][:m], v[b][:m], 1 / math.sqrt(hd)) for b, m in enumerate(keys)]
     same(out, torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want]))
+
+# ----------------------------------------------------------------- large scores
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("path", PATHS)
+@pytest.mark.parametrize("at", [0.0, 2.0 ** 12, 1e6, -1e6])
+def test_scores_far_from_zero(cuda_device, path, hd, at):
+    """Scores of `at` + u, exact in fp32 (u a multiple of 1/8, rising over the
+    keys so that every block and key range has another maximum): the weights
+    depend on u alone."""
+    c = Call(cuda_device, path, hd)
+    root = math.sqrt(abs(at))  # 0, 64 or 1000
+    for b, m in enumerate(c.keys):
+        u = torch.arange(m, device=cuda_device) * (30.0 / max(m, 1)) + 4 * torch.rand(m, device=cuda_device)
+        if c.shared and b:
+            u[:c.shared] = first[:c.shared]
+        elif b == 0:
+            first = u
+        c.q[b].zero_()
+        c.q[b][..., 0], c.q[b][..., 1] = root, 1.0
+        c.k[b].zero_()
+        c.k[b][..., 0], c.k[b][..., 1] = math.copysign(root, at), ((u * 8).round() / 8)[:, None]
+    c.run(scale=1.0)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("path", PATHS)
+def test_the_largest_finite_scores(cuda_device, path, hd):
+    """q and k at +-60000 in every column: equal scores give the mean of v, and
+    one key ahead of the others its v."""
+    c = Call(cuda_device, path, hd)
+    for sign in (1, -1):
+        for b in range(len(c.keys)):
+            c.q[b].fill_(60000.0)
+            c.k[b].fill_(sign * 60000.0)
+        c.run()
+    for b, m in enumerate(c.keys):
+        if m > max(1, c.shared):  # (the prefix's keys stay alike)
+            c.k[b][max(m - 2, c.shared)] = 30000.0
+    c.run()
