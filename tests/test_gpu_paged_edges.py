@@ -617,3 +617,85 @@ def test_the_largest_finite_scores(cuda_device, path, hd):
         if m > max(1, c.shared):  # (the prefix's keys stay alike)
             c.k[b][max(m - 2, c.shared)] = 30000.0
     c.run()
+
+
+# ------------------------------------------------------- lengths and padding
+
+@pytest.mark.parametrize("H,KV,hd", [(4, 2, 128), (32, 1, 64)])
+def test_lengths_outside_the_table(cuda_device, H, KV, hd):
+    """lens past the table's width count as the width, negative ones as none, by
+    rows, chunks and behind a prefix."""
+    dev, ps, n = cuda_device, 16, 320
+    g = torch.Generator(device=dev).manual_seed(H)
+    rnd = lambda *s: torch.randn(s, generator=g, device=dev).half()  # noqa: E731
+    lengths, new = [2 ** 31 - 1, -5, n + 1, -2 ** 31, 100], [1, 1, 3, 2, 2]
+    k, v = ([rnd(n, KV, hd) for _ in lengths] for _ in range(2))
+    for x in (k, v):
+        for y in x[1:]:
+            y[:64] = x[0][:64]
+    kp, vp, table, lens = to_pages(k, v, ps, shared=64)
+    table = table[:, :n // ps]
+    lens.copy_(torch.tensor(lengths))
+    sc, keys = 1 / math.sqrt(hd), [max(0, min(n, m)) for m in lengths]
+    q = rnd(sum(new), H, hd)
+    want = [attention_exact(a, k[b][:keys[b]], v[b][:keys[b]], sc) for b, a in enumerate(q.split(new))]
+    for max_new in (0, 3):
+        o = nb.attention_paged(q.reshape(-1, H * hd), kp, vp, table, lens, offsets(new, dev), heads=H, max_new=max_new)
+        same(o, torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want]))
+    q = rnd(len(lengths), H, hd)
+    want = [attention_exact(q[b:b + 1], k[b][:keys[b]], v[b][:keys[b]], sc) for b in range(len(lengths))]
+    for shared in (0, 64):
+        o = nb.attention_paged_decode(q.reshape(-1, H * hd), kp, vp, table, lens, heads=H, shared_len=shared)
+        same(o, torch.cat([w[0] for w in want]), torch.cat([w[1] for w in want]))
+    assert npu.device_error() == 0
+
+
+def test_a_mostly_empty_batch(cuda_device):
+    """A batch padded for a graph: 20000 rows of which 40 are in use, 300 sequences
+    of which three hold them; then none."""
+    dev, T, B, H, KV, hd, ps = cuda_device, 20000, 300, 8, 2, 128, 16
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn((T, (H + 2 * KV) * hd), generator=g, device=dev).half()
+    x[40:] = float("nan")
+    q, k, v = x[:, :H * hd], x[:, H * hd:(H + KV) * hd], x[:, (H + KV) * hd:]
+    cu = torch.full((B + 1,), 40, dtype=torch.int32, device=dev)
+    cu[:101], cu[101:201] = 0, 3  # sequence 100: 3 rows, 200: 37
+    f, pos = nb.rope_freqs(hd, device=dev), torch.zeros(T, dtype=torch.int32, device=dev)
+    pos[:40] = torch.tensor([0, 1, 2] + list(range(37)))
+    kp, vp = (torch.full((8, KV, ps, hd), 3.0, dtype=torch.float16, device=dev) for _ in range(2))
+    table = torch.full((B, 3), 1 << 30, dtype=torch.int32, device=dev)
+    table[100, 0], table[200] = 6, torch.tensor([1, 5, 0])
+    lens = torch.zeros(B, dtype=torch.int32, device=dev)
+    lens[100], lens[200] = 3, 37
+    parts = [slice(0, 3), slice(3, 40)]
+    o = torch.full((T, H * hd), 3.0, dtype=torch.float16, device=dev)
+    for _ in range(2):
+        nb.attention_packed(q, k, v, cu, H, KV, head_dim=hd, out=o)
+        rot = torch.full((T, H * hd), 3.0, dtype=torch.float16, device=dev)
+        nb.rope_paged_append(x, H, KV, hd, pos, f, kp, vp, table, cu_seqlens=cu, out=rot)
+        for r in parts:
+            n = r.stop - r.start
+            e, b = attention_exact(q[r].reshape(n, H, hd), k[r].reshape(n, KV, hd), v[r].reshape(n, KV, hd),
+                                   1 / math.sqrt(hd))
+            same(o[r], e, b)
+        assert (o[40:] == 3.0).all() and (rot[40:] == 3.0).all()
+        for max_new in (0, 2):  # sequences of 3 and 37 rows: max_new is not one of this batch's
+            out = torch.full((T, H * hd), 3.0, dtype=torch.float16, device=dev)
+            nb.attention_paged(rot, kp, vp, table, lens, cu, heads=H, max_new=max_new, out=out)
+            for r, ids in zip(parts, ([6], [1, 5, 0])):
+                n = r.stop - r.start
+                kk, vv = (p[ids].transpose(1, 2).reshape(-1, KV, hd)[:n] for p in (kp, vp))
+                m = n if max_new == 0 else min(n, 4)
+                e, b = attention_exact(rot[r].reshape(n, H, hd), kk, vv, 1 / math.sqrt(hd))
+                same(out[r][:m], e[:m], b[:m])
+                assert not out[r][m:].any()
+            assert (out[40:] == 3.0).all()
+    cu.zero_()
+    for run in (lambda y: nb.attention_packed(q, k, v, cu, H, KV, head_dim=hd, out=y),
+                lambda y: nb.attention_paged(rot, kp, vp, table, lens, cu, heads=H, out=y),
+                lambda y: nb.attention_paged(rot, kp, vp, table, lens, cu, heads=H, max_new=1, out=y),
+                lambda y: nb.rope_paged_append(x, H, KV, hd, pos, f, kp, vp, table, cu_seqlens=cu, out=y)):
+        y = torch.full((T, H * hd), 3.0, dtype=torch.float16, device=dev)
+        run(y)
+        assert (y == 3.0).all()
+    assert npu.device_error() == 0
