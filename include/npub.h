@@ -336,7 +336,9 @@ int npub_rope_paged_append(const void* qkv, int64_t ldx, void* q_out, int64_t ld
  * head_dim % 16 == 0.  head_dim > 128 or heads / kv_heads > 128 returns
  * NPUB_ERR_UNSUPPORTED.  Nothing outside a sequence reaches its results, but
  * the values of its own later rows have to be finite.  A row that sees a score
- * of NaN or +inf, or nothing but -inf, gives NaN.  Needs no workspace. */
+ * of NaN or +inf, or nothing but -inf, gives NaN.  The weights are rounded to
+ * fp16 before the product with v, so a result within 2^-10 of fp16's largest
+ * value may come out as inf.  Needs no workspace. */
 int npub_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
                           void* out, int64_t ldo, const int32_t* cu_seqlens, int batch, int total, int heads,
                           int kv_heads, int head_dim, float scale, int causal, void* stream);

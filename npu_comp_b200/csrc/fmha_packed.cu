@@ -11,7 +11,8 @@
 // G query heads, so that the group shares every K/V load and a prompt of few
 // tokens still fills rows.  A CTA takes two tiles, which share K and V:
 //   S_q(j) = Q_q K_j^T          tcgen05.mma, fp32 in TMEM
-//   P_q(j) = exp2(S c - m c)    one thread per row; fp16, over S_q's own TMEM columns
+//   P_q(j) = exp2(S c - m c)    one thread per row; fp16, over S_q's own TMEM columns (both operands of a kind::f16
+//                               MMA are fp16, as V is: half a step, 2^-11 of each weight; sums, S and O are fp32)
 //   O_q   += P_q(j) V_j         tcgen05.mma with A = P from TMEM, V read MN-major
 // O stays in TMEM over the whole key loop.  A row's reference maximum m moves
 // (and its O and sum are rescaled) only when the row maximum has grown by more
@@ -21,15 +22,18 @@
 //
 // What bounds it (clock64 stamps in one CTA, 8192 causal tokens, 32/8 heads):
 // at head_dim 128 a pair of tiles takes 2820 cycles per key block, of which
-// the tensor core runs 2048; a tile's chain is its softmax (1850: 160 to read
+// the tensor core runs 2048 (0.73; over the whole kernel, with its start, item
+// changes and end, 0.62); a tile's chain is its softmax (1850: 160 to read
 // S, 440 for the maximum and the rescale test, 1250 for the exponentials) and
-// then the second half of P V and the next S.  446 us, 1230 TFLOP/s: 0.74 of
-// the burst rate, 0.87 of the sustained one, with the clock down to 1.6 GHz
-// under the power limit.  At head_dim 64 the products are half as long and the
+// then the second half of P V and the next S.  One call after the other it takes
+// 507-514 us, 1080 TFLOP/s: 0.65 of the burst rate, 0.76 of the sustained one,
+// with the clock at 1.57 GHz under the power limit.  At head_dim 64 (414 us,
+// 660 TFLOP/s) the products are half as long and the
 // exponentials bound it (16 per cycle and SM), so a quarter of them runs as a
-// polynomial on the FMA pipe there (437 against 469 us when it was added); at
-// head_dim 128 that only costs issue slots and power (462 / 458 us).  Tried and
-// left out: P beside S at head_dim 64, so that the next S is formed during the
+// polynomial on the FMA pipe there.  The pairs of times from here on compare
+// two builds of their day in short runs at a higher clock: the polynomial 437
+// against 469 us; at head_dim 128 it only costs issue slots and power (462 / 458
+// us).  Tried and left out: P beside S at head_dim 64, so that the next S is formed during the
 // softmax (8192 tokens 207 -> 204 us, twelve ragged prompts 48 -> 51); two
 // threads per row, 16 softmax warps (454 -> 495-553 us, 48 -> 56: the pairs'
 // exchange and the second read of S, which 104 registers force); the
@@ -188,7 +192,7 @@ __device__ __forceinline__ int batch_tiles_from(const Params& p, const SeqRows& 
 
 // Where the scheduler stands.  A CTA's item numbers only ascend, so each search
 // goes on from the last one: 1000 prompts of 100 rows, 32 / 8 heads of 64, in
-// 470 us (11.9 ms with a search of the whole batch for every item, 86 us each).
+// 490 us (11.9 ms with a search of the whole batch for every item, 86 us each).
 // In shared memory: its warp's 56 registers do not hold it without spills.
 struct Place {
     int level;       // tiles of this level are handed out (sorted; else all tiles are one level)

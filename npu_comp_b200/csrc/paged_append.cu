@@ -95,7 +95,7 @@ __device__ __forceinline__ int seq_of_row(const int32_t* __restrict__ cu, int ba
 // before the block forms the angles and looks up the page.
 //
 // Measured at 8192 packed tokens of 32 / 8 heads of 128 with norms (201 MB):
-// 37.2 us with 128 threads, 5.4 TB/s or 0.83 of the copy rate (39.3 and 41.9
+// 38 us with 128 threads, 5.3 TB/s or 0.81 of the copy rate (when it was chosen 37.2; 39.3 and 41.9
 // with the heads of a token over two and three blocks); 43 with 96 or
 // 192 threads, 39.6 and 45 with two and four tokens per block, 46-48 with two
 // or three units in flight per thread (their registers cost more warps than

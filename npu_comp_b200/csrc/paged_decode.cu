@@ -16,7 +16,8 @@
 // or a shared prefix, leave partials for a second kernel.
 //
 // As in fmha_packed.cu the running maximum moves only when it has grown by
-// more than 2^8; keys past the sequence's end are masked by a select and their
+// more than 2^8, and the weights are rounded to fp16 (2^-11 of each) for the
+// product with V, all else is fp32; keys past the sequence's end are masked by a select and their
 // V rows zeroed, so stale slots of the last page never reach a result.
 #include "common.cuh"
 #include "fmha_packed.h"
