@@ -153,6 +153,32 @@ size_t npub_f16_gemm_workspace(int M, int N, int K);
  * this is the symmetric per-channel scheme its W8A16 target is defined by.) */
 int npub_quantize_w8(const float* W, int64_t ldw, int K, int N, int8_t* Wq, int64_t ldq, void* scale, void* stream);
 
+/* Matrix products in 8-bit integers with a scale for each token and channel
+ * (the quantised form of the projections of llama_layer.py:95-152; the
+ * reference has none).
+ * npub_quantize_rows: rows of fp16 [rows, cols] to int8 with one fp32 scale
+ * each, optionally behind the residual add and the RMSNorm of npub_rmsnorm:
+ *   h = fp16(x + residual), stored to h_out (residual NULL: h = x, h_out unused)
+ *   y = h / sqrt(mean(h^2) + eps) * gamma in fp32, unrounded (gamma fp16 [cols]; NULL: y = h)
+ *   scale[r] = max|y[r, :]| / 127,  q = round(127 y / max|y|), halves to even
+ * A row of zeros has scale 0; a row with an infinity or a NaN has scale NaN
+ * and q = 0.  cols % 8 == 0; ldx, ldr, ldh, ldq multiples of 8; x, residual,
+ * h_out, gamma 16-byte aligned, q 8-byte; h_out may be x or residual.
+ * npub_w8a8_gemm:
+ *   C[m, n] = fp16( a_scale[m] * w_scale[n] * sum_k A[m, k] W[n, k] (+ R[m, n]) )
+ * A int8 [M, K], W int8 [N, K] (K-major, e.g. from npub_quantize_w8), a_scale
+ * fp32 [M], w_scale fp16 [N], R and C fp16 (R may be NULL, or alias C).  The
+ * sums are exact integers, the rest is fp32 with one rounding.  swiglu != 0: W
+ * holds interleaved gate / up rows and C[m, c] = fp16(silu(z[m, 2c]) *
+ * z[m, 2c + 1]) [M, N / 2] (N even, R NULL).  K % 16 == 0, K <= 131056; lda,
+ * ldw multiples of 16, A, W 16-byte aligned.  No workspace. */
+int npub_quantize_rows(const void* x, int64_t ldx, const void* residual, int64_t ldr, void* h_out, int64_t ldh,
+                       const void* gamma, float eps, int rows, int cols, int8_t* q, int64_t ldq, float* scale,
+                       void* stream);
+int npub_w8a8_gemm(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw,
+                   const void* w_scale, void* C, int64_t ldc, const void* R, int64_t ldr, int M, int N, int K,
+                   int swiglu, void* stream);
+
 /* ---------------------------------------------------------- vector ops --
  * RMSNorm, d_compiler/npu_compiler/legalize.py:30-47, b_program_examples/llama_layer.py:79-89:
  *   y[r, :] = fp16( x[r, :] / sqrt(mean(x[r, :]^2) + eps) * gamma )   (fp32 math)

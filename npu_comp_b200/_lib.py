@@ -43,6 +43,8 @@ SIGNATURES = {
     "npub_w8a16_gemm_rms_workspace": (_sz, [_i, _i, _i]),
     "npub_w8a16_kernel_name": (ctypes.c_char_p, [_i, _i, _i]),
     "npub_w8a16_gemm_noalloc": (_i, [_p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _i, _i, _i, _f, _p]),
+    "npub_quantize_rows": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _f, _i, _i, _p, _i64, _p, _p]),
+    "npub_w8a8_gemm": (_i, [_p, _i64, _p, _p, _i64, _p, _p, _i64, _p, _i64, _i, _i, _i, _i, _p]),
     "npub_f16_gemm": (_i, [_p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _i, _i, _i, _f, _p, _sz, _p]),
     "npub_f16_gemm_workspace": (_sz, [_i, _i, _i]),
     "npub_quantize_w8": (_i, [_p, _i64, _i, _i, _p, _i64, _p, _p]),

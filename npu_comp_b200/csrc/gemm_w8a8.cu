@@ -1,0 +1,672 @@
+// Matrix products in 8-bit integers with a scale for each token and channel.
+//
+//   C[m, n] = fp16( a_scale[m] * w_scale[n] * sum_k A[m, k] W[n, k] )  (+ R[m, n])
+//   SwiGLU:   C[m, c] = fp16( silu(z[m, 2c]) * z[m, 2c + 1] ),  z the product above before rounding
+//
+// tcgen05.mma kind::i8: both operands s8 and K-major from shared memory (one
+// 128-byte swizzled row = 128 of K), the sums s32 in tensor memory, exact up to
+// |sum| < 2^31 (K * 128 * 128, which bounds K).  The scales are applied in fp32
+// and the result is rounded to fp16 once.
+//
+// Two kernels:
+//   w8a8_tile_kernel  2-CTA pairs, 256 tokens x 256 channels, persistent, the
+//                     sums double-buffered in tensor memory; tensor bound
+//   w8a8_few_kernel   128 channels x BT tokens in one CTA, the K axis over the
+//                     CTAs of a cluster, which add their sums through one
+//                     another's shared memory (integers: the order does not
+//                     matter); for few tokens, where the weights' bytes bound
+//                     it, and for products of few tiles
+// and `pick` chooses.
+#include "common.cuh"
+#include "gemm_tc.h"
+
+#include <mutex>
+
+namespace npub {
+namespace w8a8 {
+
+constexpr int BK = 128;       // K per stage: one swizzled row
+constexpr int kUmmaK = 32;    // K of one MMA
+constexpr int kMaxCluster = 8;
+
+struct Params {
+    CUtensorMap tmA, tmW;
+    int M, N, k_tiles;
+    int m_tiles, n_tiles, band;      // tile kernel
+    int per;                         // few kernel: K tiles of a CTA
+    const float* sa;
+    const __half* sw;
+    const __half* R;
+    int64_t ldr;
+    __half* C;
+    int64_t ldc;
+    int swiglu;
+    int vec;                         // rows of C (and R) and the scales can be read and written 16 bytes at a time
+    int* err;
+};
+
+__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {  // s32 sums, s8 x s8, both K-major
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void set_err(int* err, int code) {
+    if (err) atomicCAS(err, 0, code);
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16i(uint32_t taddr, int (&r)[16]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 half2_at(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+
+// ------------------------------------------------------------- 256 x 256 tiles
+
+constexpr int kTileStages = 6;
+constexpr int kTileThreads = 256;
+struct TileSmem {
+    static constexpr int kOp = 128 * BK;  // a CTA's half of either operand's tile
+    static constexpr int kOffBar = kTileStages * 2 * kOp;
+    static constexpr int kTotal = kOffBar + 256 + 1024;
+};
+
+// Tiles in bands of p.band token tiles, the channels in turn within a band, so
+// that the 74 tiles in flight share operands in L2.
+struct TileAt {
+    int m0, n0;
+};
+__device__ __forceinline__ TileAt tile_at(const Params& p, int t) {
+    const int per_band = p.band * p.n_tiles, b = t / per_band, r = t - b * per_band;
+    const int nb = min(p.band, p.m_tiles - b * p.band), n = r / nb;
+    return TileAt{(b * p.band + r - n * nb) * 256, n * 256};
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
+    w8a8_tile_kernel(const __grid_constant__ Params p) {
+    pdl_trigger();
+    using L = TileSmem;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sA = smem, *sB = smem + kTileStages * L::kOp;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar);  // [stages] (even CTA) both CTAs' operands landed
+    uint64_t* empty = full + kTileStages;                             // [stages] pair MMA done with the stage
+    uint64_t* acc_full = empty + kTileStages;                         // [2] sums ready
+    uint64_t* acc_empty = acc_full + 2;                               // [2] (even CTA) both epilogues have read them
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int cid = (int)cluster_id_x(), ncl = (int)nclusters_x();
+    const int n_all = p.m_tiles * p.n_tiles;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kTileStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], 8);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&p.tmA);
+        prefetch_tmap(&p.tmW);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {  // producer
+            uint32_t g = 0;
+            const uint32_t full0 = mapa_shared(smem_u32(&full[0]), 0);
+            for (int t = cid; t < n_all && !*abort_flag; t += ncl) {
+                const TileAt at = tile_at(p, t);
+                for (int i = 0; i < p.k_tiles; ++i, ++g) {
+                    const int s = (int)(g % kTileStages);
+                    if (!mbar_wait_cluster_bounded(&empty[s], ((g / kTileStages) & 1u) ^ 1u, abort_flag)) {
+                        *abort_flag = 1;
+                        set_err(p.err, 0x701);
+                        break;
+                    }
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], 4u * L::kOp);
+                    tma_load_3d_pair(sA + s * L::kOp, &p.tmA, full0 + (uint32_t)s * 8u, i * BK, at.m0 + (int)rank * 128, 0);
+                    tma_load_3d_pair(sB + s * L::kOp, &p.tmW, full0 + (uint32_t)s * 8u, i * BK, at.n0 + (int)rank * 128, 0);
+                }
+            }
+            // The MMA thread has waited for every load when it signals the last tile's sums.  After an abort nobody
+            // waits for those in flight: give them (microseconds) time to land before the CTAs leave.
+            if (*abort_flag) {
+                const uint64_t t0 = globaltimer_ns();
+                while (globaltimer_ns() - t0 < 1000000ull) {
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {  // MMA
+            constexpr uint32_t idesc = idesc_i8(256, 256);
+            uint32_t g = 0, n = 0;
+            bool ok = true;
+            for (int t = cid; t < n_all && ok; t += ncl, ++n) {
+                const uint32_t b = n & 1u;
+                if (!mbar_wait_cluster_bounded(&acc_empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag)) {
+                    ok = false;
+                    set_err(p.err, 0x702);
+                    break;
+                }
+                tc_fence_after();
+                for (int i = 0; i < p.k_tiles; ++i, ++g) {
+                    const int s = (int)(g % kTileStages);
+                    if (!mbar_wait_cluster_bounded(&full[s], (g / kTileStages) & 1u, abort_flag)) {
+                        ok = false;
+                        set_err(p.err, 0x703);
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(sA + s * L::kOp), w = smem_u32(sB + s * L::kOp);
+#pragma unroll
+                    for (int k = 0; k < BK / kUmmaK; ++k)
+                        mma_i8_pair(tmem + b * 256u, umma_desc_sw128(a + k * kUmmaK), umma_desc_sw128(w + k * kUmmaK), idesc,
+                                    (i > 0 || k > 0) ? 1u : 0u);
+                    tc_commit_pair(smem_u32(&empty[s]));
+                    tc_commit_pair(mapa_shared(smem_u32(&empty[s]), 1));
+                }
+                if (!ok) break;
+                tc_commit_pair(smem_u32(&acc_full[b]));
+                tc_commit_pair(mapa_shared(smem_u32(&acc_full[b]), 1));
+            }
+            if (!ok) *abort_flag = 1;
+        }
+    } else if (warp >= 4) {
+        // -------------------------------------------------------------------- epilogue: one token per lane
+        const int wq = warp & 3;
+        const uint32_t acc_empty0 = mapa_shared(smem_u32(&acc_empty[0]), 0);
+        uint32_t n = 0;
+        for (int t = cid; t < n_all; t += ncl, ++n) {
+            const TileAt at = tile_at(p, t);
+            const uint32_t b = n & 1u;
+            const int m = at.m0 + (int)rank * 128 + wq * 32 + lane;
+            const bool row = m < p.M;
+            const float sa = row ? __ldg(p.sa + m) : 0.0f;
+            bool ok = mbar_wait_cluster_bounded(&acc_full[b], (n >> 1) & 1u, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
+                set_err(p.err, 0x704);
+                *abort_flag = 1;
+                break;
+            }
+            tc_fence_after();
+            for (int c0 = 0; c0 < 256; c0 += 32) {
+                const int n0 = at.n0 + c0;
+                if (n0 >= p.N) break;
+                int acc[32];
+                tmem_ld32(tmem + ((uint32_t)(wq * 32) << 16) + b * 256u + (uint32_t)c0, acc);
+                if (!row) continue;
+                if (p.vec && n0 + 32 <= p.N) {
+                    float z[32];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint4 w = __ldg(reinterpret_cast<const uint4*>(p.sw + n0) + e);
+                        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 f = half2_at(ww[i]);
+                            z[e * 8 + 2 * i] = (float)acc[e * 8 + 2 * i] * (sa * f.x);
+                            z[e * 8 + 2 * i + 1] = (float)acc[e * 8 + 2 * i + 1] * (sa * f.y);
+                        }
+                    }
+                    if (p.swiglu) {
+                        uint4* dst = reinterpret_cast<uint4*>(p.C + (int64_t)m * p.ldc + n0 / 2);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float* g = z + e * 16 + i * 4;
+                                o[i] = pack_h2(swiglu_f(g[0], g[1]), swiglu_f(g[2], g[3]));
+                            }
+                            dst[e] = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                        continue;
+                    }
+                    if (p.R) {
+                        const uint4* r = reinterpret_cast<const uint4*>(p.R + (int64_t)m * p.ldr + n0);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint4 w = r[e];
+                            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 f = half2_at(ww[i]);
+                                z[e * 8 + 2 * i] += f.x;
+                                z[e * 8 + 2 * i + 1] += f.y;
+                            }
+                        }
+                    }
+                    uint4* dst = reinterpret_cast<uint4*>(p.C + (int64_t)m * p.ldc + n0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        dst[e] = make_uint4(pack_h2(z[e * 8], z[e * 8 + 1]), pack_h2(z[e * 8 + 2], z[e * 8 + 3]),
+                                            pack_h2(z[e * 8 + 4], z[e * 8 + 5]), pack_h2(z[e * 8 + 6], z[e * 8 + 7]));
+                    continue;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    if (n0 + i >= p.N) break;
+                    const bool two = n0 + i + 1 < p.N;
+                    float z0 = (float)acc[i] * (sa * __half2float(p.sw[n0 + i]));
+                    float z1 = two ? (float)acc[i + 1] * (sa * __half2float(p.sw[n0 + i + 1])) : 0.0f;
+                    if (p.swiglu) {
+                        p.C[(int64_t)m * p.ldc + (n0 + i) / 2] = __float2half_rn(swiglu_f(z0, z1));
+                        continue;
+                    }
+                    if (p.R) {
+                        z0 += __half2float(p.R[(int64_t)m * p.ldr + n0 + i]);
+                        if (two) z1 += __half2float(p.R[(int64_t)m * p.ldr + n0 + i + 1]);
+                    }
+                    p.C[(int64_t)m * p.ldc + n0 + i] = __float2half_rn(z0);
+                    if (two) p.C[(int64_t)m * p.ldc + n0 + i + 1] = __float2half_rn(z1);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty0 + b * 8u);
+        }
+    }
+
+    tc_fence_before();
+    cta_sync_divergent();
+    cluster_sync();  // no CTA leaves while its peer may still signal or read it
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+// ------------------------------------------------ 128 channels x BT tokens, K over a cluster
+
+constexpr int kFewThreads = 192;
+
+template <int BT>
+struct FewSmem {
+    static constexpr int kW = 128 * BK, kX = BT * BK;
+    static constexpr int kStages = BT >= 256 ? 4 : BT >= 128 ? 3 : BT >= 64 ? 4 : 5;
+    static constexpr int kOffBar = kStages * (kW + kX);
+    static constexpr int kTotal = kOffBar + 256 + 1024;
+    static constexpr int kCols = BT < 32 ? 32 : BT;  // tensor memory columns
+    static_assert(BT * 128 * 4 <= kOffBar, "the sums reuse the ring");
+};
+
+// grid (cluster * channel tiles, token tiles); CTA r of a cluster takes K tiles
+// [r * per, (r + 1) * per)
+template <int BT>
+__global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_constant__ Params p) {
+    pdl_trigger();
+    using L = FewSmem<BT>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sW = smem, *sX = smem + L::kStages * L::kW;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+    uint64_t* empty = full + L::kStages;
+    uint64_t* done = empty + L::kStages;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = (p.k_tiles + p.per - 1) / p.per;
+    const int tile = (int)blockIdx.x / S, r = (int)blockIdx.x - tile * S;
+    const int n0 = tile * 128, m0 = (int)blockIdx.y * BT;
+    const int kt0 = r * p.per, nk = min(p.per, p.k_tiles - kt0);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 4 && lane == 0) {
+        prefetch_tmap(&p.tmA);
+        prefetch_tmap(&p.tmW);
+        // the first weight tiles come to L2 while the kernel ahead still runs
+        for (int i = 0; i < min(nk, L::kStages); ++i) tma_prefetch_3d(&p.tmW, (kt0 + i) * BK, n0, 0);
+    }
+    if (warp == 5) {
+        tmem_alloc(tmem_slot, L::kCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    cta_sync_divergent();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+
+    bool ok = true;
+    if (warp == 4) {
+        if (lane == 0) {  // producer
+            int i = 0;
+            for (; i < nk; ++i) {
+                const int s = i % L::kStages;
+                ok = mbar_wait_quick(&empty[s], ((uint32_t)(i / L::kStages) & 1u) ^ 1u, abort_flag);
+                if (!ok) break;
+                mbar_arrive_expect_tx(&full[s], (uint32_t)(L::kW + L::kX));
+                tma_load_3d(sW + s * L::kW, &p.tmW, &full[s], (kt0 + i) * BK, n0, 0);
+                tma_load_3d(sX + s * L::kX, &p.tmA, &full[s], (kt0 + i) * BK, m0, 0);
+            }
+            if (!ok) {  // copies in flight land before the CTA leaves
+                *abort_flag = 1;
+                set_err(p.err, 0x711);
+                int never = 0;
+                for (int j = max(0, i - L::kStages); j < i; ++j)
+                    mbar_wait_bounded(&full[j % L::kStages], (uint32_t)(j / L::kStages) & 1u, &never, 100000000ull);
+            }
+        }
+    } else if (warp == 5) {
+        if (elect_one()) {  // MMA
+            constexpr uint32_t idesc = idesc_i8(128, BT);
+            for (int i = 0; i < nk && ok; ++i) {
+                const int s = i % L::kStages;
+                ok = mbar_wait_quick(&full[s], (uint32_t)(i / L::kStages) & 1u, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t w = smem_u32(sW + s * L::kW), x = smem_u32(sX + s * L::kX);
+#pragma unroll
+                for (int k = 0; k < BK / kUmmaK; ++k)
+                    mma_i8(tmem, umma_desc_sw128(w + k * kUmmaK), umma_desc_sw128(x + k * kUmmaK), idesc,
+                           (i > 0 || k > 0) ? 1u : 0u);
+                tc_commit(&empty[s]);
+            }
+            if (ok) tc_commit(done);
+            else {
+                *abort_flag = 1;
+                set_err(p.err, 0x712);
+            }
+        }
+    } else {
+        ok = __all_sync(0xffffffffu, mbar_wait_quick(done, 0, abort_flag));
+        tc_fence_after();
+        if (ok) {  // the ring is free: this CTA's sums [token][channel]
+            int* sums = reinterpret_cast<int*>(smem) + warp * 32 + lane;
+            const uint32_t t = tmem + ((uint32_t)(warp * 32) << 16);
+#pragma unroll 1
+            for (int c0 = 0; c0 < BT && m0 + c0 < p.M; c0 += 16) {
+                int acc[16];
+                tmem_ld16i(t + (uint32_t)c0, acc);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sums[(c0 + j) * 128] = acc[j];
+            }
+        } else if (lane == 0) {
+            *abort_flag = 1;
+            set_err(p.err, 0x713);
+        }
+    }
+    tc_fence_before();
+    if (S > 1) cluster_sync();
+    else cta_sync_divergent();
+    if (warp == 5) {
+        tc_fence_after();
+        tmem_dealloc(tmem, L::kCols);
+    }
+    if (warp < 4) {
+        const int tokens = min(BT, p.M - m0);
+        const int n = n0 + lane * 4;
+        const int left = p.N - n;  // channels of this lane
+        const uint32_t base = smem_u32(smem) + (uint32_t)lane * 16u;
+        float sw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sw[i] = i < left ? __half2float(__ldg(p.sw + n + i)) : 0.0f;
+        for (int j = r * 4 + warp; j < tokens; j += S * 4) {
+            int4 v = make_int4(0, 0, 0, 0);
+            int4 got[kMaxCluster];
+#pragma unroll
+            for (int q = 0; q < kMaxCluster; ++q)
+                if (q < S)
+                    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(got[q].x), "=r"(got[q].y), "=r"(got[q].z), "=r"(got[q].w)
+                                 : "r"(mapa_shared(base + (uint32_t)j * 512u, q))
+                                 : "memory");
+#pragma unroll
+            for (int q = 0; q < kMaxCluster; ++q)
+                if (q < S) {
+                    v.x += got[q].x;
+                    v.y += got[q].y;
+                    v.z += got[q].z;
+                    v.w += got[q].w;
+                }
+            if (left <= 0) continue;
+            const int m = m0 + j;
+            const float sa = __ldg(p.sa + m);
+            float z[4] = {(float)v.x * (sa * sw[0]), (float)v.y * (sa * sw[1]), (float)v.z * (sa * sw[2]),
+                          (float)v.w * (sa * sw[3])};
+            if (p.swiglu) {
+                __half* dst = p.C + (int64_t)m * p.ldc + n / 2;
+                const uint32_t o = pack_h2(swiglu_f(z[0], z[1]), swiglu_f(z[2], z[3]));
+                if (p.vec && left >= 4) {
+                    *reinterpret_cast<uint32_t*>(dst) = o;
+                } else {
+                    dst[0] = __ushort_as_half((unsigned short)(o & 0xffffu));
+                    if (left >= 4) dst[1] = __ushort_as_half((unsigned short)(o >> 16));
+                }
+                continue;
+            }
+            __half* dst = p.C + (int64_t)m * p.ldc + n;
+            const __half* res = p.R ? p.R + (int64_t)m * p.ldr + n : nullptr;
+            if (p.vec && left >= 4) {
+                if (res) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(res);
+                    const float2 a = half2_at(w.x), b = half2_at(w.y);
+                    z[0] += a.x;
+                    z[1] += a.y;
+                    z[2] += b.x;
+                    z[3] += b.y;
+                }
+                *reinterpret_cast<uint2*>(dst) = make_uint2(pack_h2(z[0], z[1]), pack_h2(z[2], z[3]));
+            } else {
+                for (int i = 0; i < min(4, left); ++i)
+                    dst[i] = __float2half_rn(z[i] + (res ? __half2float(res[i]) : 0.0f));
+            }
+        }
+    }
+    if (S > 1) cluster_sync();  // nobody leaves while its sums are read
+}
+
+// ---------------------------------------------------------------------- host
+
+struct Choice {
+    int bt;      // 0: tile kernel
+    int splits;
+};
+
+int few_bt(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256; }
+
+// CTAs of the few-token kernel that an SM holds (shared memory).
+int few_per_sm(int bt) { return bt >= 256 ? 1 : 2; }
+
+Choice pick(int M, int N, int k_tiles) {
+    const int sms = num_sms();
+    Choice c = {0, 1};
+    double best = 1e30;
+    // In units of one K tile of a CTA.  Tile kernel: whole waves of pairs.
+    if (M > 64) {
+        const int64_t tiles = (int64_t)((M + 255) / 256) * ((N + 255) / 256), pairs = sms / 2;
+        best = (double)((tiles + pairs - 1) / pairs) * k_tiles + 8.0;
+    }
+    for (int bt = few_bt(M); bt >= (M > 64 ? 128 : few_bt(M)); bt /= 2) {
+        const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + bt - 1) / bt);
+        const int64_t slots = (int64_t)sms * few_per_sm(bt);
+        for (int s = 1; s <= kMaxCluster && s <= k_tiles; ++s) {
+            const int per = (k_tiles + s - 1) / s, real = (k_tiles + per - 1) / per;
+            const double unit = bt >= 256 ? 1.2 : bt >= 128 ? 1.0 : 0.8;
+            const double t = (double)((tiles * real + slots - 1) / slots) * (per * unit + 6.0) + (real > 1 ? 4.0 : 0.0);
+            if (t < best) {
+                best = t;
+                c = Choice{bt, real};
+            }
+        }
+    }
+    return c;
+}
+
+template <int BT>
+int launch_few(Params& p, int splits, cudaStream_t st) {
+    using L = FewSmem<BT>;
+    static_assert(L::kTotal <= 232448, "shared memory budget");
+    auto kern = w8a8_few_kernel<BT>;
+    NPUB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
+    p.per = (p.k_tiles + splits - 1) / splits;
+    const int S = (p.k_tiles + p.per - 1) / p.per;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(S * ((p.N + 127) / 128)), (unsigned)((p.M + BT - 1) / BT));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = L::kTotal;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = npub_internal_pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = S;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    NPUB_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
+    return npub_internal_launch_status();
+}
+
+int max_pairs() {
+    static std::mutex mu;
+    static int known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return num_sms() / 2;
+    std::lock_guard<std::mutex> lk(mu);
+    if (known[dev] > 0) return known[dev];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * 256);
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = TileSmem::kTotal;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, w8a8_tile_kernel, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        n = num_sms() / 2;
+    }
+    known[dev] = n;
+    return n;
+}
+
+int launch_tile(Params& p, cudaStream_t st) {
+    static_assert(TileSmem::kTotal <= 232448, "shared memory budget");
+    NPUB_CUDA_TRY(cudaFuncSetAttribute(w8a8_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem::kTotal));
+    p.m_tiles = (p.M + 255) / 256;
+    p.n_tiles = (p.N + 255) / 256;
+    p.band = 8;
+    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+    if (tiles > 0x3fffffff) return NPUB_ERR_UNSUPPORTED;
+    const int pairs = max_pairs();
+    return launch_pdl(w8a8_tile_kernel, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), dim3(kTileThreads),
+                      TileSmem::kTotal, st, p);
+}
+
+}  // namespace w8a8
+}  // namespace npub
+
+extern "C" int npub_w8a8_gemm(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw,
+                              const void* w_scale, void* C, int64_t ldc, const void* R, int64_t ldr, int M, int N, int K,
+                              int swiglu, void* stream) {
+    using namespace npub;
+    using namespace npub::w8a8;
+    NPUB_CHECK_ARG(M >= 0 && N >= 0 && K > 0 && K % 16 == 0);
+    NPUB_CHECK_ARG(!swiglu || (N % 2 == 0 && !R));
+    if (M == 0 || N == 0) return NPUB_OK;
+    NPUB_CHECK_ARG(A && a_scale && W && w_scale && C);
+    NPUB_CHECK_ARG(lda % 16 == 0 && ldw % 16 == 0 && lda >= K && ldw >= K && npub_aligned(A, 16) && npub_aligned(W, 16));
+    NPUB_CHECK_ARG(ldc >= (swiglu ? N / 2 : N) && (!R || ldr >= N));
+    NPUB_CHECK_ARG(npub_aligned(a_scale, 4) && npub_aligned(w_scale, 2) && npub_aligned(C, 2) && npub_aligned(R, 2));
+    if (K > 131056) return NPUB_ERR_UNSUPPORTED;  // 131072 * 128 * 128 = 2^31
+    Params p;
+    memset(&p, 0, sizeof(p));
+    p.M = M;
+    p.N = N;
+    p.k_tiles = (K + BK - 1) / BK;
+    p.sa = a_scale;
+    p.sw = reinterpret_cast<const __half*>(w_scale);
+    p.C = reinterpret_cast<__half*>(C);
+    p.ldc = ldc;
+    p.R = reinterpret_cast<const __half*>(R);
+    p.ldr = ldr;
+    p.swiglu = swiglu ? 1 : 0;
+    p.vec = ldc % 8 == 0 && npub_aligned(C, 16) && npub_aligned(w_scale, 16) && (!R || (ldr % 8 == 0 && npub_aligned(R, 16)));
+    p.err = npub_internal_device_error_word();
+    const Choice c = pick(M, N, p.k_tiles);
+    if (c.bt && (M + c.bt - 1) / c.bt > 65535) return NPUB_ERR_UNSUPPORTED;
+    int rc = make_tmap_3d(&p.tmA, true, A, (uint64_t)K, (uint64_t)M, 1, (uint64_t)lda, (uint64_t)lda * M,
+                          c.bt ? (uint32_t)c.bt : 128, 1, true, BK);
+    if (rc) return rc;
+    rc = make_tmap_3d(&p.tmW, true, W, (uint64_t)K, (uint64_t)N, 1, (uint64_t)ldw, (uint64_t)ldw * N, 128, 1, true, BK);
+    if (rc) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    switch (c.bt) {
+        case 16: return launch_few<16>(p, c.splits, st);
+        case 32: return launch_few<32>(p, c.splits, st);
+        case 64: return launch_few<64>(p, c.splits, st);
+        case 128: return launch_few<128>(p, c.splits, st);
+        case 256: return launch_few<256>(p, c.splits, st);
+        default: return launch_tile(p, st);
+    }
+}

@@ -27,7 +27,7 @@ from ._lib import NpubError  # noqa: F401  (re-exported)
 __all__ = [
     "fp16", "quantize_w8", "matmul", "rmsnorm", "add", "swiglu", "softmax", "rope", "attention",
     "attention_decode", "kv_append", "rope_kv_append", "rope_kv_store", "matmul_swiglu", "interleave_gate_up",
-    "matmul_rms", "rmsnorm_parts",
+    "matmul_rms", "rmsnorm_parts", "quantize_rows", "matmul_w8a8",
     "rope_paged_append", "attention_packed", "attention_paged", "attention_paged_decode",
     "embed", "argmax", "isa_vector", "f32_to_f16_bits", "f16_bits_to_f32", "device_error", "NpubError",
 ]
@@ -304,6 +304,112 @@ def rmsnorm_parts(x: torch.Tensor, gamma: torch.Tensor, *, g_out: Optional[torch
     _lib.call("npub_rmsnorm_parts", x.data_ptr(), ldx, gamma.data_ptr(), g_out.data_ptr(), ldg, ss_out.data_ptr(),
               ss_out.stride(0), rows, d, _stream())
     return g_out, ss_out
+
+
+# ------------------------------------------------- products in 8-bit integers
+
+_i8, _f32 = torch.int8, torch.float32
+
+
+def _rows8(t: torch.Tensor, name: str, dev: Optional[int] = None):
+    """(device index, rows, columns, leading dimension) of an int8 matrix."""
+    if isinstance(t, _Tensor) and t.dtype is _i8 and t.is_cuda:
+        s = t.stride()
+        if len(s) == 2:
+            n, c = t.shape
+            if s[1] == 1 or c == 1:
+                d = t.get_device()
+                if dev is not None and d != dev:
+                    raise ValueError(f"{name} must be on the same device as the first argument")
+                return d, n, c, s[0] if n > 1 else max(s[0], c)
+    _mat(t, name, torch.int8)  # raises
+    raise ValueError(f"{name} must be a row-major int8 CUDA matrix")
+
+
+def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, dev: int) -> int:
+    if not (isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == dev and t.numel() == n
+            and t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor of {n} elements on the same device as the "
+                         "first argument")
+    return t.data_ptr()
+
+
+def quantize_rows(x: torch.Tensor, *, gamma: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                  residual: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
+    """(q int8 [rows, d], scale fp32 [rows]): the rows of x (fp16) as matmul_w8a8
+    takes them, scale[r] = max|y[r]| / 127 and q = round(127 y / max|y|), where
+    y = x, or with gamma the RMSNorm of rmsnorm(x, gamma, eps) in fp32.
+
+    With `residual`, h = fp16(x + residual) is formed first, written to
+    `residual_out` (default: a new tensor) and quantised; returns (q, scale, h).
+    A row of zeros has scale 0; one that holds an infinity or a NaN has scale
+    NaN, so what is computed from it is NaN.  d must be a multiple of 8 (of 16
+    for matmul_w8a8)."""
+    dev, rows, d, ldx = _first16(x, "x")
+    r = h = g = None
+    ldr = ldh = 0
+    if gamma is not None:
+        g = _vector(gamma, "gamma", _f16, d, dev)
+    if residual is not None:
+        n, c, ldr = _rows16(residual, "residual", dev)
+        if n != rows or c != d:
+            raise ValueError("residual must match x")
+        r = residual.data_ptr()
+        residual_out, ldh = _out16(residual_out, x, rows, d, dev)
+        h = residual_out.data_ptr()
+    if out is None:
+        out, ldq = x.new_empty((rows, d), dtype=_i8), d
+    else:
+        _, n, c, ldq = _rows8(out, "out", dev)
+        if n != rows or c != d:
+            raise ValueError(f"out must be [{rows}, {d}]")
+    if scale is None:
+        scale = x.new_empty(rows, dtype=_f32)
+    sp = _vector(scale, "scale", _f32, rows, dev)
+    with _device(dev):
+        st = _lib.bound("npub_quantize_rows")(x.data_ptr(), ldx, r, ldr, h, ldh, g, eps, rows, d, out.data_ptr(), ldq, sp,
+                                              torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail("npub_quantize_rows", st)
+    return (out, scale) if residual is None else (out, scale, residual_out)
+
+
+def matmul_w8a8(Aq: torch.Tensor, a_scale: torch.Tensor, Wq: torch.Tensor, w_scale: torch.Tensor, *,
+                residual: Optional[torch.Tensor] = None, swiglu: bool = False,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """C[M, N] = fp16(a_scale[m] * w_scale[n] * sum_k Aq[m, k] Wq[n, k] (+ residual[m, n])):
+    matmul() with 8-bit activations, exact integer sums on the tensor cores at
+    twice the fp16 rate.  Aq int8 [M, K] and a_scale fp32 [M] from quantize_rows,
+    Wq int8 [N, K] and w_scale fp16 [N] from quantize_w8; K must be a multiple of
+    16, at most 131056.
+
+    swiglu=True: Wq holds interleaved gate / up rows (interleave_gate_up) and the
+    result is fp16(silu(gate) * up) [M, N / 2]."""
+    dev, M, K, lda = _rows8(Aq, "Aq")
+    _, N, K2, ldw = _rows8(Wq, "Wq", dev)
+    if K != K2:
+        raise ValueError(f"K mismatch: Aq {tuple(Aq.shape)} vs Wq {tuple(Wq.shape)}")
+    if swiglu and (N % 2 or residual is not None):
+        raise ValueError("swiglu takes an even number of weight rows and no residual")
+    sa, sw = _vector(a_scale, "a_scale", _f32, M, dev), _vector(w_scale, "w_scale", _f16, N, dev)
+    cols = N // 2 if swiglu else N
+    if out is None:
+        out, ldc = Aq.new_empty((M, cols), dtype=_f16), cols
+    else:
+        out, ldc = _out16(out, out, M, cols, dev)
+    r, ldr = None, 0
+    if residual is not None:
+        n, c, ldr = _rows16(residual, "residual", dev)
+        if n != M or c != N:
+            raise ValueError("residual must be [M, N]")
+        r = residual.data_ptr()
+    with _device(dev):
+        st = _lib.bound("npub_w8a8_gemm")(Aq.data_ptr(), lda, sa, Wq.data_ptr(), ldw, sw, out.data_ptr(), ldc, r, ldr, M, N,
+                                          K, 1 if swiglu else 0, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail("npub_w8a8_gemm", st)
+    return out
 
 
 # ---------------------------------------------------------------- vector ops
