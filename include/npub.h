@@ -241,6 +241,24 @@ int npub_argmax_keys(const void* x, int64_t ldx, int rows, int cols, int32_t ind
                      void* stream);
 int npub_select_keys(const uint64_t* keys, int ranks, int rows, int32_t* ids, void* stream);
 
+/* One token per row from given random numbers, with temperature, top-k, top-p
+ * and min-p; the row's logits fp16 [rows, vocab] (row stride ldl, any).  In the
+ * order of descending logits, equal ones by ascending index (-0 equals +0),
+ * with w_i = exp((l_i - max) / T):
+ *   kept are the first top_k (<= 0: all); of them those whose predecessors'
+ *   weights sum to less than top_p times the sum of them all (>= 1: all); of
+ *   those the ones with w_i >= min_p; the first always
+ *   ids[r] = the first kept one at which the running sum exceeds u[r] times the
+ *   kept sum (u in [0, 1); outside of it the first or the last kept one)
+ * T <= 0 (or NaN) takes the largest logit, as npub_argmax_rows does.  Logits of
+ * -inf or NaN are never drawn; a row of nothing else gives -1; +inf takes all
+ * of the weight.  Sums are fp64 in a fixed order.  Each of temperature, top_k,
+ * top_p, min_p is an array [rows] or, where that is NULL, the one value
+ * *_all.  vocab <= 524224. */
+int npub_sample(const void* logits, int64_t ldl, int rows, int vocab, const float* u, const float* temperature,
+                float temperature_all, const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all,
+                const float* min_p, float min_p_all, int32_t* ids, void* stream);
+
 /* -------------------------------------------------------- attention ----
  * Causal prefill attention, llama_layer.py:114-137, legalize.py:117-127 for
  * every sequence b and head h: S = Q K^T * scale + mask; P = softmax(S); O = P V.

@@ -29,7 +29,7 @@ __all__ = [
     "attention_decode", "kv_append", "rope_kv_append", "rope_kv_store", "matmul_swiglu", "interleave_gate_up",
     "matmul_rms", "rmsnorm_parts", "quantize_rows", "matmul_w8a8",
     "rope_paged_append", "attention_packed", "attention_paged", "attention_paged_decode",
-    "embed", "argmax", "isa_vector", "f32_to_f16_bits", "f16_bits_to_f32", "device_error", "NpubError",
+    "embed", "argmax", "sample", "isa_vector", "f32_to_f16_bits", "f16_bits_to_f32", "device_error", "NpubError",
 ]
 
 
@@ -588,6 +588,43 @@ def select_keys(keys: torch.Tensor, ranks: int, *, ids: Optional[torch.Tensor] =
     _need(ids.is_cuda and ids.dtype == torch.int32 and ids.numel() == rows and ids.is_contiguous(),
           "ids must be contiguous int32 CUDA [rows]")
     _lib.call("npub_select_keys", keys.data_ptr(), int(ranks), rows, ids.data_ptr(), _stream())
+    return ids
+
+
+def _per_row(v, name: str, dtype: torch.dtype, rows: int, dev: int):
+    """(address of a tensor [rows] or None, the one value of all rows)"""
+    if isinstance(v, _Tensor):
+        return _vector(v, name, dtype, rows, dev), 0
+    return None, v
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+           ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token per row of logits (fp16 [rows, vocab]) from the random numbers u
+    (fp32 [rows], in [0, 1)): int32 [rows].
+
+    In the order of descending logits, equal ones by ascending index, with
+    w = exp((logit - max) / temperature): the first top_k tokens are kept (0:
+    all), of them those whose predecessors' weights sum to less than top_p times
+    the sum of them all, of those the ones with w >= min_p, the first always; the
+    token is the first kept one at which the running sum exceeds u times the kept
+    sum.  temperature 0 is argmax().  Each setting is one number or a CUDA tensor
+    [rows] (fp32; top_k int32).  Logits of -inf and NaN are never drawn; a row
+    of nothing else gives -1.  The same inputs give the same tokens."""
+    dev, rows, vocab, ldl = _first16(logits, "logits")
+    up = _vector(u, "u", _f32, rows, dev)
+    tp, t = _per_row(temperature, "temperature", _f32, rows, dev)
+    kp, k = _per_row(top_k, "top_k", _i32, rows, dev)
+    pp, p = _per_row(top_p, "top_p", _f32, rows, dev)
+    mp, m = _per_row(min_p, "min_p", _f32, rows, dev)
+    if ids is None:
+        ids = logits.new_empty(rows, dtype=_i32)
+    ip = _vector(ids, "ids", _i32, rows, dev)
+    with _device(dev):
+        st = _lib.bound("npub_sample")(logits.data_ptr(), ldl, rows, vocab, up, tp, t, kp, max(0, min(int(k), 2 ** 31 - 1)),
+                                       pp, p, mp, m, ip, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail("npub_sample", st)
     return ids
 
 
