@@ -427,6 +427,55 @@ int npub_attention_paged_decode(const void* q, int64_t ldq, const void* k_pages,
 size_t npub_attention_paged_decode_workspace(int batch, int64_t ctx_len, int shared_len, int heads, int kv_heads,
                                              int head_dim);
 
+/* ------------------------------------ paged KV cache in 8 bits ----
+ * k_pages / v_pages int8 [n_pages, kv_heads, page_size, head_dim] (contiguous,
+ * 16-byte aligned) and k_scales / v_scales fp32 [n_pages, kv_heads] (>= 0): an
+ * element stands for its integer times the scale of its page and head.  Tables,
+ * packed rows and page ids outside the pool as above; page_size 16 .. 256.
+ *
+ * npub_rope_paged_append_q8: npub_rope_paged_append with k and v held so.  The
+ * new rows of a sequence go to the slots from positions[its first row] on, one
+ * after the other (positions[t] still gives each row's angles).  For the new
+ * rows of one page and head, in fp32 behind norm and rotation:
+ *   s' = max(s, max|new rows| / 127), s = 0 where they start at the page's first slot
+ *   each new element round(y / s'); where s' > s the rows of the page ahead of
+ *   them become round(q s / s')
+ * Slots behind the new rows are left as they are.  A value that is not finite
+ * makes the scale NaN until the page is begun anew.  Sequences that write to
+ * the same page in one call leave it undefined.  head_dim <= 128 (a multiple of
+ * 16), page_size 16 .. 256; otherwise the arguments of npub_rope_paged_append.
+ *
+ * npub_attention_paged_q8 / npub_attention_paged_decode_q8: the attention of
+ * npub_attention_paged / npub_attention_paged_decode over such pages (scale >=
+ * 1e-30).  A call whose sequences have at most 64 * kv_heads / heads new rows
+ * (max_new says so; a decode step with heads <= 16 * kv_heads) reads the 8-bit
+ * keys as they are; rows of a sequence past the tiles that max_new gives are
+ * zeros, as above.  Any other call first writes the keys as fp16 (values past
+ * 65504 become infinite) to its workspace, which holds batch * ctx_len of them:
+ * there ctx_len is a limit, and the rows of a sequence with more keys than
+ * ctx_len rounded up to 128 are zeros.  ctx_len 0: the table's width.
+ * batch <= 65535. */
+int npub_rope_paged_append_q8(const void* qkv, int64_t ldx, void* q_out, int64_t ldq, int tokens, int q_heads,
+                              int kv_heads, int head_dim, int rot_dim, int interleaved, const int32_t* positions,
+                              const float* inv_freq, const void* q_gamma, const void* k_gamma, float eps,
+                              int8_t* k_pages, int8_t* v_pages, float* k_scales, float* v_scales, int n_pages,
+                              int page_size, const int32_t* page_table, int64_t ldt, int max_pages,
+                              const int32_t* cu_seqlens, int batch, void* stream);
+int npub_attention_paged_q8(const void* q, int64_t ldq, const int8_t* k_pages, const int8_t* v_pages,
+                            const float* k_scales, const float* v_scales, int n_pages, int page_size,
+                            const int32_t* page_table, int64_t ldt, int max_pages, const int32_t* lens,
+                            const int32_t* cu_seqlens, int batch, int total, int max_new, int ctx_len, void* out,
+                            int64_t ldo, int heads, int kv_heads, int head_dim, float scale, int causal,
+                            void* workspace, size_t workspace_bytes, void* stream);
+size_t npub_attention_paged_q8_workspace(int batch, int total, int max_new, int64_t ctx_len, int heads, int kv_heads,
+                                         int head_dim);
+int npub_attention_paged_decode_q8(const void* q, int64_t ldq, const int8_t* k_pages, const int8_t* v_pages,
+                                   const float* k_scales, const float* v_scales, int n_pages, int page_size,
+                                   const int32_t* page_table, int64_t ldt, int max_pages, const int32_t* lens,
+                                   int batch, int ctx_len, void* out, int64_t ldo, int heads, int kv_heads,
+                                   int head_dim, float scale, void* workspace, size_t workspace_bytes, void* stream);
+size_t npub_attention_paged_decode_q8_workspace(int batch, int64_t ctx_len, int heads, int kv_heads, int head_dim);
+
 /* ------------------------------------------------- NPU ISA semantics ----
  * One compute instruction of the NPU over PE buffers (_poc/mysim.cpp:114-141):
  * `word` is the 32-bit instruction (opcodes 0x01-0x13 vector, 0x40-0x43

@@ -8,6 +8,7 @@ from .npu import (  # noqa: F401
     quantize_w8, rmsnorm, rope, rope_freqs, rope_kv_append, rope_kv_store, softmax, swiglu, matmul_swiglu,
     interleave_gate_up, matmul_rms, rmsnorm_parts, quantize_rows, matmul_w8a8, sample,
     attention_packed, attention_paged, attention_paged_decode, rope_paged_append,
+    attention_paged_q8, attention_paged_decode_q8, rope_paged_append_q8,
 )
 
 from .llama import llama_layer  # noqa: F401,E402

@@ -49,5 +49,8 @@ int64_t fmha_packed_items(int total_q, int batch, int heads, int kv_heads, int m
 // 4-D map of a page pool [n_pages, kv_heads, page_size, head_dim], box {64, box_rows, 1, 1}, 128-byte swizzle.
 int make_tmap_pages(CUtensorMap* m, const void* base, int n_pages, int kv_heads, int page_size, int head_dim,
                     int box_rows);
+// The same of 8-bit pages: whole rows, box {64 or 128, box_rows, 1, 1} with a swizzle of its width.
+int make_tmap_pages_q8(CUtensorMap* m, const void* base, int n_pages, int kv_heads, int page_size, int head_dim,
+                       int box_rows);
 
 }  // namespace npub

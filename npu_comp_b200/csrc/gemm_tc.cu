@@ -403,6 +403,23 @@ int make_tmap_pages(CUtensorMap* m, const void* base, int n_pages, int kv_heads,
     return r == CUDA_SUCCESS ? NPUB_OK : NPUB_ERR_INVALID_ARG;
 }
 
+// The same of 8-bit pages (paged_decode_q8.cu).
+int make_tmap_pages_q8(CUtensorMap* m, const void* base, int n_pages, int kv_heads, int page_size, int head_dim,
+                       int box_rows) {
+    auto enc = encode_fn();
+    if (!enc) return NPUB_ERR_CUDA;
+    cuuint64_t gdim[4] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)kv_heads, (cuuint64_t)n_pages};
+    const cuuint64_t s1 = (cuuint64_t)head_dim;
+    cuuint64_t gstride[3] = {s1, s1 * page_size, s1 * page_size * kv_heads};
+    const bool small = head_dim <= 64;
+    cuuint32_t box[4] = {small ? 64u : 128u, (cuuint32_t)box_rows, 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), gdim, gstride, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, small ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? NPUB_OK : NPUB_ERR_INVALID_ARG;
+}
+
 template <bool A_I8, int BT, int STAGES>
 static int launch_cfg(const GemmParams& p, int grid_x, int grid_y, int grid_z, cudaStream_t st) {
     using L = GemmSmem<A_I8, BT, STAGES>;

@@ -110,10 +110,11 @@ Phase tile_phase(int total, int batch, int heads, int kv_heads, int max_new, int
 // The few-row kernel on up to `keys` keys of each sequence; behind: a shared
 // prefix's partials are combined with its own.  One of its CTAs, two of which
 // share an SM, takes 4 us (in a cluster 5) and 3 us per 128 keys of 128 columns.
-Phase few_phase(int batch, int kv_heads, int head_dim, int64_t keys, double part_us, bool behind) {
-    const Cost c = {0.0, 4.0, head_dim > 64 ? 3.0 : 1.6, 128}, cc = {0.0, 5.0, c.unit_us, 128};
+Phase few_phase(int batch, int kv_heads, int head_dim, int64_t keys, double part_us, bool behind, int tiles = 1,
+                bool q8 = false) {
+    const Cost c = {0.0, 4.0, (head_dim > 64 ? 3.0 : 1.6) * (q8 ? 0.6 : 1.0), 128}, cc = {0.0, 5.0, c.unit_us, 128};
     const bool ragged = batch > 1;
-    const int64_t items = (int64_t)batch * kv_heads, slots = 2 * num_sms();
+    const int64_t items = (int64_t)batch * kv_heads * tiles, slots = 2 * num_sms();
     Phase ph = {};
     const Split sp = pick_splits(keys, items, slots, c, ragged, 64, part_us + 0.15, 1, behind, 4.0);
     ph.splits = sp.s;
@@ -201,6 +202,78 @@ int run_plan(const Plan& pl, PackedArgs& a, void* workspace, size_t workspace_by
     if (rc || !need) return rc;
     return paged_combine(a, pl.total(), st);
 }
+
+// Over 8-bit pages: few rows on paged_decode_q8, more of them on the tile kernel behind a pass that writes the keys as
+// fp16 pages.
+constexpr int kQ8Tiles = 4;
+struct PlanQ8 {
+    Plan p;
+    int tiles;                    // paged_decode_q8: tiles of 16 rows of a sequence and kv head
+    int width;                    // tile kernel: fp16 pages of 128 keys per sequence
+    size_t parts, pages, tables;  // bytes of the partials, of the fp16 K (or V), and of their table and lengths
+    size_t bytes() const { return parts + 2 * pages + tables; }
+};
+
+PlanQ8 make_plan_q8(int batch, int total, int max_new, int64_t ctx, int heads, int kv_heads, int head_dim) {
+    PlanQ8 pl = {};
+    const int group = heads / kv_heads;
+    const double part_us = (double)total * heads * head_dim * 8.0 / 4e6;
+    if (max_new > 0 && group <= kPagedDecodeRows) {
+        const int per = kPagedDecodeRows / group;
+        const int64_t tiles = ceil_div(max_new, per);
+        if (tiles <= kQ8Tiles) pl.tiles = (int)tiles;
+    }
+    pl.p.few = pl.tiles > 0;
+    if (pl.p.few) {
+        pl.p.own = few_phase(batch, kv_heads, head_dim, ctx, part_us, false, pl.tiles, true);
+    } else {
+        pl.p.own = tile_phase(total, batch, heads, kv_heads, max_new, ctx, num_sms(), part_us, false);
+        const int64_t width = ceil_div(ctx, 128);
+        pl.width = width > 0x7fffffff ? 0x7fffffff : (int)width;
+        pl.pages = (size_t)batch * width * kv_heads * 128 * head_dim * sizeof(__half);
+        pl.tables = ((size_t)batch * (width + 1) * sizeof(int32_t) + 255) / 256 * 256;
+    }
+    pl.parts = (plan_bytes(pl.p, total, heads, head_dim) + 255) / 256 * 256;
+    return pl;
+}
+
+int run_plan_q8(const PlanQ8& pl, PackedArgs& a, const float* ks, const float* vs, void* workspace, size_t workspace_bytes,
+                cudaStream_t st) {
+    if (a.batch > 65535 || a.kv_heads > 65535) return NPUB_ERR_UNSUPPORTED;
+    if (pl.bytes()) {
+        if (!workspace || workspace_bytes < pl.bytes()) return NPUB_ERR_WORKSPACE;
+        NPUB_CHECK_ARG(npub_aligned(workspace, 256));
+    }
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (!pl.p.few) {
+        if ((int64_t)a.batch * pl.width > 0x7fffffff) return NPUB_ERR_UNSUPPORTED;
+        uint8_t *k = ws + pl.parts, *v = k + pl.pages;
+        int32_t* table = reinterpret_cast<int32_t*>(v + pl.pages);
+        int32_t* lens = table + (int64_t)a.batch * pl.width;
+        const int rc = expand_q8(a, ks, vs, pl.width, k, v, table, lens, st);
+        if (rc) return rc;
+        a.kv.k = k;
+        a.kv.v = v;
+        a.kv.table = table;
+        a.kv.ldt = a.kv.max_pages = pl.width;
+        a.kv.n_pages = a.batch * pl.width;
+        a.kv.page_size = 128;
+        a.lens = lens;
+        return run_plan(pl.p, a, workspace, pl.parts, st);
+    }
+    if (pl.parts) {
+        const size_t n = (size_t)pl.p.total() * a.total_q * a.heads;
+        a.part_ml = reinterpret_cast<float2*>(ws);
+        a.part_o = reinterpret_cast<float*>(ws + (n * sizeof(float2) + 255) / 256 * 256);
+    }
+    a.splits = pl.p.own.splits;
+    const int rc = paged_decode_q8(a, ks, vs, pl.tiles, st);
+    if (rc || !pl.parts) return rc;
+    return paged_combine(a, pl.p.total(), st);
+}
+
+// log2 of a scale over c = scale * log2(e) goes into the scores there
+bool scale_ok_q8(float scale) { return scale >= 1e-30f; }
 
 }  // namespace
 }  // namespace npub
@@ -335,4 +408,103 @@ extern "C" size_t npub_attention_paged_decode_workspace(int batch, int64_t ctx_l
         !dims_supported(heads, kv_heads, head_dim))
         return 0;
     return plan_bytes(make_plan(batch, batch, 1, ctx_len, shared_len, heads, kv_heads, head_dim), batch, heads, head_dim);
+}
+
+extern "C" int npub_attention_paged_q8(const void* q, int64_t ldq, const int8_t* k_pages, const int8_t* v_pages,
+                                       const float* k_scales, const float* v_scales, int n_pages, int page_size,
+                                       const int32_t* page_table, int64_t ldt, int max_pages, const int32_t* lens,
+                                       const int32_t* cu_seqlens, int batch, int total, int max_new, int ctx_len,
+                                       void* out, int64_t ldo, int heads, int kv_heads, int head_dim, float scale,
+                                       int causal, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace npub;
+    NPUB_CHECK_ARG(batch >= 0 && total >= 0 && max_new >= 0 && ctx_len >= 0 &&
+                   dims_ok(heads, kv_heads, head_dim, scale) && scale_ok_q8(scale));
+    if (batch == 0 || total == 0) return NPUB_OK;
+    NPUB_CHECK_ARG(q && out && lens && cu_seqlens &&
+                   pool_ok(k_pages, v_pages, n_pages, page_size, page_table, ldt, max_pages));
+    NPUB_CHECK_ARG(k_scales && v_scales && npub_aligned(k_scales, 4) && npub_aligned(v_scales, 4));
+    if (!dims_supported(heads, kv_heads, head_dim)) return NPUB_ERR_UNSUPPORTED;
+    NPUB_CHECK_ARG(ldq % 8 == 0 && ldo % 8 == 0 && ldq >= (int64_t)heads * head_dim &&
+                   ldo >= (int64_t)heads * head_dim && npub_aligned(q, 16) && npub_aligned(out, 16));
+    PackedArgs a = {};
+    a.q = q;
+    a.ldq = ldq;
+    a.out = out;
+    a.ldo = ldo;
+    a.kv.k = k_pages;
+    a.kv.v = v_pages;
+    a.kv.table = page_table;
+    a.kv.ldt = ldt;
+    a.kv.max_pages = max_pages;
+    a.kv.n_pages = n_pages;
+    a.kv.page_size = page_size;
+    a.cu = cu_seqlens;
+    a.lens = lens;
+    a.total_q = total;
+    a.batch = batch;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.scale = scale;
+    a.causal = causal;
+    const int64_t cap = (int64_t)max_pages * page_size;
+    const PlanQ8 pl = make_plan_q8(batch, total, max_new, ctx_len > 0 && ctx_len < cap ? ctx_len : cap, heads, kv_heads,
+                                   head_dim);
+    return run_plan_q8(pl, a, k_scales, v_scales, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t npub_attention_paged_q8_workspace(int batch, int total, int max_new, int64_t ctx_len, int heads,
+                                                    int kv_heads, int head_dim) {
+    using namespace npub;
+    if (batch <= 0 || total <= 0 || max_new < 0 || ctx_len < 0 || !dims_ok(heads, kv_heads, head_dim, 1.0f) ||
+        !dims_supported(heads, kv_heads, head_dim))
+        return 0;
+    return make_plan_q8(batch, total, max_new, ctx_len, heads, kv_heads, head_dim).bytes();
+}
+
+extern "C" int npub_attention_paged_decode_q8(const void* q, int64_t ldq, const int8_t* k_pages, const int8_t* v_pages,
+                                              const float* k_scales, const float* v_scales, int n_pages, int page_size,
+                                              const int32_t* page_table, int64_t ldt, int max_pages, const int32_t* lens,
+                                              int batch, int ctx_len, void* out, int64_t ldo, int heads, int kv_heads,
+                                              int head_dim, float scale, void* workspace, size_t workspace_bytes,
+                                              void* stream) {
+    using namespace npub;
+    NPUB_CHECK_ARG(batch >= 0 && ctx_len >= 0 && dims_ok(heads, kv_heads, head_dim, scale) && scale_ok_q8(scale));
+    if (batch == 0) return NPUB_OK;
+    NPUB_CHECK_ARG(q && out && lens && pool_ok(k_pages, v_pages, n_pages, page_size, page_table, ldt, max_pages));
+    NPUB_CHECK_ARG(k_scales && v_scales && npub_aligned(k_scales, 4) && npub_aligned(v_scales, 4));
+    if (!dims_supported(heads, kv_heads, head_dim)) return NPUB_ERR_UNSUPPORTED;
+    NPUB_CHECK_ARG(ldq % 8 == 0 && ldo % 8 == 0 && ldq >= (int64_t)heads * head_dim &&
+                   ldo >= (int64_t)heads * head_dim && npub_aligned(q, 16) && npub_aligned(out, 16));
+    PackedArgs a = {};
+    a.q = q;
+    a.ldq = ldq;
+    a.out = out;
+    a.ldo = ldo;
+    a.kv.k = k_pages;
+    a.kv.v = v_pages;
+    a.kv.table = page_table;
+    a.kv.ldt = ldt;
+    a.kv.max_pages = max_pages;
+    a.kv.n_pages = n_pages;
+    a.kv.page_size = page_size;
+    a.lens = lens;
+    a.total_q = batch;
+    a.batch = batch;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.scale = scale;
+    a.causal = 1;
+    const int64_t cap = (int64_t)max_pages * page_size;
+    const PlanQ8 pl = make_plan_q8(batch, batch, 1, ctx_len > 0 && ctx_len < cap ? ctx_len : cap, heads, kv_heads, head_dim);
+    return run_plan_q8(pl, a, k_scales, v_scales, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t npub_attention_paged_decode_q8_workspace(int batch, int64_t ctx_len, int heads, int kv_heads,
+                                                           int head_dim) {
+    using namespace npub;
+    if (batch <= 0 || ctx_len < 0 || !dims_ok(heads, kv_heads, head_dim, 1.0f) || !dims_supported(heads, kv_heads, head_dim))
+        return 0;
+    return make_plan_q8(batch, batch, 1, ctx_len, heads, kv_heads, head_dim).bytes();
 }

@@ -29,6 +29,7 @@ __all__ = [
     "attention_decode", "kv_append", "rope_kv_append", "rope_kv_store", "matmul_swiglu", "interleave_gate_up",
     "matmul_rms", "rmsnorm_parts", "quantize_rows", "matmul_w8a8",
     "rope_paged_append", "attention_packed", "attention_paged", "attention_paged_decode",
+    "rope_paged_append_q8", "attention_paged_q8", "attention_paged_decode_q8",
     "embed", "argmax", "sample", "isa_vector", "f32_to_f16_bits", "f16_bits_to_f32", "device_error", "NpubError",
 ]
 
@@ -772,13 +773,37 @@ def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor
     shape = k_pages.shape
     if v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must have the same shape")
+    return (shape, *_pages(page_table, dev))
+
+
+def _pages(page_table: torch.Tensor, dev: int):
+    """(batch, max_pages, leading dimension) of a page table."""
     if not (isinstance(page_table, _Tensor) and page_table.dtype is _i32 and page_table.get_device() == dev):
         raise ValueError("page_table must be int32 CUDA [batch, max_pages] on the same device as the first argument")
     s = page_table.stride()
     if len(s) != 2 or (s[1] != 1 and page_table.shape[1] != 1):
         raise ValueError("page_table must be [batch, max_pages] with unit stride along its last dim")
     B, W = page_table.shape
-    return shape, B, W, s[0] if B > 1 else max(s[0], W)
+    return B, W, s[0] if B > 1 else max(s[0], W)
+
+
+def _pool8(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+           page_table: torch.Tensor, dev: int):
+    """_pool for a cache in 8 bits."""
+    if not (isinstance(k_pages, _Tensor) and k_pages.dtype is _i8 and k_pages.get_device() == dev
+            and k_pages.dim() == 4 and k_pages.is_contiguous() and isinstance(v_pages, _Tensor)
+            and v_pages.dtype is _i8 and v_pages.get_device() == dev and v_pages.is_contiguous()):
+        raise ValueError("k_pages and v_pages must be contiguous int8 CUDA [n_pages, kv_heads, page_size, head_dim] on "
+                         "the same device as the first argument")
+    shape = k_pages.shape
+    if v_pages.shape != shape:
+        raise ValueError("k_pages and v_pages must have the same shape")
+    for t in (k_scales, v_scales):
+        if not (isinstance(t, _Tensor) and t.dtype is _f32 and t.get_device() == dev and t.is_contiguous()
+                and t.shape == shape[:2]):
+            raise ValueError("k_scales and v_scales must be contiguous fp32 CUDA [n_pages, kv_heads] on the same device as "
+                             "the first argument")
+    return (shape, *_pages(page_table, dev))
 
 
 def _out16(out: Optional[torch.Tensor], like: torch.Tensor, rows: int, cols: int, dev: int):
@@ -971,6 +996,117 @@ def attention_paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
             wsp, wsb, torch._C._cuda_getCurrentRawStream(dev))
     if st:
         _lib.fail("npub_attention_paged_decode", st)
+    return out
+
+
+# The same cache in 8 bits: k_pages / v_pages int8, and k_scales / v_scales fp32
+# [n_pages, kv_heads]: an element stands for its integer times the scale of its
+# page and head.  A page's scale is set by the appends: start with any contents.
+
+def rope_paged_append_q8(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: int, positions: torch.Tensor,
+                         inv_freq: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor,
+                         v_scales: torch.Tensor, page_table: torch.Tensor, *, cu_seqlens: Optional[torch.Tensor] = None,
+                         rot_dim: Optional[int] = None, interleaved: bool = False,
+                         q_gamma: Optional[torch.Tensor] = None, k_gamma: Optional[torch.Tensor] = None,
+                         eps: float = 1e-5, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """rope_paged_append() into a cache in 8 bits: q is returned in fp16, k and v
+    are stored as round(y / s) with the scale s of their page and head.
+
+    The new rows of a sequence go to the slots from the position of its first row
+    on, one after the other (positions still gives every row's rotation).  A
+    page's scale grows with what is appended: s' = max(s, max|new rows| / 127),
+    and where it does, the rows already there become round(q s / s'); rows that
+    start at a page's first slot begin it anew.  A value that is not finite makes
+    its page's scale NaN, until the page begins anew.  Only one sequence may
+    write to a page in a call.  head_dim at most 128, page_size 16 .. 256."""
+    dev, T, cols, ldx = _first16(qkv, "qkv")
+    R = head_dim if rot_dim is None else int(rot_dim)
+    if cols < (q_heads + 2 * kv_heads) * head_dim:
+        raise ValueError("qkv has too few columns")
+    (n_pages, kvh, ps, hd), B, W, ldt = _pool8(k_pages, v_pages, k_scales, v_scales, page_table, dev)
+    if kvh != kv_heads or hd != head_dim:
+        raise ValueError("the pages' kv_heads and head_dim must match")
+    pos = _ints(positions, "positions", T, dev)
+    fp = _vector(inv_freq, "inv_freq", _f32, R // 2, dev)
+    gq = None if q_gamma is None else _vector(q_gamma, "q_gamma", _f16, head_dim, dev)
+    gk = None if k_gamma is None else _vector(k_gamma, "k_gamma", _f16, head_dim, dev)
+    if cu_seqlens is None:
+        if B != T:
+            raise ValueError("without cu_seqlens the table needs one row per token")
+        cu = None
+    else:
+        cu = _ints(cu_seqlens, "cu_seqlens", B + 1, dev)
+    out, ldq = _out16(out, qkv, T, q_heads * head_dim, dev)
+    with _device(dev):
+        st = _lib.bound("npub_rope_paged_append_q8")(
+            qkv.data_ptr(), ldx, out.data_ptr(), ldq, T, q_heads, kv_heads, head_dim, R,
+            1 if interleaved else 0, pos, fp, gq, gk, eps, k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
+            v_scales.data_ptr(), n_pages, ps, page_table.data_ptr(), ldt, W, cu, B,
+            torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail("npub_rope_paged_append_q8", st)
+    return out
+
+
+def attention_paged_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor,
+                       v_scales: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, cu_seqlens: torch.Tensor, *,
+                       heads: int, max_new: int = 0, ctx_len: int = 0, causal: bool = True,
+                       scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """attention_paged() over a cache in 8 bits.
+
+    max_new: at least the new rows of any sequence (0: not known).  With at most
+    64 * kv_heads / heads of them the 8-bit keys are read as they are, and a
+    sequence that has more than max_new rows all the same may get zeros for those
+    past them.  Any other call first writes the keys as fp16 to its workspace,
+    batch * ctx_len of them: ctx_len is then a limit, and a sequence with more
+    keys (than ctx_len rounded up to 128; 0: the table's width) gets zeros."""
+    dev, T, qc, ldq = _first16(q, "q")
+    (n_pages, kv_heads, ps, hd), B, W, ldt = _pool8(k_pages, v_pages, k_scales, v_scales, page_table, dev)
+    if qc != heads * hd:
+        raise ValueError("q must be [total, heads * head_dim]")
+    ln = _ints(lens, "lens", B, dev)
+    cu = _ints(cu_seqlens, "cu_seqlens", B + 1, dev)
+    if scale is None:
+        scale = 1.0 / math.sqrt(max(hd, 1))
+    max_new = min(int(max_new), 2 ** 31 - 1)
+    ctx = _context(ctx_len, W * ps)
+    out, ldo = _out16(out, q, T, heads * hd, dev)
+    ws, wsp, wsb = _paged_workspace(q, dev, "npub_attention_paged_q8_workspace", B, T, max_new, ctx, heads, kv_heads, hd)
+    with _device(dev):
+        st = _lib.bound("npub_attention_paged_q8")(
+            q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), n_pages,
+            ps, page_table.data_ptr(), ldt, W, ln, cu, B, T, max_new, ctx, out.data_ptr(), ldo, heads, kv_heads, hd, scale,
+            1 if causal else 0, wsp, wsb, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail("npub_attention_paged_q8", st)
+    return out
+
+
+def attention_paged_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor,
+                              v_scales: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, *, heads: int,
+                              ctx_len: int = 0, scale: Optional[float] = None,
+                              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """attention_paged_decode() over a cache in 8 bits: q [batch, heads*hd], one
+    new row per sequence, keys 0 .. lens[b] - 1.  ctx_len: the largest lens
+    expected (0: the table's width); a limit, as in attention_paged_q8, where
+    heads > 16 * kv_heads."""
+    dev, n, qc, ldq = _first16(q, "q")
+    (n_pages, kv_heads, ps, hd), B, W, ldt = _pool8(k_pages, v_pages, k_scales, v_scales, page_table, dev)
+    if n != B or qc != heads * hd:
+        raise ValueError("q must be [batch, heads * head_dim]")
+    ln = _ints(lens, "lens", B, dev)
+    if scale is None:
+        scale = 1.0 / math.sqrt(max(hd, 1))
+    ctx = _context(ctx_len, W * ps)
+    out, ldo = _out16(out, q, B, heads * hd, dev)
+    ws, wsp, wsb = _paged_workspace(q, dev, "npub_attention_paged_decode_q8_workspace", B, ctx, heads, kv_heads, hd)
+    with _device(dev):
+        st = _lib.bound("npub_attention_paged_decode_q8")(
+            q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), n_pages,
+            ps, page_table.data_ptr(), ldt, W, ln, B, ctx, out.data_ptr(), ldo, heads, kv_heads, hd, scale, wsp, wsb,
+            torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.fail("npub_attention_paged_decode_q8", st)
     return out
 
 
