@@ -208,7 +208,7 @@ int run_plan(const Plan& pl, PackedArgs& a, void* workspace, size_t workspace_by
 constexpr int kQ8Tiles = 4;
 struct PlanQ8 {
     Plan p;
-    int tiles;                    // paged_decode_q8: tiles of 16 rows of a sequence and kv head
+    int tiles, rows;              // paged_decode_q8: tiles of a sequence and kv head, and the rows of one
     int width;                    // tile kernel: fp16 pages of 128 keys per sequence
     size_t parts, pages, tables;  // bytes of the partials, of the fp16 K (or V), and of their table and lengths
     size_t bytes() const { return parts + 2 * pages + tables; }
@@ -219,8 +219,8 @@ PlanQ8 make_plan_q8(int batch, int total, int max_new, int64_t ctx, int heads, i
     const int group = heads / kv_heads;
     const double part_us = (double)total * heads * head_dim * 8.0 / 4e6;
     if (max_new > 0 && group <= kPagedDecodeRows) {
-        const int per = kPagedDecodeRows / group;
-        const int64_t tiles = ceil_div(max_new, per);
+        pl.rows = (int64_t)max_new * group <= 8 ? 8 : kPagedDecodeRows;
+        const int64_t tiles = ceil_div(max_new, pl.rows / group);
         if (tiles <= kQ8Tiles) pl.tiles = (int)tiles;
     }
     pl.p.few = pl.tiles > 0;
@@ -267,7 +267,7 @@ int run_plan_q8(const PlanQ8& pl, PackedArgs& a, const float* ks, const float* v
         a.part_o = reinterpret_cast<float*>(ws + (n * sizeof(float2) + 255) / 256 * 256);
     }
     a.splits = pl.p.own.splits;
-    const int rc = paged_decode_q8(a, ks, vs, pl.tiles, st);
+    const int rc = paged_decode_q8(a, ks, vs, pl.rows, pl.tiles, st);
     if (rc || !pl.parts) return rc;
     return paged_combine(a, pl.p.total(), st);
 }

@@ -26,20 +26,36 @@
 #include "gemm_tc.h"
 #include "paged_decode.h"
 
+#ifndef NPUB_Q8_STEP
+#define NPUB_Q8_STEP 32
+#endif
+#ifndef NPUB_Q8_RING
+#define NPUB_Q8_RING 96
+#endif
+#ifndef NPUB_Q8_CTAS8
+#define NPUB_Q8_CTAS8 3
+#endif
+#ifndef NPUB_Q8_RING8
+#define NPUB_Q8_RING8 64
+#endif
+#ifndef NPUB_Q8_CTAS
+#define NPUB_Q8_CTAS 2
+#endif
 namespace npub {
 namespace pdq8 {
 
 constexpr int kWarps = 4;               // consumers
 constexpr int kThreads = kWarps * 32 + 32;
-constexpr int kKeys = kWarps * 16;      // keys per stage
-constexpr int kMaxRows = 16;
+constexpr int kStep = NPUB_Q8_STEP;     // keys of a stage that a warp takes
+constexpr int kKeys = kWarps * kStep;   // keys per stage
+constexpr int kGroups = kKeys / 16;     // runs of keys with the same scales
 
-template <int HD>
+template <int HD, int kMaxRows>
 struct Smem {
     static constexpr int kTile = kKeys * HD;  // K or V of a stage
-    static constexpr int kStages = HD == 128 ? 6 : 12;
-    static constexpr int kOffScale = kStages * 2 * kTile;  // [stage][group of 16 keys]: s_k, log2(s_v) / c, 1 / s_v
-    static constexpr int kOffBar = kOffScale + kStages * kWarps * 16;
+    static constexpr int kStages = (kMaxRows == 8 ? NPUB_Q8_RING8 : NPUB_Q8_RING) * 1024 / (2 * kTile);
+    static constexpr int kOffScale = kStages * 2 * kTile;  // [stage][group]: s_k, log2(s_v) / c, 1 / s_v
+    static constexpr int kOffBar = kOffScale + kStages * kGroups * 16;
     static constexpr int kTotal = kOffBar + 256;
     // The merge reuses the ring: the warps' partials, then (clusters) the CTA's own.  A lane writes runs of HD / 8
     // columns; 4 words behind each run and 4 behind a row spread the lanes over the banks.
@@ -79,6 +95,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The transpose of an 8 x 8 matrix of fp16 held by a warp, row lane / 4, columns 2 (lane & 3) and the next.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
 __device__ __forceinline__ float2 ld_cluster_f2(uint32_t a) {
     float2 v;
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
@@ -105,10 +127,17 @@ __device__ __forceinline__ void no_keys(const Params& p, bool part, int split, i
     }
 }
 
-// grid (kv_heads * splits, batch, tiles of 16 rows)
-template <int HD>
-__global__ void __launch_bounds__(kThreads, 2) paged_decode_q8_kernel(const __grid_constant__ Params p) {
-    using L = Smem<HD>;
+// grid (kv_heads * splits, batch, tiles of kMaxRows rows)
+//
+// kMaxRows 16: S = Q K^T and O = P V with the rows on the product's 16-side.
+// kMaxRows 8: transposed, S^T = K Q^T and O^T = V^T P^T with the rows on its
+// 8-side: half of the products, exponentials and sums.  A lane's integers of K
+// and V are the same in both.
+template <int HD, int kMaxRows>
+__global__ void __launch_bounds__(kThreads, kMaxRows == 8 ? NPUB_Q8_CTAS8 : NPUB_Q8_CTAS)
+    paged_decode_q8_kernel(const __grid_constant__ Params p) {
+    using L = Smem<HD, kMaxRows>;
+    constexpr bool kT = kMaxRows == 8;
     pdl_trigger();
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {
@@ -144,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_q8_kernel(const __gr
     }
     const int R = nrow * p.group;
     const int len = max(0, min(p.lens[b], p.max_keys));
-    const int per = max(2, ((len + kKeys - 1) / kKeys + p.splits - 1) / p.splits) * kKeys;
+    const int per = max(128 / kKeys, ((len + kKeys - 1) / kKeys + p.splits - 1) / p.splits) * kKeys;
     const int k0 = R == 0 ? 0 : min(len, split * per);
     const int k1 = R == 0 ? 0 : min(len, split * per + per);
     const int nst = (k1 - k0 + kKeys - 1) / kKeys;
@@ -198,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_q8_kernel(const __gr
             ok = mbar_wait_warp(&empty[s], ((uint32_t)(j / L::kStages) & 1u) ^ 1u, abort_flag);
             if (!ok) break;
             if (box < nbox) {
-                float* sc = reinterpret_cast<float*>(smem + L::kOffScale) + (s * kWarps + box * groups) * 4;
+                float* sc = reinterpret_cast<float*>(smem + L::kOffScale) + (s * kGroups + box * groups) * 4;
                 float v = isfinite(scale) ? scale : NAN;
                 if (kv) {
                     v = page < p.n_pages ? (v < 9.094947e-13f ? 9.094947e-13f : v) : 1.0f;  // 2^-40; NaN stays
@@ -232,21 +261,21 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_q8_kernel(const __gr
     }
 
     // ------------------------------------------------------------------------ consumers
-    const int ra = lane >> 2, rb = ra + 8, t4 = lane & 3;  // rows, and the lane's place among the four of a row
-    uint32_t qf[HD / 16][4];
-    {
-        const int ta = ra / p.group, tb = rb / p.group;
-        const __half* qa = p.q + (int64_t)(row0 + ta) * p.ldq + (int64_t)(kvh * p.group + ra - ta * p.group) * p.head_dim;
-        const __half* qb = p.q + (int64_t)(row0 + tb) * p.ldq + (int64_t)(kvh * p.group + rb - tb * p.group) * p.head_dim;
+    const int g8 = lane >> 2, t4 = lane & 3;  // the lane's place among eight and among four
+    // rows whose scores and output this lane holds
+    const int ra = kT ? 2 * t4 : g8, rb = kT ? ra + 1 : ra + 8;
+    constexpr int kQ = kT ? 1 : 2;  // rows of Q that a lane holds: g8 (and g8 + 8)
+    uint32_t qf[HD / 16][2 * kQ];
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) {
+        const int row = g8 + 8 * i, t = row / p.group;
+        const __half* src = p.q + (int64_t)(row0 + t) * p.ldq + (int64_t)(kvh * p.group + row - t * p.group) * p.head_dim;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {  // step kk of the lane's HD / 4 columns: 4 of them
             const int d = t4 * (HD / 4) + kk * 4;
-            const uint2 a = d < p.head_dim && ra < R ? *reinterpret_cast<const uint2*>(qa + d) : make_uint2(0, 0);
-            const uint2 c = d < p.head_dim && rb < R ? *reinterpret_cast<const uint2*>(qb + d) : make_uint2(0, 0);
-            qf[kk][0] = a.x;
-            qf[kk][1] = c.x;
-            qf[kk][2] = a.y;
-            qf[kk][3] = c.y;
+            const uint2 w = d < p.head_dim && row < R ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
+            qf[kk][i] = w.x;
+            qf[kk][kQ + i] = w.y;
         }
     }
     int lim[2] = {len, len};  // keys of rows ra and rb end here
@@ -257,103 +286,165 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_q8_kernel(const __gr
     lim[0] = min(lim[0], k1);
     lim[1] = min(lim[1], k1);
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    float o[HD / 8][4];
+    // output: kT: tile n has columns g8 HD / 8 + 2 n (e < 2) and the next (e >= 2), rows ra (even e) and rb; else tile n has
+    // column (2 t4 + (e & 1)) HD / 8 + n, rows ra (e < 2) and rb
+    constexpr int kO = kT ? HD / 16 : HD / 8;
+    float o[kO][4];
 #pragma unroll
-    for (int n = 0; n < HD / 8; ++n)
+    for (int n = 0; n < kO; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
     const float c = p.c;
+    // scores of 16 keys, [2 u + i][e]: kT: x[2 u] are keys g8 (e < 2) and g8 + 8 of rows ra (even e) and rb; else x[2 u + i]
+    // is key 8 i + 2 t4 + (e & 1) of row ra (e < 2) or rb
+    constexpr int kX = kT ? kStep / 16 : kStep / 8;
+    auto row_of = [](int e) { return kT ? e & 1 : e >> 1; };
+    auto key_of = [&](int n, int e) { return kT ? n * 16 + g8 + (e >> 1) * 8 : n * 8 + t4 * 2 + (e & 1); };
     bool ok = true;
     for (int j = 0; j < nst; ++j) {
         const int s = j % L::kStages;
         ok = mbar_wait_warp(&full[s], (uint32_t)(j / L::kStages) & 1u, abort_flag);
         if (!ok) break;
-        const int kb = k0 + j * kKeys + warp * 16;  // first key of this warp
+        const int kb = k0 + j * kKeys + warp * kStep;  // first key of this warp
         if (kb < k1) {
-            const uint8_t* kt = smem + s * 2 * L::kTile;
+            const uint8_t* kt = smem + s * 2 * L::kTile + warp * kStep * HD;
             const uint8_t* vt = kt + L::kTile;
-            const float4 sc = *reinterpret_cast<const float4*>(smem + L::kOffScale + (s * kWarps + warp) * 16);
-            float x[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+            const float4* sc = reinterpret_cast<const float4*>(smem + L::kOffScale + (s * kGroups + warp * (kStep / 16)) * 16);
+            float x[kX][4];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int key = warp * 16 + n * 8 + ra;
+            for (int u = 0; u < kStep / 16; ++u) {
+#pragma unroll
+                for (int n = u * kX * 16 / kStep; n < (u + 1) * kX * 16 / kStep; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[n][e] = 0.0f;
 #pragma unroll
                 for (int h = 0; h < HD / 64; ++h) {
-                    // columns t4 * HD / 4 + 16 h and the 15 behind them
-                    const int at = HD == 128 ? key * 128 + (((2 * t4 + h) ^ (key & 7)) << 4)
-                                             : key * 64 + ((t4 ^ ((key >> 1) & 3)) << 4);
-                    const uint4 r = *reinterpret_cast<const uint4*>(kt + at);
-                    uint32_t f[8];
-                    i8x16_to_f16x2(r, f);
+                    // keys g8 and g8 + 8 at columns t4 * HD / 4 + 16 h and the 15 behind them
+                    uint32_t f[2][8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mma16816(x[n], qf[h * 4 + i], f[2 * i], f[2 * i + 1]);
+                    for (int i = 0; i < 2; ++i) {
+                        const int key = u * 16 + i * 8 + g8;
+                        const int at = HD == 128 ? key * 128 + (((2 * t4 + h) ^ (key & 7)) << 4)
+                                                 : key * 64 + ((t4 ^ ((key >> 1) & 3)) << 4);
+                        i8x16_to_f16x2(*reinterpret_cast<const uint4*>(kt + at), f[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t(&q)[2 * kQ] = qf[h * 4 + i];
+                        if constexpr (kT) {
+                            const uint32_t a[4] = {f[0][2 * i], f[1][2 * i], f[0][2 * i + 1], f[1][2 * i + 1]};
+                            mma16816(x[u], a, q[0], q[1]);
+                        } else {
+                            mma16816(x[2 * u], q, f[0][2 * i], f[0][2 * i + 1]);
+                            mma16816(x[2 * u + 1], q, f[1][2 * i], f[1][2 * i + 1]);
+                        }
+                    }
                 }
             }
+            float inv[kStep / 16];
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int u = 0; u < kStep / 16; ++u) {
+                const float4 v = sc[u];
+                inv[u] = v.z;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[n][e] = fmaf(x[n][e], sc.x, sc.y);
-            if (kb + 16 > min(lim[0], lim[1])) {
+                for (int n = u * kX * 16 / kStep; n < (u + 1) * kX * 16 / kStep; ++n)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        x[n][e] = kb + n * 8 + t4 * 2 + (e & 1) < lim[e >> 1] ? x[n][e] : -INFINITY;
+                    for (int e = 0; e < 4; ++e) x[n][e] = fmaf(x[n][e], v.x, v.y);
             }
+            if (kb + kStep > min(lim[0], lim[1])) {
+#pragma unroll
+                for (int n = 0; n < kX; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[n][e] = kb + key_of(n, e) < lim[row_of(e)] ? x[n][e] : -INFINITY;
+            }
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < kX; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[row_of(e)] = fmaxf(mx[row_of(e)], x[n][e]);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                float mx = fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const bool need = (mx - m[r]) * c > 8.0f;
-                if (__any_sync(0xffffffffu, need)) {
-                    const float corr = need ? ex2_approx((m[r] - mx) * c) : 1.0f;
-                    if (need) m[r] = mx;
-                    l[r] *= corr;
-#pragma unroll
-                    for (int n = 0; n < HD / 8; ++n) {
-                        o[n][2 * r] *= corr;
-                        o[n][2 * r + 1] *= corr;
-                    }
-                }
-                const float ref = m[r] == -INFINITY ? 0.0f : m[r];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float pv = ex2_approx((x[n][2 * r + e] - ref) * c);
-                        x[n][2 * r + e] = pv;
-                        l[r] = fmaf(pv, sc.z, l[r]);
-                    }
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], kT ? 4 : 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], kT ? 8 : 2));
+                if (kT) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 16));
             }
-            const uint32_t pf[4] = {h2(x[0][0], x[0][1]), h2(x[0][2], x[0][3]), h2(x[1][0], x[1][1]),
-                                    h2(x[1][2], x[1][3])};
-            // V rows 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9 at the HD / 8 columns from ra * HD / 8 on
-            uint32_t v[4][HD / 32];
+            const bool need[2] = {(mx[0] - m[0]) * c > 8.0f, (mx[1] - m[1]) * c > 8.0f};
+            if (__any_sync(0xffffffffu, need[0] || need[1])) {
+                float corr[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = warp * 16 + 2 * t4 + (i & 1) + (i >> 1) * 8;
-                if (HD == 128) {
-                    const uint4 r = *reinterpret_cast<const uint4*>(vt + key * 128 + ((ra ^ (key & 7)) << 4));
-                    v[i][0] = r.x ^ 0x80808080u;
-                    v[i][1] = r.y ^ 0x80808080u;
-                    v[i][HD / 32 - 2] = r.z ^ 0x80808080u;
-                    v[i][HD / 32 - 1] = r.w ^ 0x80808080u;
+                for (int r = 0; r < 2; ++r) {
+                    corr[r] = need[r] ? ex2_approx((m[r] - mx[r]) * c) : 1.0f;
+                    if (need[r]) m[r] = mx[r];
+                    l[r] *= corr[r];
+                }
+#pragma unroll
+                for (int n = 0; n < kO; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][e] *= corr[row_of(e)];
+            }
+            const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+            for (int n = 0; n < kX; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float pv = ex2_approx((x[n][e] - ref[row_of(e)]) * c);
+                    x[n][e] = pv;
+                    l[row_of(e)] = fmaf(pv, inv[n * (kStep / 16) / kX], l[row_of(e)]);
+                }
+#pragma unroll
+            for (int u = 0; u < kStep / 16; ++u) {
+                uint32_t pf[4];
+                if constexpr (kT) {
+                    pf[0] = transpose8(h2(x[u][0], x[u][1]));  // keys 2 t4, 2 t4 + 1 of row g8
+                    pf[1] = transpose8(h2(x[u][2], x[u][3]));  // 2 t4 + 8, 2 t4 + 9
                 } else {
-                    const uint2 r = *reinterpret_cast<const uint2*>(vt + key * 64 + (((ra >> 1) ^ ((key >> 1) & 3)) << 4) +
-                                                                    (ra & 1) * 8);
-                    v[i][0] = r.x ^ 0x80808080u;
-                    v[i][1] = r.y ^ 0x80808080u;
+                    pf[0] = h2(x[2 * u][0], x[2 * u][1]);
+                    pf[1] = h2(x[2 * u][2], x[2 * u][3]);
+                    pf[2] = h2(x[2 * u + 1][0], x[2 * u + 1][1]);
+                    pf[3] = h2(x[2 * u + 1][2], x[2 * u + 1][3]);
                 }
-            }
+                // V rows 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9 of the 16 at the HD / 8 columns from g8 * HD / 8 on
+                uint32_t v[4][HD / 32];
 #pragma unroll
-            for (int w = 0; w < HD / 32; ++w) {  // 4 columns: the two keys of a pair side by side
-                const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
-                const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-                mma16816(o[4 * w], pf, f16x2_sub1152(i8_perm_lo(a0)), f16x2_sub1152(i8_perm_lo(b0)));
-                mma16816(o[4 * w + 1], pf, f16x2_sub1152(i8_perm_hi(a0)), f16x2_sub1152(i8_perm_hi(b0)));
-                mma16816(o[4 * w + 2], pf, f16x2_sub1152(i8_perm_lo(a1)), f16x2_sub1152(i8_perm_lo(b1)));
-                mma16816(o[4 * w + 3], pf, f16x2_sub1152(i8_perm_hi(a1)), f16x2_sub1152(i8_perm_hi(b1)));
+                for (int i = 0; i < 4; ++i) {
+                    const int key = u * 16 + 2 * t4 + (i & 1) + (i >> 1) * 8;
+                    if constexpr (HD == 128) {
+                        const uint4 r = *reinterpret_cast<const uint4*>(vt + key * 128 + ((g8 ^ (key & 7)) << 4));
+                        v[i][0] = r.x ^ 0x80808080u;
+                        v[i][1] = r.y ^ 0x80808080u;
+                        v[i][2] = r.z ^ 0x80808080u;
+                        v[i][3] = r.w ^ 0x80808080u;
+                    } else {
+                        const uint2 r = *reinterpret_cast<const uint2*>(
+                            vt + key * 64 + (((g8 >> 1) ^ ((key >> 1) & 3)) << 4) + (g8 & 1) * 8);
+                        v[i][0] = r.x ^ 0x80808080u;
+                        v[i][1] = r.y ^ 0x80808080u;
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < HD / 32; ++w) {  // 4 columns: the two keys of a pair side by side
+                    uint32_t a[4], b[4];
+                    const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
+                    const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
+                    a[0] = f16x2_sub1152(i8_perm_lo(a0));
+                    a[1] = f16x2_sub1152(i8_perm_hi(a0));
+                    a[2] = f16x2_sub1152(i8_perm_lo(a1));
+                    a[3] = f16x2_sub1152(i8_perm_hi(a1));
+                    b[0] = f16x2_sub1152(i8_perm_lo(b0));
+                    b[1] = f16x2_sub1152(i8_perm_hi(b0));
+                    b[2] = f16x2_sub1152(i8_perm_lo(b1));
+                    b[3] = f16x2_sub1152(i8_perm_hi(b1));
+                    if constexpr (kT) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t f[4] = {a[2 * i], a[2 * i + 1], b[2 * i], b[2 * i + 1]};
+                            mma16816(o[2 * w + i], f, pf[0], pf[1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mma16816(o[4 * w + i], pf, a[i], b[i]);
+                    }
+                }
             }
         }
         __syncwarp();
@@ -363,27 +454,36 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_q8_kernel(const __gr
         *abort_flag = 1;
         if (lane == 0) set_err(p.err, 0x722);
     }
-    // ---- merge of the four warps.  o[n][e]: column (2 t4 + (e & 1)) * HD / 8 + n of row ra (e < 2) or rb
+    // ---- merge of the four warps
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], kT ? 4 : 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], kT ? 8 : 2);
+        if (kT) l[r] += __shfl_xor_sync(0xffffffffu, l[r], 16);
     }
     consumer_bar();  // nobody reads the ring any more
     float* so = reinterpret_cast<float*>(smem);                 // [warp][row][8 runs]
     float2* sml = reinterpret_cast<float2*>(smem + L::kOffMl);  // [warp][row]
-    if (t4 == 0) {
+    if ((kT ? g8 : t4) == 0) {
         sml[warp * kMaxRows + ra] = make_float2(m[0], l[0]);
         sml[warp * kMaxRows + rb] = make_float2(m[1], l[1]);
     }
+    if constexpr (kT) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int row = e < 2 ? ra : rb;
-        if (row >= R) continue;
-        float* dst = so + (warp * kMaxRows + row) * L::kRow + (2 * t4 + (e & 1)) * (L::kRun + 4);
+        for (int r = 0; r < 2; ++r) {
+            float* dst = so + (warp * kMaxRows + ra + r) * L::kRow + g8 * (L::kRun + 4);
 #pragma unroll
-        for (int n = 0; n < HD / 8; n += 4)
-            *reinterpret_cast<float4*>(dst + n) = make_float4(o[n][e], o[n + 1][e], o[n + 2][e], o[n + 3][e]);
+            for (int n = 0; n < kO; n += 2)
+                *reinterpret_cast<float4*>(dst + 2 * n) = make_float4(o[n][r], o[n][2 + r], o[n + 1][r], o[n + 1][2 + r]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float* dst = so + (warp * kMaxRows + (e < 2 ? ra : rb)) * L::kRow + (2 * t4 + (e & 1)) * (L::kRun + 4);
+#pragma unroll
+            for (int n = 0; n < kO; n += 4)
+                *reinterpret_cast<float4*>(dst + n) = make_float4(o[n][e], o[n + 1][e], o[n + 2][e], o[n + 3][e]);
+        }
     }
     consumer_bar();
     const int cols = p.head_dim >> 2;
@@ -462,14 +562,15 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_q8_kernel(const __gr
     }
 }
 
-template <int HD>
+template <int HD, int kMaxRows>
 int launch(const Params& p, int batch, int tiles, cudaStream_t st) {
-    auto kern = paged_decode_q8_kernel<HD>;
-    NPUB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<HD>::kTotal));
+    auto kern = paged_decode_q8_kernel<HD, kMaxRows>;
+    constexpr int kTotal = Smem<HD, kMaxRows>::kTotal;
+    NPUB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kTotal));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.kv_heads * p.splits, batch, tiles);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Smem<HD>::kTotal;
+    cfg.dynamicSmemBytes = kTotal;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -533,7 +634,8 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(const int8_t* __restrict
 
 }  // namespace pdq8
 
-int paged_decode_q8(const PackedArgs& a, const float* k_scales, const float* v_scales, int tiles, cudaStream_t st) {
+int paged_decode_q8(const PackedArgs& a, const float* k_scales, const float* v_scales, int rows, int tiles,
+                    cudaStream_t st) {
     using namespace pdq8;
     Params p;
     memset(&p, 0, sizeof(p));
@@ -568,7 +670,9 @@ int paged_decode_q8(const PackedArgs& a, const float* k_scales, const float* v_s
     p.part_o = a.part_o;
     p.part_ml = a.part_ml;
     p.err = npub_internal_device_error_word();
-    return a.head_dim <= 64 ? launch<64>(p, a.batch, tiles, st) : launch<128>(p, a.batch, tiles, st);
+    const bool small = a.head_dim <= 64;
+    if (rows <= 8) return small ? launch<64, 8>(p, a.batch, tiles, st) : launch<128, 8>(p, a.batch, tiles, st);
+    return small ? launch<64, 16>(p, a.batch, tiles, st) : launch<128, 16>(p, a.batch, tiles, st);
 }
 
 int expand_q8(const PackedArgs& a, const float* k_scales, const float* v_scales, int width, void* k_out, void* v_out,
