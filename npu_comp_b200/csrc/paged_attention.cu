@@ -110,11 +110,10 @@ Phase tile_phase(int total, int batch, int heads, int kv_heads, int max_new, int
 // The few-row kernel on up to `keys` keys of each sequence; behind: a shared
 // prefix's partials are combined with its own.  One of its CTAs, two of which
 // share an SM, takes 4 us (in a cluster 5) and 3 us per 128 keys of 128 columns.
-Phase few_phase(int batch, int kv_heads, int head_dim, int64_t keys, double part_us, bool behind, int tiles = 1,
-                bool q8 = false) {
-    const Cost c = {0.0, 4.0, (head_dim > 64 ? 3.0 : 1.6) * (q8 ? 0.6 : 1.0), 128}, cc = {0.0, 5.0, c.unit_us, 128};
+Phase few_phase(int batch, int kv_heads, int head_dim, int64_t keys, double part_us, bool behind) {
+    const Cost c = {0.0, 4.0, head_dim > 64 ? 3.0 : 1.6, 128}, cc = {0.0, 5.0, c.unit_us, 128};
     const bool ragged = batch > 1;
-    const int64_t items = (int64_t)batch * kv_heads * tiles, slots = 2 * num_sms();
+    const int64_t items = (int64_t)batch * kv_heads, slots = 2 * num_sms();
     Phase ph = {};
     const Split sp = pick_splits(keys, items, slots, c, ragged, 64, part_us + 0.15, 1, behind, 4.0);
     ph.splits = sp.s;
@@ -210,6 +209,7 @@ struct PlanQ8 {
     Plan p;
     int tiles, rows;              // paged_decode_q8: tiles of a sequence and kv head, and the rows of one
     int width;                    // tile kernel: fp16 pages of 128 keys per sequence
+    bool list;                    // paged_list_q8 instead
     size_t parts, pages, tables;  // bytes of the partials, of the fp16 K (or V), and of their table and lengths
     size_t bytes() const { return parts + 2 * pages + tables; }
 };
@@ -225,7 +225,22 @@ PlanQ8 make_plan_q8(int batch, int total, int max_new, int64_t ctx, int heads, i
     }
     pl.p.few = pl.tiles > 0;
     if (pl.p.few) {
-        pl.p.own = few_phase(batch, kv_heads, head_dim, ctx, part_us, false, pl.tiles, true);
+        const int64_t items = (int64_t)batch * kv_heads * pl.tiles, blocks = ceil_div(ctx, 128);
+        // resident CTAs of the cluster kernel; ranges while they hold all of it at once
+        const int64_t slots = (pl.rows == 8 ? 3 : 2) * num_sms();
+        int64_t splits = slots / items;
+        if (splits > kPagedDecodeCluster) splits = kPagedDecodeCluster;
+        if (splits > blocks) splits = blocks;
+        if (splits < 1) splits = 1;
+        // The list takes two launches and 12 us for the smallest call, the cluster kernel 6 us and 1 to 1.5 us for each
+        // block of 128 keys that its fullest slot takes (the largest sequence's share: it is not balanced).  Measured, 32 / 8
+        // heads of 128, cluster and list: one sequence of 4096 keys 8.9 and 12.3 us, of 16384 21.9 and 17.1; 16 sequences of
+        // 16400 keys 14.6 and 19.2, of 65000 43 and 36; 64 of 16400 16.2 and 18.4, of 65000 56 and 36.
+        pl.list = ceil_div(blocks, splits) * (items * splits > slots ? items * splits : slots) > 10 * slots;
+        pl.p.own.splits = (int)splits;
+        pl.p.own.cluster = true;
+        if (pl.list) pl.parts = paged_list_q8_workspace(batch, kv_heads, head_dim, pl.rows, pl.tiles);
+        return pl;
     } else {
         pl.p.own = tile_phase(total, batch, heads, kv_heads, max_new, ctx, num_sms(), part_us, false);
         const int64_t width = ceil_div(ctx, 128);
@@ -261,15 +276,9 @@ int run_plan_q8(const PlanQ8& pl, PackedArgs& a, const float* ks, const float* v
         a.lens = lens;
         return run_plan(pl.p, a, workspace, pl.parts, st);
     }
-    if (pl.parts) {
-        const size_t n = (size_t)pl.p.total() * a.total_q * a.heads;
-        a.part_ml = reinterpret_cast<float2*>(ws);
-        a.part_o = reinterpret_cast<float*>(ws + (n * sizeof(float2) + 255) / 256 * 256);
-    }
+    if (pl.list) return paged_list_q8(a, ks, vs, pl.rows, pl.tiles, workspace, st);
     a.splits = pl.p.own.splits;
-    const int rc = paged_decode_q8(a, ks, vs, pl.rows, pl.tiles, st);
-    if (rc || !pl.parts) return rc;
-    return paged_combine(a, pl.p.total(), st);
+    return paged_decode_q8(a, ks, vs, pl.rows, pl.tiles, st);
 }
 
 // log2 of a scale over c = scale * log2(e) goes into the scores there

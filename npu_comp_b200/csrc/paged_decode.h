@@ -16,9 +16,13 @@ int paged_decode(const PackedArgs& a, cudaStream_t st);
 int paged_combine(const PackedArgs& a, int splits, cudaStream_t st);
 
 // paged_decode_q8.cu: the same over 8-bit pages with a scale for each page and kv head, for up to `tiles` tiles of `rows` (8
-// or 16) rows per kv head and sequence.  a.splits ranges: partials 0 .. splits - 1 when a.part_o is set, else the result.
+// or 16) rows per kv head and sequence: in up to kPagedDecodeCluster (a.splits) ranges that a cluster combines, or as a list
+// cut into equal parts for all warps.
 int paged_decode_q8(const PackedArgs& a, const float* k_scales, const float* v_scales, int rows, int tiles,
                     cudaStream_t st);
+size_t paged_list_q8_workspace(int batch, int kv_heads, int head_dim, int rows, int tiles);
+int paged_list_q8(const PackedArgs& a, const float* k_scales, const float* v_scales, int rows, int tiles, void* workspace,
+                  cudaStream_t st);
 // Every sequence's keys as fp16 pages of 128 keys, `width` of them per sequence (page b * width + w), with their table and
 // the lengths (0 for a sequence of more than 128 * width keys).
 int expand_q8(const PackedArgs& a, const float* k_scales, const float* v_scales, int width, void* k_out, void* v_out,

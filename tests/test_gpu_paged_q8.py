@@ -292,6 +292,57 @@ def test_decode(cuda_device, H, KV, hd, ps, keys):
             same(o[b:b + 1], want, bound)
 
 
+@pytest.mark.parametrize("H,KV,hd,ps", [(8, 8, 128, 16), (32, 8, 64, 64), (16, 1, 80, 32), (6, 3, 128, 128)])
+@pytest.mark.parametrize("seqs,most", [(1, 30000), (70, 3000), (200, 400)])
+def test_long_and_many_sequences(cuda_device, H, KV, hd, ps, seqs, most):
+    """Ragged contexts, empty ones among them, with no rows, one, or several tiles: cut over the GPU wherever it falls."""
+    g = torch.Generator().manual_seed(seqs + H)
+    keys = [int(most * x) for x in torch.rand(seqs, generator=g).square().tolist()]
+    keys[0] = most
+    if seqs > 1:
+        keys[1::7] = [0] * len(keys[1::7])
+    new = torch.randint(0, 3 * 16 * KV // H + 1, (seqs,), generator=g).clamp(max=12).tolist()
+    new[0] = max(new[0], 1)
+    check_chunks(new, keys, H, KV, hd, ps, ctx=most)
+    c = Cache(keys, KV, hd, ps, seed=seqs)
+    q = torch.randn((seqs, H * hd), generator=g).half().cuda()
+    o = nb.attention_paged_decode_q8(q, *c.args, c.lens, heads=H, ctx_len=most)
+    for b in range(0, seqs, 9):
+        want, bound = expected(c, b, q[b:b + 1].reshape(1, H, hd), 1 / math.sqrt(hd), True, False)
+        same(o[b:b + 1], want, bound)
+
+
+def planted_cache(m, KV, hd, ps, every, gen):
+    """m keys of which one at a random place of every `every` scores alike and stands out in v, the others low: a stretch
+    that is lost or weighed wrongly shows."""
+    n = (m + ps - 1) // ps
+    kq = torch.randint(-20, 21, (n, KV, ps, hd), generator=gen, dtype=torch.int8)
+    vq = torch.randint(-1, 2, (n, KV, ps, hd), generator=gen, dtype=torch.int8)
+    sign = torch.randint(0, 2, (KV, hd), generator=gen) * 2 - 1
+    first = torch.arange(0, m, every)
+    at = first + (torch.rand(len(first), generator=gen) * torch.clamp(m - first, max=every)).long()
+    kq[at // ps, :, at % ps] = (sign * 100).to(torch.int8)
+    vq[at // ps, :, at % ps] = 0
+    vq[at // ps, :, at % ps, torch.arange(len(at)) % hd] = 120
+    return kq, vq, sign.half()
+
+
+@pytest.mark.parametrize("H,KV,n", [(8, 2, 1), (16, 1, 1), (8, 2, 14)])
+def test_planted_keys_over_a_long_context(cuda_device, H, KV, n):
+    g = torch.Generator().manual_seed(H + n)
+    m, hd, ps = 100003, 128, 32
+    kq, vq, sign = planted_cache(m, KV, hd, ps, 61, g)
+    pages = kq.shape[0]
+    c = Cache.__new__(Cache)
+    c.ps, c.keys, c.kp, c.vp = ps, [m], kq.cuda(), vq.cuda()
+    c.table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    c.ks, c.vs = torch.full((pages, KV), 0.008, device="cuda"), torch.full((pages, KV), 0.02, device="cuda")
+    q = sign.repeat_interleave(H // KV, 0).reshape(1, H * hd).repeat(n, 1).cuda()
+    o = nb.attention_paged_q8(q, c.kp, c.vp, c.ks, c.vs, c.table, i32([m]), i32([0, n]), heads=H, max_new=n)
+    want, bound = expected(c, 0, q.reshape(n, H, hd), 1 / math.sqrt(hd), True, False)
+    same(o, want, bound)
+
+
 @pytest.mark.parametrize("lo,hi", [(1e-6, 10.0), (1e-12, 1e-10), (1e-38, 1.0), (5.0, 400.0)])
 def test_scales_far_apart(cuda_device, lo, hi):
     """Pages of one sequence with scales orders apart (few rows: any; the keys of both far larger than fp16 holds too)."""
