@@ -21,6 +21,7 @@
 // Bound: the logits are read once (from L1 or L2 a second time for the index);
 // what a row takes is the histogram's clearing, filling and scan.
 #include "common.cuh"
+#include "gemm_tc.h"
 
 #include <cmath>
 
@@ -33,6 +34,8 @@ constexpr int kBins = 2 * kZero;      // the last is -65504
 constexpr int kGroups = kBins / 8;    // 16 bytes of counts
 constexpr int kOwners = kGroups / 8;  // threads that hold a range of values (992)
 constexpr uint32_t kNone = 0xffffu;   // -inf and NaN: no bin
+constexpr int kMaxSegment = 65528;    // logits of a CTA: what a 16-bit count holds
+constexpr int kMaxSteps = (kMaxSegment + kThreads * 8 - 1) / (kThreads * 8);
 
 struct Args {
     const __half* x;
@@ -58,12 +61,13 @@ __device__ __forceinline__ double value_of(int bin) {
 
 // What the CTAs of a cluster tell one another.
 struct Mail {
-    double w, w_min;          // this CTA's range of values: weights, and those of at least min_p
-    double cut_w;             // a cut's weight
-    uint32_t top;             // first bin in use
-    uint32_t n, n_min;        // the same, tokens
-    uint32_t cut_n;
-    uint32_t pos, bin, rank;  // the sampled place in the order, its value, its number among the equal ones
+    double w;                   // this CTA's range of values: weight
+    double k_w, m_w, p_w;       // weight up to the cuts of top-k, min-p, top-p
+    uint32_t top;               // first bin in use
+    uint32_t n;                 // tokens of the range
+    uint32_t k_n, m_n, p_n;     // tokens up to the cuts
+    uint32_t min_bin;           // first bin of a weight below min_p
+    uint32_t pos, bin, rank;    // the sampled place in the order, its value, its number among the equal ones
 };
 
 template <int C>
@@ -123,42 +127,117 @@ __device__ __forceinline__ uint32_t group_counts(uint32_t hist, int g, uint32_t 
     return any;
 }
 
-// Weights of a thread's range of values (64 / C bins inside one binade, evenly
-// spaced): exp of a group's first value, then products with the step's ratio
-// (7 of them: within 1e-15).  The largest value of the row has weight 1.
+// exp in one place: it is long
+__device__ __noinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ double double_of(uint32_t c) {  // c < 2^32, by way of 2^52 + c
+    return __hiloint2double(0x43300000, (int)c) - 4503599627370496.0;
+}
+
+// The row's weights: exp((l - top) / T), 1 at the top.
 struct Weights {
-    double top, inv_t, ratio;
+    double top, inv_t;
     int top_bin;
-    __device__ __forceinline__ double first(int g, int& e0) const {
-        e0 = 0;
-        if (g == (top_bin >> 3)) {
-            e0 = top_bin & 7;
-            return 1.0;
-        }
-        return exp((value_of(g * 8) - top) * inv_t);
+    __device__ __forceinline__ double at(int bin) const {
+        return bin <= top_bin ? 1.0 : exp_of((value_of(bin) - top) * inv_t);
     }
 };
 
-// Walks the tokens of a thread's range in order: f(tokens before, weight before, count, weight) until it returns true.
-template <int C, typename F>
-__device__ __forceinline__ void walk(uint32_t hist, int g0, const Weights& wt, uint32_t n, double w, F f) {
-#pragma unroll 1
-    for (int j = 0; j < 8 / C; ++j) {
-        uint32_t c[8];
-        if (!group_counts<C>(hist, g0 + j, c)) continue;
-        int e0;
-        double x = wt.first(g0 + j, e0);
+__device__ __forceinline__ double scan_up(double v, int lane) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (e < e0) continue;
-            if (c[e]) {
-                if (f(n, w, c[e], x, (g0 + j) * 8 + e)) return;
-                n += c[e];
-                w += (double)c[e] * x;
+    for (int d = 1; d < 32; d <<= 1) {
+        const double u = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v = u + v;
+    }
+    return v;
+}
+__device__ __forceinline__ uint32_t scan_up(uint32_t v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += u;
+    }
+    return v;
+}
+
+// A value of the row: tokens and weight ahead of it, its count, its weight, its bin.
+struct Hit {
+    uint32_t n;
+    double w;
+    uint32_t c;
+    double y;
+    int bin;
+};
+// By a warp: the first value in use, of a thread's range from group g0 on (n tokens and the weight w ahead of it), behind
+// which crossed(tokens, weight, bin) holds; the range's last one where it holds for none.
+template <int C, typename F>
+__device__ __forceinline__ Hit locate(uint32_t hist, int g0, uint32_t n, double w, const Weights& wt, F crossed) {
+    const int lane = threadIdx.x & 31;
+    constexpr int kPer = C == 1 ? 2 : 1;  // bins per lane
+    uint32_t c[kPer];
+    double y[kPer];
+    const int first = g0 * 8 + lane * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) c[i] = 0;
+    if (lane * kPer < 64 / C) {
+#pragma unroll
+        for (int q = 0; q < C; ++q) {
+            const uint32_t v = ld_u32(addr_in<C>(hist + (uint32_t)(first >> 1) * 4u, q));
+            if constexpr (C == 1) {
+                c[0] += v & 0xffffu;
+                c[1] += v >> 16;
+            } else {
+                c[0] += (first & 1) ? v >> 16 : v & 0xffffu;
             }
-            x *= wt.ratio;
         }
     }
+    uint32_t sn = 0;
+    double sw = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        y[i] = c[i] ? wt.at(first + i) : 0.0;
+        sn += c[i];
+        sw += double_of(c[i]) * y[i];
+    }
+    const uint32_t in = scan_up(sn, lane);
+    const double iw = scan_up(sw, lane), up = __shfl_up_sync(0xffffffffu, iw, 1);
+    Hit h, last;
+    h.n = n + in - sn;
+    h.w = w + (lane ? up : 0.0);
+    bool hit = false;
+    last.c = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        if (hit || !c[i]) continue;
+        if (last.c) {
+            h.n += last.c;
+            h.w += double_of(last.c) * last.y;
+        }
+        last.c = h.c = c[i];
+        last.y = h.y = y[i];
+        h.bin = first + i;
+        hit = crossed(h.n + c[i], h.w + double_of(c[i]) * y[i], first + i);
+    }
+    const uint32_t hits = __ballot_sync(0xffffffffu, hit), used = __ballot_sync(0xffffffffu, sn != 0);
+    const int src = hits ? __ffs(hits) - 1 : 31 - __clz(used | 1u);
+    h.n = __shfl_sync(0xffffffffu, h.n, src);
+    h.w = __shfl_sync(0xffffffffu, h.w, src);
+    h.c = __shfl_sync(0xffffffffu, h.c, src);
+    h.y = __shfl_sync(0xffffffffu, h.y, src);
+    h.bin = __shfl_sync(0xffffffffu, h.bin, src);
+    return h;
+}
+
+// Eight logits from i on (-inf behind the segment's end).
+__device__ __forceinline__ uint4 load8(const __half* x, int i, int end, int vec) {
+    uint32_t w[4] = {0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u};
+    if (vec && i + 8 <= end) return __ldg(reinterpret_cast<const uint4*>(x + i));
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (i + e < end) {
+            const uint32_t h = __half_as_ushort(x[i + e]);
+            w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xffffu) | (h << 16) : (w[e >> 1] & 0xffff0000u) | h;
+        }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <int C>
@@ -167,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     extern __shared__ __align__(16) uint32_t hist[];  // [kBins / 2], two counts each
     __shared__ Mail mail;
     __shared__ double part_w[32];
-    __shared__ uint32_t part_n[32];
+    __shared__ uint32_t part_n[kMaxSteps * 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = C > 1 ? (int)cluster_ctarank() : 0;
     const int64_t row = blockIdx.x / C;
@@ -181,31 +260,22 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     const int i0 = min(a.vocab, rank * a.seg), i1 = min(a.vocab, i0 + a.seg);
     uint32_t top = kNone;
     for (int base = i0; base < i1; base += kThreads * 8) {
-        const int i = base + tid * 8;
-        uint32_t w[4] = {0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u};
-        if (a.vec && i + 8 <= i1) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + i));
-            w[0] = v.x;
-            w[1] = v.y;
-            w[2] = v.z;
-            w[3] = v.w;
-        } else {
-            for (int e = 0; e < 8; ++e)
-                if (i + e < i1) {
-                    const uint32_t h = __half_as_ushort(x[i + e]);
-                    w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xffffu) | (h << 16) : (w[e >> 1] & 0xffff0000u) | h;
-                }
+        const uint4 v = load8(x, base + tid * 8, i1, a.vec);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        // a warp of one value (a mask's) counts it at once
+        const bool flat = v.x == v.y && v.x == v.z && v.x == v.w && (v.x >> 16) == (v.x & 0xffffu);
+        const uint32_t first = __shfl_sync(0xffffffffu, v.x, 0);
+        if (__all_sync(0xffffffffu, flat && v.x == first)) {
+            const uint32_t bin = bin_of(v.x & 0xffffu);
+            top = min(top, bin);
+            if (lane == 0 && bin != kNone) atomicAdd(&hist[bin >> 1], 256u << ((bin & 1) * 16));
+            continue;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint32_t bin = bin_of((e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu);
             top = min(top, bin);
-            // a warp of one value (a mask's) counts it at once
-            if (__all_sync(0xffffffffu, bin == __shfl_sync(0xffffffffu, bin, 0))) {
-                if (lane == 0 && bin != kNone) atomicAdd(&hist[bin >> 1], 32u << ((bin & 1) * 16));
-            } else if (bin != kNone) {
-                atomicAdd(&hist[bin >> 1], 1u << ((bin & 1) * 16));
-            }
+            if (bin != kNone) atomicAdd(&hist[bin >> 1], 1u << ((bin & 1) * 16));
         }
     }
     top = __reduce_min_sync(0xffffffffu, top);
@@ -214,6 +284,14 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     const uint32_t mb = smem_u32(&mail), hb = smem_u32(hist);
     auto at = [&](int q, const void* field) {
         return addr_in<C>(mb + (uint32_t)(reinterpret_cast<const char*>(field) - reinterpret_cast<const char*>(&mail)), q);
+    };
+    auto tell_n = [&](uint32_t* field, uint32_t v) {
+#pragma unroll
+        for (int q = 0; q < C; ++q) st_u32(at(q, field), v);
+    };
+    auto tell_w = [&](double* field, double v) {
+#pragma unroll
+        for (int q = 0; q < C; ++q) st_f64(at(q, field), v);
     };
     top = kNone;
 #pragma unroll
@@ -228,201 +306,217 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         const double u = (double)a.u[row];
         const bool greedy = !(t > 0.0f);
         if (top == 0 || greedy) t = 1.0f;  // +inf takes all of the weight
-        // ---- tokens and weights of this thread's values, and their running sums
-        constexpr int G = 8 / C;
-        const bool owner = tid < kOwners;
-        const int g0 = (rank * kOwners + tid) * G;
         Weights wt;
         wt.top = value_of((int)top);
         wt.top_bin = (int)top;
         wt.inv_t = 1.0 / (double)t;
-        wt.ratio = 0.0;
-        const double min_p = (double)mf;
-        uint32_t n = 0, nm = 0;
-        double w = 0.0, wm = 0.0;
-        if (owner) {
-            // (between the second and third value: the first of bin 0's group is +inf)
-            wt.ratio = top == 0 ? 0.0 : exp((value_of(g0 * 8 + 2) - value_of(g0 * 8 + 1)) * wt.inv_t);
+        // ---- tokens and weights of this thread's values: 64 / C bins inside one binade, evenly spaced, so that the weights
+        // of a group are exp of its first value times powers of the step's ratio, and the groups' first values likewise
+        // (products of at most 63 steps: within 2e-14)
+        constexpr int G = 8 / C;
+        const int g0 = (rank * kOwners + tid) * G;
+        uint32_t n = 0;
+        double w = 0.0;
+        if (tid < kOwners) {
+            double ratio = 0.0, begin = 0.0, r8 = 0.0;
+            bool ready = false;
 #pragma unroll 1
             for (int j = 0; j < G; ++j) {
                 // lanes start at different groups: no two of a quarter warp read the same banks
-                const int g = g0 + ((j + (lane >> (C == 8 ? 3 : C == 4 ? 2 : C == 2 ? 1 : 0))) & (G - 1));
+                const int i = (j + (lane >> (C == 8 ? 3 : C == 4 ? 2 : C == 2 ? 1 : 0))) & (G - 1), g = g0 + i;
                 uint32_t c[8];
                 if (!group_counts<C>(hb, g, c)) continue;
-                int e0;
-                double y = wt.first(g, e0);
+                if (!ready) {
+                    ready = true;
+                    // (between the second and third value: the first of bin 0's group is +inf)
+                    ratio = top == 0 ? 0.0 : exp_of((value_of(g0 * 8 + 2) - value_of(g0 * 8 + 1)) * wt.inv_t);
+                    const double r2 = ratio * ratio, r4 = r2 * r2;
+                    r8 = r4 * r4;
+                    begin = g0 > wt.top_bin >> 3 ? wt.at(g0 * 8) : 0.0;
+                }
+                double y;
+                if (g0 > wt.top_bin >> 3) {
+                    const double r16 = r8 * r8;
+                    y = begin * ((i & 1) ? r8 : 1.0) * ((i & 2) ? r16 : 1.0) * ((i & 4) ? r16 * r16 : 1.0);
+                } else if (g > wt.top_bin >> 3) {
+                    y = wt.at(g * 8);
+                } else {  // the top's group: from the top on
+                    y = 1.0;
+                    const int e0 = wt.top_bin & 7;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (e < e0) continue;
-                    if (c[e]) {
-                        const double cy = (double)c[e] * y;
+                    for (int e = 0; e < 8; ++e) {
+                        if (e < e0) continue;
                         n += c[e];
-                        w += cy;
-                        if (y >= min_p) {
-                            nm += c[e];
-                            wm += cy;
-                        }
+                        w += double_of(c[e]) * y;
+                        y *= ratio;
                     }
-                    y *= wt.ratio;
+                    continue;
+                }
+                double s = double_of(c[7]);
+#pragma unroll
+                for (int e = 6; e >= 0; --e) s = fma(s, ratio, double_of(c[e]));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) n += c[e];
+                w += s * y;
+            }
+        } else if (!greedy && mf > 0.0f) {  // the last warp: where the weights fall below min_p
+            int lo = (int)top, hi = kBins;  // first bin below is in (lo, hi]; the top's weight is 1
+            if (1.0 < (double)mf) {
+                hi = lo;
+            } else {
+                while (hi - lo > 1) {
+                    const int step = (hi - lo + 31) >> 5, bin = min(hi, lo + (lane + 1) * step);
+                    const uint32_t below = __ballot_sync(0xffffffffu, bin >= hi || wt.at(bin) < (double)mf);
+                    const int f = __ffs(below) - 1;  // lanes' bins ascend
+                    hi = min(hi, lo + (f + 1) * step);
+                    lo = lo + f * step;
                 }
             }
+            if (lane == 0) mail.min_bin = (uint32_t)hi;
         }
-        uint32_t ni = n;
-        double wi = w;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t an = __shfl_up_sync(0xffffffffu, ni, d);
-            const double aw = __shfl_up_sync(0xffffffffu, wi, d);
-            if (lane >= d) {
-                ni += an;
-                wi = aw + wi;
-            }
-        }
+        // ---- running sums over the threads
+        const uint32_t ni = scan_up(n, lane);
+        const double wi = scan_up(w, lane);
         if (lane == 31) {
             part_n[warp] = ni;
             part_w[warp] = wi;
         }
         __syncthreads();
-        uint32_t bn = 0, tn = 0;
-        double bw = 0.0, tw = 0.0;
-        for (int q = 0; q < 32; ++q) {  // the warps ahead, and all of them
-            if (q == warp) {
-                bn = tn;
-                bw = tw;
+        const uint32_t pn = scan_up(part_n[lane], lane);
+        const double pw = scan_up(part_w[lane], lane);
+        uint32_t N = __shfl_sync(0xffffffffu, pn, 31), cta_n = 0;
+        double W = __shfl_sync(0xffffffffu, pw, 31), cta_w = 0.0;
+        if (C > 1) {
+            if (tid == 0) {
+                mail.n = N;
+                mail.w = W;
             }
-            tn += part_n[q];
-            tw += part_w[q];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            nm += __shfl_xor_sync(0xffffffffu, nm, d);
-            wm += __shfl_xor_sync(0xffffffffu, wm, d);
-        }
-        if (lane == 0) {
-            part_n[warp] = nm;
-            part_w[warp] = wm;
-        }
-        __syncthreads();
-        if (tid == 0) {
-            nm = 0;
-            wm = 0.0;
-            for (int q = 0; q < 32; ++q) {
-                nm += part_n[q];
-                wm += part_w[q];
-            }
-            mail.n = tn;
-            mail.w = tw;
-            mail.n_min = nm;
-            mail.w_min = wm;
-        }
-        sync_all<C>();
-        uint32_t N = 0, Nm = 0;
-        double W = 0.0, Wm = 0.0, cta_w = 0.0;
-        uint32_t cta_n = 0;
-#pragma unroll
-        for (int q = 0; q < C; ++q) {
-            if (q == rank) {
-                cta_n = N;
-                cta_w = W;
-            }
-            N += ld_u32(at(q, &mail.n));
-            W += ld_f64(at(q, &mail.w));
-            Nm += ld_u32(at(q, &mail.n_min));
-            Wm += ld_f64(at(q, &mail.w_min));
-        }
-        // [n0, n1) tokens and [w0, w1) of the running weight are this thread's.  w0 is the w1 of the thread ahead, the
-        // same sum of the same terms, so that the threads' ranges leave no gap.
-        const uint32_t n0 = cta_n + bn + ni - n, n1 = n0 + n;
-        const double up = __shfl_up_sync(0xffffffffu, wi, 1);
-        const double w0 = cta_w + (lane ? bw + up : bw), w1 = cta_w + (bw + wi);
-        auto tell = [&](uint32_t cn, double cw) {
+            sync_all<C>();
+            N = 0;
+            W = 0.0;
 #pragma unroll
             for (int q = 0; q < C; ++q) {
-                st_u32(at(q, &mail.cut_n), cn);
-                st_f64(at(q, &mail.cut_w), cw);
+                if (q == rank) {
+                    cta_n = N;
+                    cta_w = W;
+                }
+                N += ld_u32(at(q, &mail.n));
+                W += ld_f64(at(q, &mail.w));
             }
+        }
+        // [n0, n1) tokens and [w0, w1) of the running weight are this thread's.  w1 is the w0 of the thread behind, the same
+        // sum of the same terms, so that the threads' ranges leave no gap.
+        const uint32_t bn = warp ? __shfl_sync(0xffffffffu, pn, warp - 1) : 0;
+        const double up = __shfl_up_sync(0xffffffffu, wi, 1);
+        double bw = __shfl_sync(0xffffffffu, pw, max(warp - 1, 0));
+        if (warp == 0) bw = 0.0;
+        const double ew = __shfl_sync(0xffffffffu, pw, warp);
+        const uint32_t n0 = cta_n + bn + ni - n, n1 = n0 + n;
+        const double w0 = cta_w + (lane ? bw + up : bw), w1 = cta_w + (lane == 31 ? ew : bw + wi);
+        // The warp whose lane `mine` holds a place looks at that lane's values.
+        auto find = [&](bool mine, auto crossed, auto then) {
+            const uint32_t vote = __ballot_sync(0xffffffffu, mine);
+            if (!vote) return;
+            const int l = __ffs(vote) - 1;
+            const Hit h = locate<C>(hb, __shfl_sync(0xffffffffu, g0, l), __shfl_sync(0xffffffffu, n0, l),
+                                    __shfl_sync(0xffffffffu, w0, l), wt, crossed);
+            if (lane == 0) then(h);
         };
         uint32_t keep = N;
         double mass = W;
         if (greedy) {
             keep = 1;
         } else {
-            if (k > 0 && (uint32_t)k < N) {
-                if (n && n0 < (uint32_t)k && (uint32_t)k <= n1) {
-                    double cw = w1;
-                    walk<C>(hb, g0, wt, n0, w0, [&](uint32_t an, double aw, uint32_t c, double y, int) {
-                        if (an + c < (uint32_t)k) return false;
-                        cw = aw + (double)((uint32_t)k - an) * y;
-                        return true;
-                    });
-                    tell((uint32_t)k, cw);
+            const bool by_k = k > 0 && (uint32_t)k < N;
+            if (by_k || mf > 0.0f) {
+                if (mf > 0.0f && tid == 0) {  // no value below min_p: all are kept
+                    mail.m_n = N;
+                    mail.m_w = W;
+                }
+                const uint32_t min_bin = mf > 0.0f ? mail.min_bin : kBins;
+                sync_all<C>();
+                if (by_k)
+                    find(n && n0 < (uint32_t)k && (uint32_t)k <= n1,
+                         [&](uint32_t an, double, int) { return an >= (uint32_t)k; },
+                         [&](const Hit& h) {
+                             tell_n(&mail.k_n, (uint32_t)k);
+                             tell_w(&mail.k_w, h.w + double_of((uint32_t)k - h.n) * h.y);
+                         });
+                if (mf > 0.0f && min_bin < (uint32_t)kBins) {
+                    // the values ahead of min_bin: those ahead of the thread that holds it, and its own up to it
+                    const bool mine = tid < kOwners && min_bin >= (uint32_t)(g0 * 8) && min_bin < (uint32_t)((g0 + G) * 8);
+                    find(mine && n, [&](uint32_t, double, int bin) { return (uint32_t)bin >= min_bin; },
+                         [&](const Hit& h) {
+                             const bool ahead = (uint32_t)h.bin < min_bin;  // all of the range's are
+                             tell_n(&mail.m_n, ahead ? h.n + h.c : h.n);
+                             tell_w(&mail.m_w, ahead ? h.w + double_of(h.c) * h.y : h.w);
+                         });
+                    if (mine && !n) {
+                        tell_n(&mail.m_n, n0);
+                        tell_w(&mail.m_w, w0);
+                    }
                 }
                 sync_all<C>();
-                keep = mail.cut_n;
-                mass = mail.cut_w;
-                sync_all<C>();
+                if (by_k) {
+                    keep = mail.k_n;
+                    mass = mail.k_w;
+                }
             }
+            const uint32_t m_keep = mf > 0.0f ? mail.m_n : N;
+            const double m_mass = mf > 0.0f ? mail.m_w : W;
             if (pf < 1.0f) {
                 const double goal = fmax((double)pf, 0.0) * mass;
                 if (tid == 0) {
-                    mail.cut_n = keep;
-                    mail.cut_w = mass;
+                    mail.p_n = keep;
+                    mail.p_w = mass;
                 }
                 sync_all<C>();
-                if (goal <= 0.0 ? n && n0 == 0 : n && w0 < goal && goal <= w1) {
-                    uint32_t cn = n1;
-                    double cw = w1;
-                    walk<C>(hb, g0, wt, n0, w0, [&](uint32_t an, double aw, uint32_t c, double y, int) {
-                        if (goal > 0.0 && aw + (double)c * y < goal) return false;
-                        const double r = fmin(fmax(ceil((goal - aw) / y), 1.0), (double)c);
-                        cn = an + (uint32_t)r;
-                        cw = aw + r * y;
-                        return true;
-                    });
-                    if (cn < keep) tell(cn, cw);
-                }
+                find(goal <= 0.0 ? n && n0 == 0 : n && w0 < goal && goal <= w1,
+                     [&](uint32_t, double aw, int) { return aw >= goal; },
+                     [&](const Hit& h) {
+                         const double r = goal > 0.0 ? fmin(fmax(ceil((goal - h.w) / h.y), 1.0), double_of(h.c)) : 1.0;
+                         const uint32_t cn = h.n + (uint32_t)r;
+                         if (cn < keep) {
+                             tell_n(&mail.p_n, cn);
+                             tell_w(&mail.p_w, h.w + r * h.y);
+                         }
+                     });
                 sync_all<C>();
-                keep = mail.cut_n;
-                mass = mail.cut_w;
+                keep = mail.p_n;
+                mass = mail.p_w;
             }
-            if (Nm < keep) {
-                keep = Nm;
-                mass = Wm;
+            if (m_keep < keep) {
+                keep = m_keep;
+                mass = m_mass;
             }
         }
         if (keep == 0) keep = 1;  // min_p above 1
-        // ---- the place in the order, then its value
-        uint32_t pos = 0;
-        if (keep > 1) {
-            const double goal = u * mass;
-            if (tid == 0) mail.pos = goal > 0.0 ? keep - 1 : 0;
-            sync_all<C>();
-            if (n && w0 <= goal && goal < w1) {
-                uint32_t found = n1 - 1;
-                walk<C>(hb, g0, wt, n0, w0, [&](uint32_t an, double aw, uint32_t c, double y, int) {
-                    if (aw + (double)c * y <= goal) return false;
-                    found = an + (uint32_t)fmin(fmax(floor((goal - aw) / y), 0.0), (double)(c - 1));
-                    return true;
-                });
-#pragma unroll
-                for (int q = 0; q < C; ++q) st_u32(at(q, &mail.pos), found);
-            }
-            sync_all<C>();
-            pos = min(mail.pos, keep - 1);
-        }
-        if (n && n0 <= pos && pos < n1) {
-            walk<C>(hb, g0, wt, n0, w0, [&](uint32_t an, double, uint32_t c, double, int bin) {
-                if (an + c <= pos) return false;
-#pragma unroll
-                for (int q = 0; q < C; ++q) {
-                    st_u32(at(q, &mail.bin), (uint32_t)bin);
-                    st_u32(at(q, &mail.rank), pos - an);
-                }
-                return true;
-            });
-        }
+        // ---- the place in the order, and its value
+        const double goal = keep > 1 ? u * mass : 0.0;
+        if (tid == 0) mail.pos = keep > 1 && goal > 0.0 ? 0xffffffffu : 0;
+        if (tid == 0) mail.rank = 0xffffffffu;
         sync_all<C>();
+        auto tell_place = [&](uint32_t pos, const Hit& h) {
+            tell_n(&mail.pos, pos);
+            tell_n(&mail.bin, (uint32_t)h.bin);
+            tell_n(&mail.rank, pos - h.n);
+        };
+        if (keep > 1 && goal > 0.0)
+            find(n && w0 <= goal && goal < w1, [&](uint32_t, double aw, int) { return aw > goal; },
+                 [&](const Hit& h) {
+                     const double r = fmin(fmax(floor((goal - h.w) / h.y), 0.0), double_of(h.c - 1));
+                     tell_place(h.n + (uint32_t)r, h);
+                 });
+        else
+            find(n && n0 == 0, [&](uint32_t an, double, int) { return an > 0; }, [&](const Hit& h) { tell_place(0, h); });
+        sync_all<C>();
+        if (mail.pos >= keep) {  // u of 1 or more, or a border: the last one kept
+            const uint32_t pos = keep - 1;
+            sync_all<C>();
+            find(n && n0 <= pos && pos < n1, [&](uint32_t an, double, int) { return an > pos; },
+                 [&](const Hit& h) { tell_place(pos, h); });
+            sync_all<C>();
+        }
         // ---- the rank-th token of that value, by index
         const uint32_t bin = mail.bin;
         uint32_t r = mail.rank;
@@ -439,26 +533,37 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
             }
         }
         if (here && r < mine) {
-            const int per = ((i1 - i0 + kThreads - 1) / kThreads + 7) / 8 * 8;
-            const int j0 = min(i1, i0 + tid * per), j1 = min(i1, j0 + per);
-            uint32_t c = 0;
-            for (int i = j0; i < j1; ++i) c += bin_of(__half_as_ushort(x[i])) == bin;
-            uint32_t s = c;
+            // matches of every warp in every step of the segment, then the step and warp that hold the r-th, then its place
+            const int steps = (i1 - i0 + kThreads * 8 - 1) / (kThreads * 8);
+            auto matches = [&](int s, int at_warp) {
+                const uint4 v = load8(x, i0 + (s * kThreads + at_warp * 32 + lane) * 8, i1, a.vec);
+                const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+                uint32_t m = 0;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t v = __shfl_up_sync(0xffffffffu, s, d);
-                if (lane >= d) s += v;
+                for (int e = 0; e < 8; ++e)
+                    m |= (uint32_t)(bin_of((e & 1) ? h[e >> 1] >> 16 : h[e >> 1] & 0xffffu) == bin) << e;
+                return m;
+            };
+            for (int s = 0; s < steps; ++s) {
+                const uint32_t c = __reduce_add_sync(0xffffffffu, __popc(matches(s, warp)));
+                if (lane == 0) part_n[s * 32 + warp] = c;
             }
-            if (lane == 31) part_n[warp] = s;
             __syncthreads();
-            for (int q = 0; q < warp; ++q) s += part_n[q];
-            if (s - c <= r && r < s) {
-                r -= s - c;
-                for (int i = j0; i < j1; ++i)
-                    if (bin_of(__half_as_ushort(x[i])) == bin && r-- == 0) {
-                        a.ids[row] = i;
+            if (warp == 0) {
+                uint32_t before = 0;
+                for (int s = 0; s < steps; ++s) {
+                    const uint32_t c = part_n[s * 32 + lane], in = before + scan_up(c, lane);
+                    const uint32_t vote = __ballot_sync(0xffffffffu, in > r);
+                    if (vote) {
+                        const int l = __ffs(vote) - 1;
+                        before = __shfl_sync(0xffffffffu, in - c, l);
+                        const uint32_t m = matches(s, l), cm = __popc(m), im = before + scan_up(cm, lane);
+                        if (im - cm <= r && r < im)
+                            a.ids[row] = i0 + (s * kThreads + l * 32 + lane) * 8 + (int)__fns(m, 0, (int)(r - (im - cm)) + 1);
                         break;
                     }
+                    before = __shfl_sync(0xffffffffu, in, 31);
+                }
             }
         }
     }
@@ -502,7 +607,7 @@ extern "C" int npub_sample(const void* logits, int64_t ldl, int rows, int vocab,
     NPUB_CHECK_ARG(npub_aligned(u, 4) && npub_aligned(temperature, 4) && npub_aligned(top_k, 4) && npub_aligned(top_p, 4) &&
                    npub_aligned(min_p, 4) && npub_aligned(ids, 4));
     // 16-bit counts: at most 65535 logits in a CTA's histogram
-    if (vocab > 8 * 65528 || rows > 0x0fffffff) return NPUB_ERR_UNSUPPORTED;
+    if (vocab > 8 * kMaxSegment || rows > 0x0fffffff) return NPUB_ERR_UNSUPPORTED;
     Args a;
     a.x = reinterpret_cast<const __half*>(logits);
     a.ld = ldl;
@@ -518,7 +623,19 @@ extern "C" int npub_sample(const void* logits, int64_t ldl, int rows, int vocab,
     a.m = min_p;
     a.m0 = min_p_all;
     a.ids = ids;
-    const int c = vocab <= 40960 ? 1 : vocab <= 2 * 40960 ? 2 : vocab <= 4 * 40960 ? 4 : 8;
+    // CTAs of a row: waves of one CTA per SM, each about 8 us and 1 us for 8192 logits, 2 us for a cluster's barriers
+    int c = 0;
+    double best = 1e30;
+    for (int i = 1; i <= 8; i *= 2) {
+        if ((vocab + i - 1) / i > kMaxSegment - 8) continue;
+        const int64_t waves = ((int64_t)rows * i + num_sms() - 1) / num_sms();
+        const double us = (double)waves * (8.0 + (double)vocab / i / 8192.0 + (i > 1 ? 2.0 : 0.0));
+        if (us < best) {
+            best = us;
+            c = i;
+        }
+    }
+    if (c == 0) c = 8;
     a.seg = ((vocab + c - 1) / c + 7) / 8 * 8;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (c) {

@@ -71,6 +71,30 @@ def test_sizes_and_settings(cuda_device, vocab):
     check(x, torch.rand(rows, generator=g), 1.3, 0, 0.95, 0.0)
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 40000), (30, 40000), (37, 60000), (70, 60000), (148, 50000), (149, 65000), (300, 1500),
+                                        (70, 128256), (19, 300000)])
+def test_many_rows(cuda_device, rows, vocab):
+    """Every number of CTAs for a row, against the definition in whole-row fp64 operations (whose sums run in another order)."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (3.0 * torch.randn((rows, vocab), generator=g, device="cuda")).half()
+    x[:, ::5] = -math.inf
+    u = torch.rand(rows, generator=g, device="cuda")
+    pick = lambda *v: torch.tensor(v, device="cuda")[torch.randint(0, len(v), (rows,), generator=g, device="cuda")]  # noqa: E731
+    t, k = pick(0.5, 1.0, 1.7).float(), pick(0, 0, 3, 77, 1000).int()
+    p, m = pick(1.0, 0.97, 0.8, 0.2).float(), pick(0.0, 0.0, 0.003, 0.2).float()
+    l, index = torch.sort(x.double(), dim=-1, descending=True, stable=True)
+    w = torch.exp((l - l[:, :1]) / t.double()[:, None])
+    cum = torch.cumsum(w, -1)
+    n = torch.where(k > 0, k, vocab).long()[:, None]
+    kept = (torch.arange(vocab, device="cuda") < n) & (w >= m.double()[:, None])
+    goal = p.double()[:, None] * cum.gather(-1, n - 1)
+    kept &= (p >= 1.0)[:, None] | (cum - w < goal)
+    n = kept.sum(-1, keepdim=True).clamp(min=1)
+    at = torch.minimum((cum <= u.double()[:, None] * cum.gather(-1, n - 1)).sum(-1, keepdim=True), n - 1)
+    want = index.gather(-1, at)[:, 0].int()
+    assert torch.equal(nb.sample(x, u, temperature=t, top_k=k, top_p=p, min_p=m), want)
+
+
 @pytest.mark.parametrize("spread", [0.0, 1e-3, 0.05, 30.0, 20000.0])
 @pytest.mark.parametrize("t", [1e-3, 0.5, 1.0, 100.0, 1e6, math.inf])
 def test_distributions(cuda_device, spread, t):
