@@ -14,16 +14,18 @@
 // each value instead of one for each token.  Sums of weights are fp64 in a
 // fixed order, counts are integers: a token at a border of the running sum is
 // the one that the formula gives, up to 1e-13 of the sum, and the same on
-// every call.  A row of more than 40,960 logits is cut over the CTAs of a
-// cluster, which then each take a range of values out of all of their
-// histograms.
+// every call.  A row may be cut over the CTAs of a cluster, which then each take
+// a range of values out of all of their histograms.
 //
 // Bound: the logits are read once (from L1 or L2 a second time for the index);
-// what a row takes is the histogram's clearing, filling and scan.
+// what a row takes is latency: clearing the histogram (0.5 us), filling it (1.9 us
+// for 8192 logits), the weights of its values (2 to 5 us), the cuts by one warp (1.5
+// to 2 us each: fp64 exp and scans), and the barriers between them.
 #include "common.cuh"
 #include "gemm_tc.h"
 
 #include <cmath>
+#include <cstddef>
 
 namespace npub {
 namespace smp {
@@ -61,13 +63,10 @@ __device__ __forceinline__ double value_of(int bin) {
 
 // What the CTAs of a cluster tell one another.
 struct Mail {
-    double w;                   // this CTA's range of values: weight
-    double k_w, m_w, p_w;       // weight up to the cuts of top-k, min-p, top-p
-    uint32_t top;               // first bin in use
-    uint32_t n;                 // tokens of the range
-    uint32_t k_n, m_n, p_n;     // tokens up to the cuts
-    uint32_t min_bin;           // first bin of a weight below min_p
-    uint32_t pos, bin, rank;    // the sampled place in the order, its value, its number among the equal ones
+    double w[kOwners + 1];    // weight ahead of each thread's values, of the CTA's; their sum
+    uint32_t n[kOwners + 1];  // tokens, likewise
+    uint32_t top;             // first bin in use
+    uint32_t bin, rank;       // the sampled value, and its number among the equal ones
 };
 
 template <int C>
@@ -99,9 +98,6 @@ __device__ __forceinline__ uint4 ld_v4(uint32_t a) {
 }
 __device__ __forceinline__ void st_u32(uint32_t a, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
-}
-__device__ __forceinline__ void st_f64(uint32_t a, double v) {
-    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(a), "d"(v) : "memory");
 }
 
 // Counts of the 8 bins of a group over the cluster's histograms.
@@ -167,11 +163,40 @@ struct Hit {
     double y;
     int bin;
 };
-// By a warp: the first value in use, of a thread's range from group g0 on (n tokens and the weight w ahead of it), behind
-// which crossed(tokens, weight, bin) holds; the range's last one where it holds for none.
+// By a warp: the first value in use behind which crossed(tokens, weight, bin) holds (none ahead of one behind which it
+// does), or the last of the first thread's range behind which it does.  crossed is of running sums, so the search goes from
+// the CTA to the thread, 32 at a time, to its values; a sum's rounding may put it at a range's end.
 template <int C, typename F>
-__device__ __forceinline__ Hit locate(uint32_t hist, int g0, uint32_t n, double w, const Weights& wt, F crossed) {
+__device__ __noinline__ Hit locate(uint32_t hist, uint32_t mail_w, uint32_t mail_n, const Weights& wt, F crossed) {
     const int lane = threadIdx.x & 31;
+    constexpr int G = 8 / C, kAll = C * kOwners;
+    uint32_t n = 0;
+    double w = 0.0;
+    int cta = 0;
+#pragma unroll
+    for (int q = 0; q < C - 1; ++q) {
+        if (cta != q) continue;
+        const uint32_t an = n + ld_u32(addr_in<C>(mail_n + kOwners * 4u, q));
+        const double aw = w + ld_f64(addr_in<C>(mail_w + kOwners * 8u, q));
+        if (crossed(an, aw, (q + 1) * kOwners * G * 8 - 1)) continue;
+        n = an;
+        w = aw;
+        cta = q + 1;
+    }
+    int thread = 0;
+#pragma unroll
+    for (int step = 32; step >= 1; step /= 32) {
+        // the first lane's range of `step` threads behind which it holds
+        const int end = min(kOwners, thread + (lane + 1) * step);
+        const bool hit = end >= kOwners ||
+                         crossed(n + ld_u32(addr_in<C>(mail_n + (uint32_t)end * 4u, cta)),
+                                 w + ld_f64(addr_in<C>(mail_w + (uint32_t)end * 8u, cta)), (cta * kOwners + end) * G * 8 - 1);
+        thread += (__ffs(__ballot_sync(0xffffffffu, hit)) - 1) * step;
+    }
+    const int g0 = (cta * kOwners + thread) * G;
+    n += ld_u32(addr_in<C>(mail_n + (uint32_t)thread * 4u, cta));
+    w += ld_f64(addr_in<C>(mail_w + (uint32_t)thread * 8u, cta));
+    static_assert(kAll * G * 8 == kBins, "every bin has a thread");
     constexpr int kPer = C == 1 ? 2 : 1;  // bins per lane
     uint32_t c[kPer];
     double y[kPer];
@@ -219,6 +244,7 @@ __device__ __forceinline__ Hit locate(uint32_t hist, int g0, uint32_t n, double 
     }
     const uint32_t hits = __ballot_sync(0xffffffffu, hit), used = __ballot_sync(0xffffffffu, sn != 0);
     const int src = hits ? __ffs(hits) - 1 : 31 - __clz(used | 1u);
+    if (!used) h.c = 0, h.y = 0.0, h.bin = 0;
     h.n = __shfl_sync(0xffffffffu, h.n, src);
     h.w = __shfl_sync(0xffffffffu, h.w, src);
     h.c = __shfl_sync(0xffffffffu, h.c, src);
@@ -285,14 +311,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     auto at = [&](int q, const void* field) {
         return addr_in<C>(mb + (uint32_t)(reinterpret_cast<const char*>(field) - reinterpret_cast<const char*>(&mail)), q);
     };
-    auto tell_n = [&](uint32_t* field, uint32_t v) {
-#pragma unroll
-        for (int q = 0; q < C; ++q) st_u32(at(q, field), v);
-    };
-    auto tell_w = [&](double* field, double v) {
-#pragma unroll
-        for (int q = 0; q < C; ++q) st_f64(at(q, field), v);
-    };
     top = kNone;
 #pragma unroll
     for (int q = 0; q < C; ++q) top = min(top, ld_u32(at(q, &mail.top)));
@@ -318,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         uint32_t n = 0;
         double w = 0.0;
         if (tid < kOwners) {
-            double ratio = 0.0, begin = 0.0, r8 = 0.0;
+            double ratio = 0.0, begin = 0.0, r2 = 0.0, r4 = 0.0, r8 = 0.0;
             bool ready = false;
 #pragma unroll 1
             for (int j = 0; j < G; ++j) {
@@ -330,7 +348,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
                     ready = true;
                     // (between the second and third value: the first of bin 0's group is +inf)
                     ratio = top == 0 ? 0.0 : exp_of((value_of(g0 * 8 + 2) - value_of(g0 * 8 + 1)) * wt.inv_t);
-                    const double r2 = ratio * ratio, r4 = r2 * r2;
+                    r2 = ratio * ratio;
+                    r4 = r2 * r2;
                     r8 = r4 * r4;
                     begin = g0 > wt.top_bin >> 3 ? wt.at(g0 * 8) : 0.0;
                 }
@@ -352,27 +371,14 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
                     }
                     continue;
                 }
-                double s = double_of(c[7]);
+                // sum of c[e] ratio^e
+                double s[4];
 #pragma unroll
-                for (int e = 6; e >= 0; --e) s = fma(s, ratio, double_of(c[e]));
+                for (int e = 0; e < 4; ++e) s[e] = fma(double_of(c[2 * e + 1]), ratio, double_of(c[2 * e]));
+                w = fma(fma(fma(s[3], r2, s[2]), r4, fma(s[1], r2, s[0])), y, w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) n += c[e];
-                w += s * y;
             }
-        } else if (!greedy && mf > 0.0f) {  // the last warp: where the weights fall below min_p
-            int lo = (int)top, hi = kBins;  // first bin below is in (lo, hi]; the top's weight is 1
-            if (1.0 < (double)mf) {
-                hi = lo;
-            } else {
-                while (hi - lo > 1) {
-                    const int step = (hi - lo + 31) >> 5, bin = min(hi, lo + (lane + 1) * step);
-                    const uint32_t below = __ballot_sync(0xffffffffu, bin >= hi || wt.at(bin) < (double)mf);
-                    const int f = __ffs(below) - 1;  // lanes' bins ascend
-                    hi = min(hi, lo + (f + 1) * step);
-                    lo = lo + f * step;
-                }
-            }
-            if (lane == 0) mail.min_bin = (uint32_t)hi;
         }
         // ---- running sums over the threads
         const uint32_t ni = scan_up(n, lane);
@@ -384,139 +390,86 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         __syncthreads();
         const uint32_t pn = scan_up(part_n[lane], lane);
         const double pw = scan_up(part_w[lane], lane);
-        uint32_t N = __shfl_sync(0xffffffffu, pn, 31), cta_n = 0;
-        double W = __shfl_sync(0xffffffffu, pw, 31), cta_w = 0.0;
-        if (C > 1) {
-            if (tid == 0) {
-                mail.n = N;
-                mail.w = W;
-            }
-            sync_all<C>();
-            N = 0;
-            W = 0.0;
-#pragma unroll
-            for (int q = 0; q < C; ++q) {
-                if (q == rank) {
-                    cta_n = N;
-                    cta_w = W;
-                }
-                N += ld_u32(at(q, &mail.n));
-                W += ld_f64(at(q, &mail.w));
-            }
-        }
-        // [n0, n1) tokens and [w0, w1) of the running weight are this thread's.  w1 is the w0 of the thread behind, the same
-        // sum of the same terms, so that the threads' ranges leave no gap.
-        const uint32_t bn = warp ? __shfl_sync(0xffffffffu, pn, warp - 1) : 0;
-        const double up = __shfl_up_sync(0xffffffffu, wi, 1);
+        const uint32_t bn = __shfl_sync(0xffffffffu, pn - part_n[lane], warp);
         double bw = __shfl_sync(0xffffffffu, pw, max(warp - 1, 0));
         if (warp == 0) bw = 0.0;
-        const double ew = __shfl_sync(0xffffffffu, pw, warp);
-        const uint32_t n0 = cta_n + bn + ni - n, n1 = n0 + n;
-        const double w0 = cta_w + (lane ? bw + up : bw), w1 = cta_w + (lane == 31 ? ew : bw + wi);
-        // The warp whose lane `mine` holds a place looks at that lane's values.
-        auto find = [&](bool mine, auto crossed, auto then) {
-            const uint32_t vote = __ballot_sync(0xffffffffu, mine);
-            if (!vote) return;
-            const int l = __ffs(vote) - 1;
-            const Hit h = locate<C>(hb, __shfl_sync(0xffffffffu, g0, l), __shfl_sync(0xffffffffu, n0, l),
-                                    __shfl_sync(0xffffffffu, w0, l), wt, crossed);
-            if (lane == 0) then(h);
-        };
-        uint32_t keep = N;
-        double mass = W;
-        if (greedy) {
-            keep = 1;
-        } else {
-            const bool by_k = k > 0 && (uint32_t)k < N;
-            if (by_k || mf > 0.0f) {
-                if (mf > 0.0f && tid == 0) {  // no value below min_p: all are kept
-                    mail.m_n = N;
-                    mail.m_w = W;
+        const double up = __shfl_up_sync(0xffffffffu, wi, 1);
+        if (tid <= kOwners) {  // (the thread behind the last owner has the sums)
+            mail.n[tid] = bn + ni - n;
+            mail.w[tid] = lane ? bw + up : bw;
+        }
+        sync_all<C>();
+        // ---- the cuts, and the place: by one warp
+        if (rank == 0 && warp == 0) {
+            const uint32_t mn = mb + (uint32_t)offsetof(Mail, n), mw = mb + (uint32_t)offsetof(Mail, w);
+            uint32_t keep = 0;
+            double mass = 0.0;
+#pragma unroll
+            for (int q = 0; q < C; ++q) {
+                keep += ld_u32(addr_in<C>(mn + kOwners * 4u, q));
+                mass += ld_f64(addr_in<C>(mw + kOwners * 8u, q));
+            }
+            uint32_t m_keep = keep;
+            double m_mass = mass;
+            if (greedy) {
+                keep = 1;
+            } else {
+                if (k > 0 && (uint32_t)k < keep) {
+                    const Hit h = locate<C>(hb, mw, mn, wt, [=](uint32_t an, double, int) { return an >= (uint32_t)k; });
+                    keep = (uint32_t)k;
+                    mass = h.w + double_of((uint32_t)k - h.n) * h.y;
                 }
-                const uint32_t min_bin = mf > 0.0f ? mail.min_bin : kBins;
-                sync_all<C>();
-                if (by_k)
-                    find(n && n0 < (uint32_t)k && (uint32_t)k <= n1,
-                         [&](uint32_t an, double, int) { return an >= (uint32_t)k; },
-                         [&](const Hit& h) {
-                             tell_n(&mail.k_n, (uint32_t)k);
-                             tell_w(&mail.k_w, h.w + double_of((uint32_t)k - h.n) * h.y);
-                         });
-                if (mf > 0.0f && min_bin < (uint32_t)kBins) {
-                    // the values ahead of min_bin: those ahead of the thread that holds it, and its own up to it
-                    const bool mine = tid < kOwners && min_bin >= (uint32_t)(g0 * 8) && min_bin < (uint32_t)((g0 + G) * 8);
-                    find(mine && n, [&](uint32_t, double, int bin) { return (uint32_t)bin >= min_bin; },
-                         [&](const Hit& h) {
-                             const bool ahead = (uint32_t)h.bin < min_bin;  // all of the range's are
-                             tell_n(&mail.m_n, ahead ? h.n + h.c : h.n);
-                             tell_w(&mail.m_w, ahead ? h.w + double_of(h.c) * h.y : h.w);
-                         });
-                    if (mine && !n) {
-                        tell_n(&mail.m_n, n0);
-                        tell_w(&mail.m_w, w0);
+                if (mf > 0.0f) {
+                    // the first bin whose weight is below min_p, in (lo, hi]; the top's is 1
+                    int lo = (int)top, hi = kBins;
+                    if (1.0 < (double)mf) hi = lo;
+                    while (hi - lo > 1) {
+                        const int step = (hi - lo + 31) >> 5, bin = min(hi, lo + (lane + 1) * step);
+                        const bool below = bin >= hi || wt.at(bin) < (double)mf;
+                        const int f = __ffs(__ballot_sync(0xffffffffu, below)) - 1;  // the lanes' bins ascend
+                        hi = min(hi, lo + (f + 1) * step);
+                        lo += f * step;
+                    }
+                    if (hi < kBins) {
+                        const Hit h = locate<C>(hb, mw, mn, wt, [=](uint32_t, double, int bin) { return bin >= hi; });
+                        const bool ahead = h.c && h.bin < hi;  // none of the thread's values is behind the cut
+                        m_keep = ahead ? h.n + h.c : h.n;
+                        m_mass = ahead ? h.w + double_of(h.c) * h.y : h.w;
                     }
                 }
-                sync_all<C>();
-                if (by_k) {
-                    keep = mail.k_n;
-                    mass = mail.k_w;
+                if (pf < 1.0f) {
+                    const double goal = fmax((double)pf, 0.0) * mass;
+                    const Hit h = locate<C>(hb, mw, mn, wt, [=](uint32_t an, double aw, int) { return an > 0 && aw >= goal; });
+                    const double r = goal > 0.0 ? fmin(fmax(ceil((goal - h.w) / h.y), 1.0), double_of(h.c)) : 1.0;
+                    const uint32_t cn = h.n + (uint32_t)r;
+                    if (cn < keep) {
+                        keep = cn;
+                        mass = h.w + r * h.y;
+                    }
+                }
+                if (m_keep < keep) {
+                    keep = m_keep;
+                    mass = m_mass;
                 }
             }
-            const uint32_t m_keep = mf > 0.0f ? mail.m_n : N;
-            const double m_mass = mf > 0.0f ? mail.m_w : W;
-            if (pf < 1.0f) {
-                const double goal = fmax((double)pf, 0.0) * mass;
-                if (tid == 0) {
-                    mail.p_n = keep;
-                    mail.p_w = mass;
-                }
-                sync_all<C>();
-                find(goal <= 0.0 ? n && n0 == 0 : n && w0 < goal && goal <= w1,
-                     [&](uint32_t, double aw, int) { return aw >= goal; },
-                     [&](const Hit& h) {
-                         const double r = goal > 0.0 ? fmin(fmax(ceil((goal - h.w) / h.y), 1.0), double_of(h.c)) : 1.0;
-                         const uint32_t cn = h.n + (uint32_t)r;
-                         if (cn < keep) {
-                             tell_n(&mail.p_n, cn);
-                             tell_w(&mail.p_w, h.w + r * h.y);
-                         }
-                     });
-                sync_all<C>();
-                keep = mail.p_n;
-                mass = mail.p_w;
+            if (keep == 0) keep = 1;  // min_p above 1
+            uint32_t pos = 0;
+            Hit h;
+            const double goal = keep > 1 ? u * mass : 0.0;
+            if (goal > 0.0) {
+                h = locate<C>(hb, mw, mn, wt, [=](uint32_t, double aw, int) { return aw > goal; });
+                pos = h.n + (h.c ? (uint32_t)fmin(fmax(floor((goal - h.w) / h.y), 0.0), double_of(h.c - 1)) : 0);
             }
-            if (m_keep < keep) {
-                keep = m_keep;
-                mass = m_mass;
+            if (!(goal > 0.0) || pos >= keep || !h.c) {  // the first; u of 1 or more, or a sum's rounding
+                pos = min(pos, keep - 1);
+                h = locate<C>(hb, mw, mn, wt, [=](uint32_t an, double, int) { return an > pos; });
+            }
+            if (lane < C) {
+                st_u32(at(lane, &mail.bin), (uint32_t)h.bin);
+                st_u32(at(lane, &mail.rank), pos - h.n);
             }
         }
-        if (keep == 0) keep = 1;  // min_p above 1
-        // ---- the place in the order, and its value
-        const double goal = keep > 1 ? u * mass : 0.0;
-        if (tid == 0) mail.pos = keep > 1 && goal > 0.0 ? 0xffffffffu : 0;
-        if (tid == 0) mail.rank = 0xffffffffu;
         sync_all<C>();
-        auto tell_place = [&](uint32_t pos, const Hit& h) {
-            tell_n(&mail.pos, pos);
-            tell_n(&mail.bin, (uint32_t)h.bin);
-            tell_n(&mail.rank, pos - h.n);
-        };
-        if (keep > 1 && goal > 0.0)
-            find(n && w0 <= goal && goal < w1, [&](uint32_t, double aw, int) { return aw > goal; },
-                 [&](const Hit& h) {
-                     const double r = fmin(fmax(floor((goal - h.w) / h.y), 0.0), double_of(h.c - 1));
-                     tell_place(h.n + (uint32_t)r, h);
-                 });
-        else
-            find(n && n0 == 0, [&](uint32_t an, double, int) { return an > 0; }, [&](const Hit& h) { tell_place(0, h); });
-        sync_all<C>();
-        if (mail.pos >= keep) {  // u of 1 or more, or a border: the last one kept
-            const uint32_t pos = keep - 1;
-            sync_all<C>();
-            find(n && n0 <= pos && pos < n1, [&](uint32_t an, double, int) { return an > pos; },
-                 [&](const Hit& h) { tell_place(pos, h); });
-            sync_all<C>();
-        }
         // ---- the rank-th token of that value, by index
         const uint32_t bin = mail.bin;
         uint32_t r = mail.rank;
@@ -535,13 +488,17 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         if (here && r < mine) {
             // matches of every warp in every step of the segment, then the step and warp that hold the r-th, then its place
             const int steps = (i1 - i0 + kThreads * 8 - 1) / (kThreads * 8);
+            const uint32_t one = bin <= (uint32_t)kZero ? kZero - bin : 0x8000u | (bin - kZero);
+            const uint32_t wanted = one | one << 16, mask = one ? 0xffffffffu : 0x7fff7fffu;  // both zeros
             auto matches = [&](int s, int at_warp) {
                 const uint4 v = load8(x, i0 + (s * kThreads + at_warp * 32 + lane) * 8, i1, a.vec);
                 const uint32_t h[4] = {v.x, v.y, v.z, v.w};
                 uint32_t m = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    m |= (uint32_t)(bin_of((e & 1) ? h[e >> 1] >> 16 : h[e >> 1] & 0xffffu) == bin) << e;
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t eq = __vcmpeq2(h[e] & mask, wanted);
+                    m |= ((eq & 1u) | (eq >> 30 & 2u)) << (2 * e);
+                }
                 return m;
             };
             for (int s = 0; s < steps; ++s) {
@@ -623,19 +580,21 @@ extern "C" int npub_sample(const void* logits, int64_t ldl, int rows, int vocab,
     a.m = min_p;
     a.m0 = min_p_all;
     a.ids = ids;
-    // CTAs of a row: waves of one CTA per SM, each about 8 us and 1 us for 8192 logits, 2 us for a cluster's barriers
-    int c = 0;
+    // CTAs of a row.  Measured, one CTA per SM: 11, 14, 15 and 16.5 us with 1, 2, 4 and 8 of them and 1.9 us for every 8192
+    // logits of a CTA (32000: 18.4 us alone, 17.6 in two; 128256: 29, 22.6 and 20.1 in 2, 4 and 8; 64 rows of it 29, 49 and 95).
+    // Of clusters of 4 and 8 not quite all SMs hold one.
+    static const double start[4] = {11.0, 14.0, 15.0, 16.5};
+    int c = 8;
     double best = 1e30;
-    for (int i = 1; i <= 8; i *= 2) {
-        if ((vocab + i - 1) / i > kMaxSegment - 8) continue;
-        const int64_t waves = ((int64_t)rows * i + num_sms() - 1) / num_sms();
-        const double us = (double)waves * (8.0 + (double)vocab / i / 8192.0 + (i > 1 ? 2.0 : 0.0));
+    for (int i = 0; i < 4; ++i) {
+        const int n = 1 << i, at_once = num_sms() / n > 4 ? num_sms() / n - (i > 1 ? 3 : 0) : 1;
+        if ((vocab + n - 1) / n > kMaxSegment - 8) continue;
+        const double us = (double)((rows + at_once - 1) / at_once) * (start[i] + 1.9 * vocab / n / 8192.0);
         if (us < best) {
             best = us;
-            c = i;
+            c = n;
         }
     }
-    if (c == 0) c = 8;
     a.seg = ((vocab + c - 1) / c + 7) / 8 * 8;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (c) {
