@@ -20,8 +20,6 @@
 #include "common.cuh"
 #include "gemm_tc.h"
 
-#include <mutex>
-
 namespace npub {
 namespace w8a8 {
 
@@ -108,7 +106,8 @@ constexpr int kTileThreads = 256;
 struct TileSmem {
     static constexpr int kOp = 128 * BK;  // a CTA's half of either operand's tile
     static constexpr int kOffBar = kTileStages * 2 * kOp;
-    static constexpr int kTotal = kOffBar + 256 + 1024;
+    static constexpr int kOffOut = kOffBar + 256;  // epilogue warps: 32 x 32 sums, rows of 33 words
+    static constexpr int kTotal = kOffOut + 4 * 32 * 33 * 4 + 1024;
 };
 
 // Tiles in bands of p.band token tiles, the channels in turn within a band, so
@@ -251,8 +250,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
                 if (n0 >= p.N) break;
                 int acc[32];
                 tmem_ld32(tmem + ((uint32_t)(wq * 32) << 16) + b * 256u + (uint32_t)c0, acc);
-                if (!row) continue;
                 if (p.vec && n0 + 32 <= p.N) {
+                    if (!row) continue;
                     float z[32];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -300,23 +299,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
                                             pack_h2(z[e * 8 + 4], z[e * 8 + 5]), pack_h2(z[e * 8 + 6], z[e * 8 + 7]));
                     continue;
                 }
+// rows that 16 bytes at a time do not fit: through shared memory, so that the lanes store along a row
+                int* out = reinterpret_cast<int*>(smem + L::kOffOut) + wq * 32 * 33;
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    if (n0 + i >= p.N) break;
-                    const bool two = n0 + i + 1 < p.N;
-                    float z0 = (float)acc[i] * (sa * __half2float(p.sw[n0 + i]));
-                    float z1 = two ? (float)acc[i + 1] * (sa * __half2float(p.sw[n0 + i + 1])) : 0.0f;
-                    if (p.swiglu) {
-                        p.C[(int64_t)m * p.ldc + (n0 + i) / 2] = __float2half_rn(swiglu_f(z0, z1));
-                        continue;
+                for (int i = 0; i < 32; ++i) out[lane * 33 + i] = acc[i];
+                __syncwarp();
+                const int rows = min(32, p.M - (m - lane));
+                const int per = p.swiglu ? 2 : 1, n = n0 + lane * per;  // this lane's column, or the first of its two
+                const bool on = lane * per < 32 && n < p.N;
+                const float sw0 = on ? __half2float(__ldg(p.sw + n)) : 0.0f;
+                const float sw1 = on && p.swiglu ? __half2float(__ldg(p.sw + n + 1)) : 0.0f;
+                const __half* res = p.R ? p.R + (int64_t)(m - lane) * p.ldr + n : nullptr;
+                __half* dst = p.C + (int64_t)(m - lane) * p.ldc + n / per;
+                for (int q0 = 0; q0 < rows; q0 += 8) {
+                    float z[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const float sq = __shfl_sync(0xffffffffu, sa, q0 + q);
+                        const int* v = out + (q0 + q) * 33 + (lane * per & 31);
+                        z[q] = (float)v[0] * (sq * sw0);
+                        if (p.swiglu) z[q] = swiglu_f(z[q], (float)v[1] * (sq * sw1));
+                        if (res && on && q0 + q < rows) z[q] += __half2float(res[(int64_t)(q0 + q) * p.ldr]);
                     }
-                    if (p.R) {
-                        z0 += __half2float(p.R[(int64_t)m * p.ldr + n0 + i]);
-                        if (two) z1 += __half2float(p.R[(int64_t)m * p.ldr + n0 + i + 1]);
-                    }
-                    p.C[(int64_t)m * p.ldc + n0 + i] = __float2half_rn(z0);
-                    if (two) p.C[(int64_t)m * p.ldc + n0 + i + 1] = __float2half_rn(z1);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        if (on && q0 + q < rows) dst[(int64_t)(q0 + q) * p.ldc] = __float2half_rn(z[q]);
                 }
+                __syncwarp();
             }
             tc_fence_before();
             __syncwarp();
@@ -340,10 +349,9 @@ constexpr int kFewThreads = 192;
 template <int BT>
 struct FewSmem {
     static constexpr int kW = 128 * BK, kX = BT * BK;
-    static constexpr int kStages = BT >= 256 ? 4 : BT >= 128 ? 3 : BT >= 64 ? 4 : 5;
+    static constexpr int kStages = BT >= 128 ? 3 : BT >= 64 ? 4 : 5;
     static constexpr int kOffBar = kStages * (kW + kX);
     static constexpr int kTotal = kOffBar + 256 + 1024;
-    static constexpr int kCols = BT < 32 ? 32 : BT;  // tensor memory columns
     static_assert(BT * 128 * 4 <= kOffBar, "the sums reuse the ring");
 };
 
@@ -382,7 +390,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
         for (int i = 0; i < min(nk, L::kStages); ++i) tma_prefetch_3d(&p.tmW, (kt0 + i) * BK, n0, 0);
     }
     if (warp == 5) {
-        tmem_alloc(tmem_slot, L::kCols);
+        tmem_alloc(tmem_slot, BT);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -455,7 +463,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
     else cta_sync_divergent();
     if (warp == 5) {
         tc_fence_after();
-        tmem_dealloc(tmem, L::kCols);
+        tmem_dealloc(tmem, BT);
     }
     if (warp < 4) {
         const int tokens = min(BT, p.M - m0);
@@ -527,30 +535,36 @@ struct Choice {
     int splits;
 };
 
-int few_bt(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256; }
-
-// CTAs of the few-token kernel that an SM holds (shared memory).
-int few_per_sm(int bt) { return bt >= 256 ? 1 : 2; }
-
+// The estimates' terms, in us, are fitted to CUDA graphs of calls of 1 to 777 tokens (at 12288 x 4096, tile kernel 21 for up
+// to 256 tokens and 31 for 512; few-token kernel with one and two CTAs for a tile, 32 tokens 15.4 and 14.2, 64 in one tile
+// 19.5 and 16.7, 128 in two 20.5 and 26.6; 4096 x 4096 at 32 tokens with 1, 2, 4, 8: 12.6, 9.5, 7.7, 7.7).
 Choice pick(int M, int N, int k_tiles) {
+    // clusters of 1 .. 8 CTAs that 148 SMs (whole GPCs of them) hold at one CTA per SM; the few-token kernel has two
+    static const int held[kMaxCluster + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
     const int sms = num_sms();
     Choice c = {0, 1};
-    double best = 1e30;
-    // In units of one K tile of a CTA.  Tile kernel: whole waves of pairs.
-    if (M > 64) {
-        const int64_t tiles = (int64_t)((M + 255) / 256) * ((N + 255) / 256), pairs = sms / 2;
-        best = (double)((tiles + pairs - 1) / pairs) * k_tiles + 8.0;
-    }
-    for (int bt = few_bt(M); bt >= (M > 64 ? 128 : few_bt(M)); bt /= 2) {
-        const int64_t tiles = (int64_t)((N + 127) / 128) * ((M + bt - 1) / bt);
-        const int64_t slots = (int64_t)sms * few_per_sm(bt);
+    const int64_t big = (int64_t)((M + 255) / 256) * ((N + 255) / 256), pairs = sms / 2;
+    double best = 7.5 + 0.003 * (M < 1024 ? M : 1024) + (double)((big + pairs - 1) / pairs) * k_tiles * (0.3 + 0.13 * (big < 48 ? (double)big / 48.0 : 1.0));
+    for (int bt = 32; bt <= 128; bt *= 2) {
+        const int64_t token_tiles = (M + bt - 1) / bt, tiles = (int64_t)((N + 127) / 128) * token_tiles;
+        if (token_tiles > 8) continue;
+        const int stages = bt == 32 ? FewSmem<32>::kStages : bt == 64 ? FewSmem<64>::kStages : FewSmem<128>::kStages;
         for (int s = 1; s <= kMaxCluster && s <= k_tiles; ++s) {
-            const int per = (k_tiles + s - 1) / s, real = (k_tiles + per - 1) / per;
-            const double unit = bt >= 256 ? 1.2 : bt >= 128 ? 1.0 : 0.8;
-            const double t = (double)((tiles * real + slots - 1) / slots) * (per * unit + 6.0) + (real > 1 ? 4.0 : 0.0);
-            if (t < best) {
-                best = t;
-                c = Choice{bt, real};
+            const int per = (k_tiles + s - 1) / s;
+            if ((k_tiles + per - 1) / per != s) continue;
+            int64_t at_once = 2 * (int64_t)held[s] * sms / 148;
+            if (at_once < 1) at_once = 1;
+            const double waves = (double)((tiles + at_once - 1) / at_once), ctas = (double)(tiles < at_once ? tiles : at_once) * s;
+            // a K tile: a ring's latency, which grows with the weights in flight, HBM's rate, or the SM's tensor core
+            const double bytes = ctas / (double)token_tiles * 16384.0;
+            double unit = (1.0 + 0.45 * bytes / 1.57e6) / stages;
+            if (unit < bytes / 6.5e6) unit = bytes / 6.5e6;
+            const double mma = (bt < 128 ? 0.13 : 0.17) * (ctas > sms ? ctas / sms : 1.0);
+            if (unit < mma) unit = mma;
+            const double us = 4.6 + 0.004 * M + waves * (per * unit + 1.0 + bt / 51.0) + (s > 1 ? 0.5 + 0.12 * s : 0.0);
+            if (us < best) {
+                best = us;
+                c = Choice{bt, s};
             }
         }
     }
@@ -583,33 +597,6 @@ int launch_few(Params& p, int splits, cudaStream_t st) {
     return npub_internal_launch_status();
 }
 
-int max_pairs() {
-    static std::mutex mu;
-    static int known[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return num_sms() / 2;
-    std::lock_guard<std::mutex> lk(mu);
-    if (known[dev] > 0) return known[dev];
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * 256);
-    cfg.blockDim = dim3(kTileThreads);
-    cfg.dynamicSmemBytes = TileSmem::kTotal;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, w8a8_tile_kernel, &cfg) != cudaSuccess || n <= 0) {
-        cudaGetLastError();
-        n = num_sms() / 2;
-    }
-    known[dev] = n;
-    return n;
-}
-
 int launch_tile(Params& p, cudaStream_t st) {
     static_assert(TileSmem::kTotal <= 232448, "shared memory budget");
     NPUB_CUDA_TRY(cudaFuncSetAttribute(w8a8_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem::kTotal));
@@ -618,7 +605,7 @@ int launch_tile(Params& p, cudaStream_t st) {
     p.band = 8;
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
     if (tiles > 0x3fffffff) return NPUB_ERR_UNSUPPORTED;
-    const int pairs = max_pairs();
+    const int pairs = num_sms() / 2;
     return launch_pdl(w8a8_tile_kernel, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), dim3(kTileThreads),
                       TileSmem::kTotal, st, p);
 }
@@ -662,11 +649,9 @@ extern "C" int npub_w8a8_gemm(const int8_t* A, int64_t lda, const float* a_scale
     if (rc) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (c.bt) {
-        case 16: return launch_few<16>(p, c.splits, st);
         case 32: return launch_few<32>(p, c.splits, st);
         case 64: return launch_few<64>(p, c.splits, st);
         case 128: return launch_few<128>(p, c.splits, st);
-        case 256: return launch_few<256>(p, c.splits, st);
         default: return launch_tile(p, st);
     }
 }
