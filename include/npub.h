@@ -444,6 +444,8 @@ size_t npub_attention_paged_decode_workspace(int batch, int64_t ctx_len, int sha
  * makes the scale NaN until the page is begun anew.  Sequences that write to
  * the same page in one call leave it undefined.  head_dim <= 128 (a multiple of
  * 16), page_size 16 .. 256; otherwise the arguments of npub_rope_paged_append.
+ * With cu_seqlens (packed != 0 of the query) a workspace is needed, 256-byte
+ * aligned.
  *
  * npub_attention_paged_q8 / npub_attention_paged_decode_q8: the attention of
  * npub_attention_paged / npub_attention_paged_decode over such pages (scale >=
@@ -460,7 +462,9 @@ int npub_rope_paged_append_q8(const void* qkv, int64_t ldx, void* q_out, int64_t
                               const float* inv_freq, const void* q_gamma, const void* k_gamma, float eps,
                               int8_t* k_pages, int8_t* v_pages, float* k_scales, float* v_scales, int n_pages,
                               int page_size, const int32_t* page_table, int64_t ldt, int max_pages,
-                              const int32_t* cu_seqlens, int batch, void* stream);
+                              const int32_t* cu_seqlens, int batch, void* workspace, size_t workspace_bytes,
+                              void* stream);
+size_t npub_rope_paged_append_q8_workspace(int tokens, int rot_dim, int packed);
 int npub_attention_paged_q8(const void* q, int64_t ldq, const int8_t* k_pages, const int8_t* v_pages,
                             const float* k_scales, const float* v_scales, int n_pages, int page_size,
                             const int32_t* page_table, int64_t ldt, int max_pages, const int32_t* lens,

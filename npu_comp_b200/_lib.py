@@ -81,7 +81,8 @@ SIGNATURES = {
                                          _f, _p, _sz, _p]),
     "npub_attention_paged_decode_workspace": (_sz, [_i, _i64, _i, _i, _i, _i]),
     "npub_rope_paged_append_q8": (_i, [_p, _i64, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _f, _p, _p, _p, _p,
-                                       _i, _i, _p, _i64, _i, _p, _i, _p]),
+                                       _i, _i, _p, _i64, _i, _p, _i, _p, _sz, _p]),
+    "npub_rope_paged_append_q8_workspace": (_sz, [_i, _i, _i]),
     "npub_attention_paged_q8": (_i, [_p, _i64, _p, _p, _p, _p, _i, _i, _p, _i64, _i, _p, _p, _i, _i, _i, _i, _p, _i64, _i,
                                      _i, _i, _f, _i, _p, _sz, _p]),
     "npub_attention_paged_q8_workspace": (_sz, [_i, _i, _i, _i64, _i, _i, _i]),

@@ -91,6 +91,7 @@ extern "C" int npub_rope_paged_append(const void* qkv, int64_t ldx, void* q_out,
     a.max_pages = max_pages;
     a.cu = cu_seqlens;
     a.batch = batch;
+    a.turns = nullptr;
     const int total = (((q_heads + 2 * kv_heads) << a.units_log2) + 31) & ~31;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     // few tokens: blocks over the heads too, one unit per thread

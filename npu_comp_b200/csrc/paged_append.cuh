@@ -29,6 +29,7 @@ struct AppendArgs {
     int max_pages;
     const int32_t* cu;
     int batch;
+    float2* turns;  // when set: (cos, sin) of every token's pairs [tokens, half], for another kernel
 };
 
 // Eight fp16 as four pairs of fp32, and back.
@@ -110,6 +111,7 @@ __device__ __forceinline__ void append_token(const AppendArgs& a, int t, int y, 
                 float* w = reinterpret_cast<float*>(&turn[((k & 7) >> 1) * rot_units + (k >> 3)]) + (k & 1);
                 w[0] = c;
                 w[2] = s;
+                if (a.turns) a.turns[(int64_t)t * a.half + k] = make_float2(c, s);
             }
             if ((threadIdx.x >> 5) == kAppThreads / 32 - 1) {  // the last warp has the fewest angles
                 const int seq = a.cu ? seq_of_row(a.cu, a.batch, t) : t;

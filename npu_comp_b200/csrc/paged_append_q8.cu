@@ -55,6 +55,12 @@ __device__ __forceinline__ void angle(const AppendArgs& a, int p, int k, float& 
     sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
 }
 
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+    const float x = a;
+    a = x * c - b * s;
+    b = b * c + x * s;
+}
+
 // Row t's head (its first column x), by a warp: normalised by g, rotated by the angles of position p.
 __device__ __forceinline__ void head_row(const AppendArgs& a, const __half* x, const Cols& c, const __half* g, int p,
                                          float (&y)[4]) {
@@ -86,17 +92,12 @@ __device__ __forceinline__ void head_row(const AppendArgs& a, const __half* x, c
         float c0, s0, c1, s1;
         angle(a, p, c.pair, c0, s0);
         angle(a, p, c.pair + 1, c1, s1);
-        const float a0 = y[0], a1 = y[1], b0 = y[2], b1 = y[3];
-        if (a.interleaved) {  // pairs (a0, a1) and (b0, b1)
-            y[0] = a0 * c0 - a1 * s0;
-            y[1] = a1 * c0 + a0 * s0;
-            y[2] = b0 * c1 - b1 * s1;
-            y[3] = b1 * c1 + b0 * s1;
-        } else {  // pairs (a0, b0) and (a1, b1)
-            y[0] = a0 * c0 - b0 * s0;
-            y[1] = a1 * c1 - b1 * s1;
-            y[2] = b0 * c0 + a0 * s0;
-            y[3] = b1 * c1 + a1 * s1;
+        if (a.interleaved) {
+            turn(y[0], y[1], c0, s0);
+            turn(y[2], y[3], c1, s1);
+        } else {
+            turn(y[0], y[2], c0, s0);
+            turn(y[1], y[3], c1, s1);
         }
     }
 }
@@ -122,8 +123,10 @@ __device__ __forceinline__ Step step_of(float before, uint32_t top) {
     s.old = s.scale > before && s.scale > 1e-37f ? before / s.scale : 1.0f;
     return s;
 }
-__device__ __forceinline__ uint32_t q8(float y, float inv) {
-    return (uint32_t)(int)fminf(fmaxf(rintf(y * inv), -127.0f), 127.0f) & 0xffu;
+// round(y / s') in the low byte: |y inv| is at most 127 (1 + 2^-22), and adding 1.5 * 2^23 rounds it, halves to even.
+__device__ __forceinline__ uint32_t q8(float y, float inv) { return __float_as_uint(fmaf(y, inv, 12582912.0f)); }
+__device__ __forceinline__ uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 __device__ __forceinline__ uint32_t rescaled(uint32_t w, float f) {
     uint32_t r = 0;
@@ -172,8 +175,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32) append_decode_q8_kernel(con
     const Step s = step_of(before, __reduce_max_sync(0xffffffffu, max_bits(y)));
     if (c.on) {
         int8_t* dst = rows + (int64_t)slot * a.hd;
-        *reinterpret_cast<uint16_t*>(dst + c.ca) = (uint16_t)(q8(y[0], s.inv) | q8(y[1], s.inv) << 8);
-        *reinterpret_cast<uint16_t*>(dst + c.cb) = (uint16_t)(q8(y[2], s.inv) | q8(y[3], s.inv) << 8);
+        const uint32_t w = bytes4(q8(y[0], s.inv), q8(y[1], s.inv), q8(y[2], s.inv), q8(y[3], s.inv));
+        *reinterpret_cast<uint16_t*>(dst + c.ca) = (uint16_t)w;
+        *reinterpret_cast<uint16_t*>(dst + c.cb) = (uint16_t)(w >> 16);
     }
     if (s.old != 1.0f) {
         uint4* w = reinterpret_cast<uint4*>(rows);
@@ -187,34 +191,44 @@ __global__ void __launch_bounds__(kDecodeWarps * 32) append_decode_q8_kernel(con
 }
 
 // ------------------------------------------------------------------ packed rows
-// Blocks of windows first: (window of p.window packed rows, k or v head); each
-// takes the pages whose first new row lies in its window, one after the other,
-// all of a page's rows at once (in shared memory in fp32 between the maximum and
-// the store).  Then one block per token for its query heads.
-__global__ void __launch_bounds__(kAppThreads) append_packed_q8_kernel(const Q8Args p) {
+// One block per token for its query heads, in a launch of their own: they are
+// three quarters of the bytes, and need neither the registers nor the shared
+// memory of the others.  They leave the angles for the k heads, which would form
+// them once for each head and page.
+__global__ void __launch_bounds__(kAppThreads) append_query_kernel(const AppendArgs a) {
     pdl_trigger();
-    extern __shared__ __align__(16) float ys[];  // [page_size][hd + 4]
-    __shared__ uint32_t part[kAppThreads / 32];
+    pdl_wait();
+    append_token(a, blockIdx.x, 0, 1);
+}
+
+// Blocks of (window of p.window packed rows, k or v head): each takes the pages
+// whose first new row lies in its window, one after the other.  A thread holds
+// one 16-element unit (as in append_token) of up to kUnits rows of the page in
+// registers, so that all of a page's loads are in flight at once and its rows
+// stay there between the maximum and the store.
+constexpr int kUnits = 4;
+constexpr int kMaxPackedThreads = 512;  // 256 rows of 8 units
+__global__ void __launch_bounds__(kMaxPackedThreads, 1) append_packed_q8_kernel(const Q8Args p) {
+    pdl_trigger();
+    __shared__ uint32_t part[kMaxPackedThreads / 32];
     pdl_wait();
     const AppendArgs& a = p.q;
     const int heads = 2 * p.hk;
-    const int page_blocks = p.windows * heads;
-    if ((int)blockIdx.x >= page_blocks) {
-        append_token(a, (int)blockIdx.x - page_blocks, 0, 1);
-        return;
-    }
     const int win = (int)blockIdx.x / heads, head = (int)blockIdx.x - win * heads;
     const bool isv = head >= p.hk;
     const int kvh = isv ? head - p.hk : head;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int ps = 1 << a.page_shift, ld = a.hd + 4;
-    const Cols c = lane_cols(a, !isv);
-    const __half* g = isv ? nullptr : a.gk;
+    const int threads = (int)blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int ps = 1 << a.page_shift;
+    // this thread's unit: two 8-element chunks, the halves of a rotated pair or neighbours
+    const int u = threadIdx.x & (a.units_p2 - 1), row_of = threadIdx.x >> a.units_log2, stride = threads >> a.units_log2;
+    const bool act = u < a.units, turns = !isv && u < a.half >> 3, split = turns && !a.interleaved;
+    const int c0 = split ? u * 8 : u * 16, c1 = split ? c0 + a.half : c0 + 8;
+    const bool norm = !isv && a.gk;
     const int row_end = min(p.rows, (win + 1) * p.window);
     for (int t0 = win * p.window; t0 < row_end; t0 += 32) {
         // the page that starts with row t0 + lane: its sequence, first slot, rows
         const int t = t0 + lane;
-        int page = -1, slot = 0, n = 0, pos = 0;
+        int page = -1, slot = 0, n = 0;
         if (t < row_end && t >= __ldg(a.cu) && t < __ldg(a.cu + a.batch)) {
             int lo = 0, hi = a.batch;  // the first sequence that ends behind t
             while (lo < hi) {
@@ -243,47 +257,93 @@ __global__ void __launch_bounds__(kAppThreads) append_packed_q8_kernel(const Q8A
             float* scale = (isv ? p.vs : p.ks) + at;
             int8_t* dst = (isv ? p.vp : p.kp) + (at << a.page_shift) * a.hd;
             const float before = sl ? *scale : 0.0f;
-            uint32_t top = 0;
             const __half* x = a.x + (int64_t)row0 * a.ldx + (int64_t)(a.hq + head) * a.hd;
-            for (int r = warp; r < rows; r += kAppThreads / 32) {
-                pos = isv ? 0 : __ldg(a.pos + row0 + r);
-                float y[4];
-                head_row(a, x + (int64_t)r * a.ldx, c, g, pos, y);
-                top = max(top, max_bits(y));
-                if (c.on) {
-                    *reinterpret_cast<float2*>(ys + r * ld + c.ca) = make_float2(y[0], y[1]);
-                    *reinterpret_cast<float2*>(ys + r * ld + c.cb) = make_float2(y[2], y[3]);
+            uint4 raw[kUnits][2];
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int r = row_of + i * stride;
+                raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+                if (act && r < rows) {
+                    raw[i][0] = *reinterpret_cast<const uint4*>(x + (int64_t)r * a.ldx + c0);
+                    raw[i][1] = *reinterpret_cast<const uint4*>(x + (int64_t)r * a.ldx + c1);
+                }
+            }
+            float y[kUnits][16];
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int r = row_of + i * stride;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float2 f = __half22float2(reinterpret_cast<const __half2*>(&raw[i][e >> 2])[e & 3]);
+                    y[i][2 * e] = f.x;
+                    y[i][2 * e + 1] = f.y;
+                }
+                if (norm) {
+                    float ss = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) ss = fmaf(y[i][e], y[i][e], ss);
+                    for (int m = a.units_p2 >> 1; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+                    const float inv = rsqrtf(ss * a.inv_hd + a.eps);
+                    uint4 g[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+                    if (act) {
+                        g[0] = __ldg(reinterpret_cast<const uint4*>(a.gk + c0));
+                        g[1] = __ldg(reinterpret_cast<const uint4*>(a.gk + c1));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 f = __half22float2(reinterpret_cast<const __half2*>(&g[e >> 2])[e & 3]);
+                        y[i][2 * e] *= inv * f.x;
+                        y[i][2 * e + 1] *= inv * f.y;
+                    }
+                }
+                if (turns && r < rows) {  // pairs (e, e + 8), or (2 e, 2 e + 1), by the angles of the token's pairs 8 u + e
+                    const float4* w = reinterpret_cast<const float4*>(a.turns + (int64_t)(row0 + r) * a.half + u * 8);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float4 cs = *(w + e);
+                        if (split) {
+                            turn(y[i][2 * e], y[i][2 * e + 8], cs.x, cs.y);
+                            turn(y[i][2 * e + 1], y[i][2 * e + 9], cs.z, cs.w);
+                        } else {
+                            turn(y[i][4 * e], y[i][4 * e + 1], cs.x, cs.y);
+                            turn(y[i][4 * e + 2], y[i][4 * e + 3], cs.z, cs.w);
+                        }
+                    }
+                }
+                if (act && r < rows) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(y[i][e]) & 0x7fffffffu);
                 }
             }
             top = __reduce_max_sync(0xffffffffu, top);
             if (lane == 0) part[warp] = top;
             __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kAppThreads / 32; ++w) top = max(top, part[w]);
+            for (int w = 0; w < threads >> 5; ++w) top = max(top, part[w]);
             const Step s = step_of(before, top);
-            const int units = a.hd / 16;  // 16 columns per thread and step
-            uint4* out = reinterpret_cast<uint4*>(dst + (int64_t)sl * a.hd);
-            for (int i = threadIdx.x; i < rows * units; i += kAppThreads) {
-                const int r = i / units;
-                const float4* y = reinterpret_cast<const float4*>(ys + r * ld + (i - r * units) * 16);
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const int r = row_of + i * stride;
+                if (!act || r >= rows) continue;
                 uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float4 v = y[e];
-                    w[e] = q8(v.x, s.inv) | q8(v.y, s.inv) << 8 | q8(v.z, s.inv) << 16 | q8(v.w, s.inv) << 24;
-                }
-                out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int e = 0; e < 4; ++e)
+                    w[e] = bytes4(q8(y[i][4 * e], s.inv), q8(y[i][4 * e + 1], s.inv), q8(y[i][4 * e + 2], s.inv),
+                                  q8(y[i][4 * e + 3], s.inv));
+                int8_t* out = dst + (int64_t)(sl + r) * a.hd;
+                *reinterpret_cast<uint2*>(out + c0) = make_uint2(w[0], w[1]);
+                *reinterpret_cast<uint2*>(out + c1) = make_uint2(w[2], w[3]);
             }
             if (s.old != 1.0f) {
                 uint4* old = reinterpret_cast<uint4*>(dst);
-                for (int i = threadIdx.x; i < sl * units; i += kAppThreads) {
+                for (int i = threadIdx.x; i < sl * (a.hd / 16); i += threads) {
                     const uint4 v = old[i];
                     old[i] = make_uint4(rescaled(v.x, s.old), rescaled(v.y, s.old), rescaled(v.z, s.old),
                                         rescaled(v.w, s.old));
                 }
             }
             if (threadIdx.x == 0) *scale = s.scale;
-            __syncthreads();  // ys and part are free
+            __syncthreads();  // part is free
         }
     }
 }
@@ -291,13 +351,18 @@ __global__ void __launch_bounds__(kAppThreads) append_packed_q8_kernel(const Q8A
 }  // namespace
 }  // namespace npub
 
+extern "C" size_t npub_rope_paged_append_q8_workspace(int tokens, int rot_dim, int packed) {
+    return packed && tokens > 0 && rot_dim > 0 ? (size_t)tokens * (rot_dim / 2) * sizeof(float2) : 0;
+}
+
 extern "C" int npub_rope_paged_append_q8(const void* qkv, int64_t ldx, void* q_out, int64_t ldq, int tokens, int q_heads,
                                          int kv_heads, int head_dim, int rot_dim, int interleaved,
                                          const int32_t* positions, const float* inv_freq, const void* q_gamma,
                                          const void* k_gamma, float eps, int8_t* k_pages, int8_t* v_pages,
                                          float* k_scales, float* v_scales, int n_pages, int page_size,
                                          const int32_t* page_table, int64_t ldt, int max_pages,
-                                         const int32_t* cu_seqlens, int batch, void* stream) {
+                                         const int32_t* cu_seqlens, int batch, void* workspace, size_t workspace_bytes,
+                                         void* stream) {
     using namespace npub;
     NPUB_CHECK_ARG(tokens >= 0 && batch >= 0 && q_heads > 0 && kv_heads > 0 && q_heads + 2 * (int64_t)kv_heads <= 65536);
     if (tokens == 0) return NPUB_OK;
@@ -353,9 +418,14 @@ extern "C" int npub_rope_paged_append_q8(const void* qkv, int64_t ldx, void* q_o
     // short sequences start several pages in the rows of one
     p.window = tokens / batch >= page_size ? page_size : 16;
     p.windows = (tokens + p.window - 1) / p.window;
-    const int64_t blocks = (int64_t)p.windows * 2 * kv_heads + tokens;
+    const int64_t blocks = (int64_t)p.windows * 2 * kv_heads;
+    if (!workspace || workspace_bytes < npub_rope_paged_append_q8_workspace(tokens, rot_dim, 1)) return NPUB_ERR_WORKSPACE;
+    NPUB_CHECK_ARG(npub_aligned(workspace, 256));
+    a.turns = reinterpret_cast<float2*>(workspace);
     if (blocks > 0x7fffffff) return NPUB_ERR_UNSUPPORTED;
-    const size_t smem = (size_t)page_size * (head_dim + 4) * sizeof(float);
-    NPUB_CUDA_TRY(cudaFuncSetAttribute(append_packed_q8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 256 * 132 * 4));
-    return launch_pdl(append_packed_q8_kernel, dim3((unsigned)blocks), dim3(kAppThreads), smem, st, p);
+    const int rc = launch_pdl(append_query_kernel, dim3(tokens), dim3(kAppThreads), 0, st, p.q);
+    if (rc) return rc;
+    int threads = (page_size << a.units_log2) / kUnits;
+    if (threads < 32) threads = 32;
+    return launch_pdl(append_packed_q8_kernel, dim3((unsigned)blocks), dim3(threads), 0, st, p);
 }

@@ -8,13 +8,14 @@
 // The norm's factor cancels in q, so one pass over the row collects the sum of
 // squares and the largest |t| together, and the row stays in registers for the
 // second.  q is exactly the definition's: t is exact in fp32 (a product of two
-// fp16), and where the fp32 quotient comes within 1e-4 of a half the remainder
+// fp16), and where the fp32 quotient comes within 2e-5 of a half the remainder
 // 127 t - q max|t| is formed in fp64, which holds it exactly.
 // A row with a NaN or an infinity gets the scale NaN and q = 0; a row of zeros
 // the scale 0.
 //
 // Bound: HBM, 2 bytes read and 1 written per element (6 and 3 with a residual).
 #include "common.cuh"
+#include "gemm_tc.h"
 
 namespace npub {
 namespace {
@@ -61,8 +62,15 @@ __device__ __forceinline__ void times_gamma(const uint4& v, const uint4& g, floa
     }
 }
 
+// The larger magnitude, NaN when one is.
+__device__ __forceinline__ float top_of(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
+
 // rint(127 t / most), halves to even, from the fp32 quotient's q, where that is near a half.
-__device__ __noinline__ int beside_half(float t, float most, int q) {
+__device__ __forceinline__ int beside_half(float t, float most, int q) {
     const double e = 127.0 * (double)t - (double)q * (double)most, half = 0.5 * (double)most;
     if (e > half || (e == half && (q & 1))) return q + 1;
     if (e < -half || (e == -half && (q & 1))) return q - 1;
@@ -72,7 +80,9 @@ __device__ __noinline__ int beside_half(float t, float most, int q) {
 // One row per block; V 8-element vectors of it in the registers of a thread,
 // those behind them (rows of more than 8 V THREADS elements) read again.
 //
-// Measured: 2048 rows of 11008 in 13 us, 5.2 TB/s; 8192 of 4096 with gamma in 24.
+// Measured: 32 rows of 4096 with gamma 2.6 us, 2048 of 11008 17.5 (3.9 TB/s), 8192 of 11008 54 (5.0), 8192 of 4096 with gamma
+// 32 (3.1), without 21.5: with gamma the instructions bound it. (rintf, a conversion and the fp64 path as a call: 4.1, 29, 108,
+// 40 and 37.)
 template <int THREADS, int V, bool GAMMA>
 __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const QuantArgs a) {
     pdl_trigger();
@@ -84,6 +94,7 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const QuantArgs 
     uint4 v[V];
     float ss = 0.0f;
     uint32_t top = 0;  // bits of the largest |t|: ordered as integers, NaN above infinity
+    float most = 0.0f;
     auto gamma_at = [&](int c) { return GAMMA ? __ldg(reinterpret_cast<const uint4*>(a.g + c)) : make_uint4(0, 0, 0, 0); };
     auto look = [&](int c, const uint4& u) {
         if (GAMMA) {
@@ -96,7 +107,7 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const QuantArgs 
                 ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(t[i]) & 0x7fffffffu);
+            for (int i = 0; i < 8; ++i) most = top_of(most, t[i]);
         } else {  // fp16 magnitudes, two in a word
             const uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu),
                                         __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
@@ -118,7 +129,8 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const QuantArgs 
         load_h(a, row, c, u);
         look(c, u);
     }
-    if (!GAMMA) top = __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(top & 0xffffu, top >> 16))));
+    if (GAMMA) top = __float_as_uint(most);
+    else top = __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(top & 0xffffu, top >> 16))));
     if (GAMMA) {
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
@@ -135,7 +147,8 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const QuantArgs 
         ss += part_ss[w];
         top = max(top, part_top[w]);
     }
-    float most = __uint_as_float(top), y = most;
+    most = __uint_as_float(top);
+    float y = most;
     if (GAMMA) y = most * (1.0f / sqrtf(ss / (float)a.cols + a.eps));
     const bool fine = top < 0x7f800000u;
     if (threadIdx.x == 0) a.scale[row] = fine ? y / 127.0f : NAN;
@@ -153,7 +166,7 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const QuantArgs 
             q[i] = __float_as_uint(m);
             off = fmaxf(off, fabsf(y - (m - 12582912.0f)));
         }
-        if (off > 0.4999f) {  // near a half: y's two roundings, 127 * 2^-23, are far inside 1e-4
+        if (off > 0.49998f) {  // near a half: y's two roundings are within 127 * 2^-23 = 1.52e-5
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = (uint32_t)beside_half(t[i], most, (int)q[i] - 0x4b400000);
         }
@@ -212,6 +225,10 @@ extern "C" int npub_quantize_rows(const void* x, int64_t ldx, const void* residu
     a.eps = eps;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int vecs = cols / 8;
+    if (rows <= num_sms() && vecs > 256) {  // one block on an SM: a row's latency counts
+        if (vecs <= 512) return launch_quantize<512, 1>(a, rows, st);
+        return launch_quantize<512, 3>(a, rows, st);
+    }
     if (vecs <= 256) return launch_quantize<128, 2>(a, rows, st);
     if (vecs <= 512) return launch_quantize<256, 2>(a, rows, st);
     if (vecs <= 768) return launch_quantize<256, 3>(a, rows, st);

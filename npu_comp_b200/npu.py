@@ -1033,15 +1033,17 @@ def rope_paged_append_q8(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_di
     if cu_seqlens is None:
         if B != T:
             raise ValueError("without cu_seqlens the table needs one row per token")
-        cu = None
+        cu = wsp = None
+        wsb = 0
     else:
         cu = _ints(cu_seqlens, "cu_seqlens", B + 1, dev)
+        ws, wsp, wsb = _paged_workspace(qkv, dev, "npub_rope_paged_append_q8_workspace", T, R, 1)
     out, ldq = _out16(out, qkv, T, q_heads * head_dim, dev)
     with _device(dev):
         st = _lib.bound("npub_rope_paged_append_q8")(
             qkv.data_ptr(), ldx, out.data_ptr(), ldq, T, q_heads, kv_heads, head_dim, R,
             1 if interleaved else 0, pos, fp, gq, gk, eps, k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(),
-            v_scales.data_ptr(), n_pages, ps, page_table.data_ptr(), ldt, W, cu, B,
+            v_scales.data_ptr(), n_pages, ps, page_table.data_ptr(), ldt, W, cu, B, wsp, wsb,
             torch._C._cuda_getCurrentRawStream(dev))
     if st:
         _lib.fail("npub_rope_paged_append_q8", st)

@@ -119,6 +119,23 @@ def test_append(cuda_device, new, start, H, KV, hd, rot, inter, norm, ps, packed
     check_append(new, start, H, KV, hd, rot, inter, norm, ps, packed, scale_spread=scale_spread, extra=2 if packed else 0)
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-5])
+def test_append_norm_of_few_rows(cuda_device, eps):
+    """Rows that do not fill a page's threads, with eps 0 too."""
+    g = torch.Generator().manual_seed(2)
+    H, KV, hd, ps = 2, 1, 80, 64
+    x = torch.randn((3, (H + 2 * KV) * hd), generator=g).half().cuda()
+    kp = torch.zeros((1, KV, ps, hd), dtype=torch.int8, device="cuda")
+    vp, ks, vs = kp.clone(), torch.ones(1, KV, device="cuda"), torch.ones(1, KV, device="cuda")
+    f, gam = nb.rope_freqs(hd, device="cuda"), torch.ones(hd, device="cuda").half()
+    pos = i32([0, 1, 2])
+    nb.rope_paged_append_q8(x, H, KV, hd, pos, f, kp, vp, ks, vs, i32([[0]]), cu_seqlens=i32([0, 3]), q_gamma=gam, k_gamma=gam,
+                            eps=eps)
+    _, (ke, _) = append64(x.view(3, -1, hd), H, KV, pos, f, hd, False, gam, gam, eps)
+    assert torch.isfinite(ks).all()
+    assert ((kp[0, 0, :3].double() * ks.item() - ke[:, 0]).abs() <= 0.501 * ks.item()).all()
+
+
 def test_append_wide_values(cuda_device):
     check_append([40], [8], 2, 2, 64, 64, False, False, 32, True, spread=300.0)
     check_append([40], [8], 2, 2, 64, 64, False, False, 32, True, spread=1e-6, scale_spread=1e-8)

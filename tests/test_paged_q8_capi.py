@@ -10,9 +10,9 @@ BYTE = ctypes.c_void_p(4097)
 
 
 def append(lib, qkv=P, ldx=1024, q=P, ldq=512, tokens=4, hq=4, hk=2, hd=128, rot=128, pos=P, f=P, gq=None, kp=P, vp=P, ks=P,
-           vs=P, n_pages=8, ps=16, table=P, ldt=4, width=4, cu=None, batch=4):
+           vs=P, n_pages=8, ps=16, table=P, ldt=4, width=4, cu=None, batch=4, ws=None, wsb=0):
     return lib.npub_rope_paged_append_q8(qkv, ldx, q, ldq, tokens, hq, hk, hd, rot, 0, pos, f, gq, None, 1e-5, kp, vp, ks, vs,
-                                         n_pages, ps, table, ldt, width, cu, batch, None)
+                                         n_pages, ps, table, ldt, width, cu, batch, ws, wsb, None)
 
 
 def test_append_refusals(libnpub_path):
@@ -25,6 +25,10 @@ def test_append_refusals(libnpub_path):
                dict(ps=24), dict(ps=512), dict(width=0), dict(ldt=3), dict(batch=3), dict(batch=0, cu=P)):
         assert append(lib, **kw) == -1, kw
     assert append(lib, hd=144, rot=16, ldx=2048, ldq=1024) == -2
+    n = lib.npub_rope_paged_append_q8_workspace(4, 128, 1)
+    assert n == 4 * 64 * 8 and lib.npub_rope_paged_append_q8_workspace(4, 128, 0) == 0
+    assert append(lib, cu=P, batch=2) == -4 and append(lib, cu=P, batch=2, ws=P, wsb=n - 1) == -4
+    assert append(lib, cu=P, batch=2, ws=ODD, wsb=n) == -1
 
 
 def paged(lib, q=P, ldq=512, kp=P, ks=P, vs=P, n_pages=8, ps=16, table=P, ldt=4, width=4, lens=P, cu=P, batch=2, total=8,
