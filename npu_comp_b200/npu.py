@@ -360,7 +360,7 @@ def quantize_rows(x: torch.Tensor, *, gamma: Optional[torch.Tensor] = None, eps:
         residual_out, ldh = _out16(residual_out, x, rows, d, dev)
         h = residual_out.data_ptr()
     if out is None:
-        out, ldq = x.new_empty((rows, d), dtype=_i8), d
+        out, ldq = (torch.empty_like(x, dtype=_i8) if ldx == d else x.new_empty((rows, d), dtype=_i8)), d
     else:
         _, n, c, ldq = _rows8(out, "out", dev)
         if n != rows or c != d:
@@ -396,7 +396,7 @@ def matmul_w8a8(Aq: torch.Tensor, a_scale: torch.Tensor, Wq: torch.Tensor, w_sca
     sa, sw = _vector(a_scale, "a_scale", _f32, M, dev), _vector(w_scale, "w_scale", _f16, N, dev)
     cols = N // 2 if swiglu else N
     if out is None:
-        out, ldc = Aq.new_empty((M, cols), dtype=_f16), cols
+        out, ldc = w_scale.new_empty(M, cols), cols  # (fp16, on the device of Aq)
     else:
         out, ldc = _out16(out, out, M, cols, dev)
     r, ldr = None, 0
