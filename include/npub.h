@@ -448,14 +448,14 @@ size_t npub_attention_paged_decode_workspace(int batch, int64_t ctx_len, int sha
  * aligned.
  *
  * npub_attention_paged_q8 / npub_attention_paged_decode_q8: the attention of
- * npub_attention_paged / npub_attention_paged_decode over such pages (scale >=
- * 1e-30).  A call whose sequences have at most 64 * kv_heads / heads new rows
- * (max_new says so; a decode step with heads <= 16 * kv_heads) reads the 8-bit
- * keys as they are; rows of a sequence past the tiles that max_new gives are
- * zeros, as above.  Any other call first writes the keys as fp16 (values past
- * 65504 become infinite) to its workspace, which holds batch * ctx_len of them:
- * there ctx_len is a limit, and the rows of a sequence with more keys than
- * ctx_len rounded up to 128 are zeros.  ctx_len 0: the table's width.
+ * npub_attention_paged / npub_attention_paged_decode over such pages.  A call
+ * with max_new > 0 and max_new * heads <= 128 * kv_heads (every
+ * decode step) reads the 8-bit keys as they are; rows of a sequence past its
+ * first max_new may be zeros, as above.  Any other call first writes the keys
+ * as fp16 (values past 65504 become infinite) to its workspace, which holds
+ * batch * ctx_len of them: there ctx_len is a limit, and the rows of a sequence
+ * with more keys than ctx_len rounded up to 128 are zeros.  ctx_len 0: the
+ * table's width.  heads <= 128 * kv_heads.
  * batch <= 65535. */
 int npub_rope_paged_append_q8(const void* qkv, int64_t ldx, void* q_out, int64_t ldq, int tokens, int q_heads,
                               int kv_heads, int head_dim, int rot_dim, int interleaved, const int32_t* positions,

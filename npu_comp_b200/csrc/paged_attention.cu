@@ -202,9 +202,11 @@ int run_plan(const Plan& pl, PackedArgs& a, void* workspace, size_t workspace_by
     return paged_combine(a, pl.total(), st);
 }
 
-// Over 8-bit pages: few rows on paged_decode_q8, more of them on the tile kernel behind a pass that writes the keys as
-// fp16 pages.
-constexpr int kQ8Tiles = 4;
+// Over 8-bit pages: few rows on paged_decode_q8.cu, more of them on the tile kernel behind a pass that writes the keys as
+// fp16 pages.  Measured on 70001 keys, 32 / 8 heads of 128, ragged rows, with the tiles of the longest sequence, as they
+// are and behind the pass: 24 sequences of 6 tiles 88 and 153 us, of 9 tiles 142 and 169, of 14 tiles 226 and 173; 4
+// sequences of 5 tiles 133 and 156, of 10 tiles 220 and 160.
+constexpr int kQ8Tiles = 8;
 struct PlanQ8 {
     Plan p;
     int tiles, rows;              // paged_decode_q8: tiles of a sequence and kv head, and the rows of one
@@ -218,10 +220,10 @@ PlanQ8 make_plan_q8(int batch, int total, int max_new, int64_t ctx, int heads, i
     PlanQ8 pl = {};
     const int group = heads / kv_heads;
     const double part_us = (double)total * heads * head_dim * 8.0 / 4e6;
-    if (max_new > 0 && group <= kPagedDecodeRows) {
-        pl.rows = (int64_t)max_new * group <= 8 ? 8 : kPagedDecodeRows;
-        const int64_t tiles = ceil_div(max_new, pl.rows / group);
-        if (tiles <= kQ8Tiles) pl.tiles = (int)tiles;
+    if (max_new > 0) {
+        const int64_t rows = (int64_t)max_new * group;
+        pl.rows = rows <= 8 ? 8 : kPagedDecodeRows;
+        if (ceil_div(rows, pl.rows) <= kQ8Tiles) pl.tiles = (int)ceil_div(rows, pl.rows);
     }
     pl.p.few = pl.tiles > 0;
     if (pl.p.few) {
@@ -280,9 +282,6 @@ int run_plan_q8(const PlanQ8& pl, PackedArgs& a, const float* ks, const float* v
     a.splits = pl.p.own.splits;
     return paged_decode_q8(a, ks, vs, pl.rows, pl.tiles, st);
 }
-
-// log2 of a scale over c = scale * log2(e) goes into the scores there
-bool scale_ok_q8(float scale) { return scale >= 1e-30f; }
 
 }  // namespace
 }  // namespace npub
@@ -427,7 +426,7 @@ extern "C" int npub_attention_paged_q8(const void* q, int64_t ldq, const int8_t*
                                        int causal, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace npub;
     NPUB_CHECK_ARG(batch >= 0 && total >= 0 && max_new >= 0 && ctx_len >= 0 &&
-                   dims_ok(heads, kv_heads, head_dim, scale) && scale_ok_q8(scale));
+                   dims_ok(heads, kv_heads, head_dim, scale));
     if (batch == 0 || total == 0) return NPUB_OK;
     NPUB_CHECK_ARG(q && out && lens && cu_seqlens &&
                    pool_ok(k_pages, v_pages, n_pages, page_size, page_table, ldt, max_pages));
@@ -478,7 +477,7 @@ extern "C" int npub_attention_paged_decode_q8(const void* q, int64_t ldq, const 
                                               int head_dim, float scale, void* workspace, size_t workspace_bytes,
                                               void* stream) {
     using namespace npub;
-    NPUB_CHECK_ARG(batch >= 0 && ctx_len >= 0 && dims_ok(heads, kv_heads, head_dim, scale) && scale_ok_q8(scale));
+    NPUB_CHECK_ARG(batch >= 0 && ctx_len >= 0 && dims_ok(heads, kv_heads, head_dim, scale));
     if (batch == 0) return NPUB_OK;
     NPUB_CHECK_ARG(q && out && lens && pool_ok(k_pages, v_pages, n_pages, page_size, page_table, ldt, max_pages));
     NPUB_CHECK_ARG(k_scales && v_scales && npub_aligned(k_scales, 4) && npub_aligned(v_scales, 4));

@@ -23,8 +23,8 @@
 //     the V product; the swizzle of the tile keeps the loads free of bank
 //     conflicts.
 //
-// Rows: a tile is 8 or 16 of a kv head (token x grouped head); more in further
-// tiles, which find K and V in L2.
+// Rows: a tile is 8 or 16 of a kv head, (token, grouped head) in order; more in
+// further tiles, which find K and V in L2.
 //
 // Two kernels.  paged_decode_q8_kernel: one CTA per (sequence, kv head, tile,
 // range of keys), up to eight ranges of an item a cluster that combines through
@@ -184,14 +184,14 @@ struct WarpTile {
         ra = kT ? 2 * t4 : g8;
         rb = kT ? ra + 1 : ra + 8;
     }
-    // The R rows from row0 on of head kvh, the first of them number `first` of a sequence of nseq rows and len keys, over
-    // keys up to k1.
-    __device__ __forceinline__ void start(const Params& p, int row0, int R, int kvh, int first, int nseq, int len, int k1) {
+    // R rows of head kvh from number f0 on, (token, grouped head) in order, of the sequence of nseq tokens from row0 on and
+    // len keys, over keys up to k1.
+    __device__ __forceinline__ void start(const Params& p, int row0, int R, int kvh, int f0, int nseq, int len, int k1) {
 #pragma unroll
         for (int i = 0; i < kQ; ++i) {
-            const int row = g8 + 8 * i, t = row / p.group;
+            const int row = g8 + 8 * i, t = (f0 + row) / p.group;
             const __half* src =
-                p.q + (int64_t)(row0 + t) * p.ldq + (int64_t)(kvh * p.group + row - t * p.group) * p.head_dim;
+                p.q + (int64_t)(row0 + t) * p.ldq + (int64_t)(kvh * p.group + f0 + row - t * p.group) * p.head_dim;
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk) {  // step kk of the lane's HD / 4 columns: 4 of them
                 const int d = t4 * (HD / 4) + kk * 4;
@@ -216,8 +216,8 @@ struct WarpTile {
         }
         lim[0] = lim[1] = len;
         if (p.causal) {
-            lim[0] = len - nseq + first + ra / p.group + 1;
-            lim[1] = len - nseq + first + rb / p.group + 1;
+            lim[0] = len - nseq + (f0 + ra) / p.group + 1;
+            lim[1] = len - nseq + (f0 + rb) / p.group + 1;
         }
         lim[0] = min(lim[0], k1);
         lim[1] = min(lim[1], k1);
@@ -428,25 +428,20 @@ __global__ void __launch_bounds__(kThreads, kMaxRows == 8 ? 3 : 2)
     const int kvh = (int)blockIdx.x / p.splits, split = (int)blockIdx.x - kvh * p.splits, b = blockIdx.y;
     pdl_wait();
     // this CTA's rows, the sequence's keys, and the range of them
-    int row0 = b, nseq = 1, nrow = 1, first = 0;
+    int row0 = b, nseq = 1;
     if (p.cu) {
-        const int per_tile = kMaxRows / p.group;
         row0 = max(0, min(p.total_q, p.cu[b]));
         nseq = max(0, min(p.total_q, p.cu[b + 1]) - row0);
-        first = (int)blockIdx.z * per_tile;
-        nrow = max(0, min(nseq - first, per_tile));
-        const int covered = (int)gridDim.z * per_tile;
-        if (blockIdx.z == gridDim.z - 1 && covered < nseq && split == 0) {
-            // a caller's max_new below the sequence's rows: the rest are zeros
-            const int rest = (nseq - covered) * p.group;
-            for (int i = threadIdx.x; i < rest; i += kThreads) {
-                const int t = i / p.group;
-                zero_row(p, row0 + covered + t, kvh * p.group + i - t * p.group);
-            }
-        }
-        row0 += first;
     }
-    const int R = nrow * p.group;
+    const int f0 = (int)blockIdx.z * kMaxRows;  // (token, grouped head) in order
+    const int64_t all = (int64_t)nseq * p.group;
+    const int R = (int)max((int64_t)0, min(all - f0, (int64_t)kMaxRows));
+    if (blockIdx.z == gridDim.z - 1 && split == 0) {  // a caller's max_new below the sequence's rows: the rest are zeros
+        for (int64_t f = (int64_t)gridDim.z * kMaxRows + threadIdx.x; f < all; f += kThreads) {
+            const int t = (int)(f / p.group);
+            zero_row(p, row0 + t, kvh * p.group + (int)(f - (int64_t)t * p.group));
+        }
+    }
     const int len = max(0, min(p.lens[b], p.max_keys));
     const int per = max(128 / kKeys, ((len + kKeys - 1) / kKeys + p.splits - 1) / p.splits) * kKeys;
     const int k0 = R == 0 ? 0 : min(len, split * per);
@@ -454,8 +449,8 @@ __global__ void __launch_bounds__(kThreads, kMaxRows == 8 ? 3 : 2)
     const int nst = (k1 - k0 + kKeys - 1) / kKeys;
     if (nst == 0) {
         for (int r = threadIdx.x; r < R; r += kThreads) {
-            const int t = r / p.group;
-            if (split == 0) zero_row(p, row0 + t, kvh * p.group + r - t * p.group);
+            const int t = (f0 + r) / p.group;
+            if (split == 0) zero_row(p, row0 + t, kvh * p.group + f0 + r - t * p.group);
         }
         return;
     }
@@ -534,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, kMaxRows == 8 ? 3 : 2)
 
     // ------------------------------------------------------------------------ consumers
     WarpTile<HD, kMaxRows> w;
-    w.start(p, row0, R, kvh, first, nseq, len, k1);
+    w.start(p, row0, R, kvh, f0, nseq, len, k1);
     bool ok = true;
     for (int j = 0; j < nst; ++j) {
         const int s = j % L::kStages;
@@ -589,9 +584,9 @@ __global__ void __launch_bounds__(kThreads, kMaxRows == 8 ? 3 : 2)
             acc[2] += f * v.z;
             acc[3] += f * v.w;
         }
-        const int t = r / p.group, head = kvh * p.group + r - t * p.group;
+        const int t = (f0 + r) / p.group, head = kvh * p.group + f0 + r - t * p.group;
         // keys, but all scores -inf: 0 / 0 in the formula, (-inf, 1) for a combination
-        const bool flat = mm == -INFINITY && sum == 0.0f && (p.causal ? min(k1, len - nseq + first + t + 1) : k1) > k0;
+        const bool flat = mm == -INFINITY && sum == 0.0f && (p.causal ? min(k1, len - nseq + t + 1) : k1) > k0;
         if (flat) sum = 1.0f;
         if (p.cluster) {
             if (d == 0) *reinterpret_cast<float2*>(smem + L::kOffOwnMl + r * 8) = make_float2(mm, sum);
@@ -633,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, kMaxRows == 8 ? 3 : 2)
             uint2 w;
             w.x = sum != 0.0f ? h2(acc[0] * inv, acc[1] * inv) : 0u;
             w.y = sum != 0.0f ? h2(acc[2] * inv, acc[3] * inv) : 0u;
-            const int t = r / p.group, head = kvh * p.group + r - t * p.group;
+            const int t = (f0 + r) / p.group, head = kvh * p.group + f0 + r - t * p.group;
             *reinterpret_cast<uint2*>(p.out + (int64_t)(row0 + t) * p.ldo + (int64_t)head * p.head_dim + d) = w;
         }
         cluster_arrive();  // nobody leaves while its shared memory is read
@@ -688,8 +683,7 @@ __device__ __forceinline__ Seq seq_at(const Params& p, int rows_of_tile, int b) 
         s.rows = max(0, min(p.total_q, __ldg(p.cu + b + 1)) - s.row0);
     }
     s.len = max(0, min(__ldg(p.lens + b), p.max_keys));
-    const int per = rows_of_tile / p.group;
-    s.tiles = min(p.tiles, (s.rows + per - 1) / per);
+    s.tiles = (int)min((int64_t)p.tiles, ((int64_t)s.rows * p.group + rows_of_tile - 1) / rows_of_tile);
     s.steps = (int)(((int64_t)s.len + kStep - 1) / kStep);
     s.items = s.steps > 0 ? s.tiles * p.kv_heads : 0;
     return s;
@@ -829,13 +823,12 @@ __global__ void __launch_bounds__(kWarps * 32, kListCtas) paged_list_q8_kernel(c
 
     // ---- the steps
     WarpTile<HD, kMaxRows> w;
-    const int per = kMaxRows / p.group;
     const float skc = p.c * kSubnormal;
     int src[kStep / 16];  // the lane of the K piece that holds 16 keys (V's is the next)
 #pragma unroll
     for (int u = 0; u < kStep / 16; ++u) src[u] = 2 * (u * 16 / p.box_rows);
     int begun = now.step;  // first step of the current item that is this warp's
-    int row0 = 0, R = 0;
+    int row0 = 0, f0 = 0, R = 0;
     bool fresh = true;  // the current item is the first of this warp's
     // j: steps of this warp ahead of the item's
     auto open = [&](int j) {
@@ -846,10 +839,10 @@ __global__ void __launch_bounds__(kWarps * 32, kListCtas) paged_list_q8_kernel(c
                 make_int2(2 * (int)id + (fresh ? 0 : 1), last - (int)id + 1);
         }
         const Seq s = seq_at(p, kMaxRows, now.b);
-        const int first = now.tile * per;
-        row0 = s.row0 + first;
-        R = min(per, s.rows - first) * p.group;
-        w.start(p, row0, R, now.kvh, first, s.rows, s.len, s.len);
+        row0 = s.row0;
+        f0 = now.tile * kMaxRows;
+        R = (int)min((int64_t)kMaxRows, (int64_t)s.rows * p.group - f0);
+        w.start(p, row0, R, now.kvh, f0, s.rows, s.len, s.len);
     };
     open(0);
     int never = 0;
@@ -894,9 +887,9 @@ __global__ void __launch_bounds__(kWarps * 32, kListCtas) paged_list_q8_kernel(c
                 w.runs([&](int r, int col, const float (&o)[HD / 8]) {
                     const int row = r ? w.rb : w.ra;
                     if (row >= R || col >= p.head_dim) return;
-                    const int t = row / p.group;
+                    const int t = (f0 + row) / p.group;
                     __half* dst = p.out + (int64_t)(row0 + t) * p.ldo +
-                                  (int64_t)(now.kvh * p.group + row - t * p.group) * p.head_dim + col;
+                                  (int64_t)(now.kvh * p.group + f0 + row - t * p.group) * p.head_dim + col;
                     const bool any = w.l[r] != 0.0f || flat[r];
 #pragma unroll
                     for (int i = 0; i < HD / 8; i += 8)
@@ -954,8 +947,9 @@ __global__ void __launch_bounds__(kCoop ? 256 : 128) paged_list_combine_kernel(c
         b = lo;
     }
     const Seq s = seq_at(p, kMaxRows, b);
-    const int per = kMaxRows / p.group, kvh = head / p.group;
-    const int tile = (row - s.row0) / per;
+    const int kvh = head / p.group;
+    const int64_t f = (int64_t)(row - s.row0) * p.group + head - kvh * p.group;  // (token, grouped head) in order
+    const int64_t tile = f / kMaxRows;
     __half* dst = p.out + (int64_t)row * p.ldo + (int64_t)head * p.head_dim + lane * 4;
     const bool act = lane * 4 < p.head_dim;
     if (s.items == 0 || tile >= s.tiles || row < s.row0) {
@@ -965,7 +959,7 @@ __global__ void __launch_bounds__(kCoop ? 256 : 128) paged_list_combine_kernel(c
     const int2 at = p.parts[((int64_t)b * p.kv_heads + kvh) * p.tiles + tile];
     const int n = at.y;
     if (n <= 1) return;  // one warp had it whole
-    const int r = (row - s.row0 - tile * per) * p.group + head - kvh * p.group;  // row of the tile
+    const int r = (int)(f - tile * kMaxRows);  // row of the tile
     // the first part's warp had other items ahead of this one or not; of the others it is the first
     auto slot = [&](int i) { return (int64_t)(i ? (at.x & ~1) + 2 * i : at.x) * kMaxRows + r; };
     float m = -INFINITY, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;

@@ -1057,7 +1057,7 @@ def attention_paged_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     """attention_paged() over a cache in 8 bits.
 
     max_new: at least the new rows of any sequence (0: not known).  With at most
-    64 * kv_heads / heads of them the 8-bit keys are read as they are, and a
+    128 * kv_heads / heads of them the 8-bit keys are read as they are, and a
     sequence that has more than max_new rows all the same may get zeros for those
     past them.  Any other call first writes the keys as fp16 to its workspace,
     batch * ctx_len of them: ctx_len is then a limit, and a sequence with more
@@ -1090,8 +1090,7 @@ def attention_paged_decode_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: t
                               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """attention_paged_decode() over a cache in 8 bits: q [batch, heads*hd], one
     new row per sequence, keys 0 .. lens[b] - 1.  ctx_len: the largest lens
-    expected (0: the table's width); a limit, as in attention_paged_q8, where
-    heads > 16 * kv_heads."""
+    expected (0: the table's width), which only decides how the work is split."""
     dev, n, qc, ldq = _first16(q, "q")
     (n_pages, kv_heads, ps, hd), B, W, ldt = _pool8(k_pages, v_pages, k_scales, v_scales, page_table, dev)
     if n != B or qc != heads * hd:

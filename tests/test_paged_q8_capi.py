@@ -49,7 +49,7 @@ def test_attention_refusals(libnpub_path):
     for kw in (dict(q=None), dict(kp=None), dict(ks=None), dict(vs=None), dict(table=None), dict(lens=None), dict(out=None),
                dict(q=ODD), dict(kp=ODD), dict(out=ODD), dict(ks=BYTE), dict(vs=BYTE), dict(ldq=504), dict(ldo=500),
                dict(n_pages=0), dict(ps=8), dict(ps=48), dict(ps=512), dict(width=0), dict(ldt=3), dict(h=3), dict(hd=8),
-               dict(scale=-1.0), dict(scale=1e-31), dict(ctx=-1), dict(batch=-1)):
+               dict(scale=-1.0), dict(scale=0.0), dict(ctx=-1), dict(batch=-1)):
         assert paged(lib, **kw) == -1, kw
         assert decode(lib, **kw) == -1, kw
     assert paged(lib, cu=None) == -1 and paged(lib, max_new=-1) == -1
@@ -67,5 +67,6 @@ def test_workspace_queries(libnpub_path):
     n = p(3, 300, 100, 1000, 8, 2, 128)
     keys = 3 * 1024 * 2 * 128 * 2 * 2
     assert n >= keys + 3 * 9 * 4
-    assert p(3, 300, 16, 1000, 8, 2, 128) < keys  # at most 64 rows of a kv head: read as they are
+    assert p(3, 300, 32, 1000, 8, 2, 128) != p(3, 300, 33, 1000, 8, 2, 128)  # at most 128 rows of a kv head: read as they are
+    assert d(3, 1000, 128, 1, 128) < p(3, 3, 0, 1000, 128, 1, 128)
     assert p(0, 8, 0, 100, 4, 2, 128) == 0
