@@ -9,14 +9,25 @@
 // and the result is rounded to fp16 once.
 //
 // Two kernels:
-//   w8a8_tile_kernel  2-CTA pairs, 256 tokens x 256 channels, persistent, the
-//                     sums double-buffered in tensor memory; tensor bound
+//   w8a8_tile_kernel  persistent, 256 channels x 256 tokens (two MMAs share the
+//                     channels' tile; the sums fill tensor memory) or x 128
+//                     (the sums of two tiles, so that the epilogue runs behind
+//                     the next tile's MMAs)
 //   w8a8_few_kernel   128 channels x BT tokens in one CTA, the K axis over the
 //                     CTAs of a cluster, which add their sums through one
 //                     another's shared memory (integers: the order does not
 //                     matter); for few tokens, where the weights' bytes bound
 //                     it, and for products of few tiles
 // and `pick` chooses.
+//
+// What bounds the tile kernel: an MMA of 128 x 256 x 32 reads 12 KB of shared
+// memory in its 128 cycles, and the copies write 64 KB (256 tokens) for 8 of
+// them, 48 KB (128) for 4: 160 and 192 bytes a cycle where the SM has 128, so
+// 80 % and 67 % of the tensor rate at the same clock.  8192 x 22016 x 4096 runs
+// into the power limit first (542 us, 2730 TOP/s at 1.45 - 1.5 GHz; 128 tokens
+// 571), 2048 x 4096 x 11008 takes 78 us in one wave of 256 tokens and 85 in two
+// of 128, 1024 x 12288 x 4096 59 and 51.5, 256 x 12288 x 4096 33 and 22.  Stages
+// of 64 of K instead of 128, twice as many: 569 and 704 us on the first.
 #include "common.cuh"
 #include "gemm_tc.h"
 
@@ -51,14 +62,6 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
@@ -99,171 +102,188 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
 }
 __device__ __forceinline__ float2 half2_at(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
-// ------------------------------------------------------------- 256 x 256 tiles
+// ------------------------------------------------------------- tiles of 256 channels
 
-constexpr int kTileStages = 6;
-constexpr int kTileThreads = 256;
+constexpr int kTileThreads = 384;
+// MH halves of 128 tokens.  The sums take all of tensor memory: with MH = 2 one
+// tile's two halves, each read by four epilogue warps, with MH = 1 two tiles',
+// each read by all eight.
+template <int MH>
 struct TileSmem {
-    static constexpr int kOp = 128 * BK;  // a CTA's half of either operand's tile
-    static constexpr int kOffBar = kTileStages * 2 * kOp;
+    static constexpr int kOp = 128 * BK;  // 128 rows of either operand
+    static constexpr int kStage = (MH + 2) * kOp;
+    static constexpr int kStages = MH == 2 ? 3 : 4;
+    static constexpr int kOffBar = kStages * kStage;
     static constexpr int kOffOut = kOffBar + 256;  // epilogue warps: 32 x 32 sums, rows of 33 words
-    static constexpr int kTotal = kOffOut + 4 * 32 * 33 * 4 + 1024;
+    static constexpr int kTotal = kOffOut + 8 * 32 * 33 * 4 + 1024;
+    static_assert((2 * kStages + 5) * 8 + 8 <= 256, "the barriers' part");
 };
 
 // Tiles in bands of p.band token tiles, the channels in turn within a band, so
-// that the 74 tiles in flight share operands in L2.
+// that the tiles in flight share operands in L2.
 struct TileAt {
     int m0, n0;
 };
+template <int MH>
 __device__ __forceinline__ TileAt tile_at(const Params& p, int t) {
     const int per_band = p.band * p.n_tiles, b = t / per_band, r = t - b * per_band;
     const int nb = min(p.band, p.m_tiles - b * p.band), n = r / nb;
-    return TileAt{(b * p.band + r - n * nb) * 256, n * 256};
+    return TileAt{(b * p.band + r - n * nb) * 128 * MH, n * 256};
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
-    w8a8_tile_kernel(const __grid_constant__ Params p) {
-    pdl_trigger();
-    using L = TileSmem;
+template <int MH>
+__global__ void __launch_bounds__(kTileThreads, 1) w8a8_tile_kernel(const __grid_constant__ Params p) {
+    using L = TileSmem<MH>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *sA = smem, *sB = smem + kTileStages * L::kOp;
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar);  // [stages] (even CTA) both CTAs' operands landed
-    uint64_t* empty = full + kTileStages;                             // [stages] pair MMA done with the stage
-    uint64_t* acc_full = empty + kTileStages;                         // [2] sums ready
-    uint64_t* acc_empty = acc_full + 2;                               // [2] (even CTA) both epilogues have read them
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar);  // [stages] both operands landed
+    uint64_t* empty = full + L::kStages;                              // [stages] the MMAs are done with the stage
+    uint64_t* acc_full = empty + L::kStages;                          // [2] sums ready
+    uint64_t* acc_empty = acc_full + 2;                               // [2] the epilogue has read them
+    uint64_t* drained = acc_empty + 2;                                // after an abort: the MMAs are done
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_ctarank();
-    const int cid = (int)cluster_id_x(), ncl = (int)nclusters_x();
     const int n_all = p.m_tiles * p.n_tiles;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kTileStages; ++s) {
+        for (int s = 0; s < L::kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], 8);
+            mbar_init(&acc_empty[b], MH == 2 ? 4 : 8);
         }
+        mbar_init(drained, 1);
         *abort_flag = 0;
         fence_barrier_init();
-    }
-    if (warp == 0 && lane == 0) {
         prefetch_tmap(&p.tmA);
         prefetch_tmap(&p.tmW);
     }
     if (warp == 1) {
-        tmem_alloc_pair(tmem_slot, 512);
-        tmem_relinquish_pair();
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
     }
     tc_fence_before();
-    cluster_sync();
+    cta_sync_divergent();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    pdl_wait();
 
     if (warp == 0) {
         if (lane == 0) {  // producer
             uint32_t g = 0;
-            const uint32_t full0 = mapa_shared(smem_u32(&full[0]), 0);
-            for (int t = cid; t < n_all && !*abort_flag; t += ncl) {
-                const TileAt at = tile_at(p, t);
+            bool ok = true;
+            for (int t = (int)blockIdx.x; t < n_all && ok; t += (int)gridDim.x) {
+                const TileAt at = tile_at<MH>(p, t);
                 for (int i = 0; i < p.k_tiles; ++i, ++g) {
-                    const int s = (int)(g % kTileStages);
-                    if (!mbar_wait_cluster_bounded(&empty[s], ((g / kTileStages) & 1u) ^ 1u, abort_flag)) {
-                        *abort_flag = 1;
-                        set_err(p.err, 0x701);
-                        break;
-                    }
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], 4u * L::kOp);
-                    tma_load_3d_pair(sA + s * L::kOp, &p.tmA, full0 + (uint32_t)s * 8u, i * BK, at.m0 + (int)rank * 128, 0);
-                    tma_load_3d_pair(sB + s * L::kOp, &p.tmW, full0 + (uint32_t)s * 8u, i * BK, at.n0 + (int)rank * 128, 0);
+                    const int s = (int)(g % L::kStages);
+                    ok = mbar_wait_quick(&empty[s], ((g / L::kStages) & 1u) ^ 1u, abort_flag);
+                    if (!ok) break;
+                    uint8_t* st = smem + s * L::kStage;
+                    mbar_arrive_expect_tx(&full[s], (uint32_t)L::kStage);
+                    tma_load_3d(st, &p.tmA, &full[s], i * BK, at.m0, 0);
+                    tma_load_3d(st + MH * L::kOp, &p.tmW, &full[s], i * BK, at.n0, 0);
                 }
             }
-            // The MMA thread has waited for every load when it signals the last tile's sums.  After an abort nobody
-            // waits for those in flight: give them (microseconds) time to land before the CTAs leave.
-            if (*abort_flag) {
-                const uint64_t t0 = globaltimer_ns();
-                while (globaltimer_ns() - t0 < 1000000ull) {
-                }
+            if (!ok) {  // copies in flight land before the CTA leaves (the MMA thread has waited for them otherwise)
+                *abort_flag = 1;
+                set_err(p.err, 0x701);
+                int never = 0;
+                for (uint32_t j = g < (uint32_t)L::kStages ? 0 : g - L::kStages; j < g; ++j)
+                    mbar_wait_bounded(&full[j % L::kStages], (j / L::kStages) & 1u, &never, 100000000ull);
             }
         }
     } else if (warp == 1) {
-        if (rank == 0 && elect_one()) {  // MMA
-            constexpr uint32_t idesc = idesc_i8(256, 256);
+        if (elect_one()) {  // MMA
+            constexpr uint32_t idesc = idesc_i8(128, 256);
             uint32_t g = 0, n = 0;
-            bool ok = true;
-            for (int t = cid; t < n_all && ok; t += ncl, ++n) {
-                const uint32_t b = n & 1u;
-                if (!mbar_wait_cluster_bounded(&acc_empty[b], ((n >> 1) & 1u) ^ 1u, abort_flag)) {
-                    ok = false;
-                    set_err(p.err, 0x702);
-                    break;
-                }
-                tc_fence_after();
-                for (int i = 0; i < p.k_tiles; ++i, ++g) {
-                    const int s = (int)(g % kTileStages);
-                    if (!mbar_wait_cluster_bounded(&full[s], (g / kTileStages) & 1u, abort_flag)) {
-                        ok = false;
-                        set_err(p.err, 0x703);
+            int code = 0;
+            for (int t = (int)blockIdx.x; t < n_all && !code; t += (int)gridDim.x, ++n) {
+                for (int i = 0; i < p.k_tiles && !code; ++i, ++g) {
+                    const int s = (int)(g % L::kStages);
+                    if (!mbar_wait_quick(&full[s], (g / L::kStages) & 1u, abort_flag)) {
+                        code = 0x703;
                         break;
                     }
-                    tc_fence_after();
-                    const uint32_t a = smem_u32(sA + s * L::kOp), w = smem_u32(sB + s * L::kOp);
+                    const uint32_t a = smem_u32(smem + s * L::kStage), w = a + MH * L::kOp;
 #pragma unroll
-                    for (int k = 0; k < BK / kUmmaK; ++k)
-                        mma_i8_pair(tmem + b * 256u, umma_desc_sw128(a + k * kUmmaK), umma_desc_sw128(w + k * kUmmaK), idesc,
-                                    (i > 0 || k > 0) ? 1u : 0u);
-                    tc_commit_pair(smem_u32(&empty[s]));
-                    tc_commit_pair(mapa_shared(smem_u32(&empty[s]), 1));
+                    for (int h = 0; h < MH; ++h) {
+                        const uint32_t b = MH == 2 ? h : n & 1u, ph = MH == 2 ? n & 1u : (n >> 1) & 1u;
+                        if (i == 0 && !mbar_wait_quick(&acc_empty[b], ph ^ 1u, abort_flag)) {
+                            code = 0x702;
+                            break;
+                        }
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 0; k < BK / kUmmaK; ++k)
+                            mma_i8(tmem + b * 256u, umma_desc_sw128(a + h * L::kOp + k * kUmmaK),
+                                   umma_desc_sw128(w + k * kUmmaK), idesc, (i > 0 || k > 0) ? 1u : 0u);
+                        if (i == p.k_tiles - 1) tc_commit(&acc_full[b]);
+                    }
+                    if (!code) tc_commit(&empty[s]);
                 }
-                if (!ok) break;
-                tc_commit_pair(smem_u32(&acc_full[b]));
-                tc_commit_pair(mapa_shared(smem_u32(&acc_full[b]), 1));
             }
-            if (!ok) *abort_flag = 1;
+            if (code) {
+                set_err(p.err, code);
+                *abort_flag = 1;
+                int never = 0;
+                tc_commit(drained);
+                mbar_wait_bounded(drained, 0, &never, 100000000ull);
+            }
         }
     } else if (warp >= 4) {
         // -------------------------------------------------------------------- epilogue: one token per lane
-        const int wq = warp & 3;
-        const uint32_t acc_empty0 = mapa_shared(smem_u32(&acc_empty[0]), 0);
+        const int wq = warp & 3, group = (warp - 4) >> 2;
+        // of this warp: 32 x 32 sums on their way out, or the channels' 256 scales
+        int* out = reinterpret_cast<int*>(smem + L::kOffOut) + (warp - 4) * 32 * 33;
         uint32_t n = 0;
-        for (int t = cid; t < n_all; t += ncl, ++n) {
-            const TileAt at = tile_at(p, t);
-            const uint32_t b = n & 1u;
-            const int m = at.m0 + (int)rank * 128 + wq * 32 + lane;
+        for (int t = (int)blockIdx.x; t < n_all; t += (int)gridDim.x, ++n) {
+            const TileAt at = tile_at<MH>(p, t);
+            const int b = MH == 2 ? group : (int)(n & 1u);
+            const uint32_t sums = tmem + ((uint32_t)(wq * 32) << 16) + (uint32_t)b * 256u;
+            const int m = at.m0 + (MH == 2 ? group * 128 : 0) + wq * 32 + lane;
             const bool row = m < p.M;
+            const int rows = min(32, p.M - (m - lane));              // of this warp, may be negative
+            const int c0 = MH == 2 ? 0 : group * 4;                  // its chunks of 32 channels
+            const int chunks = rows > 0 ? min(MH == 2 ? 8 : c0 + 4, (p.N - at.n0 + 31) / 32) : 0;
             const float sa = row ? __ldg(p.sa + m) : 0.0f;
-            bool ok = mbar_wait_cluster_bounded(&acc_full[b], (n >> 1) & 1u, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) {
-                set_err(p.err, 0x704);
-                *abort_flag = 1;
-                break;
+            const __half* res = p.R ? p.R + (int64_t)m * p.ldr + at.n0 : nullptr;
+            uint4 r[4];  // the residual of the chunk to come, where it can be read 16 bytes at a time
+            auto fetch = [&](int c) {
+                if (!p.vec || !res || !row || c >= 8 || at.n0 + c * 32 + 32 > p.N) return;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r[e] = *(reinterpret_cast<const uint4*>(res + c * 32) + e);
+            };
+            fetch(c0);
+            if (p.vec) {
+                if (at.n0 + lane * 8 + 8 <= p.N)
+                    *(reinterpret_cast<uint4*>(out) + lane) = __ldg(reinterpret_cast<const uint4*>(p.sw + at.n0) + lane);
+                __syncwarp();
             }
-            tc_fence_after();
-            for (int c0 = 0; c0 < 256; c0 += 32) {
-                const int n0 = at.n0 + c0;
-                if (n0 >= p.N) break;
-                int acc[32];
-                tmem_ld32(tmem + ((uint32_t)(wq * 32) << 16) + b * 256u + (uint32_t)c0, acc);
+            // sums of 32 channels to C
+            auto finish = [&](int c, int (&acc)[32]) {
+                const int n0 = at.n0 + c * 32;
                 if (p.vec && n0 + 32 <= p.N) {
-                    if (!row) continue;
                     float z[32];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint4 w = __ldg(reinterpret_cast<const uint4*>(p.sw + n0) + e);
-                        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+                        const uint4 w = *(reinterpret_cast<const uint4*>(out) + c * 4 + e);
+                        const uint32_t ww[4] = {w.x, w.y, w.z, w.w}, rr[4] = {r[e].x, r[e].y, r[e].z, r[e].w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float2 f = half2_at(ww[i]);
                             z[e * 8 + 2 * i] = (float)acc[e * 8 + 2 * i] * (sa * f.x);
                             z[e * 8 + 2 * i + 1] = (float)acc[e * 8 + 2 * i + 1] * (sa * f.y);
+                            if (res) {
+                                const float2 g = half2_at(rr[i]);
+                                z[e * 8 + 2 * i] += g.x;
+                                z[e * 8 + 2 * i + 1] += g.y;
+                            }
                         }
                     }
+                    fetch(c + 1);
+                    if (!row) return;
                     if (p.swiglu) {
                         uint4* dst = reinterpret_cast<uint4*>(p.C + (int64_t)m * p.ldc + n0 / 2);
 #pragma unroll
@@ -276,42 +296,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
                             }
                             dst[e] = make_uint4(o[0], o[1], o[2], o[3]);
                         }
-                        continue;
-                    }
-                    if (p.R) {
-                        const uint4* r = reinterpret_cast<const uint4*>(p.R + (int64_t)m * p.ldr + n0);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint4 w = r[e];
-                            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float2 f = half2_at(ww[i]);
-                                z[e * 8 + 2 * i] += f.x;
-                                z[e * 8 + 2 * i + 1] += f.y;
-                            }
-                        }
+                        return;
                     }
                     uint4* dst = reinterpret_cast<uint4*>(p.C + (int64_t)m * p.ldc + n0);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         dst[e] = make_uint4(pack_h2(z[e * 8], z[e * 8 + 1]), pack_h2(z[e * 8 + 2], z[e * 8 + 3]),
                                             pack_h2(z[e * 8 + 4], z[e * 8 + 5]), pack_h2(z[e * 8 + 6], z[e * 8 + 7]));
-                    continue;
+                    return;
                 }
-// rows that 16 bytes at a time do not fit: through shared memory, so that the lanes store along a row
-                int* out = reinterpret_cast<int*>(smem + L::kOffOut) + wq * 32 * 33;
+                // rows that 16 bytes at a time do not fit: through shared memory, so that the lanes store along a row
+                __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 32; ++i) out[lane * 33 + i] = acc[i];
                 __syncwarp();
-                const int rows = min(32, p.M - (m - lane));
                 const int per = p.swiglu ? 2 : 1, n = n0 + lane * per;  // this lane's column, or the first of its two
                 const bool on = lane * per < 32 && n < p.N;
                 const float sw0 = on ? __half2float(__ldg(p.sw + n)) : 0.0f;
                 const float sw1 = on && p.swiglu ? __half2float(__ldg(p.sw + n + 1)) : 0.0f;
-                const __half* res = p.R ? p.R + (int64_t)(m - lane) * p.ldr + n : nullptr;
+                const __half* add = p.R ? p.R + (int64_t)(m - lane) * p.ldr + n : nullptr;
                 __half* dst = p.C + (int64_t)(m - lane) * p.ldc + n / per;
-                for (int q0 = 0; q0 < rows; q0 += 8) {
+#pragma unroll
+                for (int q0 = 0; q0 < 32; q0 += 8) {
                     float z[8];
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
@@ -319,26 +325,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1)
                         const int* v = out + (q0 + q) * 33 + (lane * per & 31);
                         z[q] = (float)v[0] * (sq * sw0);
                         if (p.swiglu) z[q] = swiglu_f(z[q], (float)v[1] * (sq * sw1));
-                        if (res && on && q0 + q < rows) z[q] += __half2float(res[(int64_t)(q0 + q) * p.ldr]);
+                        if (add && on && q0 + q < rows) z[q] += __half2float(add[(int64_t)(q0 + q) * p.ldr]);
                     }
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
                         if (on && q0 + q < rows) dst[(int64_t)(q0 + q) * p.ldc] = __float2half_rn(z[q]);
                 }
                 __syncwarp();
+            };
+            const bool ok = __all_sync(0xffffffffu, mbar_wait_quick(&acc_full[b], MH == 2 ? n & 1u : (n >> 1) & 1u, abort_flag));
+            if (!ok) {
+                if (lane == 0) {
+                    set_err(p.err, 0x704);
+                    *abort_flag = 1;
+                }
+                break;
             }
+            tc_fence_after();
+            // the last two chunks go to registers ahead of their turn, and the MMAs may have the sums' place again
+            int acc[32], last[32];
+#pragma unroll 1
+            for (int c = c0; c < chunks - 2; ++c) {
+                tmem_ld32(sums + (uint32_t)(c * 32), acc);
+                finish(c, acc);
+            }
+            if (chunks - 2 >= c0) tmem_ld32(sums + (uint32_t)((chunks - 2) * 32), acc);
+            if (chunks - 1 >= c0) tmem_ld32(sums + (uint32_t)((chunks - 1) * 32), last);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty0 + b * 8u);
+            if (lane == 0) mbar_arrive(&acc_empty[b]);
+            if (chunks - 2 >= c0) finish(chunks - 2, acc);
+            if (chunks - 1 >= c0) finish(chunks - 1, last);
+            __syncwarp();  // `out` is read
         }
     }
 
     tc_fence_before();
     cta_sync_divergent();
-    cluster_sync();  // no CTA leaves while its peer may still signal or read it
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc_pair(tmem, 512);
+        tmem_dealloc(tmem, 512);
     }
 }
 
@@ -359,7 +385,6 @@ struct FewSmem {
 // [r * per, (r + 1) * per)
 template <int BT>
 __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_constant__ Params p) {
-    pdl_trigger();
     using L = FewSmem<BT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -397,6 +422,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
     cta_sync_divergent();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    pdl_trigger();  // behind the allocation: a successor's CTA that waits for this grid may hold columns of its own
     pdl_wait();
 
     bool ok = true;
@@ -530,21 +556,26 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
 
 // ---------------------------------------------------------------------- host
 
+constexpr int kTile1 = 1, kTile2 = 2;  // the tile kernel with 128 and 256 tokens
 struct Choice {
-    int bt;      // 0: tile kernel
+    int bt;      // kTile1, kTile2, or the tokens of the few-token kernel's tiles
     int splits;
 };
 
-// The estimates' terms, in us, are fitted to CUDA graphs of calls of 1 to 777 tokens (at 12288 x 4096, tile kernel 21 for up
-// to 256 tokens and 31 for 512; few-token kernel with one and two CTAs for a tile, 32 tokens 15.4 and 14.2, 64 in one tile
-// 19.5 and 16.7, 128 in two 20.5 and 26.6; 4096 x 4096 at 32 tokens with 1, 2, 4, 8: 12.6, 9.5, 7.7, 7.7).
-Choice pick(int M, int N, int k_tiles) {
+// The estimates' terms, in us, are fitted to CUDA graphs of calls of 1 to 8192 tokens: those above; few-token kernel at 12288
+// x 4096 with one and two CTAs for a tile, 32 tokens 15.4 and 14.2, 64 in one tile 19.5 and 16.7, 128 in two 20.5 and 26.6;
+// 4096 x 4096 at 32 tokens with 1, 2, 4, 8: 12.6, 9.5, 7.7, 7.7.  Rows that are not written 16 bytes at a time, 777 x 1003 x
+// 2064: few-token kernel 14, tiles of 128 tokens 23, of 256 36.
+Choice pick(int M, int N, int k_tiles, bool vec) {
     // clusters of 1 .. 8 CTAs that 148 SMs (whole GPCs of them) hold at one CTA per SM; the few-token kernel has two
     static const int held[kMaxCluster + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
     const int sms = num_sms();
-    Choice c = {0, 1};
-    const int64_t big = (int64_t)((M + 255) / 256) * ((N + 255) / 256), pairs = sms / 2;
-    double best = 7.5 + 0.003 * (M < 1024 ? M : 1024) + (double)((big + pairs - 1) / pairs) * k_tiles * (0.3 + 0.13 * (big < 48 ? (double)big / 48.0 : 1.0));
+    const int64_t wide = (N + 255) / 256, t1 = (int64_t)((M + 127) / 128) * wide, t2 = (int64_t)((M + 255) / 256) * wide;
+    const double some1 = t1 < sms ? (double)t1 / sms : 1.0, some2 = t2 < sms ? (double)t2 / sms : 1.0;
+    const double us1 = (vec ? 4.1 : 13.0) + (double)((t1 + sms - 1) / sms) * k_tiles * (0.40 + 0.07 * some1);
+    const double us2 = (vec ? 4.5 : 22.0) + (double)((t2 + sms - 1) / sms) * (k_tiles * (0.61 + 0.17 * some2) + 4.0);
+    Choice c = {us1 <= us2 ? kTile1 : kTile2, 1};
+    double best = us1 <= us2 ? us1 : us2;
     for (int bt = 32; bt <= 128; bt *= 2) {
         const int64_t token_tiles = (M + bt - 1) / bt, tiles = (int64_t)((N + 127) / 128) * token_tiles;
         if (token_tiles > 8) continue;
@@ -597,17 +628,19 @@ int launch_few(Params& p, int splits, cudaStream_t st) {
     return npub_internal_launch_status();
 }
 
+template <int MH>
 int launch_tile(Params& p, cudaStream_t st) {
-    static_assert(TileSmem::kTotal <= 232448, "shared memory budget");
-    NPUB_CUDA_TRY(cudaFuncSetAttribute(w8a8_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem::kTotal));
-    p.m_tiles = (p.M + 255) / 256;
-    p.n_tiles = (p.N + 255) / 256;
-    p.band = 8;
+    using L = TileSmem<MH>;
+    static_assert(L::kTotal <= 232448, "shared memory budget");
+    NPUB_CUDA_TRY(cudaFuncSetAttribute(w8a8_tile_kernel<MH>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
+    p.m_tiles = (p.M - 1) / (128 * MH) + 1;
+    p.n_tiles = (p.N - 1) / 256 + 1;
+    p.band = 16 / MH;
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
     if (tiles > 0x3fffffff) return NPUB_ERR_UNSUPPORTED;
-    const int pairs = num_sms() / 2;
-    return launch_pdl(w8a8_tile_kernel, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), dim3(kTileThreads),
-                      TileSmem::kTotal, st, p);
+    const int sms = num_sms();
+    w8a8_tile_kernel<MH><<<(unsigned)(tiles < sms ? tiles : sms), kTileThreads, L::kTotal, st>>>(p);
+    return npub_internal_launch_status();
 }
 
 }  // namespace w8a8
@@ -626,6 +659,7 @@ extern "C" int npub_w8a8_gemm(const int8_t* A, int64_t lda, const float* a_scale
     NPUB_CHECK_ARG(ldc >= (swiglu ? N / 2 : N) && (!R || ldr >= N));
     NPUB_CHECK_ARG(npub_aligned(a_scale, 4) && npub_aligned(w_scale, 2) && npub_aligned(C, 2) && npub_aligned(R, 2));
     if (K > 131056) return NPUB_ERR_UNSUPPORTED;  // 131072 * 128 * 128 = 2^31
+    if (M > 0x7fffff00 || N > 0x7fffff00) return NPUB_ERR_UNSUPPORTED;
     Params p;
     memset(&p, 0, sizeof(p));
     p.M = M;
@@ -640,18 +674,19 @@ extern "C" int npub_w8a8_gemm(const int8_t* A, int64_t lda, const float* a_scale
     p.swiglu = swiglu ? 1 : 0;
     p.vec = ldc % 8 == 0 && npub_aligned(C, 16) && npub_aligned(w_scale, 16) && (!R || (ldr % 8 == 0 && npub_aligned(R, 16)));
     p.err = npub_internal_device_error_word();
-    const Choice c = pick(M, N, p.k_tiles);
-    if (c.bt && (M + c.bt - 1) / c.bt > 65535) return NPUB_ERR_UNSUPPORTED;
-    int rc = make_tmap_3d(&p.tmA, true, A, (uint64_t)K, (uint64_t)M, 1, (uint64_t)lda, (uint64_t)lda * M,
-                          c.bt ? (uint32_t)c.bt : 128, 1, true, BK);
+    const Choice c = pick(M, N, p.k_tiles, p.vec);
+    const bool tile = c.bt < 32;
+    const uint32_t rows_a = tile ? 128 * c.bt : c.bt, rows_w = tile ? 256 : 128;
+    int rc = make_tmap_3d(&p.tmA, true, A, (uint64_t)K, (uint64_t)M, 1, (uint64_t)lda, (uint64_t)lda * M, rows_a, 1, true, BK);
     if (rc) return rc;
-    rc = make_tmap_3d(&p.tmW, true, W, (uint64_t)K, (uint64_t)N, 1, (uint64_t)ldw, (uint64_t)ldw * N, 128, 1, true, BK);
+    rc = make_tmap_3d(&p.tmW, true, W, (uint64_t)K, (uint64_t)N, 1, (uint64_t)ldw, (uint64_t)ldw * N, rows_w, 1, true, BK);
     if (rc) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (c.bt) {
         case 32: return launch_few<32>(p, c.splits, st);
         case 64: return launch_few<64>(p, c.splits, st);
         case 128: return launch_few<128>(p, c.splits, st);
-        default: return launch_tile(p, st);
+        case kTile1: return launch_tile<1>(p, st);
+        default: return launch_tile<2>(p, st);
     }
 }

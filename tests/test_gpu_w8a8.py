@@ -131,6 +131,30 @@ def test_matmul_forms(cuda_device, M, kw):
         check(M, N, 528, **kw)
 
 
+@pytest.mark.parametrize("M,N,K", [(1200, 11200, 64), (1024, 18688, 4096), (2100, 9000, 2304), (4000, 2500, 4096)])
+@pytest.mark.parametrize("kw", [{}, dict(res=True), dict(swiglu=True), dict(res=True, ldc=3)])
+def test_matmul_several_tiles_of_a_cta(cuda_device, M, N, K, kw):
+    check(M, N, K, **kw)
+
+
+def test_many_calls_in_flight(cuda_device):
+    """Rows quantised and multiplied again and again: every call ends, with the same bits."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for M, N, K in ((4096, 11008, 2048), (2048, 18688, 4096), (64, 4096, 4096)):
+        x = torch.randn((M, K), generator=g, device="cuda").half()
+        gamma = torch.ones(K, device="cuda", dtype=torch.float16)
+        w = torch.randint(-127, 128, (N, K), generator=g, device="cuda", dtype=torch.int8)
+        ws = torch.full((N,), 1e-3, device="cuda", dtype=torch.float16)
+        first = None
+        for i in range(400):
+            q, s = nb.quantize_rows(x, gamma=gamma)
+            c = nb.matmul_w8a8(q, s, w, ws, swiglu=True)
+            if i % 100 == 0:
+                first = c if first is None else first
+                assert torch.equal(c, first)
+        assert torch.equal(c, first) and npu.device_error() == 0
+
+
 def test_matmul_largest_sums(cuda_device):
     """-128 * -128 over the longest K: 2^31 - 2^18 exactly, and its negative side."""
     for M in (2, 300):
