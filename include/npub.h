@@ -451,9 +451,8 @@ size_t npub_attention_paged_decode_workspace(int batch, int64_t ctx_len, int sha
  * npub_attention_paged / npub_attention_paged_decode over such pages.  A call
  * with max_new > 0 and max_new * heads <= 128 * kv_heads (every
  * decode step) reads the 8-bit keys as they are; rows of a sequence past its
- * first max_new may be zeros, as above.  Any other call first writes the keys
- * as fp16 (values past 65504 become infinite) to its workspace, which holds
- * batch * ctx_len of them: there ctx_len is a limit, and the rows of a sequence
+ * first max_new may be zeros, as above.  Any other call first writes the keys'
+ * integers as fp16 to its workspace, which holds batch * ctx_len of them: there ctx_len is a limit, and the rows of a sequence
  * with more keys than ctx_len rounded up to 128 are zeros.  ctx_len 0: the
  * table's width.  heads <= 128 * kv_heads.
  * batch <= 65535. */

@@ -40,6 +40,10 @@ struct PackedArgs {
     // [splits, total_q, heads]: (row's reference score, sum of exponentials); (-inf, 0) where the row has no key
     // in the range, (-inf, 1) where all its scores there are -inf (part_o is not written then)
     float2* part_ml;
+    // pages of whole numbers (null: of values): for every 16 keys, [batch, kv_heads, max_pages * page_size / 16],
+    // (log2(e) scale s_k, log2 s_v), with which a score's sum of products becomes the exponent of its weight times s_v;
+    // part_ml's references are such exponents
+    const float2* key_scale;
 };
 
 int fmha_packed(const PackedArgs& a, cudaStream_t st);

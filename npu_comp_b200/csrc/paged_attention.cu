@@ -212,8 +212,9 @@ struct PlanQ8 {
     int tiles, rows;              // paged_decode_q8: tiles of a sequence and kv head, and the rows of one
     int width;                    // tile kernel: fp16 pages of 128 keys per sequence
     bool list;                    // paged_list_q8 instead
-    size_t parts, pages, tables;  // bytes of the partials, of the fp16 K (or V), and of their table and lengths
-    size_t bytes() const { return parts + 2 * pages + tables; }
+    size_t parts, pages, scales, tables;  // bytes of the partials, of the fp16 K (or V), of two scales for 16 keys, and
+                                          // of the table and lengths
+    size_t bytes() const { return parts + 2 * pages + scales + tables; }
 };
 
 PlanQ8 make_plan_q8(int batch, int total, int max_new, int64_t ctx, int heads, int kv_heads, int head_dim) {
@@ -248,6 +249,7 @@ PlanQ8 make_plan_q8(int batch, int total, int max_new, int64_t ctx, int heads, i
         const int64_t width = ceil_div(ctx, 128);
         pl.width = width > 0x7fffffff ? 0x7fffffff : (int)width;
         pl.pages = (size_t)batch * width * kv_heads * 128 * head_dim * sizeof(__half);
+        pl.scales = ((size_t)batch * width * kv_heads * 8 * sizeof(float2) + 255) / 256 * 256;
         pl.tables = ((size_t)batch * (width + 1) * sizeof(int32_t) + 255) / 256 * 256;
     }
     pl.parts = (plan_bytes(pl.p, total, heads, head_dim) + 255) / 256 * 256;
@@ -265,10 +267,13 @@ int run_plan_q8(const PlanQ8& pl, PackedArgs& a, const float* ks, const float* v
     if (!pl.p.few) {
         if ((int64_t)a.batch * pl.width > 0x7fffffff) return NPUB_ERR_UNSUPPORTED;
         uint8_t *k = ws + pl.parts, *v = k + pl.pages;
-        int32_t* table = reinterpret_cast<int32_t*>(v + pl.pages);
+        float2* key_scale = reinterpret_cast<float2*>(v + pl.pages);
+        int32_t* table = reinterpret_cast<int32_t*>(v + pl.pages + pl.scales);
         int32_t* lens = table + (int64_t)a.batch * pl.width;
-        const int rc = expand_q8(a, ks, vs, pl.width, k, v, table, lens, st);
+        const int rc = expand_q8(a, ks, vs, pl.width, k, v, table, lens, key_scale, st);
         if (rc) return rc;
+        a.key_scale = key_scale;
+        a.scale = 0.6931472f;  // of exponents of 2, where partials are joined
         a.kv.k = k;
         a.kv.v = v;
         a.kv.table = table;

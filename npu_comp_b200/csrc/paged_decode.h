@@ -23,9 +23,9 @@ int paged_decode_q8(const PackedArgs& a, const float* k_scales, const float* v_s
 size_t paged_list_q8_workspace(int batch, int kv_heads, int head_dim, int rows, int tiles);
 int paged_list_q8(const PackedArgs& a, const float* k_scales, const float* v_scales, int rows, int tiles, void* workspace,
                   cudaStream_t st);
-// Every sequence's keys as fp16 pages of 128 keys, `width` of them per sequence (page b * width + w), with their table and
-// the lengths (0 for a sequence of more than 128 * width keys).
+// Every sequence's whole numbers as fp16 pages of 128 keys, `width` of them per sequence (page b * width + w), with their
+// table, the lengths (0 for a sequence of more than 128 * width keys) and PackedArgs::key_scale.
 int expand_q8(const PackedArgs& a, const float* k_scales, const float* v_scales, int width, void* k_out, void* v_out,
-              int32_t* table_out, int32_t* lens_out, cudaStream_t st);
+              int32_t* table_out, int32_t* lens_out, float2* key_scale, cudaStream_t st);
 
 }  // namespace npub

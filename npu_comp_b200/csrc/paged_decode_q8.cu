@@ -1041,15 +1041,16 @@ int launch_list(const Params& p, int ctas, cudaStream_t st) {
     return launch_pdl(paged_list_combine_kernel<HD, kMaxRows, false>, dim3((unsigned)((n + 3) / 4)), dim3(128), 0, st, p);
 }
 
-// 16 columns of a key per thread and step: s q in fp16 (2^-11; the products with fp16 take no more), one block per
-// (key block of 128, kv head, sequence).
+// 16 columns of a key per thread and step: the whole numbers as fp16, which holds them exactly, and the scales of every 16
+// keys; one block per (key block of 128, kv head, sequence).
 __global__ void __launch_bounds__(256) expand_q8_kernel(const int8_t* __restrict__ kp, const int8_t* __restrict__ vp,
                                                         const float* __restrict__ ks, const float* __restrict__ vs,
                                                         const int32_t* __restrict__ table, int64_t ldt, int n_pages,
                                                         int page_shift, int max_keys, const int32_t* __restrict__ lens,
                                                         int kv_heads, int head_dim, int width, __half* __restrict__ k_out,
                                                         __half* __restrict__ v_out, int32_t* __restrict__ table_out,
-                                                        int32_t* __restrict__ lens_out) {
+                                                        int32_t* __restrict__ lens_out, float c,
+                                                        float2* __restrict__ key_scale) {
     pdl_trigger();
     pdl_wait();
     const int w = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
@@ -1060,6 +1061,17 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(const int8_t* __restrict
         if (w == 0) lens_out[b] = len;
     }
     const int n = min(128, len - w * 128);
+    if (threadIdx.x < 8 && n > 0) {  // of keys behind the last one too: they weigh nothing times this
+        const int key = w * 128 + (int)threadIdx.x * 16;
+        const int id = key < len ? __ldg(table + (int64_t)b * ldt + (key >> page_shift)) : -1;
+        const bool in = id >= 0 && id < n_pages;
+        const float sk = in ? __ldg(ks + (int64_t)id * kv_heads + kvh) : 0.0f;
+        const float sv = in ? __ldg(vs + (int64_t)id * kv_heads + kvh) : 0.0f;
+        // log2 s_v is an addend of the exponents: within [-60, 60], below which a V is zero in fp16 and above which infinite
+        const float e = fminf(fmaxf(log2f(sv), -60.0f), 60.0f);
+        const int64_t g = ((int64_t)b * kv_heads + kvh) * width * 8 + w * 8 + threadIdx.x;
+        key_scale[g] = isfinite(sk) && isfinite(sv) ? make_float2(c * sk, sv > 0.0f ? e : -60.0f) : make_float2(NAN, NAN);
+    }
     const int units = head_dim / 16;
     const int64_t to = ((int64_t)(b * (int64_t)width + w) * kv_heads + kvh) * 128 * head_dim;
     for (int i = threadIdx.x; i < n * units * 2; i += 256) {
@@ -1070,16 +1082,16 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(const int8_t* __restrict
         uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if (id >= 0 && id < n_pages) {
             const int64_t at = (int64_t)id * kv_heads + kvh;
-            const float s = __ldg((v ? vs : ks) + at);
             const uint4 r = *reinterpret_cast<const uint4*>(
                 (v ? vp : kp) + ((at << page_shift) + (key & ((1 << page_shift) - 1))) * head_dim + col);
             const uint32_t x[4] = {r.x, r.y, r.z, r.w};
             uint32_t* y = reinterpret_cast<uint32_t*>(o);
-            const float fs = isfinite(s) ? s : NAN;
+            if (!v || !(__ldg(vs + at) < 0x1p-60f)) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                y[2 * e] = h2((float)(int8_t)x[e] * fs, (float)(int8_t)(x[e] >> 8) * fs);
-                y[2 * e + 1] = h2((float)(int8_t)(x[e] >> 16) * fs, (float)(int8_t)(x[e] >> 24) * fs);
+                for (int e = 0; e < 4; ++e) {
+                    y[2 * e] = h2((float)(int8_t)x[e], (float)(int8_t)(x[e] >> 8));
+                    y[2 * e + 1] = h2((float)(int8_t)(x[e] >> 16), (float)(int8_t)(x[e] >> 24));
+                }
             }
         }
         uint4* dst = reinterpret_cast<uint4*>((v ? v_out : k_out) + to + (int64_t)row * head_dim + col);
@@ -1166,7 +1178,7 @@ int paged_list_q8(const PackedArgs& a, const float* k_scales, const float* v_sca
 }
 
 int expand_q8(const PackedArgs& a, const float* k_scales, const float* v_scales, int width, void* k_out, void* v_out,
-              int32_t* table_out, int32_t* lens_out, cudaStream_t st) {
+              int32_t* table_out, int32_t* lens_out, float2* key_scale, cudaStream_t st) {
     int shift = 0;
     while ((1 << shift) < a.kv.page_size) ++shift;
     const int64_t mk = (int64_t)a.kv.max_pages << shift;
@@ -1174,7 +1186,7 @@ int expand_q8(const PackedArgs& a, const float* k_scales, const float* v_scales,
                       reinterpret_cast<const int8_t*>(a.kv.k), reinterpret_cast<const int8_t*>(a.kv.v), k_scales, v_scales,
                       a.kv.table, a.kv.ldt, a.kv.n_pages, shift, (int)(mk > 0x7ff00000 ? 0x7ff00000 : mk), a.lens,
                       a.kv_heads, a.head_dim, width, reinterpret_cast<__half*>(k_out), reinterpret_cast<__half*>(v_out),
-                      table_out, lens_out);
+                      table_out, lens_out, a.scale * 1.4426950408889634f, key_scale);
 }
 
 }  // namespace npub

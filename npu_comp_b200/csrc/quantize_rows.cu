@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const QuantArgs 
     }
     most = __uint_as_float(top);
     float y = most;
-    if (GAMMA) y = most * (1.0f / sqrtf(ss / (float)a.cols + a.eps));
+    if (GAMMA && most > 0.0f) y = most * (1.0f / sqrtf(ss / (float)a.cols + a.eps));  // zeros stay zeros with eps = 0 too
     const bool fine = top < 0x7f800000u;
     if (threadIdx.x == 0) a.scale[row] = fine ? y / 127.0f : NAN;
     // the smallest |t| that is not 0 is 2^-48

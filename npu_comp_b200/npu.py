@@ -1059,7 +1059,7 @@ def attention_paged_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     max_new: at least the new rows of any sequence (0: not known).  With at most
     128 * kv_heads / heads of them the 8-bit keys are read as they are, and a
     sequence that has more than max_new rows all the same may get zeros for those
-    past them.  Any other call first writes the keys as fp16 to its workspace,
+    past them.  Any other call first writes the keys' integers as fp16 to its workspace,
     batch * ctx_len of them: ctx_len is then a limit, and a sequence with more
     keys (than ctx_len rounded up to 128; 0: the table's width) gets zeros."""
     dev, T, qc, ldq = _first16(q, "q")

@@ -81,6 +81,16 @@ def test_quantize_rows_halves_extremes_and_values_that_are_not_finite(cuda_devic
     assert torch.isnan(z[:3]).all() and torch.isfinite(z[3]).all()
 
 
+def test_quantize_rows_of_zeros(cuda_device):
+    x = torch.zeros((3, 64), device="cuda", dtype=torch.float16)
+    x[1, 7] = 2.0
+    for gamma in (None, torch.ones(64, device="cuda").half()):
+        for eps in (1e-5, 0.0):
+            q, s = nb.quantize_rows(x, gamma=gamma, eps=eps)
+            assert s[0] == 0 and s[2] == 0 and not q[0].any() and not q[2].any()
+            assert q[1, 7] == 127 and q[1].count_nonzero() == 1
+
+
 def product64(q, s, w, ws, res=None, swiglu=False):
     z = (q.double() @ w.double().T) * s.double()[:, None] * ws.double()
     if swiglu:
