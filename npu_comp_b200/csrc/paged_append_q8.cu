@@ -78,7 +78,7 @@ __device__ __forceinline__ void head_row(const AppendArgs& a, const __half* x, c
         float ss = y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3];
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-        const float inv = rsqrtf(ss * a.inv_hd + a.eps);
+        const float inv = 1.0f / sqrtf(ss * a.inv_hd + a.eps);
         if (c.on) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(g + c.ca));
             const float2 h = __half22float2(*reinterpret_cast<const __half2*>(g + c.cb));
@@ -109,8 +109,8 @@ __device__ __forceinline__ uint32_t max_bits(const float (&y)[4]) {  // as integ
     return m;
 }
 
-// The page's scale behind rows of the largest magnitude `top` (bits), what they are multiplied with, and what the rows
-// ahead of them are (1: left).
+// The page's scale behind rows of the largest magnitude `top` (bits), its reciprocal (0 where all is 0), and what the rows
+// ahead of them are multiplied with (1: left).
 struct Step {
     float scale, inv, old;
 };
@@ -123,8 +123,13 @@ __device__ __forceinline__ Step step_of(float before, uint32_t top) {
     s.old = s.scale > before && s.scale > 1e-37f ? before / s.scale : 1.0f;
     return s;
 }
-// round(y / s') in the low byte: |y inv| is at most 127 (1 + 2^-22), and adding 1.5 * 2^23 rounds it, halves to even.
-__device__ __forceinline__ uint32_t q8(float y, float inv) { return __float_as_uint(fmaf(y, inv, 12582912.0f)); }
+// round(y / s') in the low byte: |y / s'| is at most 127 (1 + 2^-22), and adding 1.5 * 2^23 rounds it, halves to even.  The
+// quotient y inv is corrected by its remainder: halves are not rare (half of the largest value is 63.5), and with the
+// reciprocal's rounding alone they fall to either side (error of a prompt's keys and values against 64 bits a third more).
+__device__ __forceinline__ uint32_t q8(float y, const Step& s) {
+    const float t = y * s.inv;
+    return __float_as_uint(fmaf(fmaf(-t, s.scale, y), s.inv, t) + 12582912.0f);
+}
 __device__ __forceinline__ uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
@@ -175,7 +180,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32) append_decode_q8_kernel(con
     const Step s = step_of(before, __reduce_max_sync(0xffffffffu, max_bits(y)));
     if (c.on) {
         int8_t* dst = rows + (int64_t)slot * a.hd;
-        const uint32_t w = bytes4(q8(y[0], s.inv), q8(y[1], s.inv), q8(y[2], s.inv), q8(y[3], s.inv));
+        const uint32_t w = bytes4(q8(y[0], s), q8(y[1], s), q8(y[2], s), q8(y[3], s));
         *reinterpret_cast<uint16_t*>(dst + c.ca) = (uint16_t)w;
         *reinterpret_cast<uint16_t*>(dst + c.cb) = (uint16_t)(w >> 16);
     }
@@ -284,7 +289,7 @@ __global__ void __launch_bounds__(kMaxPackedThreads, 1) append_packed_q8_kernel(
 #pragma unroll
                     for (int e = 0; e < 16; ++e) ss = fmaf(y[i][e], y[i][e], ss);
                     for (int m = a.units_p2 >> 1; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-                    const float inv = rsqrtf(ss * a.inv_hd + a.eps);
+                    const float inv = 1.0f / sqrtf(ss * a.inv_hd + a.eps);
                     uint4 g[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
                     if (act) {
                         g[0] = __ldg(reinterpret_cast<const uint4*>(a.gk + c0));
@@ -328,8 +333,8 @@ __global__ void __launch_bounds__(kMaxPackedThreads, 1) append_packed_q8_kernel(
                 uint32_t w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    w[e] = bytes4(q8(y[i][4 * e], s.inv), q8(y[i][4 * e + 1], s.inv), q8(y[i][4 * e + 2], s.inv),
-                                  q8(y[i][4 * e + 3], s.inv));
+                    w[e] = bytes4(q8(y[i][4 * e], s), q8(y[i][4 * e + 1], s), q8(y[i][4 * e + 2], s),
+                                  q8(y[i][4 * e + 3], s));
                 int8_t* out = dst + (int64_t)(sl + r) * a.hd;
                 *reinterpret_cast<uint2*>(out + c0) = make_uint2(w[0], w[1]);
                 *reinterpret_cast<uint2*>(out + c1) = make_uint2(w[2], w[3]);
