@@ -17,8 +17,12 @@
 // offsets alone: one block (packed rows) or one warp (decode steps) takes a
 // page's new rows of one head, finds their maximum, and stores.
 //
-// Bound: HBM for prompts (the qkv rows read, q and the 8-bit rows written); the
-// launch and a few memory latencies for a decode step.
+// Bound: the launch and a few memory latencies for a decode step (250 rows of 32 /
+// 8 heads of 128: 5.5 us).  For prompts HBM (the qkv rows read, q and the 8-bit
+// rows written) is the floor, 14 us for 4096 rows of those heads with norms; they
+// take 33.7, the query heads' launch about 14 at half of the issue slots, the
+// pages' the rest, on 16 warps an SM (a thread holds 64 values) that first look
+// for their pages.  8192 rows: 54 us.
 #include "gemm_tc.h"
 #include "paged_append.cuh"
 
