@@ -969,6 +969,7 @@ __global__ void __launch_bounds__(kCoop ? 256 : 128) paged_list_combine_kernel(c
     // the first part's warp had other items ahead of this one or not; of the others it is the first
     auto slot = [&](int i) { return (int64_t)(i ? (at.x & ~1) + 2 * i : at.x) * kMaxRows + r; };
     float m = -INFINITY, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+    bool any = false;  // a part with a key
     constexpr int kStride = kCoop ? 8 : 1;
     for (int i0 = kCoop ? warp : 0; i0 < n; i0 += 8 * kStride) {  // eight loads in flight
         float4 v[8];
@@ -986,15 +987,18 @@ __global__ void __launch_bounds__(kCoop ? 256 : 128) paged_list_combine_kernel(c
         float mm = m;
 #pragma unroll
         for (int i = 0; i < 8; ++i) mm = fmaxf(mm, ml[i].x);
-        const float f0 = sum != 0.0f ? ex2_approx(m - mm) : 0.0f;
+        const float ref = mm == -INFINITY ? 0.0f : mm, f0 = ex2_approx(m - ref);
         m = mm;
         sum *= f0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = f0 != 0.0f ? acc[e] * f0 : 0.0f;
+        for (int e = 0; e < 4; ++e) acc[e] *= f0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float f = ml[i].y != 0.0f ? ex2_approx(ml[i].x - mm) : 0.0f;
-            if (f == 0.0f) continue;  // no key, or no weight beside the others
+            // A part without a finite score weighs nothing beside others, but its sum counts where it is NaN (0 * NaN).
+            // O is finite unless the sum is NaN.
+            if (ml[i].y == 0.0f) continue;  // no key
+            any = true;
+            const float f = ex2_approx(ml[i].x - ref);
             sum += f * ml[i].y;
             acc[0] += f * v[i].x;
             acc[1] += f * v[i].y;
@@ -1004,15 +1008,17 @@ __global__ void __launch_bounds__(kCoop ? 256 : 128) paged_list_combine_kernel(c
     }
     if (kCoop) {
         sums[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        if (lane == 0) tops[warp] = make_float2(m, sum);
+        if (lane == 0) tops[warp] = make_float2(m, any && sum == 0.0f ? 1.0f : sum);  // (-inf, 1) as the parts are
         __syncthreads();
         if (warp) return;
         m = -INFINITY;
         for (int i = 0; i < 8; ++i) m = fmaxf(m, tops[i].x);
+        const float ref = m == -INFINITY ? 0.0f : m;
         sum = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
         for (int i = 0; i < 8; ++i) {
-            const float f = tops[i].y != 0.0f ? ex2_approx(tops[i].x - m) : 0.0f;
-            if (f == 0.0f) continue;
+            if (tops[i].y == 0.0f) continue;
+            any = true;
+            const float f = ex2_approx(tops[i].x - ref);
             const float4 v = sums[i][lane];
             sum += f * tops[i].y;
             acc[0] += f * v.x;
@@ -1021,6 +1027,7 @@ __global__ void __launch_bounds__(kCoop ? 256 : 128) paged_list_combine_kernel(c
             acc[3] += f * v.w;
         }
     }
+    if (any && m == -INFINITY) sum = NAN;  // keys, but all scores -inf: 0 / 0
     if (!act) return;
     const float inv = 1.0f / sum;
     uint2 o;

@@ -1,0 +1,91 @@
+"""Scales that are not finite in a long 8-bit paged cache: rows that see such a
+page are NaN in that head, wherever the keys are cut, and all others are as the
+64-bit form has them (bounds of test_gpu_paged_q8)."""
+import math
+
+import pytest
+import torch
+
+import npu_comp_b200 as nb
+from npu_comp_b200 import _lib, npu
+from paged_exact import same
+from test_gpu_paged_q8 import Cache, expected, i32, offsets
+
+pytestmark = pytest.mark.gpu
+
+
+def spoil(c, b, lo, hi, head, which, value):
+    """The scale of every page of sequence b that holds one of its keys lo .. hi - 1."""
+    pages = c.table[b, lo // c.ps:(hi - 1) // c.ps + 1].long()
+    (c.ks if which == "k" else c.vs)[pages, head] = value
+
+
+def attend(c, q, new, H, **kw):
+    o = (nb.attention_paged_decode_q8(q, *c.args, c.lens, heads=H) if kw.pop("decode", False)
+         else nb.attention_paged_q8(q, *c.args, c.lens, offsets(new), heads=H, **kw))
+    assert npu.device_error() == 0
+    return o
+
+
+def is_list(B, total, max_new, keys, H, KV, hd, ps):
+    """The call takes the list of all sequences' steps: the only few-row kernel with a workspace."""
+    ctx = ((max(keys) + ps - 1) // ps + 1) * ps  # the table's width
+    return _lib.query("npub_attention_paged_q8_workspace", B, total, max_new, ctx, H, KV, hd) > 0
+
+
+@pytest.mark.parametrize("which,value", [("k", math.nan), ("v", math.nan), ("k", math.inf), ("v", -math.inf)])
+@pytest.mark.parametrize("ps", [16, 128, 256])
+@pytest.mark.parametrize("where", ["first", "middle", "last", "one page"])
+@pytest.mark.parametrize("n", [1, 6])
+def test_one_long_sequence(cuda_device, which, value, ps, where, n):
+    """16384 keys of 8 heads are 1024 parts of 128 keys: whole parts have no finite score (few rows: the combination by
+    blocks)."""
+    H, KV, hd, m = 32, 8, 128, 16384
+    assert is_list(1, n, n, [m], H, KV, hd, ps)
+    c = Cache([m], KV, hd, ps, seed=ps + n)
+    lo, hi = {"first": (0, 512), "middle": (7936, 8448), "last": (m - 512, m), "one page": (5120, 5121)}[where]
+    spoil(c, 0, lo, hi, 3, which, value)
+    q = torch.randn((n, H * hd), generator=torch.Generator().manual_seed(n)).half().cuda()
+    o = attend(c, q, [n], H, decode=n == 1, **({} if n == 1 else {"max_new": n}))
+    nan = torch.isnan(o.view(n, KV, -1))
+    assert nan[:, 3].all() and not nan[:, :3].any() and not nan[:, 4:].any()
+    want, bound = expected(c, 0, q.view(n, H, hd), 1 / math.sqrt(hd), True)
+    same(o, want, bound)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("ps", [32, 256])
+@pytest.mark.parametrize("n", [1, 2])
+def test_many_long_sequences(cuda_device, which, ps, n):
+    """24 sequences, the combination by warps: parts of several hundred keys, of which some sequences' are all spoilt."""
+    H, KV, hd, B = 32, 8, 128, 24
+    keys = [6000 + 100 * b for b in range(B)]
+    assert is_list(B, B * n, n, keys, H, KV, hd, ps)
+    c = Cache(keys, KV, hd, ps, seed=ps + n)
+    at = {b: 0 if b % 2 else keys[b] - 2600 for b in range(0, B, 3)}
+    for b, lo in at.items():
+        spoil(c, b, lo, lo + 2500, b % KV, which, math.nan)
+    q = torch.randn((B * n, H * hd), generator=torch.Generator().manual_seed(n)).half().cuda()
+    o = attend(c, q, [n] * B, H, max_new=n).view(B, n, KV, -1)
+    nan = torch.isnan(o)
+    for b in range(B):
+        for h in range(KV):
+            assert nan[b, :, h].all() if b in at and h == b % KV else not nan[b, :, h].any(), (b, h)
+    for b in (0, 1, 9, B - 1):
+        want, bound = expected(c, b, q[b * n:b * n + n].view(n, H, hd), 1 / math.sqrt(hd), True)
+        same(o[b].reshape(n, -1), want, bound)
+
+
+def test_nan_beside_scores_far_above(cuda_device):
+    """A part with a NaN and finite scores more than 126 powers of two below the others'."""
+    H, KV, hd, ps, m = 8, 8, 128, 16, 32768
+    assert is_list(1, 1, 1, [m], H, KV, hd, ps)
+    c = Cache([m], KV, hd, ps, seed=5)
+    q = torch.ones((1, H * hd)).half().cuda()
+    c.kp[:] = 1
+    c.ks[:] = 1.0
+    c.ks[c.table[0, :128].long()] = 30.0  # the first 2048 keys score 30 * 128 / sqrt(128), the others a thirtieth of it
+    spoil(c, 0, 20000, 20001, 2, "k", math.nan)
+    o = attend(c, q, [1], H, decode=True)
+    nan = torch.isnan(o.view(KV, -1))
+    assert nan[2].all() and not nan[:2].any() and not nan[3:].any()
