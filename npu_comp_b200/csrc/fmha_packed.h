@@ -42,6 +42,7 @@ struct PackedArgs {
     float2* part_ml;
     // pages of whole numbers (null: of values): for every 16 keys, [batch, kv_heads, max_pages * page_size / 16],
     // (log2(e) scale s_k, log2 s_v), with which a score's sum of products becomes the exponent of its weight times s_v;
+    // (NaN, 0) where a scale is not finite;
     // part_ml's references are such exponents
     const float2* key_scale;
 };

@@ -133,7 +133,8 @@ __device__ __forceinline__ float usable(float scale, bool v, bool in_pool) {
     return v && scale < 9.094947e-13f ? 9.094947e-13f : scale;
 }
 
-// c s_k 2^24 of a usable K scale; log2 and reciprocal of a usable V scale (to 2^-22 and 2^-23: as close as the scores)
+// c s_k 2^24 of a usable K scale; log2 and reciprocal of a usable V scale (to 2^-22 and 2^-23: as close as the scores).  The
+// reciprocal of NaN is 1: the scores carry the NaN to the rows that see the page, and masked ones weigh 0 times this.
 constexpr float kSubnormal = 16777216.0f;
 __device__ __forceinline__ float log2_of(float v) {
     float r;
@@ -143,7 +144,7 @@ __device__ __forceinline__ float log2_of(float v) {
 __device__ __forceinline__ float inverse_of(float v) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
+    return isnan(v) ? 1.0f : r;
 }
 // 16 int8 as fp16 pairs (q + 128) 2^-24.
 __device__ __forceinline__ void bytes_to_subnormals(uint4 raw, uint32_t (&f)[8]) {
@@ -1084,7 +1085,8 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(const int8_t* __restrict
         // log2 s_v is an addend of the exponents: within [-60, 60], below which a V is zero in fp16 and above which infinite
         const float e = fminf(fmaxf(log2f(sv), -60.0f), 60.0f);
         const int64_t g = ((int64_t)b * kv_heads + kvh) * width * 8 + w * 8 + threadIdx.x;
-        key_scale[g] = isfinite(sk) && isfinite(sv) ? make_float2(c * sk, sv > 0.0f ? e : -60.0f) : make_float2(NAN, NAN);
+        // a scale that is not finite: NaN scores, which a mask replaces, and a finite addend, which it leaves in the sum
+        key_scale[g] = isfinite(sk) && isfinite(sv) ? make_float2(c * sk, sv > 0.0f ? e : -60.0f) : make_float2(NAN, 0.0f);
     }
     const int units = head_dim / 16;
     const int64_t to = ((int64_t)(b * (int64_t)width + w) * kv_heads + kvh) * 128 * head_dim;

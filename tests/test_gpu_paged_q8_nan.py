@@ -89,3 +89,32 @@ def test_nan_beside_scores_far_above(cuda_device):
     o = attend(c, q, [1], H, decode=True)
     nan = torch.isnan(o.view(KV, -1))
     assert nan[2].all() and not nan[:2].any() and not nan[3:].any()
+
+
+@pytest.mark.parametrize("which,value", [("k", math.nan), ("v", math.nan), ("v", math.inf)])
+@pytest.mark.parametrize("m,n,max_new,hd", [
+    (208, 32, 32, 128),     # one CTA
+    (1010, 24, 24, 64),     # ranges of a cluster
+    (16400, 24, 24, 128),   # the list
+    (300, 100, 100, 128),   # tiles
+    (5005, 30, 0, 64),      # tiles, keys in parts
+    (36000, 200, 200, 128),
+])
+def test_pages_behind_a_row(cuda_device, which, value, m, n, max_new, hd):
+    """Rows that the causal mask keeps from a page whose scale is not finite do not see it; the rows behind them do."""
+    H, KV, ps = 4, 4, 16
+    c = Cache([m, 40], KV, hd, ps, seed=m)
+    from_key = (m - 1) // ps * ps  # of the last page
+    clean = n - (m - from_key)     # rows that end ahead of it
+    assert 0 < clean < n
+    q = torch.randn((n + 1, H * hd), generator=torch.Generator().manual_seed(n)).half().cuda()
+    want, bound = expected(c, 0, q[:n].view(n, H, hd), 1 / math.sqrt(hd), True)
+    alone, alone_bound = expected(c, 1, q[n:].view(1, H, hd), 1 / math.sqrt(hd), True)
+    spoil(c, 0, from_key, m, 1, which, value)
+    o = attend(c, q, [n, 1], H, max_new=max_new)
+    nan = torch.isnan(o[:n].view(n, H, hd))
+    assert nan[clean:, 1].all()
+    assert not nan[clean:, 0].any() and not nan[clean:, 2:].any() and not nan[:clean].any()
+    want.view(n, H, hd)[clean:, 1] = math.nan
+    same(o[:n], want, bound)
+    same(o[n:], alone, alone_bound)
