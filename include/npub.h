@@ -452,9 +452,11 @@ size_t npub_attention_paged_decode_workspace(int batch, int64_t ctx_len, int sha
  * with max_new > 0 and max_new * heads <= 128 * kv_heads (every
  * decode step) reads the 8-bit keys as they are; rows of a sequence past its
  * first max_new may be zeros, as above.  Any other call first writes the keys'
- * integers as fp16 to its workspace, which holds batch * ctx_len of them: there ctx_len is a limit, and the rows of a sequence
- * with more keys than ctx_len rounded up to 128 are zeros.  ctx_len 0: the
- * table's width.  heads <= 128 * kv_heads.
+ * integers as fp16 to its workspace, which holds ctx_len of them for each
+ * sequence, up to 2 GiB; where that is less than the batch needs (but one
+ * sequence's at least), the sequences take turns in it.  There ctx_len is a
+ * limit: the rows of a sequence with more keys than ctx_len rounded up to 128
+ * are zeros.  ctx_len 0: the table's width.  heads <= 128 * kv_heads.
  * batch <= 65535. */
 int npub_rope_paged_append_q8(const void* qkv, int64_t ldx, void* q_out, int64_t ldq, int tokens, int q_heads,
                               int kv_heads, int head_dim, int rot_dim, int interleaved, const int32_t* positions,

@@ -207,10 +207,15 @@ int run_plan(const Plan& pl, PackedArgs& a, void* workspace, size_t workspace_by
 // are and behind the pass: 24 sequences of 6 tiles 88 and 153 us, of 9 tiles 142 and 169, of 14 tiles 226 and 173; 4
 // sequences of 5 tiles 133 and 156, of 10 tiles 220 and 160.
 constexpr int kQ8Tiles = 8;
+// Bytes of the fp16 copy (one sequence's at least): the sequences take turns in it, each group of them behind the one before.
+// Measured, 32 / 8 heads of 128, all sequences at once, groups of 4, 2 and 1 GiB: 16 of 65000 keys (4 GiB at once) 3330, 3391,
+// 3339 and 4137 us; one of 65000 and 15 of 3000 697, 669, 735 and 969; 64 of 1000 keys in a table of 131072 (32 GiB) without
+// ctx_len 1098, 1650, 2442 and 5200, with it 231.
+constexpr int64_t kQ8Copy = (int64_t)1 << 31;
 struct PlanQ8 {
     Plan p;
     int tiles, rows;              // paged_decode_q8: tiles of a sequence and kv head, and the rows of one
-    int width;                    // tile kernel: fp16 pages of 128 keys per sequence
+    int width, seqs;              // tile kernel: fp16 pages of 128 keys per sequence, sequences of a group
     bool list;                    // paged_list_q8 instead
     size_t parts, pages, scales, tables;  // bytes of the partials, of the fp16 K (or V), of two scales for 16 keys, and
                                           // of the table and lengths
@@ -245,12 +250,19 @@ PlanQ8 make_plan_q8(int batch, int total, int max_new, int64_t ctx, int heads, i
         if (pl.list) pl.parts = paged_list_q8_workspace(batch, kv_heads, head_dim, pl.rows, pl.tiles);
         return pl;
     } else {
-        pl.p.own = tile_phase(total, batch, heads, kv_heads, max_new, ctx, num_sms(), part_us, false);
         const int64_t width = ceil_div(ctx, 128);
         pl.width = width > 0x7fffffff ? 0x7fffffff : (int)width;
-        pl.pages = (size_t)batch * width * kv_heads * 128 * head_dim * sizeof(__half);
-        pl.scales = ((size_t)batch * width * kv_heads * 8 * sizeof(float2) + 255) / 256 * 256;
-        pl.tables = ((size_t)batch * (width + 1) * sizeof(int32_t) + 255) / 256 * 256;
+        const int64_t copy = width * kv_heads * 128 * head_dim * (int64_t)sizeof(__half);  // of a sequence's K
+        const int64_t meta = width * kv_heads * 8 * (int64_t)sizeof(float2), ids = (width + 1) * (int64_t)sizeof(int32_t);
+        int64_t most = kQ8Copy / (2 * copy + meta + ids);
+        if (most < 1) most = 1;
+        const int64_t groups = ceil_div(batch, most);
+        pl.seqs = (int)ceil_div(batch, groups);
+        pl.pages = (size_t)(pl.seqs * copy);
+        pl.scales = ((size_t)(pl.seqs * meta) + 255) / 256 * 256;
+        pl.tables = ((size_t)(pl.seqs * ids) + 255) / 256 * 256;
+        // a group has its share of the rows, but its partials are numbered through all of them
+        pl.p.own = tile_phase((int)ceil_div(total, groups), pl.seqs, heads, kv_heads, max_new, ctx, num_sms(), part_us, false);
     }
     pl.parts = (plan_bytes(pl.p, total, heads, head_dim) + 255) / 256 * 256;
     return pl;
@@ -265,23 +277,32 @@ int run_plan_q8(const PlanQ8& pl, PackedArgs& a, const float* ks, const float* v
     }
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     if (!pl.p.few) {
-        if ((int64_t)a.batch * pl.width > 0x7fffffff) return NPUB_ERR_UNSUPPORTED;
+        if ((int64_t)pl.seqs * pl.width > 0x7fffffff) return NPUB_ERR_UNSUPPORTED;
         uint8_t *k = ws + pl.parts, *v = k + pl.pages;
         float2* key_scale = reinterpret_cast<float2*>(v + pl.pages);
         int32_t* table = reinterpret_cast<int32_t*>(v + pl.pages + pl.scales);
-        int32_t* lens = table + (int64_t)a.batch * pl.width;
-        const int rc = expand_q8(a, ks, vs, pl.width, k, v, table, lens, key_scale, st);
-        if (rc) return rc;
-        a.key_scale = key_scale;
-        a.scale = 0.6931472f;  // of exponents of 2, where partials are joined
-        a.kv.k = k;
-        a.kv.v = v;
-        a.kv.table = table;
-        a.kv.ldt = a.kv.max_pages = pl.width;
-        a.kv.n_pages = a.batch * pl.width;
-        a.kv.page_size = 128;
-        a.lens = lens;
-        return run_plan(pl.p, a, workspace, pl.parts, st);
+        int32_t* lens = table + (int64_t)pl.seqs * pl.width;
+        for (int b0 = 0; b0 < a.batch; b0 += pl.seqs) {
+            PackedArgs g = a;  // sequences b0 .. : rows outside of their offsets are left as they are
+            g.batch = a.batch - b0 < pl.seqs ? a.batch - b0 : pl.seqs;
+            g.cu = a.cu + b0;
+            g.lens = a.lens + b0;
+            g.kv.table = a.kv.table + b0 * a.kv.ldt;
+            int rc = expand_q8(g, ks, vs, pl.width, k, v, table, lens, key_scale, st);
+            if (rc) return rc;
+            g.key_scale = key_scale;
+            g.scale = 0.6931472f;  // of exponents of 2, where partials are joined
+            g.kv.k = k;
+            g.kv.v = v;
+            g.kv.table = table;
+            g.kv.ldt = g.kv.max_pages = pl.width;
+            g.kv.n_pages = g.batch * pl.width;
+            g.kv.page_size = 128;
+            g.lens = lens;
+            rc = run_plan(pl.p, g, workspace, pl.parts, st);
+            if (rc) return rc;
+        }
+        return NPUB_OK;
     }
     if (pl.list) return paged_list_q8(a, ks, vs, pl.rows, pl.tiles, workspace, st);
     a.splits = pl.p.own.splits;

@@ -1059,9 +1059,11 @@ def attention_paged_q8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     max_new: at least the new rows of any sequence (0: not known).  With at most
     128 * kv_heads / heads of them the 8-bit keys are read as they are, and a
     sequence that has more than max_new rows all the same may get zeros for those
-    past them.  Any other call first writes the keys' integers as fp16 to its workspace,
-    batch * ctx_len of them: ctx_len is then a limit, and a sequence with more
-    keys (than ctx_len rounded up to 128; 0: the table's width) gets zeros."""
+    past them.  Any other call first writes the keys' integers as fp16 to its
+    workspace, ctx_len of them for each sequence, up to 2 GiB; where that is less
+    than the batch needs (but one sequence's at least), the sequences take turns
+    in it.  ctx_len is then a limit, and a sequence with more keys (than ctx_len
+    rounded up to 128; 0: the table's width) gets zeros."""
     dev, T, qc, ldq = _first16(q, "q")
     (n_pages, kv_heads, ps, hd), B, W, ldt = _pool8(k_pages, v_pages, k_scales, v_scales, page_table, dev)
     if qc != heads * hd:
