@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) w8a8_tile_kernel(const __grid
                     tma_load_3d(st + MH * L::kOp, &p.tmW, &full[s], i * BK, at.n0, 0);
                 }
             }
-            if (!ok) {  // copies in flight land before the CTA leaves (the MMA thread has waited for them otherwise)
+            if (!ok) {  // copies in flight land before the CTA leaves (the MMA thread waits for them otherwise)
                 *abort_flag = 1;
                 set_err(p.err, 0x701);
                 int never = 0;
@@ -230,6 +230,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) w8a8_tile_kernel(const __grid
                 int never = 0;
                 tc_commit(drained);
                 mbar_wait_bounded(drained, 0, &never, 100000000ull);
+                for (uint32_t j = g; j < g + (uint32_t)L::kStages; ++j)  // copies that nobody has waited for
+                    mbar_wait_bounded(&full[j % L::kStages], (j / L::kStages) & 1u, &never, 100000000ull);
             }
         }
     } else if (warp >= 4) {
@@ -448,7 +450,8 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
     } else if (warp == 5) {
         if (elect_one()) {  // MMA
             constexpr uint32_t idesc = idesc_i8(128, BT);
-            for (int i = 0; i < nk && ok; ++i) {
+            int i = 0;
+            for (; i < nk; ++i) {
                 const int s = i % L::kStages;
                 ok = mbar_wait_quick(&full[s], (uint32_t)(i / L::kStages) & 1u, abort_flag);
                 if (!ok) break;
@@ -460,14 +463,20 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
                            (i > 0 || k > 0) ? 1u : 0u);
                 tc_commit(&empty[s]);
             }
-            if (ok) tc_commit(done);
-            else {
+            if (!ok) {
                 *abort_flag = 1;
                 set_err(p.err, 0x712);
             }
+            tc_commit(done);
+            if (!ok) {  // the MMAs end, and the copies that nobody has waited for land, before the CTA leaves
+                int never = 0;
+                mbar_wait_bounded(done, 0, &never, 100000000ull);
+                for (int j = i; j < min(nk, i + L::kStages); ++j)
+                    mbar_wait_bounded(&full[j % L::kStages], (uint32_t)(j / L::kStages) & 1u, &never, 100000000ull);
+            }
         }
     } else {
-        ok = __all_sync(0xffffffffu, mbar_wait_quick(done, 0, abort_flag));
+        ok = __all_sync(0xffffffffu, mbar_wait_quick(done, 0, abort_flag) && !*abort_flag);
         tc_fence_after();
         if (ok) {  // the ring is free: this CTA's sums [token][channel]
             int* sums = reinterpret_cast<int*>(smem) + warp * 32 + lane;
@@ -492,6 +501,13 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
         tmem_dealloc(tmem, BT);
     }
     if (warp < 4) {
+        // a CTA of the cluster that gave up has no sums: nothing is stored (looked up here, needed behind the sums' loads)
+        uint32_t gave_up = 0;
+        if (lane < S)
+            asm volatile("ld.shared::cluster.u32 %0, [%1];"
+                         : "=r"(gave_up)
+                         : "r"(S > 1 ? mapa_shared(smem_u32((const void*)abort_flag), (uint32_t)lane) : smem_u32((const void*)abort_flag))
+                         : "memory");
         const int tokens = min(BT, p.M - m0);
         const int n = n0 + lane * 4;
         const int left = p.N - n;  // channels of this lane
@@ -517,7 +533,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
                     v.z += got[q].z;
                     v.w += got[q].w;
                 }
-            if (left <= 0) continue;
+            if (__any_sync(0xffffffffu, gave_up != 0) || left <= 0) continue;
             const int m = m0 + j;
             const float sa = __ldg(p.sa + m);
             float z[4] = {(float)v.x * (sa * sw[0]), (float)v.y * (sa * sw[1]), (float)v.z * (sa * sw[2]),
