@@ -89,6 +89,7 @@ struct Params {
     float2* part_ml;
     int2* parts;
     int batch, tiles;  // tiles of a sequence at most
+    int slots;         // of partials, two for each warp
     int* err;
 };
 
@@ -965,7 +966,11 @@ __global__ void __launch_bounds__(kCoop ? 256 : 128) paged_list_combine_kernel(c
     }
     const int2 at = p.parts[((int64_t)b * p.kv_heads + kvh) * p.tiles + tile];
     const int n = at.y;
-    if (n <= 1) return;  // one warp had it whole
+    if (n == 1) return;  // one warp had it whole
+    if (at.x < 0 || at.x >= p.slots || n < 1 || n > (p.slots - (at.x & ~1)) / 2) {  // never written: that warp gave up on a wait
+        if (act && (!kCoop || warp == 0)) *reinterpret_cast<uint2*>(dst) = make_uint2(0x7fff7fffu, 0x7fff7fffu);  // NaN
+        return;
+    }
     const int r = (int)(f - tile * kMaxRows);  // row of the tile
     // the first part's warp had other items ahead of this one or not; of the others it is the first
     auto slot = [&](int i) { return (int64_t)(i ? (at.x & ~1) + 2 * i : at.x) * kMaxRows + r; };
@@ -1188,6 +1193,7 @@ int paged_list_q8(const PackedArgs& a, const float* k_scales, const float* v_sca
     ws += up256(n * (a.head_dim <= 64 ? 64 : 128) * sizeof(float));
     p.part_ml = reinterpret_cast<float2*>(ws);
     p.parts = reinterpret_cast<int2*>(ws + up256(n * sizeof(float2)));
+    p.slots = 2 * ctas * kWarps;
     const bool small = a.head_dim <= 64;
     if (rows <= 8) return small ? launch_list<64, 8>(p, ctas, st) : launch_list<128, 8>(p, ctas, st);
     return small ? launch_list<64, 16>(p, ctas, st) : launch_list<128, 16>(p, ctas, st);
