@@ -539,7 +539,8 @@ __global__ void __launch_bounds__(kThreads, kMaxRows == 8 ? 3 : 2)
     WarpTile<HD, kMaxRows> w;
     w.start(p, row0, R, kvh, f0, nseq, len, k1);
     bool ok = true;
-    for (int j = 0; j < nst; ++j) {
+    int j = 0;
+    for (; j < nst; ++j) {
         const int s = j % L::kStages;
         ok = mbar_wait_warp(&full[s], (uint32_t)(j / L::kStages) & 1u, abort_flag);
         if (!ok) break;
@@ -553,9 +554,14 @@ __global__ void __launch_bounds__(kThreads, kMaxRows == 8 ? 3 : 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
     }
-    if (!ok) {
+    if (!ok) {  // copies in flight land before the ring is used again and the CTA leaves; the rows are NaN
         *abort_flag = 1;
         if (lane == 0) set_err(p.err, 0x722);
+        int never = 0;
+        for (int i = j; i < min(nst, j + L::kStages); ++i)
+            mbar_wait_bounded(&full[i % L::kStages], (uint32_t)(i / L::kStages) & 1u, &never, 100000000ull);
+        __syncwarp();
+        w.l[0] = w.l[1] = NAN;
     }
     // ---- merge of the four warps
     w.sum_lanes();

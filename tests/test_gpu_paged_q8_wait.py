@@ -94,3 +94,13 @@ def test_list(broken, seqs, keys, H, KV):
     if (seqs, KV) == (70, 8):
         nan = torch.isnan(got[(at + 1) // KV, (at + 1) % KV])
         assert bool(nan.all())
+
+
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 128), (16, 1, 64), (4, 4, 64)])
+@pytest.mark.parametrize("keys,key", [([100, 90], 16), ([700, 5000, 900], 4999), ([2000], 0)])
+def test_ranges(broken, keys, key, H, KV, hd):
+    """One CTA for an item, or a cluster: all its rows are NaN, whichever range waited in vain."""
+    assert getattr(broken, NAME + "_workspace")(len(keys), max(keys), H, KV, hd) == 0
+    b, h = len(keys) // 2, KV - 1
+    got = check(broken, keys, H, KV, hd, 32, (b, key, h), (0x721, 0x722), lambda i, j: (i, j) != (b, h))
+    assert torch.isnan(got[b, h]).all()
