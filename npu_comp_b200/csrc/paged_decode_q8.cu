@@ -57,7 +57,7 @@ template <int HD, int kMaxRows>
 struct Smem {
     static constexpr int kTile = kKeys * HD;  // K or V of a stage
     static constexpr int kStages = (kMaxRows == 8 ? 64 : 96) * 1024 / (2 * kTile);
-    static constexpr int kOffScale = kStages * 2 * kTile;  // [stage][group]: c s_k 2^24, log2(s_v), 1 / s_v
+    static constexpr int kOffScale = kStages * 2 * kTile;  // [stage][group]: c s_k, log2(s_v), 1 / s_v
     static constexpr int kOffBar = kOffScale + kStages * kGroups * 16;
     static constexpr int kTotal = kOffBar + 256;
     // The merge reuses the ring: the warps' partials, then (clusters) the CTA's own.  A lane writes runs of HD / 8
@@ -134,7 +134,9 @@ __device__ __forceinline__ float usable(float scale, bool v, bool in_pool) {
     return v && scale < 9.094947e-13f ? 9.094947e-13f : scale;
 }
 
-// c s_k 2^24 of a usable K scale; log2 and reciprocal of a usable V scale (to 2^-22 and 2^-23: as close as the scores).  The
+// A score's integer sum is its products' sum 2^24 - 128 sum(q), in one rounding; the scales come behind it, so that scores
+// are right as far as fp32 holds them (2^24 in the scale ran over from c s_k = 2e31 on).
+// log2 and reciprocal of a usable V scale (to 2^-22 and 2^-23: as close as the scores).  The
 // reciprocal of NaN is 1: the scores carry the NaN to the rows that see the page, and masked ones weigh 0 times this.
 constexpr float kSubnormal = 16777216.0f;
 __device__ __forceinline__ float log2_of(float v) {
@@ -178,7 +180,7 @@ struct WarpTile {
     uint32_t qf[HD / 16][2 * kQ];
     int lim[2];  // keys of rows ra and rb end here
     float m[2], l[2];
-    float bias[2];  // 128 sum(q) 2^-24 of rows ra and rb
+    float bias[2];  // 128 sum(q) of rows ra and rb
     float o[kO][4];
 
     __device__ __forceinline__ static int row_of(int e) { return kT ? e & 1 : e >> 1; }
@@ -216,7 +218,7 @@ struct WarpTile {
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            bias[i] = sum * (128.0f / kSubnormal);
+            bias[i] = sum * 128.0f;
         }
         if (kT) {  // that of row g8 is in its lanes
             bias[1] = __shfl_sync(0xffffffffu, bias[0], rb * 4);
@@ -236,7 +238,7 @@ struct WarpTile {
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
     }
-    // kStep keys from kb on at kt and vt; sc(u): {c s_k 2^24, log2(s_v), 1 / s_v} of its u-th 16 keys.
+    // kStep keys from kb on at kt and vt; sc(u): {c s_k, log2(s_v), 1 / s_v} of its u-th 16 keys.
     template <typename Scales>
     __device__ __forceinline__ void step(const uint8_t* kt, const uint8_t* vt, int kb, Scales sc) {
         float x[kX][4];
@@ -275,11 +277,10 @@ struct WarpTile {
         for (int u = 0; u < kStep / 16; ++u) {
             const float4 v = sc(u);
             inv[u] = v.z;
-            const float off[2] = {fmaf(-v.x, bias[0], v.y), fmaf(-v.x, bias[1], v.y)};
 #pragma unroll
             for (int n = u * kX * 16 / kStep; n < (u + 1) * kX * 16 / kStep; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[n][e] = fmaf(x[n][e], v.x, off[row_of(e)]);
+                for (int e = 0; e < 4; ++e) x[n][e] = fmaf(fmaf(x[n][e], kSubnormal, -bias[row_of(e)]), v.x, v.y);
         }
         if (kb + kStep > min(lim[0], lim[1])) {
 #pragma unroll
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, kMaxRows == 8 ? 3 : 2)
                         sc[g * 4 + 2] = inverse_of(v);
                     }
                 } else {
-                    for (int g = 0; g < groups; ++g) sc[g * 4] = v * p.c * kSubnormal;
+                    for (int g = 0; g < groups; ++g) sc[g * 4] = v * p.c;
                 }
             }
             __syncwarp();
@@ -837,7 +838,6 @@ __global__ void __launch_bounds__(kWarps * 32, kListCtas) paged_list_q8_kernel(c
 
     // ---- the steps
     WarpTile<HD, kMaxRows> w;
-    const float skc = p.c * kSubnormal;
     int src[kStep / 16];  // the lane of the K piece that holds 16 keys (V's is the next)
 #pragma unroll
     for (int u = 0; u < kStep / 16; ++u) src[u] = 2 * (u * 16 / p.box_rows);
@@ -872,7 +872,7 @@ __global__ void __launch_bounds__(kWarps * 32, kListCtas) paged_list_q8_kernel(c
             return;
         }
         const float v = usable(scale[0], kv, pool[0]);
-        const float first_of = kv ? log2_of(v) : v * skc, inv = inverse_of(v);
+        const float first_of = kv ? log2_of(v) : v * p.c, inv = inverse_of(v);
         const uint8_t* kt = ring + slot * 2 * L::kTile;
         w.step(kt, kt + L::kTile, now.step * kStep, [&](int u) {
             return make_float4(__shfl_sync(0xffffffffu, first_of, src[u]), __shfl_sync(0xffffffffu, first_of, src[u] + 1),

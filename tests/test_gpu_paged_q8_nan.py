@@ -118,3 +118,26 @@ def test_pages_behind_a_row(cuda_device, which, value, m, n, max_new, hd):
     want.view(n, H, hd)[clean:, 1] = math.nan
     same(o[:n], want, bound)
     same(o[n:], alone, alone_bound)
+
+
+@pytest.mark.parametrize("scale,spread", [(1e30, 100.0), (1e-3, 1e36), (1e34, 1e-3)])
+@pytest.mark.parametrize("m,n,hd", [(500, 1, 128), (1000, 9, 64), (16400, 2, 128), (600, 80, 128)])
+def test_scores_of_any_size(cuda_device, scale, spread, m, n, hd):
+    """Finite scores of 1e30 and more: the largest takes all of the weight."""
+    H, KV, ps = 8, 2, 16
+    c = Cache([m], KV, hd, ps, seed=m + n)
+    c.ks[c.table[0, :(m + ps - 1) // ps].long()] = spread
+    q = (torch.randn((n, H * hd), generator=torch.Generator().manual_seed(n)) / 8).half().cuda()
+    k, v, _, _ = c.seq(0)
+    x = torch.einsum("nhd,mhd->hnm", q.view(n, H, hd).double(), k.repeat_interleave(H // KV, 1) / spread)
+    seen = torch.arange(m, device="cuda")[None] <= (m - n + torch.arange(n, device="cuda"))[:, None]
+    best = x.masked_fill(~seen, -math.inf).topk(2, -1)
+    # fp32 roundings of 255 sum |q| (two for a bit each at every one of hd terms), and exp(-scale * spread * gap) is 0 beyond
+    off = hd * 2.0 ** -22 * 255 * q.view(n, H, hd).double().abs().sum(-1).T
+    clear = best.values[..., 0] - best.values[..., 1] > off
+    assert clear.double().mean() > 0.9 and (best.values[..., 0] * scale * spread * 1.45 < 3e38).all()
+    o = attend(c, q, [n], H, max_new=n, scale=scale)
+    assert torch.isfinite(o).all()
+    want = v.repeat_interleave(H // KV, 1)[best.indices[..., 0], torch.arange(H, device="cuda")[:, None]].transpose(0, 1)
+    err = (o.view(n, H, hd).double() - want).abs()
+    assert (err[clear.T] <= 1.25 * 2.0 ** -11 * want.abs()[clear.T] + 2.0 ** -24).all()
