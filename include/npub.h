@@ -430,8 +430,12 @@ size_t npub_attention_paged_decode_workspace(int batch, int64_t ctx_len, int sha
 /* ------------------------------------ paged KV cache in 8 bits ----
  * k_pages / v_pages int8 [n_pages, kv_heads, page_size, head_dim] (contiguous,
  * 16-byte aligned) and k_scales / v_scales fp32 [n_pages, kv_heads] (>= 0): an
- * element stands for its integer times the scale of its page and head.  Tables,
- * packed rows and page ids outside the pool as above; page_size 16 .. 256.
+ * element stands for its integer times the scale of its page and head.  Rows
+ * that see a key of a page whose scale is not finite are NaN in that head.  V
+ * scales below 2^-40 add less than 2^-33 to a result and may count as 2^-40 or
+ * as 0; a call that copies the keys (below) takes those above 2^60 as 2^60.
+ * Tables, packed rows and page ids outside the pool as above; page_size
+ * 16 .. 256.
  *
  * npub_rope_paged_append_q8: npub_rope_paged_append with k and v held so.  The
  * new rows of a sequence go to the slots from positions[its first row] on, one

@@ -103,6 +103,8 @@ __device__ __forceinline__ TileCoord tile_coord(const PairParams& p, int tile, i
 template <int BT, int STAGES, int CSTAGES, int G>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_for<G>(), 1)
     w8a16_pair_kernel(const __grid_constant__ PairParams p) {
+    // Ahead of the allocation below: a successor's CTA that held tensor memory on this SM and waited for this grid would stop
+    // both, but with the 208 KB of shared memory and more of a CTA here none that allocates any (97 KB and more) finds room.
     pdl_trigger();
     using L = Smem<BT, STAGES, CSTAGES>;
     static_assert(STAGES % G == 0 && CSTAGES >= G && CSTAGES >= 2, "see kPairStages*: converter groups take turns");

@@ -580,8 +580,13 @@ struct Choice {
 
 // The estimates' terms, in us, are fitted to CUDA graphs of calls of 1 to 8192 tokens: those above; few-token kernel at 12288
 // x 4096 with one and two CTAs for a tile, 32 tokens 15.4 and 14.2, 64 in one tile 19.5 and 16.7, 128 in two 20.5 and 26.6;
-// 4096 x 4096 at 32 tokens with 1, 2, 4, 8: 12.6, 9.5, 7.7, 7.7.  Rows that are not written 16 bytes at a time, 777 x 1003 x
-// 2064: few-token kernel 14, tiles of 128 tokens 23, of 256 36.
+// 4096 x 4096 at 32 tokens with 1, 2, 4, 8: 12.6, 9.5, 7.7, 7.7.
+// Rows that are not written 16 bytes at a time, few-token kernel, tiles of 128 and of 256 tokens: 777 x 1003 x 2064 13.6, 22.6
+// and 35.0; tiles alone, 4000 x 1003 x 4096 24 and 41, 4000 x 5001 x 4096 73 and 110, 8000 x 12289 x 4096 319 and 393, with a
+// residual 732 and 763.  The two constants for such rows are the first of these sizes', for any number of waves, and the few-token
+// kernel's stores count nothing there, so that up to 800 tokens of many channels it is taken where tiles of 128 are better
+// (777 x 5001 x 2064 29.5 and 23.3, 777 x 12289 x 11008 168 and 113), and with a residual and K of 11008 tiles of 256 (4000 x 2049
+// 115 and 97, 2000 x 12289 317 and 234).
 Choice pick(int M, int N, int k_tiles, bool vec) {
     // clusters of 1 .. 8 CTAs that 148 SMs (whole GPCs of them) hold at one CTA per SM; the few-token kernel has two
     static const int held[kMaxCluster + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};

@@ -20,9 +20,13 @@
 // Bound: the launch and a few memory latencies for a decode step (250 rows of 32 /
 // 8 heads of 128: 5.5 us).  For prompts HBM (the qkv rows read, q and the 8-bit
 // rows written) is the floor, 14 us for 4096 rows of those heads with norms; they
-// take 33.7, the query heads' launch about 14 at half of the issue slots, the
-// pages' the rest, on 16 warps an SM (a thread holds 64 values) that first look
-// for their pages.  8192 rows: 54 us.
+// take 34, the query heads' launch about 14 at half of the issue slots, the
+// pages' the rest, on 16 warps an SM (a thread holds 64 values) that look for
+// their pages again, which the query heads' launch has done for every token.  8192
+// rows: 54 us.  The fp16 append (paged_append.cu), one launch, takes 22.5 and 40.
+//
+// A prompt's q rows are normalised with rsqrtf and sums of pairs (paged_append.cuh),
+// a decode step's with 1 / sqrtf: the same row can differ in its last bit.
 #include "gemm_tc.h"
 #include "paged_append.cuh"
 

@@ -9,14 +9,19 @@
 //     fp16); a step of 16 keys lies in one page, so its scales are two numbers.
 //   * an integer q of K goes in as the byte q + 128, which as the bits of an fp16
 //     is the subnormal (q + 128) 2^-24: one byte permutation for two of them, and
-//     128 sum(q_row) is taken off the score.  (Not for V: the weights' sum times
-//     128 would drown an average over many keys.  There it is two instructions.)
+//     128 sum(q_row) is taken off the score (whose fp32 sums round relative to
+//     255 sum |q_row| for it).  (Not for V: the weights' sum times 128 would drown
+//     an average over many keys.  There it is two instructions.)
 //   * s_k multiplies the scores; s_v goes into the exponent: with z = c s_k (q . k)
 //     + log2(s_v), c = scale log2(e), the weights 2^(z - m) carry s_v, O takes them
 //     times the integers, and the row's sum takes them times 1 / s_v.  The running
-//     reference m is of z, so a weight's rounding to fp16 (2^-11) is relative to
-//     what it adds to the result.  (s_v below 2^-40 counts as 2^-40: what it
-//     adds to a result is below 2^-33.)
+//     reference m is of z, so a weight's rounding to fp16 (2^-11, for the product
+//     with V) is relative to what it adds to the result: off by 0.00023 to 0.00029
+//     against 64 bits, where the output's rounding alone is 0.00021.  (s_v below
+//     2^-40 counts as 2^-40: what it adds to a result is below 2^-33.)
+//   * a scale that is not finite makes the scores of its keys NaN, and with them
+//     the sum of every row that sees one; a part of an item whose sum is NaN is
+//     never left out of a merge.
 //   * an element's place in the product's inner dimension is free, as long as
 //     both operands agree: a lane takes 16 neighbouring columns of a key with one
 //     16-byte load, which are 4 steps of the K product, or 16 of the columns of

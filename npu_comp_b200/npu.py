@@ -1002,6 +1002,7 @@ def attention_paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
 # The same cache in 8 bits: k_pages / v_pages int8, and k_scales / v_scales fp32
 # [n_pages, kv_heads]: an element stands for its integer times the scale of its
 # page and head.  A page's scale is set by the appends: start with any contents.
+# Rows that see a key of a page whose scale is not finite are NaN in that head.
 
 def rope_paged_append_q8(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: int, positions: torch.Tensor,
                          inv_freq: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor,
