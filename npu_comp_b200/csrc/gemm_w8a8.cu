@@ -501,14 +501,13 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
         tmem_dealloc(tmem, BT);
     }
     if (warp < 4) {
+        const int tokens = min(BT, p.M - m0);
         // a CTA of the cluster that gave up has no sums: nothing is stored (looked up here, needed behind the sums' loads)
         uint32_t gave_up = 0;
-        if (lane < S)
-            asm volatile("ld.shared::cluster.u32 %0, [%1];"
-                         : "=r"(gave_up)
-                         : "r"(S > 1 ? mapa_shared(smem_u32((const void*)abort_flag), (uint32_t)lane) : smem_u32((const void*)abort_flag))
-                         : "memory");
-        const int tokens = min(BT, p.M - m0);
+        if (lane < S && r * 4 + warp < tokens) {
+            const uint32_t flag = smem_u32((const void*)abort_flag);
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(gave_up) : "r"(S > 1 ? mapa_shared(flag, lane) : flag) : "memory");
+        }
         const int n = n0 + lane * 4;
         const int left = p.N - n;  // channels of this lane
         const uint32_t base = smem_u32(smem) + (uint32_t)lane * 16u;
