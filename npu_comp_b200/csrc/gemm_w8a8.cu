@@ -396,6 +396,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
     uint64_t* done = empty + L::kStages;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* no_sums = abort_flag + 1;  // a CTA of the cluster gave up
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int S = (p.k_tiles + p.per - 1) / p.per;
     const int tile = (int)blockIdx.x / S, r = (int)blockIdx.x - tile * S;
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
             mbar_init(&empty[s], 1);
         }
         mbar_init(done, 1);
-        *abort_flag = 0;
+        *abort_flag = *no_sums = 0;
         fence_barrier_init();
     }
     if (warp == 4 && lane == 0) {
@@ -428,6 +429,12 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
     pdl_wait();
 
     bool ok = true;
+    auto give_up = [&](int code) {
+        *abort_flag = 1;
+        set_err(p.err, code);
+        for (int q = 0; q < S; ++q)
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(smem_u32((const void*)no_sums), q)), "r"(1) : "memory");
+    };
     if (warp == 4) {
         if (lane == 0) {  // producer
             int i = 0;
@@ -440,8 +447,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
                 tma_load_3d(sX + s * L::kX, &p.tmA, &full[s], (kt0 + i) * BK, m0, 0);
             }
             if (!ok) {  // copies in flight land before the CTA leaves
-                *abort_flag = 1;
-                set_err(p.err, 0x711);
+                give_up(0x711);
                 int never = 0;
                 for (int j = max(0, i - L::kStages); j < i; ++j)
                     mbar_wait_bounded(&full[j % L::kStages], (uint32_t)(j / L::kStages) & 1u, &never, 100000000ull);
@@ -463,10 +469,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
                            (i > 0 || k > 0) ? 1u : 0u);
                 tc_commit(&empty[s]);
             }
-            if (!ok) {
-                *abort_flag = 1;
-                set_err(p.err, 0x712);
-            }
+            if (!ok) give_up(0x712);
             tc_commit(done);
             if (!ok) {  // the MMAs end, and the copies that nobody has waited for land, before the CTA leaves
                 int never = 0;
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
             }
         }
     } else {
-        ok = __all_sync(0xffffffffu, mbar_wait_quick(done, 0, abort_flag) && !*abort_flag);
+        ok = __all_sync(0xffffffffu, mbar_wait_quick(done, 0, abort_flag));
         tc_fence_after();
         if (ok) {  // the ring is free: this CTA's sums [token][channel]
             int* sums = reinterpret_cast<int*>(smem) + warp * 32 + lane;
@@ -489,8 +492,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
                 for (int j = 0; j < 16; ++j) sums[(c0 + j) * 128] = acc[j];
             }
         } else if (lane == 0) {
-            *abort_flag = 1;
-            set_err(p.err, 0x713);
+            give_up(0x713);
         }
     }
     tc_fence_before();
@@ -500,14 +502,8 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
         tc_fence_after();
         tmem_dealloc(tmem, BT);
     }
-    if (warp < 4) {
+    if (warp < 4 && !*no_sums) {
         const int tokens = min(BT, p.M - m0);
-        // a CTA of the cluster that gave up has no sums: nothing is stored (looked up here, needed behind the sums' loads)
-        uint32_t gave_up = 0;
-        if (lane < S && r * 4 + warp < tokens) {
-            const uint32_t flag = smem_u32((const void*)abort_flag);
-            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(gave_up) : "r"(S > 1 ? mapa_shared(flag, lane) : flag) : "memory");
-        }
         const int n = n0 + lane * 4;
         const int left = p.N - n;  // channels of this lane
         const uint32_t base = smem_u32(smem) + (uint32_t)lane * 16u;
@@ -532,7 +528,7 @@ __global__ void __launch_bounds__(kFewThreads) w8a8_few_kernel(const __grid_cons
                     v.z += got[q].z;
                     v.w += got[q].w;
                 }
-            if (__any_sync(0xffffffffu, gave_up != 0) || left <= 0) continue;
+            if (left <= 0) continue;
             const int m = m0 + j;
             const float sa = __ldg(p.sa + m);
             float z[4] = {(float)v.x * (sa * sw[0]), (float)v.y * (sa * sw[1]), (float)v.z * (sa * sw[2]),
